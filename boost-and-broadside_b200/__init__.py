@@ -15,6 +15,7 @@ from .yemong.encoder import BulletEncoder, ShipEncoder
 from .yemong.heads import HeadMLP, NextStateHead, TeamPMA, evaluate_action, sample_action
 from .yemong.griffin import CONV_KERNEL, RGLRU, GriffinTemporalBlock, YemongBlock
 from .yemong.policy import YemongPolicy
+from .yemong.selective import causal_conv, causal_conv_step, selective_scan, selective_step
 from .yemong.trunk import YemongTrunk, RaggedBatch
 
 __all__ = [
@@ -33,6 +34,10 @@ __all__ = [
     "YemongBlock",
     "YemongPolicy",
     "YemongTrunk",
+    "causal_conv",
+    "causal_conv_step",
     "evaluate_action",
     "sample_action",
+    "selective_scan",
+    "selective_step",
 ]

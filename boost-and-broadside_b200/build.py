@@ -3,7 +3,7 @@
     python boost-and-broadside_b200/build.py [--force]
 
 The library lands beside this file as ``libbnb_trunk.so``; it is what ``_capi`` loads.  Beside it lands
-``_host_path.so``, the CPython module with the host side of a call (csrc/host_path.cpp), linked
+``_host_path.so``, the CPython module with the host side of a call (csrc/host_path.cpp, csrc/host_sequences.cpp), linked
 against the library.
 """
 
@@ -19,7 +19,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbnb_trunk.so")
 HOST_MODULE = os.path.join(HERE, "_host_path.so")
-SOURCES = ["capi.cu", "exact_kernels.cu", "tensor_kernels.cu", "bullet_kv.cu", "pipelined_tile_kernel.cu", "static_scratch.cu", "grad_kernels.cu", "mlp_kernels.cu", "head_tiles.cu", "policy_tail.cu", "train_attention.cu", "train_mlp.cu", "train_linear.cu", "split_kernels.cu"]
+SOURCES = ["capi.cu", "exact_kernels.cu", "tensor_kernels.cu", "bullet_kv.cu", "pipelined_tile_kernel.cu", "static_scratch.cu", "grad_kernels.cu", "mlp_kernels.cu", "head_tiles.cu", "policy_tail.cu", "train_attention.cu", "train_mlp.cu", "train_linear.cu", "split_kernels.cu", "causal_conv.cu", "selective_scan.cu", "selective_scan_bwd.cu"]
+HOST_SOURCES = ["host_path.cpp", "host_sequences.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",
@@ -41,28 +42,28 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def _host_compile() -> tuple[str, list[str]]:
-    """Object file and compiler command of the host module (torch's own headers and C++ ABI)."""
+def _host_compile(src: str) -> tuple[str, list[str]]:
+    """Object file and compiler command of a part of the host module (torch's own headers and C++ ABI)."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
-    obj = os.path.join(HERE, "build", "host_path.o")
+    obj = os.path.join(HERE, "build", src.replace(".cpp", ".o"))
     os.makedirs(os.path.dirname(obj), exist_ok=True)
     includes = [*cpp_extension.include_paths(), os.path.dirname(os.path.dirname(_nvcc())) + "/include",
                 sysconfig.get_paths()["include"], os.path.join(ROOT, "include"), CSRC]
     flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_API_INCLUDE_EXTENSION_H",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
-    cmd = ["g++", *flags, *[a for i in includes for a in ("-isystem", i)], "-c", os.path.join(CSRC, "host_path.cpp"), "-o", obj]
+    cmd = ["g++", *flags, *[a for i in includes for a in ("-isystem", i)], "-c", os.path.join(CSRC, src), "-o", obj]
     return obj, cmd
 
 
-def _link_host(obj: str) -> list[str]:
+def _link_host(objs: list[str]) -> list[str]:
     from torch.utils import cpp_extension
 
     libs = [a for p in cpp_extension.library_paths() for a in ("-L", p)]
-    return ["g++", "-shared", "-o", HOST_MODULE, obj, "-L", HERE, "-l:libbnb_trunk.so", *libs, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+    return ["g++", "-shared", "-o", HOST_MODULE, *objs, "-L", HERE, "-l:libbnb_trunk.so", *libs, "-lc10", "-lc10_cuda", "-ltorch_cpu",
             "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
 
 
@@ -72,8 +73,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     objs = []
     procs = []
-    host_obj, host_cmd = _host_compile()
-    procs.append(("host_path.cpp", subprocess.Popen(host_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    host_objs = []
+    for src in HOST_SOURCES:
+        obj, cmd = _host_compile(src)
+        host_objs.append(obj)
+        procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     for src in SOURCES:
         obj = os.path.join(HERE, "build", src.replace(".cu", ".o"))
         os.makedirs(os.path.dirname(obj), exist_ok=True)
@@ -89,7 +93,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
             sys.stderr.write(out)
         if p.returncode:
             raise RuntimeError(f"nvcc failed on {src}")
-    for link in ([_nvcc(), "-shared", "-o", LIB, *objs, "-lcudart"], _link_host(host_obj)):
+    for link in ([_nvcc(), "-shared", "-o", LIB, *objs, "-lcudart"], _link_host(host_objs)):
         r = subprocess.run(link, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
         if r.returncode:
             sys.stderr.write(r.stdout)

@@ -24,14 +24,13 @@
 
 #include "bnb_trunk.h"
 #include "host_calls.h"
+#include "host_tensors.h"
 #include "mlp_kernels.h"
 #include "policy_tail.h"
 #include "split_kernels.h"
 #include "tensor_kernels.h"
 
-namespace py = pybind11;
-using at::Tensor;
-using OptTensor = c10::optional<Tensor>;
+using namespace bnb::host;
 
 namespace {
 
@@ -148,39 +147,6 @@ py::object trunk_params(const py::sequence& blocks, bool has_fields) {
 
 constexpr int kEngineSimt = BNB_ENGINE_SIMT;
 
-const void* ptr(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
-
-Tensor f32c(const Tensor& t) {
-  if (t.scalar_type() == at::kBFloat16 && t.is_cuda() && t.is_contiguous() && t.numel() % 8 == 0 &&
-      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) {
-    const c10::cuda::CUDAGuard guard(t.device());
-    const Tensor f = at::empty(t.sizes(), t.options().dtype(at::kFloat));
-    if (bnb::host::widen(t.data_ptr(), static_cast<float*>(f.data_ptr()), (size_t)t.numel(), at::cuda::getCurrentCUDAStream(t.device().index()).stream()) != BNB_OK)
-      throw std::runtime_error("the bfloat16 conversion could not be launched");
-    return f;
-  }
-  const Tensor f = t.scalar_type() == at::kFloat ? t : t.to(at::kFloat);
-  return f.is_contiguous() ? f : f.contiguous();
-}
-Tensor contiguous(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
-// One byte per element: a bool tensor as it is, anything else compared with zero.
-OptTensor bytes_of(const OptTensor& t) {
-  if (!t.has_value()) return c10::nullopt;
-  return t->scalar_type() == at::kBool ? contiguous(*t) : contiguous(t->ne(0));
-}
-const float* parameter(const Tensor& t, const c10::Device& dev, const char* what) {
-  if (t.device() != dev)
-    throw std::runtime_error(std::string(what) + " parameter is on " + t.device().str() + ", input on " + dev.str());
-  if (t.scalar_type() != at::kFloat || !t.is_contiguous())
-    throw std::runtime_error(std::string(what) + " parameter must be contiguous float32 (got " + c10::toString(t.scalar_type()) + ")");
-  return static_cast<const float*>(t.data_ptr());
-}
-void check(const char* fn, int status) {
-  if (status == BNB_OK) return;
-  const std::string text = std::string(fn) + ": " + bnb_status_string(status);
-  if (status == BNB_ERR_UNSUPPORTED_DIMS) throw py::value_error(text);
-  throw std::runtime_error(text + " (status " + std::to_string(status) + ")");
-}
 // A bounded wait of an earlier call on this device ran out (its kernels drained and its outputs were
 // garbage): say so once, at the next call, without synchronising.
 void raise_pending_status(const c10::Device& dev) {
@@ -487,14 +453,6 @@ std::tuple<Tensor, Tensor, Tensor> trunk_forward_train(const Tensor& x, const Op
   if (x.scalar_type() == at::kBFloat16) y = y.to(at::kBFloat16);
   return {y, hout, kept};
 }
-
-// Behind the gradients of a backward pass that is itself recorded (create_graph=True): the trunk has no second-order
-// gradient, and whoever asks for one is told so, as by an operator without an autograd formula.
-struct NoSecondOrder : public torch::autograd::Node {
-  torch::autograd::variable_list apply(torch::autograd::variable_list&&) override {
-    throw std::runtime_error("the gradients of the CUDA trunk cannot be differentiated again (a second-order gradient through it was asked for)");
-  }
-};
 
 // The autograd node of an eager differentiated call: what the operators' formulas do, without Python in
 // the backward pass.
@@ -875,6 +833,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_tail(const Tensor& x_in, const
 }  // namespace
 
 PYBIND11_MODULE(_host_path, m) {
+  bnb::host::bind_sequences(m);
   m.def("trunk_params", &trunk_params);
   m.def("keep_activations", [](const c10::Device& dev, const std::vector<int64_t>& geom, int64_t d_model, int64_t n_bullets) {
     return keep_activations(dev, Geometry(geom), d_model, n_bullets);

@@ -1,0 +1,368 @@
+// The selective state space recurrence, forward: whole sequences and single tokens.  For every row, channel and state n
+//
+//   p = softplus(delta + bias),  h_n = exp(p a_n) h_n + p u b_n,  y = (sum_n c_n h_n + d u) silu(z)
+//
+// A sequence reads u, delta, z and writes y, eight bytes a channel and step in 16 bits, and computes an exponential for each state: with 16
+// states the exponentials (16 a clock and SM) bound it, not memory.  selective_scan.cuh describes how the work is laid out.
+// A single token reads and writes the state, eight bytes for each of its elements: memory bounds it.
+#include "selective_scan.cuh"
+
+namespace bnb {
+namespace scan {
+
+int check(const BnbSelectiveScan* a) {
+  if (!a) return BNB_ERR_NULL_POINTER;
+  if (a->steps < 0 || a->rows < 0 || a->width < 0 || a->element < 0 || a->element > 2) return BNB_ERR_BAD_ARGUMENT;
+  if (a->states < 1 || a->states > 64) return BNB_ERR_UNSUPPORTED_DIMS;
+  if (a->groups < 1 || a->width % a->groups) return BNB_ERR_BAD_ARGUMENT;
+  if (a->rows == 0 || a->width == 0) return BNB_OK;
+  if (!a->a) return BNB_ERR_NULL_POINTER;
+  if (a->steps && (!a->u.data || !a->delta.data || !a->b.data || !a->c.data)) return BNB_ERR_NULL_POINTER;
+  if ((reinterpret_cast<uintptr_t>(a->state_in) | reinterpret_cast<uintptr_t>(a->state_out) | reinterpret_cast<uintptr_t>(a->a) |
+       reinterpret_cast<uintptr_t>(a->kept)) & 15) return BNB_ERR_MISALIGNED;
+  if ((int64_t)a->rows * a->width > (int64_t)1 << 40) return BNB_ERR_BAD_ARGUMENT;
+  return BNB_OK;
+}
+
+namespace {
+
+constexpr int L = 16;    // steps of a chunk
+constexpr int CT = 32;   // channels of a CTA
+
+enum Pass : int { WHOLE, LOCAL, JOINED };   // one split; what a split leaves of a zero start; from its starting state
+
+struct Work {
+  float* local;       // (splits, rows, width, 4 KL)
+  float* sum_p;       // (splits, rows, width)
+  uint8_t* cut;       // (splits, rows)
+  Splits splits;
+  int tiles_a_group;
+};
+
+template <typename T, int KL, Pass PASS>
+__global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSelectiveScan q, Work w) {
+  constexpr int THREADS = CT * KL, NP = NS * KL, PER = L / KL;   // elements a thread prepares of every (L, CT) array
+  constexpr int BC = (L * NP + THREADS - 1) / THREADS;           // and of b and c
+  __shared__ float p_s[L][CT], pu_s[L][CT], y_s[PASS == LOCAL ? 1 : L][CT];
+  __shared__ __align__(16) float b_s[L][NP], c_s[PASS == LOCAL ? 1 : L][NP];
+  const int tid = threadIdx.x, cl = tid / KL, lane = tid % KL;
+  const int tiles = w.tiles_a_group * q.groups, share = q.width / q.groups;
+  const int r = blockIdx.x / tiles, tile = blockIdx.x - r * tiles, group = tile / w.tiles_a_group;
+  const int c0 = group * share + (tile - group * w.tiles_a_group) * CT, c_end = min((group + 1) * share, c0 + CT);   // channels [c0, c_end)
+  const int ch = c0 + cl;
+  const bool owns = ch < c_end, wide = q.states % NS == 0;
+  const int n = row_steps(q.lengths, r, q.steps);
+  const int split = blockIdx.y, first = split * w.splits.steps, last = min(q.steps, first + w.splits.steps);
+  const int64_t rc = (int64_t)r * q.width + ch;
+
+  float rate[NS], h[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) rate[i] = h[i] = 0.f;
+  if (owns) {
+    load_states(rate, q.a + (int64_t)ch * q.states, NS * lane, q.states, wide);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) rate[i] *= LOG2E;
+    if constexpr (PASS == WHOLE) {
+      if (q.state_in) load_states(h, q.state_in + rc * q.states, NS * lane, q.states, wide);
+    } else if constexpr (PASS == JOINED) {
+      load_states(h, w.local + ((int64_t)split * q.rows * q.width + rc) * NP, NS * lane, NP, true);
+    }
+  }
+
+  // what this thread prepares: steps t0 + tid / CT + k KL of channel c0 + tid % CT
+  const int pc = tid % CT, pt = tid / CT;
+  const bool prepares = c0 + pc < c_end;
+  const float bias = prepares && q.delta_bias ? q.delta_bias[c0 + pc] : 0.f, skip = prepares && q.d ? q.d[c0 + pc] : 0.f;
+  const T* up = static_cast<const T*>(q.u.data) + r * q.u.row + c0 + pc;
+  const T* dp = static_cast<const T*>(q.delta.data) + r * q.delta.row + c0 + pc;
+  const T* zp = static_cast<const T*>(q.z.data) + r * q.z.row + c0 + pc;
+  const T* bp = static_cast<const T*>(q.b.data) + r * q.b.row + group * q.b.group;
+  const T* cp = static_cast<const T*>(q.c.data) + r * q.c.row + group * q.c.group;
+  T* yp = static_cast<T*>(q.y.data) + r * q.y.row + c0 + pc;
+  const bool gated = q.z.data != nullptr;
+  const T none = from_f<T>(0.f);
+  T u_r[PER], d_r[PER], z_r[PER], b_r[BC], c_r[BC];
+  unsigned cuts = 0, cuts_next = 0;   // bit k: an episode ended before step t0 + k
+  auto fetch = [&](int t0) {
+    if (q.done) {
+      const int t = t0 + (tid & 31) - 1;
+      cuts_next = __ballot_sync(0xffffffffu, (tid & 31) < L && t >= 0 && t + 1 < n && q.done[(int64_t)max(t, 0) * q.rows + r]);
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int t = t0 + pt + k * KL;
+      const bool on = prepares && t < min(n, last);
+      u_r[k] = on ? up[t * q.u.step] : none;
+      d_r[k] = on ? dp[t * q.delta.step] : none;
+      z_r[k] = PASS != LOCAL && gated && on ? zp[t * q.z.step] : none;
+    }
+#pragma unroll
+    for (int k = 0; k < BC; ++k) {
+      const int e = tid + k * THREADS, t = t0 + e / NP, s = e % NP;
+      const bool on = e < L * NP && s < q.states && t < min(n, last);
+      b_r[k] = on ? bp[t * q.b.step + s] : none;
+      if (PASS != LOCAL) c_r[k] = on ? cp[t * q.c.step + s] : none;
+    }
+  };
+  float sum_p = 0.f;
+  bool any_cut = false;
+  const int live = min(n, last);
+  if (first < live) fetch(first);
+#pragma unroll 1
+  for (int t0 = first; t0 < live; t0 += L) {
+    float u_f[PER], gate[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      u_f[k] = to_f(u_r[k]);
+      const float p = t0 + pt + k * KL < live ? step_size(to_f(d_r[k]) + bias, q.softplus) : 0.f;
+      p_s[pt + k * KL][pc] = p;
+      pu_s[pt + k * KL][pc] = p * u_f[k];
+      if (PASS != LOCAL) {
+        const float z = to_f(z_r[k]);
+        gate[k] = gated ? z * sigmoid<T>(z) : 1.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < BC; ++k) {
+      const int e = tid + k * THREADS;
+      if (e < L * NP) {
+        (&b_s[0][0])[e] = to_f(b_r[k]);
+        if (PASS != LOCAL) (&c_s[0][0])[e] = to_f(c_r[k]);
+      }
+    }
+    cuts = cuts_next;
+    any_cut |= cuts != 0;
+    __syncthreads();
+    if (t0 + L < live) fetch(t0 + L);
+    constexpr int GROUP = KL > 4 ? KL : 4;
+#pragma unroll 1
+    for (int g0 = 0; g0 < L; g0 += GROUP) {
+      float y[GROUP];
+#pragma unroll
+      for (int k = 0; k < GROUP; ++k) {
+        const int t = g0 + k;
+        if (PASS != LOCAL && t % KEEP == 0 && q.kept && owns && t0 + t < live)
+          store_states(q.kept + ((int64_t)((t0 + t) / KEEP) * q.rows * q.width + rc) * NP, h, NS * lane, NP, true);
+        if ((cuts >> t) & 1) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i) h[i] = 0.f;
+        }
+        const float p = p_s[t][cl], pu = pu_s[t][cl];
+        const float4 b4 = *reinterpret_cast<const float4*>(&b_s[t][NS * lane]);
+        const float b[NS] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+        for (int i = 0; i < NS; ++i) h[i] = fmaf(ex2(p * rate[i]), h[i], pu * b[i]);
+        if (PASS == LOCAL) {
+          sum_p += p;
+        } else {
+          const float4 c4 = *reinterpret_cast<const float4*>(&c_s[t][NS * lane]);
+          y[k] = fmaf(c4.x, h[0], c4.y * h[1]) + fmaf(c4.z, h[2], c4.w * h[3]);
+        }
+      }
+      if constexpr (PASS != LOCAL) {
+        constexpr int BITS = KL == 1 ? 0 : KL == 2 ? 1 : KL == 4 ? 2 : KL == 8 ? 3 : 4;
+        const int at = sum_lanes<GROUP, 0, BITS>(y);
+#pragma unroll
+        for (int k = 0; k < (GROUP >> BITS); ++k) y_s[g0 + at + k][cl] = y[k];
+      }
+    }
+    __syncthreads();
+    if constexpr (PASS != LOCAL) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int t = t0 + pt + k * KL;
+        if (prepares && t < live) yp[t * q.y.step] = from_f<T>(fmaf(skip, u_f[k], y_s[pt + k * KL][pc]) * gate[k]);
+      }
+    }
+  }
+  if constexpr (PASS == LOCAL) {
+    if (owns) {
+      store_states(w.local + ((int64_t)split * q.rows * q.width + rc) * NP, h, NS * lane, NP, true);
+      if (lane == 0) w.sum_p[(int64_t)split * q.rows * q.width + rc] = sum_p;
+    }
+    if (tid == 0 && tile == 0) w.cut[(int64_t)split * q.rows + r] = any_cut;
+  } else {
+    if (prepares)
+      for (int t = max(first, n) + pt; t < last; t += KL) yp[t * q.y.step] = none;
+    // the split that holds the row's last step has its state; a row without steps, the first one
+    if (owns && q.state_out && ((first < n && n <= last) || (n == 0 && split == 0)))
+      store_states(q.state_out + rc * q.states, h, NS * lane, q.states, wide);
+  }
+}
+
+// One token a row.  A thread keeps the constants of its channel's states and goes over rows ROWS at a time, so that their
+// states are in flight together.
+template <typename T, int KL, int ROWS, bool WIDE>
+__global__ void __launch_bounds__(256) k_step(const __grid_constant__ BnbSelectiveScan q) {
+  constexpr int BITS = KL == 1 ? 0 : KL == 2 ? 1 : KL == 4 ? 2 : KL == 8 ? 3 : 4;
+  const int lane = threadIdx.x % KL, ch = blockIdx.y * (256 / KL) + threadIdx.x / KL;
+  const bool on = ch < q.width;
+  const int c = on ? ch : 0, group = c / (q.width / q.groups), n0 = NS * lane;
+  float rate[NS];
+  load_states(rate, q.a + (int64_t)c * q.states, n0, q.states, WIDE);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) rate[i] *= LOG2E;
+  const float bias = q.delta_bias ? q.delta_bias[c] : 0.f, skip = q.d ? q.d[c] : 0.f;
+  const bool real = n0 < q.states;
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < q.rows; r0 += (int64_t)gridDim.x * ROWS) {
+    float h[ROWS][NS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t r = r0 + k;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) h[k][i] = 0.f;
+      if (r < q.rows && on && real && q.state_in && !(q.reset && q.reset[r])) load_states(h[k], q.state_in + (r * q.width + c) * q.states, n0, q.states, WIDE);
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t r = r0 + k;
+      if (r >= q.rows) break;
+      const float u = to_f(static_cast<const T*>(q.u.data)[r * q.u.row + c]);
+      const float p = step_size(to_f(static_cast<const T*>(q.delta.data)[r * q.delta.row + c]) + bias, q.softplus), pu = p * u;
+      const T* b = static_cast<const T*>(q.b.data) + r * q.b.row + group * q.b.group + n0;
+      const T* cc = static_cast<const T*>(q.c.data) + r * q.c.row + group * q.c.group + n0;
+      float y = 0.f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const bool has = WIDE ? real : n0 + i < q.states;
+        h[k][i] = fmaf(ex2(p * rate[i]), h[k][i], has ? pu * to_f(b[i]) : 0.f);
+        if (has) y = fmaf(to_f(cc[i]), h[k][i], y);
+      }
+#pragma unroll
+      for (int o = 1; o < KL; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      if (on && real) store_states(q.state_out + (r * q.width + c) * q.states, h[k], n0, q.states, WIDE);
+      if (on && lane == 0) {
+        y = fmaf(skip, u, y);
+        if (q.z.data) {
+          const float z = to_f(static_cast<const T*>(q.z.data)[r * q.z.row + c]);
+          y *= z * sigmoid<T>(z);
+        }
+        static_cast<T*>(q.y.data)[r * q.y.row + c] = from_f<T>(y);
+      }
+    }
+  }
+}
+
+// Sixteen warps of each SM with two CTAs to spare: what the splits aim at.
+Splits splits(const BnbSelectiveScan& a, int kl, int tiles) {
+  return splits_of(a.steps, (int64_t)tiles * a.rows, 148 * std::max(1, 1024 / (CT * kl)));
+}
+int tiles_a_group(const BnbSelectiveScan& a) { return (a.width / a.groups + CT - 1) / CT; }
+
+struct Scratch { size_t local, sum_p, cut, total; };
+Scratch scratch_of(const BnbSelectiveScan& a, const Splits& s, int kl) {
+  Scratch o{};
+  if (s.count == 1) return o;
+  const size_t cells = (size_t)s.count * a.rows * a.width;
+  o.sum_p = round256(cells * NS * kl * 4);
+  o.cut = o.sum_p + round256(cells * 4);
+  o.total = o.cut + round256((size_t)s.count * a.rows);
+  return o;
+}
+
+template <typename T, int KL>
+int launch(const BnbSelectiveScan& a, uint8_t* scratch, cudaStream_t st) {
+  Work w{};
+  w.tiles_a_group = tiles_a_group(a);
+  const int64_t tiles = (int64_t)w.tiles_a_group * a.groups;
+  w.splits = splits(a, KL, (int)tiles);
+  if (tiles * a.rows > INT32_MAX || w.splits.count > 65535) return BNB_ERR_UNSUPPORTED_DIMS;
+  const dim3 grid((unsigned)(tiles * a.rows), w.splits.count);
+  if (w.splits.count == 1) {
+    count_launch();
+    k_scan<T, KL, WHOLE><<<grid, CT * KL, 0, st>>>(a, w);
+  } else {
+    const Scratch s = scratch_of(a, w.splits, KL);
+    w.local = reinterpret_cast<float*>(scratch);
+    w.sum_p = reinterpret_cast<float*>(scratch + s.sum_p);
+    w.cut = scratch + s.cut;
+    count_launch();
+    k_scan<T, KL, LOCAL><<<grid, CT * KL, 0, st>>>(a, w);
+    const int64_t cells = (int64_t)a.rows * a.width * NS * KL;
+    count_launch();
+    k_join<false><<<(unsigned)((cells + 255) / 256), 256, 0, st>>>(w.local, w.sum_p, w.cut, a.a, a.state_in, w.splits.count, a.rows, a.width, a.states, NS * KL);
+    count_launch();
+    k_scan<T, KL, JOINED><<<grid, CT * KL, 0, st>>>(a, w);
+  }
+  return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;
+}
+
+template <typename T, int KL>
+int launch_step(const BnbSelectiveScan& a, cudaStream_t st) {
+  constexpr int ROWS = 4;
+  const int tiles = (a.width * KL + 255) / 256;
+  if (tiles > 65535) return BNB_ERR_UNSUPPORTED_DIMS;
+  const int64_t groups = (a.rows + ROWS - 1) / ROWS, fit = std::max(1, 148 * 8 / tiles);
+  count_launch();
+  if (groups < fit) {   // fewer rows than it takes to fill the chip: one each
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, fit), tiles);
+    if (a.states % NS == 0) k_step<T, KL, 1, true><<<grid, 256, 0, st>>>(a);
+    else k_step<T, KL, 1, false><<<grid, 256, 0, st>>>(a);
+  } else {
+    const dim3 grid((unsigned)fit, tiles);
+    if (a.states % NS == 0) k_step<T, KL, ROWS, true><<<grid, 256, 0, st>>>(a);
+    else k_step<T, KL, ROWS, false><<<grid, 256, 0, st>>>(a);
+  }
+  return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;
+}
+
+template <typename T>
+int run(const BnbSelectiveScan& a, uint8_t* scratch, cudaStream_t st) {
+  switch (lanes_of(a.states)) {
+    case 1: return launch<T, 1>(a, scratch, st);
+    case 2: return launch<T, 2>(a, scratch, st);
+    case 4: return launch<T, 4>(a, scratch, st);
+    case 8: return launch<T, 8>(a, scratch, st);
+    default: return launch<T, 16>(a, scratch, st);
+  }
+}
+template <typename T>
+int run_step(const BnbSelectiveScan& a, cudaStream_t st) {
+  switch (lanes_of(a.states)) {
+    case 1: return launch_step<T, 1>(a, st);
+    case 2: return launch_step<T, 2>(a, st);
+    case 4: return launch_step<T, 4>(a, st);
+    case 8: return launch_step<T, 8>(a, st);
+    default: return launch_step<T, 16>(a, st);
+  }
+}
+
+}  // namespace
+}  // namespace scan
+}  // namespace bnb
+
+using namespace bnb;
+
+extern "C" size_t bnb_selective_scan_kept_bytes(const BnbSelectiveScan* a) {
+  if (scan::check(a)) return 0;
+  return (size_t)((a->steps + scan::KEEP - 1) / scan::KEEP) * a->rows * a->width * scan::NS * scan::lanes_of(a->states) * 4;
+}
+
+extern "C" size_t bnb_selective_scan_scratch_bytes(const BnbSelectiveScan* a) {
+  if (scan::check(a) || a->rows == 0 || a->width == 0) return 0;
+  const int kl = scan::lanes_of(a->states);
+  return scan::scratch_of(*a, scan::splits(*a, kl, scan::tiles_a_group(*a) * a->groups), kl).total;
+}
+
+extern "C" int bnb_selective_scan_fwd(const BnbSelectiveScan* a, void* scratch, size_t scratch_bytes, void* stream) {
+  if (const int st = scan::check(a)) return st;
+  if (a->rows == 0 || a->width == 0) return BNB_OK;
+  if (a->reset || (a->state_in && a->state_in == a->state_out)) return BNB_ERR_BAD_ARGUMENT;
+  if (!a->state_out || (a->steps && !a->y.data)) return BNB_ERR_NULL_POINTER;
+  const size_t need = bnb_selective_scan_scratch_bytes(a);
+  if (need && (!scratch || scratch_bytes < need)) return BNB_ERR_SCRATCH_TOO_SMALL;
+  const auto s = static_cast<cudaStream_t>(stream);
+  auto* at = static_cast<uint8_t*>(scratch);
+  return a->element == BNB_ELEM_F32 ? scan::run<float>(*a, at, s)
+       : a->element == BNB_ELEM_BF16 ? scan::run<__nv_bfloat16>(*a, at, s) : scan::run<__half>(*a, at, s);
+}
+
+extern "C" int bnb_selective_step(const BnbSelectiveScan* a, void* stream) {
+  if (const int st = scan::check(a)) return st;
+  if (a->rows == 0 || a->width == 0) return BNB_OK;
+  if (a->steps != 1 || a->done || a->lengths || a->kept) return BNB_ERR_BAD_ARGUMENT;
+  if (!a->state_out || !a->y.data) return BNB_ERR_NULL_POINTER;
+  const auto s = static_cast<cudaStream_t>(stream);
+  return a->element == BNB_ELEM_F32 ? scan::run_step<float>(*a, s)
+       : a->element == BNB_ELEM_BF16 ? scan::run_step<__nv_bfloat16>(*a, s) : scan::run_step<__half>(*a, s);
+}

@@ -1,0 +1,137 @@
+// What the forward and the backward of the selective state space recurrence share (selective_scan.cu,
+// selective_scan_bwd.cu).
+//
+// Layout of the work.  KL neighbouring lanes own a channel of a row, four states each (KL = states / 4 rounded up to a power of two;
+// states behind the last have a = 0 and b = c = 0, so they stay 0).  A CTA walks along time in chunks with a tile of channels of one
+// row: what is per channel and step (softplus, gate, p u) is computed once by the CTA's threads together and stands in shared memory,
+// and so do the chunk's b and c, which the tile's channels share.  Steps at and behind a row's length get p = 0 and b = c = 0, which
+// makes them the identity.
+//
+// Few rows do not fill the chip.  Then time is cut into splits: a first pass over the splits computes the state each would leave
+// from a zero start, and the sum of its p, since the product of a split's decays is exp(a sum p); a short pass along the splits
+// turns these into every split's starting state; the last pass is the ordinary one, started there.  That computes the decays twice, so it is
+// taken where it at least triples the CTAs at work.
+#pragma once
+
+#include <algorithm>
+
+#include "launch_count.h"
+#include "sequence_rows.cuh"
+
+namespace bnb {
+namespace scan {
+
+using namespace seq;
+
+constexpr int NS = 4;         // states of a thread
+constexpr int KEEP = 8;       // steps from one kept state to the next
+constexpr int MIN_SPLIT = 64; // steps
+
+struct Splits {
+  int steps;   // of a split, a multiple of 16
+  int count;
+};
+// a power of two of lanes with four states each
+inline int lanes_of(int states) {
+  int k = 1;
+  while (NS * k < states) k *= 2;
+  return k;
+}
+inline Splits splits_of(int steps, int64_t ctas_a_split, int ctas_wanted) {
+  int64_t count = std::min<int64_t>(ctas_wanted / std::max<int64_t>(1, ctas_a_split), steps / MIN_SPLIT);
+  if (count < 3) return {(steps + 15) / 16 * 16, 1};
+  const int len = (int)(((steps + count - 1) / count + 15) / 16 * 16);
+  return {len, (steps + len - 1) / len};
+}
+
+// Sum over the lanes of a warp that differ in the bits [LO, HI) of their number: NV values a lane go in; afterwards v[0] ..
+// v[left - 1] hold the totals of the values from `first` on, left = max(1, NV >> (HI - LO)).  A lane passes on half of its values in
+// every round, so that NV values take about NV exchanges and not NV log2(lanes).
+template <int NV, int LO, int HI>
+__device__ __forceinline__ int sum_lanes(float* v) {
+  if constexpr (HI == LO) {
+    return 0;
+  } else {
+    const bool up = (threadIdx.x >> (HI - 1)) & 1;
+    if constexpr (NV > 1) {
+      constexpr int H = NV / 2;
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const float mine = up ? v[H + i] : v[i], other = up ? v[i] : v[H + i];
+        v[i] = mine + __shfl_xor_sync(0xffffffffu, other, 1 << (HI - 1));
+      }
+      return (up ? H : 0) + sum_lanes<H, LO, HI - 1>(v);
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1 << (HI - 1));
+      return sum_lanes<1, LO, HI - 1>(v);
+    }
+  }
+}
+// Whether this lane is the one to write what sum_lanes left of NV values over these bits (others hold the same).
+template <int NV, int LO, int HI>
+__device__ __forceinline__ bool writes_sum() {
+  int left = HI - LO, halvings = 0;
+  for (int n = NV; n > 1 && halvings < left; n /= 2) ++halvings;
+  return ((threadIdx.x >> LO) & ((1 << (left - halvings)) - 1)) == 0;
+}
+
+// log(1 + e^v) as max(v, 0) + log(1 + x) with x = e^-|v| <= 1, and log(1 + x) = 2 atanh(s), s = x / (2 + x) <= 1/3, by its Taylor series:
+// the first term left out, s^14 / 15, is 1.4e-8 of the sum.  Half the instructions of log1pf(expf(v)), without a branch,
+// and good to some units in the last place, which the gradients of a need: they are long sums.
+__device__ __forceinline__ float step_size(float v, bool with_softplus) {
+  if (!with_softplus) return v;
+  const float x = expf(-fabsf(v)), s = __fdividef(x, 2.0f + x), q = s * s;
+  float series = fmaf(q, 1.0f / 13.0f, 1.0f / 11.0f);
+  series = fmaf(q, series, 1.0f / 9.0f);
+  series = fmaf(q, series, 1.0f / 7.0f);
+  series = fmaf(q, series, 1.0f / 5.0f);
+  series = fmaf(q, series, 1.0f / 3.0f);
+  series = fmaf(q, series, 1.0f);
+  return fmaf(2.0f * s, series, fmaxf(v, 0.0f));
+}
+
+// The four states of a lane, n0 .. n0 + 3, of a (.., states) array that may end inside them.
+__device__ __forceinline__ void load_states(float (&h)[NS], const float* at, int n0, int states, bool wide) {
+  if (wide) {
+    const float4 v = *reinterpret_cast<const float4*>(at + n0);
+    h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) h[i] = n0 + i < states ? at[n0 + i] : 0.f;
+  }
+}
+__device__ __forceinline__ void store_states(float* at, const float (&h)[NS], int n0, int states, bool wide) {
+  if (wide) {
+    *reinterpret_cast<float4*>(at + n0) = make_float4(h[0], h[1], h[2], h[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) if (n0 + i < states) at[n0 + i] = h[i];
+  }
+}
+
+// Starting states of the splits from what each leaves of a zero start: local (count, rows, width, 4 KL) holds that on the way in and the
+// starting state on the way out.  REVERSE: the same for the adjoint, from the last split to the first.
+//   sum_p (count, rows, width); cut (count, rows): the split does not pass on what it starts with
+//   start (rows, width, states) or null; end: where the state behind the last split goes (REVERSE: not wanted)
+template <bool REVERSE>
+__global__ void __launch_bounds__(256) k_join(float* local, const float* sum_p, const uint8_t* cut, const float* a, const float* start,
+                                              int count, int rows, int width, int states, int padded) {
+  const int64_t cells = (int64_t)rows * width * padded, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= cells) return;
+  const int64_t rc = i / padded;
+  const int n = (int)(i - rc * padded), r = (int)(rc / width), c = (int)(rc - (int64_t)r * width);
+  const bool real = n < states;
+  const float rate = real ? a[(int64_t)c * states + n] * LOG2E : 0.f;
+  float run = real && start ? start[rc * states + n] : 0.f;
+  for (int k = 0; k < count; ++k) {
+    const int s = REVERSE ? count - 1 - k : k;
+    const float left = local[s * cells + i];
+    local[s * cells + i] = run;
+    run = (cut[(int64_t)s * rows + r] ? 0.f : ex2(rate * sum_p[s * (int64_t)rows * width + rc]) * run) + left;
+  }
+}
+
+int check(const BnbSelectiveScan* a);
+
+}  // namespace scan
+}  // namespace bnb

@@ -476,6 +476,99 @@ int bnb_pack_temporal(const BnbTemporalWeights* w, int d_model, void* packed, vo
 int bnb_pack_trunk(const BnbSpatialWeights* spatial, int n_spatial_total, const BnbTemporalWeights* temporal,
                    int n_temporal_total, int d_model, int n_heads, void* stream);
 
+/* ------------------------------------------------------------------ recurrent layers outside the trunk
+ *
+ * No counterpart in the reference, whose temporal sublayer (griffin.py:222-286) has one fixed recurrence.
+ * Sequences are time-major: (steps, rows, width), every row a sequence of its own, innermost stride 1.  */
+typedef enum { BNB_ELEM_F32 = 0, BNB_ELEM_BF16 = 1, BNB_ELEM_F16 = 2 } BnbElement;
+typedef enum { BNB_ACT_NONE = 0, BNB_ACT_SILU = 1, BNB_ACT_GELU = 2 /* erf */ } BnbActivation;
+
+/* A (steps, rows, ...) tensor of a call's element type; strides in elements. */
+typedef struct {
+  void* data;
+  int64_t step;
+  int64_t row;
+  int64_t group;            /* (steps, rows, groups, states) tensors only */
+} BnbView;
+
+/* pre[t] = bias + sum_j weight[:, taps-1-j] x[t-j], y = act(pre): the causal depthwise convolution.  Taps before
+ * step 0 come from state_in; taps of an earlier episode count as zero.
+ *   element: type of x and y; parameters and states are float32
+ *   weight (width, taps), 2 <= taps <= 4; bias (width) or NULL; activation BNB_ACT_NONE or BNB_ACT_SILU
+ *   state_in, state_out (rows, taps-1, width), oldest first; state_in NULL: zeros.  They may be one buffer
+ *     in calls of a single step.
+ *   done (steps, rows) bytes or NULL: an episode ends behind the step (as in bnb_trunk_sequence, an end behind the
+ *     last step leaves the returned state alone)
+ *   lengths (rows) or NULL: steps at and behind a row's length are not read, y is zero there, and the
+ *     state is the one after the row's last step.  Values are clamped to 0..steps.
+ *   reset (rows) bytes or NULL: rows whose state counts as zero before the first step */
+typedef struct {
+  int32_t steps, rows, width, taps, element, activation;
+  BnbView x, y;
+  const float* weight;
+  const float* bias;
+  const float* state_in;
+  float* state_out;
+  const uint8_t* done;
+  const int32_t* lengths;
+  const uint8_t* reset;
+} BnbCausalConv;
+int bnb_causal_conv_fwd(const BnbCausalConv* call, void* stream);
+
+/* Gradients of the above (y and state_out of the call are not read; reset must be NULL): dx, dstate_in and the sums
+ * dweight (width, taps), dbias (width) of given dy and dstate_out (NULL: zero).  dstate_in and dbias may be NULL. */
+typedef struct {
+  BnbView dy, dx;
+  const float* dstate_out;
+  float* dstate_in;
+  float* dweight;
+  float* dbias;
+} BnbCausalConvGrads;
+size_t bnb_causal_conv_bwd_scratch_bytes(const BnbCausalConv* call);
+int bnb_causal_conv_bwd(const BnbCausalConv* call, const BnbCausalConvGrads* grads, void* scratch, size_t scratch_bytes,
+                        void* stream);
+
+/* The selective state space recurrence, for every row, channel c and state n < states:
+ *   p = softplus(delta + delta_bias) (softplus = 0: p = delta + delta_bias),
+ *   h_n = exp(p a[c, n]) h_n + p u b_n,  y = (sum_n c_n h_n + d u) silu(z).
+ * b and c are shared by the width / groups channels of a group.  1 <= states <= 64, groups divide width.
+ *   element: type of u, delta, z, b, c, y; a (width, states), d, delta_bias (width) and states are float32
+ *   z.data NULL: no gate; d, delta_bias NULL: zeros
+ *   state_in, state_out (rows, width, states), 16-byte aligned; state_in NULL: zeros.  They may be one buffer in bnb_selective_step.
+ *   done, lengths, reset: as above; reset in bnb_selective_step only, which takes no done and no lengths
+ *   kept: NULL, or bnb_selective_scan_kept_bytes bytes that the backward reads */
+typedef struct {
+  int32_t steps, rows, width, states, groups, element, softplus;
+  BnbView u, delta, z, b, c, y;
+  const float* a;
+  const float* d;
+  const float* delta_bias;
+  const float* state_in;
+  float* state_out;
+  const uint8_t* done;
+  const int32_t* lengths;
+  const uint8_t* reset;
+  float* kept;
+} BnbSelectiveScan;
+size_t bnb_selective_scan_kept_bytes(const BnbSelectiveScan* call);
+size_t bnb_selective_scan_scratch_bytes(const BnbSelectiveScan* call);
+int bnb_selective_scan_fwd(const BnbSelectiveScan* call, void* scratch, size_t scratch_bytes, void* stream);
+int bnb_selective_step(const BnbSelectiveScan* call, void* stream);   /* steps = 1 */
+
+/* Gradients: du, ddelta, dz (with z), db, dc, dstate_in, da, dd, ddelta_bias of given dy and dstate_out (NULL:
+ * zero).  dd, ddelta_bias, dstate_in may be NULL.  The call's `kept` as the forward left it. */
+typedef struct {
+  BnbView dy, du, ddelta, dz, db, dc;
+  const float* dstate_out;
+  float* dstate_in;
+  float* da;
+  float* dd;
+  float* ddelta_bias;
+} BnbSelectiveScanGrads;
+size_t bnb_selective_scan_bwd_scratch_bytes(const BnbSelectiveScan* call);
+int bnb_selective_scan_bwd(const BnbSelectiveScan* call, const BnbSelectiveScanGrads* grads, void* scratch,
+                           size_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
