@@ -12,6 +12,7 @@ the C-ABI library ``libbnb_trunk.so`` (include/bnb_trunk.h).  There is no CPU pa
 from .config import ModelConfig
 from .yemong.attention import GatedMLP, TransformerBlock
 from .yemong.encoder import BulletEncoder, ShipEncoder
+from .yemong.gated import gated_mlp
 from .yemong.heads import HeadMLP, NextStateHead, TeamPMA, evaluate_action, sample_action
 from .yemong.griffin import CONV_KERNEL, RGLRU, GriffinTemporalBlock, YemongBlock
 from .yemong.policy import YemongPolicy
@@ -37,6 +38,7 @@ __all__ = [
     "causal_conv",
     "causal_conv_step",
     "evaluate_action",
+    "gated_mlp",
     "sample_action",
     "selective_scan",
     "selective_step",

@@ -132,7 +132,7 @@ EXPORTS = {
     "bnb_last_status": (C.c_int, []),
     "bnb_clear_status": (None, []),
     "bnb_debug_wait_test": (None, [C.c_int, C.c_int]),
-    # the recurrent layers outside the trunk; their structs are filled in native code (csrc/host_sequences.cpp)
+    # the operators outside the trunk; their structs are filled in native code (csrc/host_operators.cpp)
     "bnb_causal_conv_fwd": (C.c_int, [_fp, _fp]),
     "bnb_causal_conv_bwd_scratch_bytes": (C.c_size_t, [_fp]),
     "bnb_causal_conv_bwd": (C.c_int, [_fp, _fp, _fp, C.c_size_t, _fp]),
@@ -142,6 +142,10 @@ EXPORTS = {
     "bnb_selective_step": (C.c_int, [_fp, _fp]),
     "bnb_selective_scan_bwd_scratch_bytes": (C.c_size_t, [_fp]),
     "bnb_selective_scan_bwd": (C.c_int, [_fp, _fp, _fp, C.c_size_t, _fp]),
+    "bnb_gated_block_kept_bytes": (C.c_size_t, [_fp]),
+    "bnb_gated_block_scratch_bytes": (C.c_size_t, [_fp, C.c_int]),
+    "bnb_gated_block_fwd": (C.c_int, [_fp, _fp, C.c_size_t, _fp]),
+    "bnb_gated_block_bwd": (C.c_int, [_fp, _fp, _fp, C.c_size_t, _fp]),
 }
 
 

@@ -3,7 +3,7 @@
     python boost-and-broadside_b200/build.py [--force]
 
 The library lands beside this file as ``libbnb_trunk.so``; it is what ``_capi`` loads.  Beside it lands
-``_host_path.so``, the CPython module with the host side of a call (csrc/host_path.cpp, csrc/host_sequences.cpp), linked
+``_host_path.so``, the CPython module with the host side of a call (csrc/host_path.cpp, csrc/host_operators.cpp), linked
 against the library.
 """
 
@@ -19,8 +19,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbnb_trunk.so")
 HOST_MODULE = os.path.join(HERE, "_host_path.so")
-SOURCES = ["capi.cu", "exact_kernels.cu", "tensor_kernels.cu", "bullet_kv.cu", "pipelined_tile_kernel.cu", "static_scratch.cu", "grad_kernels.cu", "mlp_kernels.cu", "head_tiles.cu", "policy_tail.cu", "train_attention.cu", "train_mlp.cu", "train_linear.cu", "split_kernels.cu", "causal_conv.cu", "selective_scan.cu", "selective_scan_bwd.cu"]
-HOST_SOURCES = ["host_path.cpp", "host_sequences.cpp"]
+SOURCES = ["capi.cu", "exact_kernels.cu", "tensor_kernels.cu", "bullet_kv.cu", "pipelined_tile_kernel.cu", "static_scratch.cu", "grad_kernels.cu", "mlp_kernels.cu", "head_tiles.cu", "policy_tail.cu", "train_attention.cu", "train_mlp.cu", "train_linear.cu", "split_kernels.cu", "causal_conv.cu", "selective_scan.cu", "selective_scan_bwd.cu", "gated_mlp.cu"]
+HOST_SOURCES = ["host_path.cpp", "host_operators.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

@@ -1,4 +1,4 @@
-// The host side of the recurrent layers outside the trunk (yemong/selective.py): checks, outputs from torch's
+// The host side of the operators outside the trunk (yemong/selective.py, yemong/gated.py): checks, outputs from torch's
 // allocator, the launch, and the autograd nodes of eager calls.  Scratch comes from torch's allocator call by call, so that
 // captured graphs and streams never share any.
 #include "host_tensors.h"
@@ -447,9 +447,106 @@ Tensor scan_step(const Tensor& u, const Tensor& delta, const Tensor& a, const Te
   return y;
 }
 
+// ------------------------------------------------------------------ gated feed-forward block
+
+struct GatedCall {
+  BnbGatedBlock c{};
+  std::vector<Tensor> held;
+};
+// x as (rows, width), its rows contiguous elements.
+Tensor rows_of(const Tensor& t) {
+  const Tensor v = t.reshape({-1, t.size(-1)});
+  return v.stride(1) == 1 || v.size(1) <= 1 ? v : v.contiguous();
+}
+int64_t row_stride(const Tensor& v) { return v.size(0) > 1 ? v.stride(0) : v.size(1); }
+GatedCall gated_call(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int activation) {
+  const char* fn = "gated_mlp";
+  expect_cuda(fn, x);
+  if (x.dim() < 1) refuse("gated_mlp: x must have shape (.., D)");
+  const int64_t D = x.size(-1);
+  const c10::Device dev = x.device();
+  GatedCall k;
+  BnbGatedBlock& c = k.c;
+  c.element = element_of(fn, x);
+  if (gate.dim() != 2) refuse("gated_mlp: gate_w must have shape (F, " + std::to_string(D) + "), got " + shape_text(gate.sizes()));
+  const int64_t F = gate.size(0);
+  if (D < 1 || F < 1) throw py::value_error("gated_mlp: width and hidden size must be at least 1");
+  expect(fn, "gate_w", gate, {F, D}, dev);
+  expect(fn, "up_w", up, {F, D}, dev);
+  expect(fn, "down_w", down, {D, F}, dev);
+  for (const Tensor* w : {&gate, &up, &down})
+    if (w->scalar_type() != gate.scalar_type() || (w->scalar_type() != x.scalar_type() && w->scalar_type() != at::kFloat))
+      refuse(std::string("gated_mlp: the weights must all be float32 or all of the input's type ") + c10::toString(x.scalar_type()));
+  const Tensor flat = rows_of(x);
+  k.held.push_back(flat);
+  c.rows = flat.size(0);
+  c.width = fits_int(fn, D);
+  c.hidden = fits_int(fn, F);
+  c.weight_element = element_of(fn, gate);
+  c.activation = activation;
+  c.x = flat.data_ptr();
+  c.x_row = row_stride(flat);
+  const void** at[] = {&c.gate_w, &c.up_w, &c.down_w};
+  int i = 0;
+  for (const Tensor* w : {&gate, &up, &down}) {
+    k.held.push_back(contiguous(*w));
+    *at[i++] = k.held.back().data_ptr();
+  }
+  return k;
+}
+
+// (y, what the backward reads: empty unless asked for)
+std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int activation, bool keep) {
+  const c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
+  GatedCall k = gated_call(x, gate, up, down, activation);
+  raise_pending_status(x.device());
+  const Tensor y = at::empty(x.sizes(), x.options());
+  const Tensor kept = at::empty({keep ? (int64_t)bnb_gated_block_kept_bytes(&k.c) : 0}, x.options().dtype(at::kByte));
+  k.c.y = y.data_ptr();
+  k.c.kept = keep ? kept.data_ptr() : nullptr;
+  const Tensor scratch = scratch_of(bnb_gated_block_scratch_bytes(&k.c, 0), x);
+  check("bnb_gated_block_fwd", bnb_gated_block_fwd(&k.c, scratch.data_ptr(), (size_t)scratch.numel(), stream_of(x.device())));
+  return {y, kept};
+}
+
+// Gradients of x, gate_w, up_w and down_w.
+std::vector<Tensor> gated_backward(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int activation, const Tensor& kept, const Tensor& dy) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  GatedCall k = gated_call(x, gate, up, down, activation);
+  Tensor held = contiguous(kept).to(x.device());
+  if (held.scalar_type() != at::kByte || (size_t)held.numel() != bnb_gated_block_kept_bytes(&k.c))
+    refuse("gated_mlp: the kept activations came back as another tensor: saved-tensor hooks have to return type and shape as they were");
+  if (reinterpret_cast<uintptr_t>(held.data_ptr()) % 16) held = held.clone();
+  expect("gated_mlp", "the gradient of y", dy, x.sizes(), x.device());
+  const Tensor gy = rows_of(dy.to(x.scalar_type()));
+  const Tensor dx = at::empty(x.sizes(), x.options()), dg = at::empty(gate.sizes(), gate.options()), du = at::empty(up.sizes(), up.options()),
+               dd = at::empty(down.sizes(), down.options());
+  k.c.kept = held.data_ptr();
+  const BnbGatedBlockGrads g{gy.data_ptr(), row_stride(gy), dx.data_ptr(), dg.data_ptr(), du.data_ptr(), dd.data_ptr()};
+  const Tensor scratch = scratch_of(bnb_gated_block_scratch_bytes(&k.c, 1), x);
+  check("bnb_gated_block_bwd", bnb_gated_block_bwd(&k.c, &g, scratch.data_ptr(), (size_t)scratch.numel(), stream_of(x.device())));
+  return {dx, dg, du, dd};
+}
+
+Tensor gated(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, int activation) {
+  const variable_list inputs{x, gate, up, down};
+  if (!wants_grad(inputs)) return std::get<0>(gated_forward(x, gate, up, down, activation, false));
+  Tensor y, kept;
+  {
+    const at::NoGradGuard no_grad;
+    std::tie(y, kept) = gated_forward(x, gate, up, down, activation, true);
+  }
+  auto node = node_of(inputs, {kept}, [activation](const std::vector<Tensor>& s, const variable_list& g) -> variable_list {
+    if (!g[0].defined()) return variable_list(4);
+    return gated_backward(s[0], s[1], s[2], s[3], activation, s[4], g[0]);
+  });
+  torch::autograd::create_gradient_edge(y, node);
+  return y;
+}
+
 }  // namespace
 
-void bind_sequences(py::module& m) {
+void bind_operators(py::module& m) {
   m.def("causal_conv_forward", &conv_forward);
   m.def("causal_conv_backward", &conv_backward);
   m.def("causal_conv", torch::wrap_pybind_function(conv));
@@ -458,6 +555,9 @@ void bind_sequences(py::module& m) {
   m.def("selective_scan_backward", &scan_backward);
   m.def("selective_scan", torch::wrap_pybind_function(scan));
   m.def("selective_step", &scan_step);
+  m.def("gated_mlp_forward", &gated_forward);
+  m.def("gated_mlp_backward", &gated_backward);
+  m.def("gated_mlp", torch::wrap_pybind_function(gated));
 }
 
 }  // namespace host

@@ -147,16 +147,6 @@ py::object trunk_params(const py::sequence& blocks, bool has_fields) {
 
 constexpr int kEngineSimt = BNB_ENGINE_SIMT;
 
-// A bounded wait of an earlier call on this device ran out (its kernels drained and its outputs were
-// garbage): say so once, at the next call, without synchronising.
-void raise_pending_status(const c10::Device& dev) {
-  const int st = bnb_last_status();
-  if (!st) return;
-  bnb_clear_status();
-  throw std::runtime_error("an earlier tensor-core call on " + dev.str() + " gave up a bounded wait: " + bnb_status_string(st) +
-                           " (status " + std::to_string(st) + "); its outputs, and any state carried from them, are invalid");
-}
-
 constexpr int N_SPATIAL = 7, N_TEMPORAL = 15;   // parameters of a sublayer, + bullets / field substitute
 
 // The integers of a call (yemong/_ops.py names the entries).
@@ -833,7 +823,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_tail(const Tensor& x_in, const
 }  // namespace
 
 PYBIND11_MODULE(_host_path, m) {
-  bnb::host::bind_sequences(m);
+  bnb::host::bind_operators(m);
   m.def("trunk_params", &trunk_params);
   m.def("keep_activations", [](const c10::Device& dev, const std::vector<int64_t>& geom, int64_t d_model, int64_t n_bullets) {
     return keep_activations(dev, Geometry(geom), d_model, n_bullets);

@@ -1,4 +1,4 @@
-// What the parts of the host module share (host_path.cpp, host_sequences.cpp): conversions and checks of tensors, the
+// What the parts of the host module share (host_path.cpp, host_operators.cpp): conversions and checks of tensors, the
 // library's status as an exception, the refusal of second-order gradients.
 #pragma once
 #include <torch/extension.h>
@@ -52,7 +52,16 @@ inline void check(const char* fn, int status) {
   if (status == BNB_ERR_UNSUPPORTED_DIMS) throw py::value_error(text);
   throw std::runtime_error(text + " (status " + std::to_string(status) + ")");
 }
-// Behind the gradients of a backward pass that is itself recorded (create_graph=True): the trunk has no second-order
+// A bounded wait of an earlier call on this device ran out (its kernels drained and its outputs were
+// garbage): say so once, at the next call, without synchronising.
+inline void raise_pending_status(const c10::Device& dev) {
+  const int st = bnb_last_status();
+  if (!st) return;
+  bnb_clear_status();
+  throw std::runtime_error("an earlier tensor-core call on " + dev.str() + " gave up a bounded wait: " + bnb_status_string(st) +
+                           " (status " + std::to_string(st) + "); its outputs, and any state carried from them, are invalid");
+}
+// Behind the gradients of a backward pass that is itself recorded (create_graph=True): the kernels have no second-order
 // gradient, and whoever asks for one is told so, as by an operator without an autograd formula.
 struct NoSecondOrder : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list&&) override {
@@ -60,8 +69,8 @@ struct NoSecondOrder : public torch::autograd::Node {
   }
 };
 
-// The recurrent layers outside the trunk (host_sequences.cpp).
-void bind_sequences(py::module& m);
+// The operators outside the trunk (host_operators.cpp).
+void bind_operators(py::module& m);
 
 }  // namespace host
 }  // namespace bnb

@@ -1,6 +1,6 @@
-"""Opaque ``torch.library`` operators of the recurrent layers outside the trunk (``selective.py``), for callers
+"""Opaque ``torch.library`` operators of the layers outside the trunk (``selective.py``, ``gated.py``), for callers
 that have to see them: a compiler, a tracer, a dispatch mode.  Same reason and same form as ``_ops.py``;
-eager calls go to the native code (csrc/host_sequences.cpp) directly, autograd nodes included.
+eager calls go to the native code (csrc/host_operators.cpp) directly, autograd nodes included.
 """
 
 from __future__ import annotations
@@ -151,3 +151,50 @@ def selective_step(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
 @selective_step.register_fake
 def _(u, delta, A, B, C, D, state, z, delta_bias, reset, softplus):
     return u.new_empty(u.shape)
+
+
+# ----------------------------------------------------------------------------- gated feed-forward block
+
+
+@torch.library.custom_op("bnb_b200::gated_mlp", mutates_args=(), device_types="cuda")
+def gated_mlp(x: Tensor, gate_w: Tensor, up_w: Tensor, down_w: Tensor, activation: int, keep: bool) -> Tuple[Tensor, Tensor]:
+    """``bnb_gated_block_fwd``: x (.., D) -> (y like x, what the backward reads: empty without ``keep``)."""
+    return _capi.host.gated_mlp_forward(x, gate_w, up_w, down_w, activation, keep)
+
+
+@gated_mlp.register_fake
+def _(x, gate_w, up_w, down_w, activation, keep):
+    rows = x.numel() // x.shape[-1]
+    bytes_ = 2 * rows * ((gate_w.shape[0] + 7) // 8 * 8) * x.element_size()
+    return x.new_empty(x.shape), x.new_empty(bytes_ if keep else 0, dtype=torch.uint8)
+
+
+@torch.library.custom_op("bnb_b200::gated_mlp_backward", mutates_args=(), device_types="cuda")
+def gated_mlp_backward(x: Tensor, gate_w: Tensor, up_w: Tensor, down_w: Tensor, activation: int, kept: Tensor, dy: Tensor) -> List[Tensor]:
+    """Gradients of x, gate_w, up_w and down_w."""
+    return _capi.host.gated_mlp_backward(x, gate_w, up_w, down_w, activation, kept, dy)
+
+
+@gated_mlp_backward.register_fake
+def _(x, gate_w, up_w, down_w, activation, kept, dy):
+    return [t.new_empty(t.shape) for t in (x, gate_w, up_w, down_w)]
+
+
+def _gated_context(ctx, inputs, output):
+    x, gate_w, up_w, down_w, activation, keep = inputs
+    ctx.activation, ctx.keep = activation, keep
+    ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, gate_w, up_w, down_w, output[1])
+
+
+def _gated_formula(ctx, dy, _dkept):
+    if not ctx.keep:
+        raise RuntimeError("gated_mlp was called without keeping what its backward reads")
+    x, gate_w, up_w, down_w, kept = ctx.saved_tensors
+    if dy is None:
+        return (None,) * 6
+    return (*gated_mlp_backward(x, gate_w, up_w, down_w, ctx.activation, kept, dy), None, None)
+
+
+gated_mlp.register_autograd(_gated_formula, setup_context=_gated_context)

@@ -15,13 +15,15 @@ import torch.nn as nn
 from .. import _capi
 from . import _ops
 from ._weights import spatial_tensors
+from .gated import gated_mlp
 
 
 class GatedMLP(nn.Module):
     """down_proj(gelu(gate_proj(x)) * up_proj(x)), no biases (attention.py:21-37).
 
     Inside a sublayer the product runs fused in the sublayer kernels; ``forward`` serves callers
-    that use the module on its own (the reference's tests do) through ``bnb_gated_mlp_fwd``.
+    that use the module on its own (the reference's tests do) through ``bnb_gated_mlp_fwd``, or, for an
+    input that requires grad, through ``gated_mlp``, which has a backward.
     """
 
     def __init__(self, d_model: int, expand: int = 4) -> None:
@@ -41,10 +43,11 @@ class GatedMLP(nn.Module):
         if x.shape[-1] != D:
             raise RuntimeError(f"expected x of shape (..., {D}), got {tuple(x.shape)}")
         _capi.require_cuda(x, "x")
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise NotImplementedError("the CUDA trunk is forward-only; call it under torch.no_grad()")
         dev = x.device
         precision = _capi.current_precision(dev)
+        if torch.is_grad_enabled() and x.requires_grad:
+            return gated_mlp(x.to(torch.bfloat16 if precision == _capi.BNB_BF16 else torch.float32), self.gate_proj.weight,
+                             self.up_proj.weight, self.down_proj.weight)
         with torch.cuda.device(dev):
             flat = _capi.f32c(x).reshape(-1, D)
             y = torch.empty_like(flat)

@@ -569,6 +569,41 @@ size_t bnb_selective_scan_bwd_scratch_bytes(const BnbSelectiveScan* call);
 int bnb_selective_scan_bwd(const BnbSelectiveScan* call, const BnbSelectiveScanGrads* grads, void* scratch,
                            size_t scratch_bytes, void* stream);
 
+/* y = (act(x gate_w^T) * (x up_w^T)) down_w^T on tensor-core tiles, any width and hidden size.
+ *   element: type of x and y; 16-bit ones are the operands of the products, float32 ones go through exact pieces
+ *   weight_element: type of the weights: element, or BNB_ELEM_F32, which a call of 16-bit elements rounds as autocast does
+ *   gate_w, up_w (hidden, width), down_w (width, hidden) contiguous; x (rows, width), x_row elements between rows;
+ *   y (rows, width) contiguous; activation BNB_ACT_SILU or BNB_ACT_GELU
+ *   kept: NULL, or bnb_gated_block_kept_bytes bytes that the backward reads
+ *   y, kept, scratch 16-byte aligned.  Waits are bounded: see the status word above (the host word alone is written). */
+typedef struct {
+  int64_t rows;
+  int32_t width, hidden, element, weight_element, activation;
+  const void* x;
+  int64_t x_row;
+  const void* gate_w;
+  const void* up_w;
+  const void* down_w;
+  void* y;
+  void* kept;
+} BnbGatedBlock;
+size_t bnb_gated_block_kept_bytes(const BnbGatedBlock* call);
+size_t bnb_gated_block_scratch_bytes(const BnbGatedBlock* call, int backward);
+int bnb_gated_block_fwd(const BnbGatedBlock* call, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Gradients of given dy (rows, width), dy_row elements between rows: dx (rows, width) of x's type, the others of the weights'.
+ * Any may be NULL, dgate_w and dup_w together.  The call's `kept` as the forward left it; its y is not read. */
+typedef struct {
+  const void* dy;
+  int64_t dy_row;
+  void* dx;
+  void* dgate_w;
+  void* dup_w;
+  void* ddown_w;
+} BnbGatedBlockGrads;
+int bnb_gated_block_bwd(const BnbGatedBlock* call, const BnbGatedBlockGrads* grads, void* scratch, size_t scratch_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -110,6 +110,49 @@ def test_c_entry_points_check_their_arguments():
     assert lib.bnb_selective_scan_bwd(C.byref(long), None, None, 0, None) == 1
 
 
+class Gated(C.Structure):
+    _fields_ = [("rows", C.c_int64)] + [(n, C.c_int32) for n in ("width", "hidden", "element", "weight_element", "activation")] + [
+        ("x", C.c_void_p), ("x_row", C.c_int64)] + [(n, C.c_void_p) for n in ("gate_w", "up_w", "down_w", "y", "kept")]
+
+
+class GatedGrads(C.Structure):
+    _fields_ = [("dy", C.c_void_p), ("dy_row", C.c_int64)] + [(n, C.c_void_p) for n in ("dx", "dgate_w", "dup_w", "ddown_w")]
+
+
+def test_gated_block_checks_its_arguments():
+    import boost_and_broadside_b200 as bnb
+    from boost_and_broadside_b200 import _capi
+
+    x, w = torch.zeros(3, 8), torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        bnb.gated_mlp(x, w, w, w.t())
+    with pytest.raises(ValueError, match="activation"):
+        bnb.gated_mlp(x, w, w, w.t(), activation="relu")
+    lib, fake = _capi.lib, 0x1000
+
+    def call(**over):
+        c = Gated(100, 64, 128, 1, 1, 2, fake, 64, fake, fake, fake, fake, None)
+        for k, v in over.items():
+            setattr(c, k, v)
+        return c
+
+    fwd = lambda **over: lib.bnb_gated_block_fwd(C.byref(call(**over)), over.pop("scratch", None), 0, None)  # noqa: E731
+    assert fwd(width=0) == 3 and fwd(hidden=0) == 3 and fwd(weight_element=2) == 3
+    assert fwd(activation=0) == 5 and fwd(element=3) == 5 and fwd(rows=-1) == 5
+    assert fwd(gate_w=None) == 1 and fwd(x=None) == 1 and fwd(y=None) == 1
+    assert fwd(y=fake + 4) == 2 and fwd() == 6
+    assert fwd(rows=0) == 0
+    c = call()
+    assert lib.bnb_gated_block_scratch_bytes(C.byref(c), 0) >= 100 * 128 * 2
+    assert lib.bnb_gated_block_scratch_bytes(C.byref(c), 1) > lib.bnb_gated_block_scratch_bytes(C.byref(c), 0)
+    assert lib.bnb_gated_block_kept_bytes(C.byref(c)) == 2 * 100 * 128 * 2
+    g = GatedGrads(fake, 64, fake, fake, None, fake)
+    assert lib.bnb_gated_block_bwd(C.byref(call(kept=fake)), C.byref(g), None, 0, None) == 1     # half of the gate's pair
+    g = GatedGrads(fake, 64, fake, fake, fake, fake)
+    assert lib.bnb_gated_block_bwd(C.byref(call()), C.byref(g), None, 0, None) == 1              # nothing kept
+    assert lib.bnb_gated_block_bwd(C.byref(call(kept=fake)), C.byref(g), None, 0, None) == 6
+
+
 def test_split_sequences_join():
     """The 64-bit implementations themselves: a sequence in two calls, episode ends and lengths included, is the sequence in one."""
     g = torch.Generator().manual_seed(0)
@@ -145,4 +188,6 @@ def test_operators_have_shape_only_fakes():
         y, st, kept = ops.selective_scan(x, x, A, B, B, None, None, None, None, None, None, True, True)
         assert y.shape == x.shape and st.shape == (3, 8, 11) and kept.numel() == 1 * 3 * 8 * 16
         assert ops.selective_scan(x, x, A, B, B, None, None, None, None, None, None, True, False)[2].numel() == 0
+        y, kept = ops.gated_mlp(x, torch.empty(20, 8, device="cuda"), torch.empty(20, 8, device="cuda"), torch.empty(8, 20, device="cuda"), 2, True)
+        assert y.shape == x.shape and kept.numel() == 2 * 15 * 24 * 2
         assert ops.selective_step(x[0], x[0], A, B[0], B[0], None, st, None, None, None, True).shape == (3, 8)
