@@ -5,10 +5,11 @@
 //
 // Six width x hidden products a row forward and twelve backward: the tensor cores bound it, from widths on whose rows cost more
 // than their memory.  Forward is two launches: both projections, the activation and their product in one, where g and u of a tile
-// meet in tensor memory, and the down projection.  Backward is four: dh with the gate's derivatives (and h once more, which is cheaper to
-// form again than to keep), dx over both halves, dWg and dWu, dWd.  product_tiles.cuh has the products.
+// meet in tensor memory, and the down projection.  Backward is four: dh with the gate's derivatives (and h once more), dx over both
+// halves, dWg and dWu, dWd.  product_tiles.cuh has the products.
 //
-// h, dg and du are rounded to the operands' type between the products: they are operands of the next one.  Sums over the
+// h, dg and du are rounded to the operands' type between the products: they are operands of the next one.  g and u are not: they
+// enter the backward as float32, either kept by the forward or, where that is cheaper, computed once more (see recomputes).  Sums over the
 // depth are float32; where the depth is cut into parts (few tiles), the parts are added in a fixed order.
 #include <algorithm>
 #include <mutex>
@@ -57,6 +58,7 @@ __global__ void __launch_bounds__(256) k_add_parts(const float* part, int splits
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= cells * jobs) return;
   float v = 0.f;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) v += part[s * cells * jobs + i];
   void* out = i < cells ? out0 : out1;
   const int64_t at = i < cells ? i : i - cells;
@@ -97,23 +99,25 @@ bool map_of(CUtensorMap& m, const Operand& o, int pieces, int box_rows, bool hal
 constexpr int SMS = 148;
 
 struct Shaped { int bn, tiles, splits, split_steps; };
-// The width of a tile: the one with the least time by a tile's columns and its fixed cost (about 48 columns' worth of fetching, issuing
-// and taking out the last tile) over the rounds that the tiles make.  Then, where tiles leave SMs idle and results can be
-// added, the depth is cut so that all have work, no part below 8 stages.
-Shaped shape_of(int64_t m, int64_t n, int jobs, int steps, int least, int out_of_bn, bool may_split) {
+// The width of a tile: the one with the least time.  A stage moves (128 + BN) rows of 128 bytes into shared memory and the products read
+// them once from there, at 128 bytes a clock: 2 (128 + BN) clocks, more than the products themselves take at any BN up to 256 (measured:
+// 790 clocks a stage at 256).  A tile's fixed cost (fill, the last results) is about 1200.  Then, where tiles leave SMs idle and results can be
+// added, the depth is cut so that all have work, no part below 8 stages; the sums' launch costs some 6000 clocks.
+Shaped shape_of(int64_t m, int64_t n, int jobs, int steps, int most, int least, int out_of_bn, bool may_split) {
   const int64_t mt = (m + BM - 1) / BM;
   Shaped best{};
   double cost = 0;
-  for (int bn = 256; bn >= least; bn /= 2) {
+  for (int bn = most; bn >= least; bn /= 2) {
     const int64_t tiles = mt * ((n + bn / out_of_bn - 1) / (bn / out_of_bn)) * jobs;
-    int splits = 1;
-    if (may_split && tiles < SMS) splits = (int)std::max<int64_t>(1, std::min<int64_t>(SMS / tiles, steps / 8));
-    const int split_steps = (steps + splits - 1) / splits;
-    splits = (steps + split_steps - 1) / split_steps;
-    const double rounds = (double)((tiles * splits + SMS - 1) / SMS), c = rounds * (split_steps * (double)bn + 48.0 * 8) + (splits > 1 ? 2000.0 : 0.0);
-    if (best.bn == 0 || c < cost) {
-      best = {bn, (int)tiles, splits, split_steps};
-      cost = c;
+    for (int cut = 0; cut <= (may_split && tiles < SMS ? 1 : 0); ++cut) {
+      int splits = cut ? (int)std::max<int64_t>(1, std::min<int64_t>(SMS / tiles, steps / 8)) : 1;
+      const int split_steps = (steps + splits - 1) / splits;
+      splits = (steps + split_steps - 1) / split_steps;
+      const double rounds = (double)((tiles * splits + SMS - 1) / SMS), c = rounds * (split_steps * 2.0 * (BM + bn) + 1200.0) + (splits > 1 ? 6000.0 : 0.0);
+      if (best.bn == 0 || c < cost) {
+        best = {bn, (int)tiles, splits, split_steps};
+        cost = c;
+      }
     }
   }
   return best;
@@ -121,21 +125,31 @@ Shaped shape_of(int64_t m, int64_t n, int jobs, int steps, int least, int out_of
 
 template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT>
 int launch(const Product& p, int tiles, cudaStream_t st) {
-  constexpr uint32_t bytes = Shape<A_MN, B_MN, BN>::BYTES;
+  constexpr uint32_t bytes = Shape<BN, OUT>::BYTES;
   auto kernel = k_product<E, PIECES, A_MN, B_MN, BN, OUT>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return BNB_ERR_LAUNCH;
-  count_launch();
-  kernel<<<std::min(tiles, SMS), CTA, bytes, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;
+  return launch_after(kernel, dim3(std::min(tiles, SMS)), CTA, bytes, st, p);
 }
 
 // Pieces of a float32 product that are not below 2^-24 of it, smallest first.
 constexpr int PAIRS[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
 
-struct Sides { Operand a[2], b[2]; int segments; };   // segments: a[s] b[s]^T are added
+struct Sides { Operand a[2], b[3]; int segments; };   // segments: a[s] b[s]^T are added
+
+// Widths of tiles that are built: two sets of accumulators are 512 columns, and float32 adds runs in a third.
+template <int PIECES> constexpr int MOST = PIECES > 1 ? 128 : 256;
 
 template <typename E, int PIECES, bool A_MN, bool B_MN, Out OUT>
-int multiply(const Sides& s, int64_t m, int64_t n, int64_t depth, int jobs, Epilogue e, float* part, cudaStream_t st) {
+int at_width(const Product& p, int bn, int tiles, cudaStream_t st) {
+  if constexpr (PIECES == 1)
+    if (bn == 256) return launch<E, PIECES, A_MN, B_MN, 256, OUT>(p, tiles, st);
+  if (bn == 128) return launch<E, PIECES, A_MN, B_MN, 128, OUT>(p, tiles, st);
+  if constexpr (OUT != Out::GATE) return launch<E, PIECES, A_MN, B_MN, 64, OUT>(p, tiles, st);
+  return BNB_ERR_BAD_ARGUMENT;
+}
+
+template <typename E, int PIECES, bool A_MN, bool B_MN, Out OUT>
+int multiply(const Sides& s, int64_t m, int64_t n, int64_t depth, int jobs, const Epilogue& e, float* part, cudaStream_t st) {
   Product p{};
   p.e = e;
   p.m = m;
@@ -149,40 +163,40 @@ int multiply(const Sides& s, int64_t m, int64_t n, int64_t depth, int jobs, Epil
     p.a_piece[t] = PIECES > 1 ? (uint8_t)PAIRS[pair][0] : 0;
     p.b_piece[t] = PIECES > 1 ? (uint8_t)PAIRS[pair][1] : 0;
   }
-  const bool splits_allowed = OUT == Out::VALUES;
+  constexpr bool again = OUT == Out::AGAIN;
   constexpr int LEAST = OUT == Out::GATE ? 128 : 64, OF = OUT == Out::GATE ? 2 : 1;
-  const Shaped z = shape_of(m, n, jobs, p.k_steps * p.terms, LEAST, OF, splits_allowed);
+  Shaped z = again ? Shaped{64, (int)((m + BM - 1) / BM * ((n + 63) / 64)), 1, p.k_steps}
+                   : shape_of(m, n, jobs, p.k_steps * p.terms, MOST<PIECES>, LEAST, OF, OUT == Out::VALUES);
   p.splits = z.splits;
   p.split_steps = z.split_steps;
   p.m_tiles = (int)((m + BM - 1) / BM);
   p.n_tiles = (int)((n + z.bn / OF - 1) / (z.bn / OF));
   p.host_status = host_status_word(st);
   constexpr bool half = std::is_same<E, __half>::value;
-  const int a_maps = jobs > 1 ? jobs : s.segments, b_maps = OUT == Out::GATE ? 2 : s.segments;
+  const int a_maps = again ? 2 : jobs > 1 ? jobs : s.segments, b_maps = again ? 3 : OUT == Out::GATE ? 2 : s.segments;
   bool ok = has_context();
   for (int i = 0; i < a_maps; ++i) ok = ok && map_of(p.a[i], s.a[i], PIECES, A_MN ? BK : BM, half);
-  for (int i = 0; i < b_maps; ++i) ok = ok && map_of(p.b[i], s.b[i], PIECES, B_MN ? BK : z.bn / OF, half);
+  for (int i = 0; i < b_maps; ++i) ok = ok && map_of(p.b[i], s.b[i], PIECES, again || B_MN ? BK : z.bn / OF, half);
   if (!ok) return BNB_ERR_LAUNCH;
   const int total = z.tiles * z.splits;
-  if constexpr (OUT == Out::VALUES) {
+  if constexpr (again) {
+    return launch<E, PIECES, false, false, 192, OUT>(p, total, st);
+  } else if constexpr (OUT == Out::VALUES) {
     if (z.splits > 1) {
       p.e.part = part;
-      int st_ = z.bn == 256 ? launch<E, PIECES, A_MN, B_MN, 256, Out::PARTIAL>(p, total, st)
-              : z.bn == 128 ? launch<E, PIECES, A_MN, B_MN, 128, Out::PARTIAL>(p, total, st) : launch<E, PIECES, A_MN, B_MN, 64, Out::PARTIAL>(p, total, st);
-      if (st_) return st_;
+      if (const int r = at_width<E, PIECES, A_MN, B_MN, Out::PARTIAL>(p, z.bn, total, st)) return r;
       const int64_t cells = m * n;
       count_launch();
       k_add_parts<E><<<(unsigned)((cells * jobs + 255) / 256), 256, 0, st>>>(part, z.splits, cells, jobs, e.out[0], e.out[1], e.out_kind);
       return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;
     }
+    return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, st);
+  } else {
+    return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, st);
   }
-  if (z.bn == 256) return launch<E, PIECES, A_MN, B_MN, 256, OUT>(p, total, st);
-  if (z.bn == 128) return launch<E, PIECES, A_MN, B_MN, 128, OUT>(p, total, st);
-  if constexpr (OUT != Out::GATE) return launch<E, PIECES, A_MN, B_MN, 64, OUT>(p, total, st);
-  return BNB_ERR_BAD_ARGUMENT;
 }
-size_t part_bytes(int64_t m, int64_t n, int64_t depth, int jobs, int terms) {
-  const Shaped z = shape_of(m, n, jobs, (int)((depth + BK - 1) / BK) * terms, 64, 1, true);
+size_t part_bytes(int64_t m, int64_t n, int64_t depth, int jobs, int terms, int most) {
+  const Shaped z = shape_of(m, n, jobs, (int)((depth + BK - 1) / BK) * terms, most, 64, 1, true);
   return z.splits > 1 ? round256((size_t)z.splits * jobs * m * n * 4) : 0;
 }
 
@@ -198,6 +212,12 @@ int check(const BnbGatedBlock* c) {
   return BNB_OK;
 }
 
+// Whether the backward computes g and u once more.  Kept in float32 they cost 16 bytes a row and hidden column, forward and backward,
+// which is 4 ps; computed, 28 clocks of a tile's 128 x 64 for each 64 of the width, 0.012 ps for each of it.  So up to a width of 384,
+// in 16 bits; float32 takes six times the products, and keeps.
+bool recomputes(const BnbGatedBlock& c) { return c.element != BNB_ELEM_F32 && c.width <= 384; }
+
+int64_t round32(int64_t v) { return (v + 31) / 32 * 32; }
 bool lies_well(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 
 // Where everything of a call stands in its scratch; sizes alone with base = null.
@@ -230,15 +250,15 @@ struct Layout {
     up = operand(c.up_w, F, D, D, c.weight_element);
     down = operand(c.down_w, D, F, F, c.weight_element);
     h = between();
-    const int t = pieces > 1 ? 6 : 1;
+    const int t = pieces > 1 ? 6 : 1, most = pieces > 1 ? MOST<3> : MOST<1>;
     size_t parts = 0;
     if (!backward) {
-      parts = part_bytes(M, D, F, 1, t);
+      parts = part_bytes(M, D, F, 1, t, most);
     } else {
       dy = operand(dy_in, M, D, dy_ld, c.element);
       dg = between();
       du = between();
-      parts = std::max({part_bytes(M, D, F, 1, 2 * t), part_bytes(F, D, M, 2, t), part_bytes(D, F, M, 1, t)});
+      parts = std::max({part_bytes(M, D, F, 1, 2 * t, most), part_bytes(F, D, M, 2, t, most), part_bytes(D, F, M, 1, t, most)});
     }
     part = reinterpret_cast<float*>(take(parts));
   }
@@ -254,9 +274,7 @@ int pack(const Layout& l, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;
 }
 
-template <typename E, int PIECES>
 Epilogue between(const BnbGatedBlock& c, const Layout& l) {
-  using V = typename Kind<E, PIECES>::Value;
   Epilogue e{};
   e.activation = c.activation;
   e.ld_h = l.ld_h;
@@ -264,9 +282,9 @@ Epilogue between(const BnbGatedBlock& c, const Layout& l) {
   e.h = const_cast<void*>(l.h.data);
   e.dg = const_cast<void*>(l.dg.data);
   e.du = const_cast<void*>(l.du.data);
-  if (c.kept) {
-    e.g = c.kept;
-    e.u = static_cast<V*>(c.kept) + l.M * l.ld_h;
+  if (c.kept && !recomputes(c)) {
+    e.g = static_cast<float*>(c.kept);
+    e.u = e.g + round32(l.M) * round32(l.F);
   }
   return e;
 }
@@ -275,7 +293,7 @@ template <typename E, int PIECES>
 int forward(const BnbGatedBlock& c, const Layout& l, cudaStream_t st) {
   if (const int r = pack<E, PIECES>(l, st)) return r;
   const Sides up{{l.x, {}}, {l.gate, l.up}, 1};
-  if (const int r = multiply<E, PIECES, false, false, Out::GATE>(up, l.M, l.F, l.D, 1, between<E, PIECES>(c, l), nullptr, st)) return r;
+  if (const int r = multiply<E, PIECES, false, false, Out::GATE>(up, l.M, l.F, l.D, 1, between(c, l), nullptr, st)) return r;
   Epilogue e{};
   e.out[0] = c.y;
   e.ld_out = l.D;
@@ -286,21 +304,28 @@ int forward(const BnbGatedBlock& c, const Layout& l, cudaStream_t st) {
 template <typename E, int PIECES>
 int backward(const BnbGatedBlock& c, const BnbGatedBlockGrads& g, const Layout& l, cudaStream_t st) {
   if (const int r = pack<E, PIECES>(l, st)) return r;
-  if (const int r = multiply<E, PIECES, false, true, Out::BACK>({{l.dy, {}}, {l.down, {}}, 1}, l.M, l.F, l.D, 1, between<E, PIECES>(c, l), nullptr, st)) return r;
+  int r;
+  if constexpr (PIECES == 1) {
+    r = recomputes(c) ? multiply<E, PIECES, false, false, Out::AGAIN>({{l.x, l.dy}, {l.gate, l.up, l.down}, 1}, l.M, l.F, l.D, 1, between(c, l), nullptr, st)
+                      : multiply<E, PIECES, false, true, Out::BACK>({{l.dy, {}}, {l.down, {}}, 1}, l.M, l.F, l.D, 1, between(c, l), nullptr, st);
+  } else {
+    r = multiply<E, PIECES, false, true, Out::BACK>({{l.dy, {}}, {l.down, {}}, 1}, l.M, l.F, l.D, 1, between(c, l), nullptr, st);
+  }
+  if (r) return r;
   Epilogue e{};
   const int own = PIECES > 1 ? 0 : 1, weights = c.weight_element == BNB_ELEM_F32 ? 0 : 1;
   if (g.dx) {
     e.out[0] = g.dx;
     e.ld_out = l.D;
     e.out_kind = own;
-    if (const int r = multiply<E, PIECES, false, true, Out::VALUES>({{l.dg, l.du}, {l.gate, l.up}, 2}, l.M, l.D, l.F, 1, e, l.part, st)) return r;
+    if (r = multiply<E, PIECES, false, true, Out::VALUES>({{l.dg, l.du}, {l.gate, l.up}, 2}, l.M, l.D, l.F, 1, e, l.part, st); r) return r;
   }
   e.out_kind = weights;
   if (g.dgate_w && g.dup_w) {
     e.out[0] = g.dgate_w;
     e.out[1] = g.dup_w;
     e.ld_out = l.D;
-    if (const int r = multiply<E, PIECES, true, true, Out::VALUES>({{l.dg, l.du}, {l.x, {}}, 1}, l.F, l.D, l.M, 2, e, l.part, st)) return r;
+    if (r = multiply<E, PIECES, true, true, Out::VALUES>({{l.dg, l.du}, {l.x, {}}, 1}, l.F, l.D, l.M, 2, e, l.part, st); r) return r;
   }
   if (g.ddown_w) {
     e.out[0] = g.ddown_w;
@@ -320,7 +345,7 @@ using namespace bnb::product;
 
 extern "C" size_t bnb_gated_block_kept_bytes(const BnbGatedBlock* c) {
   if (check(c)) return 0;
-  return (size_t)2 * c->rows * round8(c->hidden) * (c->element == BNB_ELEM_F32 ? 4 : 2);
+  return recomputes(*c) ? 0 : (size_t)2 * round32(c->rows) * round32(c->hidden) * 4;
 }
 
 extern "C" size_t bnb_gated_block_scratch_bytes(const BnbGatedBlock* c, int backward) {
@@ -351,7 +376,7 @@ extern "C" int bnb_gated_block_bwd(const BnbGatedBlock* c, const BnbGatedBlockGr
       if (p && cudaMemsetAsync(p, 0, cells, s) != cudaSuccess) return BNB_ERR_LAUNCH;
     return BNB_OK;
   }
-  if (!g->dy || !c->kept || (g->dgate_w == nullptr) != (g->dup_w == nullptr)) return BNB_ERR_NULL_POINTER;
+  if (!g->dy || (!c->kept && !recomputes(*c)) || (g->dgate_w == nullptr) != (g->dup_w == nullptr)) return BNB_ERR_NULL_POINTER;
   if ((reinterpret_cast<uintptr_t>(c->kept) | reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(g->dx) | reinterpret_cast<uintptr_t>(g->dgate_w) |
        reinterpret_cast<uintptr_t>(g->dup_w) | reinterpret_cast<uintptr_t>(g->ddown_w)) & 15) return BNB_ERR_MISALIGNED;
   const Layout l(*c, g->dy, g->dy_row, true, static_cast<uint8_t*>(scratch));

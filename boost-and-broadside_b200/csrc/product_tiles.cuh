@@ -3,19 +3,22 @@
 //
 // out (m, n) = sum over terms of A_t (m, k) B_t (n, k)^T.  One persistent CTA per SM walks over tiles of 128 x BN; a warp fetches (TMA
 // boxes of 64 elements by 64 to 256, 128-byte swizzle, zeros outside the tensors, so that no size has to be a multiple of a
-// tile), a warp issues the products, eight warps take finished accumulators out of tensor memory.  There are two accumulators: a tile's
+// tile), a warp issues the products, sixteen warps take finished accumulators out of tensor memory.  There are two accumulators: a tile's
 // products run while the tile before is written out.
 //
 // An operand may lie in memory with its depth innermost (K-major) or with its rows innermost (MN-major): the same boxes, other descriptor
 // bits.  So no operand of the backward is transposed in memory.
 //
 // 16-bit operands take one term.  Float32 ones are split into three bfloat16 pieces whose sum is exact to 24 bits, and the
-// product into the six products of pieces that are not below 2^-24 of it, smallest first: six terms of the same loop.
+// product into the six products of pieces that are not below 2^-24 of it, smallest first: six terms of the same loop.  The tensor cores
+// truncate every addition to an accumulator, 2^-25 of it on average and always towards zero; so the last term, the only one of full size, is
+// cut into runs of FLUSH stages (16 additions), and the runs are added, rounded, by the warps that take results out.
 #pragma once
 
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include "launch_after.h"
 #include "tile_rows.cuh"
 
 namespace bnb {
@@ -25,32 +28,35 @@ using namespace tensor;
 
 constexpr int BM = 128, BK = 64;              // tile rows; depth of a stage
 constexpr int MAX_TERMS = 12;                 // two segments of six
-constexpr int OUT_WARPS = 8, CTA = 32 * (2 + OUT_WARPS);
+constexpr int FLUSH = 4;                      // stages of a run
+constexpr int OUT_WARPS = 16, PARTS = OUT_WARPS / 4, CTA = 32 * (2 + OUT_WARPS);
 constexpr uint32_t A_BYTES = BM * BK * 2, SLAB = 64 * BK * 2;   // SLAB: 64 rows or columns by 64
+constexpr uint32_t OUT_BYTES = 2048;          // shared memory of a warp that takes out
 enum : int { W_FULL = 101, W_EMPTY = 102, W_ACC = 103, W_DRAINED = 104 };
-
-enum class Out : int { VALUES, PARTIAL, GATE, BACK };
 
 // What a tile's results become.
 //   VALUES   out[job] (m, n), of type `out_kind`
 //   PARTIAL  float32 sums of a part of the depth: part (splits, jobs, m, n)
 //   GATE     columns come in pairs of tiles, g and u: h = act(g) u as operand pieces; g and u themselves where they are kept
-//   BACK     columns are dh: dg = dh u act'(g), du = dh act(g), h = act(g) u as operand pieces
+//   BACK     columns are dh: dg = dh u act'(g), du = dh act(g), h = act(g) u as operand pieces, from the kept g and u
+//   AGAIN    the same with g and u computed once more: a stage holds x and dy, and 64 columns of all three weights
+enum class Out : int { VALUES, PARTIAL, GATE, BACK, AGAIN };
+
 struct Epilogue {
   void* out[2];
   float* part;
   void* h;              // operand pieces (pieces, m, ld_h)
   void* dg;
   void* du;
-  void* g;              // values (m, ld_h)
-  void* u;
+  float* g;             // kept: blocks of 32 rows by 32 columns, see kept_at
+  float* u;
   int64_t ld_out, ld_h, piece_stride;
   int out_kind;         // 0: float32, 1: the operands' type
   int activation;       // BNB_ACT_SILU or BNB_ACT_GELU
 };
 
 struct Product {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a[2], b[3];
   Epilogue e;
   int64_t m;
   int n, k_steps, terms;       // k_steps: stages of a term
@@ -107,16 +113,6 @@ __device__ __forceinline__ void activate(int kind, float g, float& a, float& da)
   da = cdf + density;
 }
 
-// Eight neighbouring results of a row.
-__device__ __forceinline__ void put8(float* at, const float (&v)[8], int left, bool wide) {
-  if (wide && left >= 8) {
-    reinterpret_cast<float4*>(at)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(at)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < left) at[i] = v[i];
-  }
-}
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -126,33 +122,15 @@ __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v
 __device__ __forceinline__ float up(__half v) { return __half2float(v); }
 __device__ __forceinline__ void down(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void down(__half& o, float v) { o = __float2half_rn(v); }
-template <typename E>
-__device__ __forceinline__ void put8(E* at, const float (&v)[8], int left, bool wide) {
-  if (wide && left >= 8) {
-    *reinterpret_cast<uint4*>(at) = make_uint4(pair_of(v[0], v[1], E{}), pair_of(v[2], v[3], E{}), pair_of(v[4], v[5], E{}), pair_of(v[6], v[7], E{}));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) if (i < left) down(at[i], v[i]);
-  }
-}
-__device__ __forceinline__ void get8(const float* at, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(at)[0], b = reinterpret_cast<const float4*>(at)[1];
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-template <typename E>
-__device__ __forceinline__ void get8(const E* at, float (&v)[8]) {
-  const uint4 raw = *reinterpret_cast<const uint4*>(at);
-  const E* e = reinterpret_cast<const E*>(&raw);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = up(e[i]);
-}
+__device__ __forceinline__ void down(float& o, float v) { o = v; }
+
 // The operand pieces of eight values: one rounding, or three bfloat16 numbers that add up to the value.
 template <typename E, int PIECES>
 __device__ __forceinline__ void put_operand(void* base, int64_t piece_stride, int64_t at, float (&v)[8]) {
 #pragma unroll
   for (int p = 0; p < PIECES; ++p) {
-    E* to = static_cast<E*>(base) + p * piece_stride + at;
-    put8(to, v, 8, true);
+    *reinterpret_cast<uint4*>(static_cast<E*>(base) + p * piece_stride + at) =
+        make_uint4(pair_of(v[0], v[1], E{}), pair_of(v[2], v[3], E{}), pair_of(v[4], v[5], E{}), pair_of(v[6], v[7], E{}));
     if constexpr (PIECES > 1) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -164,33 +142,74 @@ __device__ __forceinline__ void put_operand(void* base, int64_t piece_stride, in
   }
 }
 
-template <typename E, int PIECES> struct Kind {
-  using Value = E;
-  static constexpr uint32_t FORMAT = 0;
-};
-template <> struct Kind<__nv_bfloat16, 1> {
-  using Value = __nv_bfloat16;
-  static constexpr uint32_t FORMAT = (1u << 7) | (1u << 10);
-};
-template <> struct Kind<__nv_bfloat16, 3> {
-  using Value = float;
-  static constexpr uint32_t FORMAT = (1u << 7) | (1u << 10);
+template <typename E> struct Format { static constexpr uint32_t BITS = 0; };
+template <> struct Format<__nv_bfloat16> { static constexpr uint32_t BITS = (1u << 7) | (1u << 10); };
+
+template <int BN, Out OUT>
+struct Shape {
+  static constexpr uint32_t B_BYTES = BN * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
+  static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_WARPS * OUT_BYTES) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
+  static constexpr uint32_t OUT_AT = STAGES * STAGE, FRAME = OUT_AT + OUT_WARPS * OUT_BYTES, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
+  static constexpr int COLS = OUT == Out::GATE ? BN / 2 : OUT == Out::AGAIN ? BN / 3 : BN;   // of the output
 };
 
-template <bool A_MN, bool B_MN, int BN>
-struct Shape {
-  static constexpr uint32_t B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
-  static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_WARPS * 4096) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
-  static constexpr uint32_t OUT = STAGES * STAGE, FRAME = OUT + OUT_WARPS * 4096, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
-};
+// 32 rows, a row a lane, of CW values to memory: through shared memory (rows of RB bytes, pieces of 16 bytes swizzled so that neither side
+// meets a bank twice), so that a request writes whole sectors of neighbouring rows.  f(row, first column, the 16 bytes) writes.
+template <int RB, class F>
+__device__ __forceinline__ void through(uint8_t* stage, int lane, const uint4 (&v)[RB / 16], F f) {
+  constexpr int PER = RB / 16;
+  auto at = [](int r, int q) { return r * RB + ((RB == 64 ? q ^ ((r >> 1) & 3) : q ^ ((r >> 2) & 1)) << 4); };
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < PER; ++q) *reinterpret_cast<uint4*>(stage + at(lane, q)) = v[q];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = i * (32 / PER) + lane / PER, q = lane % PER;
+    f(r, q, *reinterpret_cast<const uint4*>(stage + at(r, q)));
+  }
+}
+// CW values a lane as elements of type E.
+template <typename E, int CW, class F>
+__device__ __forceinline__ void emit(uint8_t* stage, int lane, const float (&v)[CW], F f) {
+  if constexpr (sizeof(E) == 4) {
+#pragma unroll
+    for (int h = 0; h < CW / 16; ++h) {
+      uint4 c[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        c[q] = make_uint4(__float_as_uint(v[16 * h + 4 * q]), __float_as_uint(v[16 * h + 4 * q + 1]), __float_as_uint(v[16 * h + 4 * q + 2]), __float_as_uint(v[16 * h + 4 * q + 3]));
+      through<64>(stage, lane, c, [&](int r, int q, uint4 raw) { f(r, 16 * h + 4 * q, raw); });
+    }
+  } else {
+    uint4 c[CW / 8];
+#pragma unroll
+    for (int q = 0; q < CW / 8; ++q)
+      c[q] = make_uint4(pair_of(v[8 * q], v[8 * q + 1], E{}), pair_of(v[8 * q + 2], v[8 * q + 3], E{}), pair_of(v[8 * q + 4], v[8 * q + 5], E{}), pair_of(v[8 * q + 6], v[8 * q + 7], E{}));
+    through<2 * CW>(stage, lane, c, [&](int r, int q, uint4 raw) { f(r, 8 * q, raw); });
+  }
+}
+// The 16 bytes of a row from column `col` on: whole where they may be, else element by element up to `cols`.
+template <typename E>
+__device__ __forceinline__ void put16(E* row, int col, int cols, bool wide, uint4 raw) {
+  constexpr int N = 16 / sizeof(E);
+  if (wide && col + N <= cols) {
+    *reinterpret_cast<uint4*>(row + col) = raw;
+  } else {
+    const E* e = reinterpret_cast<const E*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (col + i < cols) row[col + i] = e[i];
+  }
+}
 
 template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT>
 __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Product p) {
-  using S = Shape<A_MN, B_MN, BN>;
-  using V = typename Kind<E, PIECES>::Value;
+  using S = Shape<BN, OUT>;
   constexpr bool EXACT = PIECES > 1;
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  static_assert(!EXACT || 3 * BN <= 512, "two sets of accumulators and their sum");
+  constexpr uint32_t SUM = 2 * BN;   // float32: where runs are added
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   Frame2& f = *reinterpret_cast<Frame2*>(smem + S::FRAME);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -215,9 +234,14 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  let_next_start();
+  wait_for_previous();
   const uint32_t tmem = f.tmem, base = smem_u32(smem);
   auto wait = [&](uint64_t& bar, uint32_t parity, int code) { mbar_wait(smem_u32(&bar), parity & 1u, &f.status, f.aborted, code); };
   const int tiles = p.m_tiles * p.n_tiles * p.jobs * p.splits, all_steps = p.k_steps * p.terms;
+  // The end of the run of stages that begins at s: all of a tile's, or, in float32, all of the small terms, then FLUSH at a time.
+  const int small = EXACT ? all_steps - all_steps / 6 : all_steps;
+  auto run_end = [&](int s, int s1) { return !EXACT ? s1 : s < small ? min(s1, small) : min(s1, s + FLUSH); };
 
   if (warp == 0) {
     // fetching
@@ -227,30 +251,39 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
       const Tile t = tile_of(p, i);
       const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps);
       int term = s0 / p.k_steps, k = s0 - term * p.k_steps;
-      const int m0 = t.m * BM, n0 = t.n * (OUT == Out::GATE ? BN / 2 : BN);
+      const int m0 = t.m * BM, n0 = t.n * S::COLS;
       for (int s = s0; s < s1; ++s, ++step) {
         const int slot = step % S::STAGES;
         if (step >= S::STAGES) wait(f.empty[slot], step / S::STAGES - 1, W_EMPTY);
         if (el) {
-          const uint32_t bar = smem_u32(&f.full[slot]), at = base + slot * S::STAGE, bt = at + A_BYTES;
+          const uint32_t bar = smem_u32(&f.full[slot]), at = base + slot * S::STAGE;
           const CUtensorMap* am = &p.a[p.jobs > 1 ? t.job : p.a_map[term]];
           const CUtensorMap* bm = &p.b[p.b_map[term]];
           const int ap = p.a_piece[term], bp = p.b_piece[term], kc = k * BK;
           mbar_expect_tx(bar, S::STAGE);
-          if constexpr (A_MN) {
+          if constexpr (OUT == Out::AGAIN) {
+            tma_load(at, &p.a[0], kc, m0, 0, bar);
+            tma_load(at + A_BYTES, &p.a[1], kc, m0, 0, bar);
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load(at + j * SLAB, am, m0 + 64 * j, kc, ap, bar);
+            for (int j = 0; j < 2; ++j) tma_load(at + 2 * A_BYTES + j * SLAB, &p.b[j], kc, n0, 0, bar);
+            tma_load(at + 2 * A_BYTES + 2 * SLAB, &p.b[2], n0, kc, 0, bar);
           } else {
-            tma_load(at, am, kc, m0, ap, bar);
-          }
-          if constexpr (OUT == Out::GATE) {
-            tma_load(bt, &p.b[0], kc, n0, bp, bar);
-            tma_load(bt + S::B_BYTES / 2, &p.b[1], kc, n0, bp, bar);
-          } else if constexpr (B_MN) {
+            const uint32_t bt = at + A_BYTES;
+            if constexpr (A_MN) {
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j) tma_load(bt + j * SLAB, bm, n0 + 64 * j, kc, bp, bar);
-          } else {
-            tma_load(bt, bm, kc, n0, bp, bar);
+              for (int j = 0; j < BM / 64; ++j) tma_load(at + j * SLAB, am, m0 + 64 * j, kc, ap, bar);
+            } else {
+              tma_load(at, am, kc, m0, ap, bar);
+            }
+            if constexpr (OUT == Out::GATE) {
+              tma_load(bt, &p.b[0], kc, n0, bp, bar);
+              tma_load(bt + S::B_BYTES / 2, &p.b[1], kc, n0, bp, bar);
+            } else if constexpr (B_MN) {
+#pragma unroll
+              for (int j = 0; j < BN / 64; ++j) tma_load(bt + j * SLAB, bm, n0 + 64 * j, kc, bp, bar);
+            } else {
+              tma_load(bt, bm, kc, n0, bp, bar);
+            }
           }
         }
         __syncwarp();
@@ -261,146 +294,192 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
     for (int s = max(0, step - S::STAGES); s < step; ++s) wait(f.full[s % S::STAGES], s / S::STAGES, W_FULL);
   } else if (warp == 1) {
     // issuing
-    constexpr uint32_t IDESC = (1u << 4) | Kind<E, PIECES>::FORMAT | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24) |
-                               (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+    constexpr uint32_t COMMON = (1u << 4) | Format<E>::BITS | ((uint32_t)(BM >> 4) << 24);
+    constexpr uint32_t MN_A = 1u << 15, MN_B = 1u << 16;
     constexpr uint32_t A_K = A_MN ? 128 : 2, B_K = B_MN ? 128 : 2;   // 16 of depth in descriptor units (16 bytes)
     const uint32_t el = elect_one(), tm = uniform(tmem);
     auto low = [](uint32_t addr, bool mn) { return ((addr & 0x3FFFFu) >> 4) | (mn ? (SLAB >> 4) << 16 : 1u << 16); };
     int step = 0, done = 0;
-    for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++done) {
+    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
       const Tile t = tile_of(p, i);
-      const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps), set = done & 1;
-      if (done >= 2) wait(f.drained[set], done / 2 - 1, W_DRAINED);
-      tc_fence_after();
-      for (int s = s0; s < s1; ++s, ++step) {
-        const int slot = step % S::STAGES;
-        wait(f.full[slot], step / S::STAGES, W_FULL);
+      const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps);
+      for (int s = s0; s < s1; ++done) {
+        const int set = done & 1, end = run_end(s, s1);
+        if (done >= 2) wait(f.drained[set], done / 2 - 1, W_DRAINED);
         tc_fence_after();
-        const uint32_t at = base + slot * S::STAGE, a_lo = uniform(low(at, A_MN)), b_lo = uniform(low(at + A_BYTES, B_MN));
+        for (uint32_t acc = 0; s < end; ++s, ++step, acc = 1) {
+          const int slot = step % S::STAGES;
+          wait(f.full[slot], step / S::STAGES, W_FULL);
+          tc_fence_after();
+          const uint32_t at = base + slot * S::STAGE;
+          if constexpr (OUT == Out::AGAIN) {
+            const uint32_t x = uniform(low(at, false)), dy = uniform(low(at + A_BYTES, false)), w = uniform(low(at + 2 * A_BYTES, false)),
+                           d = uniform(low(at + 2 * A_BYTES + 2 * SLAB, true));
 #pragma unroll
-        for (uint32_t k = 0; k < BK / 16; ++k)
-          mma_one<false>(el, tm + set * BN, a_lo + A_K * k, b_lo + B_K * k, IDESC, s > s0 || k ? 1u : 0u);
-        tc_commit_if(el, smem_u32(&f.empty[slot]));
+            for (uint32_t k = 0; k < BK / 16; ++k)
+              mma_one<false>(el, tm + set * BN, x + 2 * k, w + 2 * k, COMMON | ((uint32_t)(128 >> 3) << 17), acc || k ? 1u : 0u);
+#pragma unroll
+            for (uint32_t k = 0; k < BK / 16; ++k)
+              mma_one<false>(el, tm + set * BN + 128, dy + 2 * k, d + 128 * k, COMMON | ((uint32_t)(64 >> 3) << 17) | MN_B, acc || k ? 1u : 0u);
+          } else {
+            constexpr uint32_t IDESC = COMMON | ((uint32_t)(BN >> 3) << 17) | (A_MN ? MN_A : 0u) | (B_MN ? MN_B : 0u);
+            const uint32_t a_lo = uniform(low(at, A_MN)), b_lo = uniform(low(at + A_BYTES, B_MN));
+#pragma unroll
+            for (uint32_t k = 0; k < BK / 16; ++k)
+              mma_one<false>(el, tm + set * BN, a_lo + A_K * k, b_lo + B_K * k, IDESC, acc || k ? 1u : 0u);
+          }
+          tc_commit_if(el, smem_u32(&f.empty[slot]));
+        }
+        tc_commit_if(el, smem_u32(&f.acc[set]));
+        __syncwarp();
       }
-      tc_commit_if(el, smem_u32(&f.acc[set]));
-      __syncwarp();
     }
   } else {
-    // taking out: this warp's 32 rows (a quarter of tensor memory is a warp's by its number) and half of the columns
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* stage = smem + S::OUT + (warp - 2) * 4096;
+    // taking out: this warp's 32 rows (a quarter of tensor memory is a warp's by its number) and a part of the columns
+    constexpr int MINE = S::COLS / PARTS, CW = MINE < 32 || OUT == Out::BACK ? 16 : 32;   // BACK holds four values a column
+    static_assert(MINE % CW == 0 && (CW == 16 || CW == 32), "a warp takes 16 or 32 columns at a time");
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
+    uint8_t* stage = smem + S::OUT_AT + (warp - 2) * OUT_BYTES;
     const Epilogue& e = p.e;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
     int done = 0;
-    for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++done) {
-      const Tile t = tile_of(p, i);
-      const int set = done & 1;
-      wait(f.acc[set], done / 2, W_ACC);
-      tc_fence_after();
-      const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + set * BN;
-      const int64_t row0 = (int64_t)t.m * BM + 32 * quarter;
-      // 32 columns from a row per lane to eight neighbours of a row per lane: request q, row 8 q + lane / 4, columns 8 (lane % 4) ..
-      auto stage_in = [&](const float (&v)[32]) {
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          *reinterpret_cast<float4*>(stage + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        __syncwarp();
-      };
-      auto staged = [&](int q, float (&v)[8]) {
-        const int r = 8 * q + (lane >> 2), c = 2 * (lane & 3);
-        const float4 a = *reinterpret_cast<const float4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
-        const float4 b = *reinterpret_cast<const float4*>(stage + r * 128 + (((c + 1) ^ (r & 7)) << 4));
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      };
-      const int my_cols = OUT == Out::GATE ? BN / 4 : BN / 2;   // of the output
-      static_assert(OUT == Out::GATE ? BN >= 128 : BN >= 64, "a warp takes 32 columns at a time");
-#pragma unroll 1
-      for (int c0 = half * my_cols; c0 < (half + 1) * my_cols; c0 += 32) {
-        const int col0 = t.n * (OUT == Out::GATE ? BN / 2 : BN) + c0, col = col0 + 8 * (lane & 3);
-        if (col0 >= p.n) break;
-        uint32_t bits[32];
-        float v[32];
-        tmem_ld32(acc + c0, bits);
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(bits[k]);
-        if constexpr (OUT == Out::GATE) {
-          tmem_ld32(acc + BN / 2 + c0, bits);
-          if (e.g) {
-            stage_in(v);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int64_t r = row0 + 8 * q + (lane >> 2);
-              float o[8];
-              staged(q, o);
-              if (r < p.m && col < e.ld_h) put8(static_cast<V*>(e.g) + r * e.ld_h + col, o, 8, true);
-            }
-            float w[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) w[k] = __uint_as_float(bits[k]);
-            stage_in(w);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int64_t r = row0 + 8 * q + (lane >> 2);
-              float o[8];
-              staged(q, o);
-              if (r < p.m && col < e.ld_h) put8(static_cast<V*>(e.u) + r * e.ld_h + col, o, 8, true);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            float a, da;
-            activate<EXACT>(e.activation, v[k], a, da);
-            v[k] = a * __uint_as_float(bits[k]);
-          }
-          stage_in(v);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int64_t r = row0 + 8 * q + (lane >> 2);
-            float o[8];
-            staged(q, o);
-            if (r < p.m && col < e.ld_h) put_operand<E, PIECES>(e.h, e.piece_stride, r * e.ld_h + col, o);
-          }
-        } else {
-          stage_in(v);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int64_t r = row0 + 8 * q + (lane >> 2);
-            float o[8];
-            staged(q, o);
-            if constexpr (OUT == Out::BACK) {
-              if (r < p.m && col < e.ld_h) {
-                const int64_t at = r * e.ld_h + col;
-                float g[8], u[8], dg[8], du[8], h[8];
-                get8(static_cast<const V*>(e.g) + at, g);
-                get8(static_cast<const V*>(e.u) + at, u);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  float a, da;
-                  activate<EXACT>(e.activation, g[k], a, da);
-                  dg[k] = o[k] * u[k] * da;
-                  du[k] = o[k] * a;
-                  h[k] = a * u[k];
-                }
-                put_operand<E, PIECES>(e.dg, e.piece_stride, at, dg);
-                put_operand<E, PIECES>(e.du, e.piece_stride, at, du);
-                put_operand<E, PIECES>(e.h, e.piece_stride, at, h);
-              }
-            } else if (r < p.m && col < p.n) {
-              const int left = p.n - col;
-              if constexpr (OUT == Out::PARTIAL) {
-                put8(e.part + (((int64_t)t.split * p.jobs + t.job) * p.m + r) * p.n + col, o, left, p.n % 4 == 0);
-              } else if (e.out_kind == 0) {
-                put8(static_cast<float*>(e.out[t.job]) + r * e.ld_out + col, o, left, e.ld_out % 4 == 0);
-              } else {
-                put8(static_cast<E*>(e.out[t.job]) + r * e.ld_out + col, o, left, e.ld_out % 8 == 0);
-              }
-            }
-          }
-        }
-      }
+    auto release = [&](int set) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&f.drained[set]));
+    };
+    auto load = [&](uint32_t at, float (&v)[CW]) {
+      uint32_t bits[CW];
+      tmem_ld_cols<CW>(at, bits);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < CW; ++k) v[k] = __uint_as_float(bits[k]);
+    };
+    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+      const Tile t = tile_of(p, i);
+      uint32_t acc = lanes + (done & 1) * BN;
+      if constexpr (EXACT) {
+        const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps);
+        for (int s = s0; s < s1; ++done) {
+          const int set = done & 1;
+          wait(f.acc[set], done / 2, W_ACC);
+          tc_fence_after();
+          // its share of the accumulators' columns, in GATE of both halves
+#pragma unroll 1
+          for (int c0 = part * (BN / PARTS); c0 < (part + 1) * (BN / PARTS); c0 += 8) {
+            uint32_t v[8], w[8];
+            const int c = OUT == Out::GATE ? (c0 - part * (BN / PARTS) < MINE ? part * MINE + (c0 - part * (BN / PARTS)) : BN / 2 + part * MINE + (c0 - part * (BN / PARTS) - MINE)) : c0;
+            tmem_ld8_nowait(lanes + set * BN + c, v);
+            if (s > s0) tmem_ld8_nowait(lanes + SUM + c, w);
+            tmem_wait_ld();
+            if (s > s0)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) + __uint_as_float(w[k]));
+            tmem_st8_nowait(lanes + SUM + c, v);
+          }
+          tmem_wait_st();
+          release(set);
+          s = run_end(s, s1);
+        }
+        acc = lanes + SUM;
+      }
+      const int set = done & 1;
+      const int64_t row0 = (int64_t)t.m * BM + 32 * quarter;
+      auto operand_out = [&](void* base_, int col0, float (&v)[CW]) {   // (pieces, m, ld_h)
+#pragma unroll
+        for (int piece = 0; piece < PIECES; ++piece) {
+          E* to = static_cast<E*>(base_) + piece * e.piece_stride;
+          emit<E, CW>(stage, lane, v, [&](int r, int c, uint4 raw) {
+            if (row0 + r < p.m && col0 + c < e.ld_h) *reinterpret_cast<uint4*>(to + (row0 + r) * e.ld_h + col0 + c) = raw;
+          });
+          if constexpr (PIECES > 1) {
+#pragma unroll
+            for (int k = 0; k < CW; ++k) {
+              E r;
+              down(r, v[k]);
+              v[k] -= up(r);
+            }
+          }
+        }
+      };
+      // kept g and u: a block of 32 x 32 is eight requests of a float4 a lane, its row's
+      auto kept_at = [&](float* base_, int col0, int q) {
+        const int64_t block = (row0 >> 5) * ((e.ld_h + 31) >> 5) + (col0 >> 5);
+        return reinterpret_cast<float4*>(base_) + (block * 8 + ((col0 & 31) >> 2) + q) * 32 + lane;
+      };
+      bool waited = EXACT;
+#pragma unroll 1
+      for (int c0 = part * MINE; c0 < (part + 1) * MINE; c0 += CW) {
+        const int col0 = t.n * S::COLS + c0;
+        if (col0 >= p.n) break;
+        const bool in = row0 < p.m;
+        if constexpr (OUT == Out::GATE || OUT == Out::BACK || OUT == Out::AGAIN) {
+          float g[CW], u[CW];
+          if constexpr (OUT == Out::BACK) {
+#pragma unroll
+            for (int q = 0; q < CW / 4; ++q) {
+              const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), gq = in ? *kept_at(e.g, col0, q) : zero, uq = in ? *kept_at(e.u, col0, q) : zero;
+              g[4 * q] = gq.x, g[4 * q + 1] = gq.y, g[4 * q + 2] = gq.z, g[4 * q + 3] = gq.w;
+              u[4 * q] = uq.x, u[4 * q + 1] = uq.y, u[4 * q + 2] = uq.z, u[4 * q + 3] = uq.w;
+            }
+          }
+          if (!waited) wait(f.acc[set], done / 2, W_ACC), waited = true;
+          tc_fence_after();
+          if constexpr (OUT != Out::BACK) {
+            load(acc + c0, g);
+            load(acc + S::COLS + c0, u);
+          }
+          if constexpr (OUT == Out::GATE) {
+            if (e.g && in)
+#pragma unroll
+              for (int q = 0; q < CW / 4; ++q) {
+                *kept_at(e.g, col0, q) = make_float4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
+                *kept_at(e.u, col0, q) = make_float4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
+              }
+#pragma unroll
+            for (int k = 0; k < CW; ++k) {
+              float a, da;
+              activate<EXACT>(e.activation, g[k], a, da);
+              u[k] *= a;
+            }
+            operand_out(e.h, col0, u);
+          } else {
+            float dh[CW], h[CW];
+            load(acc + (OUT == Out::AGAIN ? 128 : 0) + c0, dh);
+#pragma unroll
+            for (int k = 0; k < CW; ++k) {
+              float a, da;
+              activate<EXACT>(e.activation, g[k], a, da);
+              h[k] = a * u[k];
+              g[k] = dh[k] * u[k] * da;
+              dh[k] *= a;
+            }
+            operand_out(e.h, col0, h);
+            operand_out(e.dg, col0, g);
+            operand_out(e.du, col0, dh);
+          }
+        } else {
+          if (!waited) wait(f.acc[set], done / 2, W_ACC), waited = true;
+          tc_fence_after();
+          float v[CW];
+          load(acc + c0, v);
+          auto rows_out = [&](auto* to, int64_t ld) {
+            using O = std::remove_pointer_t<decltype(to)>;
+            const bool wide = ld % (16 / (int)sizeof(O)) == 0;
+            emit<O, CW>(stage, lane, v, [&](int r, int c, uint4 raw) {
+              if (row0 + r < p.m) put16(to + (row0 + r) * ld, col0 + c, p.n, wide, raw);
+            });
+          };
+          if constexpr (OUT == Out::PARTIAL) rows_out(e.part + (int64_t)(t.split * p.jobs + t.job) * p.m * p.n, p.n);
+          else if (e.out_kind == 0) rows_out(static_cast<float*>(e.out[t.job]), e.ld_out);
+          else rows_out(static_cast<E*>(e.out[t.job]), e.ld_out);
+        }
+      }
+      if constexpr (!EXACT) {
+        if (!waited) wait(f.acc[set], done / 2, W_ACC);
+        release(set);
+        ++done;
+      }
     }
   }
   tc_fence_before();

@@ -145,11 +145,12 @@ def test_gated_block_checks_its_arguments():
     c = call()
     assert lib.bnb_gated_block_scratch_bytes(C.byref(c), 0) >= 100 * 128 * 2
     assert lib.bnb_gated_block_scratch_bytes(C.byref(c), 1) > lib.bnb_gated_block_scratch_bytes(C.byref(c), 0)
-    assert lib.bnb_gated_block_kept_bytes(C.byref(c)) == 2 * 100 * 128 * 2
+    assert lib.bnb_gated_block_kept_bytes(C.byref(c)) == 0                                        # narrow: computed once more
+    assert lib.bnb_gated_block_kept_bytes(C.byref(call(width=400))) == 2 * 128 * 128 * 4          # whole blocks of 32 x 32
     g = GatedGrads(fake, 64, fake, fake, None, fake)
     assert lib.bnb_gated_block_bwd(C.byref(call(kept=fake)), C.byref(g), None, 0, None) == 1     # half of the gate's pair
     g = GatedGrads(fake, 64, fake, fake, fake, fake)
-    assert lib.bnb_gated_block_bwd(C.byref(call()), C.byref(g), None, 0, None) == 1              # nothing kept
+    assert lib.bnb_gated_block_bwd(C.byref(call(width=400)), C.byref(g), None, 0, None) == 1     # nothing kept
     assert lib.bnb_gated_block_bwd(C.byref(call(kept=fake)), C.byref(g), None, 0, None) == 6
 
 
@@ -189,5 +190,5 @@ def test_operators_have_shape_only_fakes():
         assert y.shape == x.shape and st.shape == (3, 8, 11) and kept.numel() == 1 * 3 * 8 * 16
         assert ops.selective_scan(x, x, A, B, B, None, None, None, None, None, None, True, False)[2].numel() == 0
         y, kept = ops.gated_mlp(x, torch.empty(20, 8, device="cuda"), torch.empty(20, 8, device="cuda"), torch.empty(8, 20, device="cuda"), 2, True)
-        assert y.shape == x.shape and kept.numel() == 2 * 15 * 24 * 2
+        assert y.shape == x.shape and kept.numel() == 0
         assert ops.selective_step(x[0], x[0], A, B[0], B[0], None, st, None, None, None, True).shape == (3, 8)
