@@ -52,14 +52,21 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJobs j
   }
 }
 
-// Sums of the parts of a depth, in their order.
+// Sums of the parts of a depth: four threads share a cell's parts, each in their order, and are added in theirs.
 template <typename E>
 __global__ void __launch_bounds__(256) k_add_parts(const float* part, int splits, int64_t cells, int jobs, void* out0, void* out1, int out_kind) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= cells * jobs) return;
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane;
   float v = 0.f;
+  if (i < cells * jobs) {
 #pragma unroll 8
-  for (int s = 0; s < splits; ++s) v += part[s * cells * jobs + i];
+    for (int s = q; s < splits; s += 4) v += part[s * cells * jobs + i];
+  }
+  sums[q][lane] = v;
+  __syncthreads();
+  if (q || i >= cells * jobs) return;
+  v = (v + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
   void* out = i < cells ? out0 : out1;
   const int64_t at = i < cells ? i : i - cells;
   if (out_kind == 0) static_cast<float*>(out)[at] = v;
@@ -187,7 +194,7 @@ int multiply(const Sides& s, int64_t m, int64_t n, int64_t depth, int jobs, cons
       if (const int r = at_width<E, PIECES, A_MN, B_MN, Out::PARTIAL>(p, z.bn, total, st)) return r;
       const int64_t cells = m * n;
       count_launch();
-      k_add_parts<E><<<(unsigned)((cells * jobs + 255) / 256), 256, 0, st>>>(part, z.splits, cells, jobs, e.out[0], e.out[1], e.out_kind);
+      k_add_parts<E><<<(unsigned)((cells * jobs + 63) / 64), 256, 0, st>>>(part, z.splits, cells, jobs, e.out[0], e.out[1], e.out_kind);
       return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;
     }
     return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, st);

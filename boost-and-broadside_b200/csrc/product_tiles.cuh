@@ -88,29 +88,60 @@ struct Frame2 {
   uint32_t tmem;
 };
 
-// act(g) and act'(g).  e^(-g^2/2) serves the distribution function and its density: for 16-bit results by the approximation 7.1.26
-// of Abramowitz and Stegun's Handbook (absolute error 1.5e-7), for float32 by erff.
-template <bool EXACT>
-__device__ __forceinline__ void activate(int kind, float g, float& a, float& da) {
+// act(g) and, where wanted, act'(g) of neighbouring columns, two in an instruction.  e^(-g^2/2) serves the distribution function and its
+// density.  16-bit results: that function as 1/2 + sign(g) (1/2 - tail), the tail by the approximation 7.1.26 of Abramowitz and Stegun's
+// Handbook (absolute error 1.5e-7); float32: by erff.  With one element at a time and divisions that scale, 38 instructions an element
+// instead of 14.
+template <bool SLOPE>
+__device__ __forceinline__ void activate_pair(int kind, F2 g, F2& a, F2& da) {
+  const float2 gs = halves(g);
   if (kind == BNB_ACT_SILU) {
-    const float s = EXACT ? 1.0f / (1.0f + expf(-g)) : __fdividef(1.0f, 1.0f + __expf(-g));
-    a = g * s;
-    da = s * fmaf(g, 1.0f - s, 1.0f);
+    const float2 m = halves(mul(g, f2(-1.4426950408889634f))), den = halves(add(f2(ex2_fast(m.x), ex2_fast(m.y)), f2(1.0f)));
+    const F2 s = f2(rcp_fast(den.x), rcp_fast(den.y));
+    a = mul(g, s);
+    if (SLOPE) da = mul(s, fma(g, fma(s, f2(-1.0f), f2(1.0f)), f2(1.0f)));
     return;
   }
-  float cdf, density;   // density: g e^(-g^2/2) / sqrt(2 pi)
+  const float2 den = halves(fma(f2(fabsf(gs.x), fabsf(gs.y)), f2(0.3275911f * 0.70710678118654752440f), f2(1.0f)));
+  const float2 m = halves(mul(mul(g, g), f2(-0.5f * 1.4426950408889634f)));
+  const F2 t = f2(rcp_fast(den.x), rcp_fast(den.y)), q = f2(ex2_fast(m.x), ex2_fast(m.y));
+  F2 poly = fma(t, f2(-0.5f * 1.061405429f), f2(0.5f * 1.453152027f));   // half of the series, negative
+  poly = fma(t, poly, f2(-0.5f * 1.421413741f));
+  poly = fma(t, poly, f2(0.5f * 0.284496736f));
+  poly = fma(t, poly, f2(-0.5f * 0.254829592f));
+  const float2 rest = halves(fma(mul(t, poly), q, f2(0.5f)));   // 1/2 - tail
+  const F2 cdf = add(f2(copysignf(rest.x, gs.x), copysignf(rest.y, gs.y)), f2(0.5f));
+  a = mul(g, cdf);
+  if (SLOPE) da = fma(mul(g, q), f2(0.39894228040143267794f), cdf);
+}
+template <bool EXACT, bool SLOPE, int N>
+__device__ __forceinline__ void activate(int kind, const float (&g)[N], float (&a)[N], float (&da)[N]) {
   if constexpr (EXACT) {
-    cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752440f));
-    density = g * expf(-0.5f * g * g) * 0.39894228040143267794f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (kind == BNB_ACT_SILU) {
+        const float s = 1.0f / (1.0f + expf(-g[k]));
+        a[k] = g[k] * s;
+        da[k] = s * fmaf(g[k], 1.0f - s, 1.0f);
+      } else {
+        const float cdf = 0.5f * (1.0f + erff(g[k] * 0.70710678118654752440f));
+        a[k] = g[k] * cdf;
+        da[k] = fmaf(g[k] * 0.39894228040143267794f, expf(-0.5f * g[k] * g[k]), cdf);
+      }
+    }
   } else {
-    const float x = fabsf(g) * 0.70710678118654752440f, t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f)), q = __expf(-0.5f * g * g);
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * poly * q;   // of |g|
-    cdf = g < 0.f ? tail : 1.0f - tail;
-    density = g * q * 0.39894228040143267794f;
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      F2 v, d;
+      activate_pair<SLOPE>(kind, f2(g[k], g[k + 1]), v, d);
+      const float2 vs = halves(v);
+      a[k] = vs.x, a[k + 1] = vs.y;
+      if (SLOPE) {
+        const float2 ds = halves(d);
+        da[k] = ds.x, da[k + 1] = ds.y;
+      }
+    }
   }
-  a = g * cdf;
-  da = cdf + density;
 }
 
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
@@ -348,13 +379,7 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&f.drained[set]));
     };
-    auto load = [&](uint32_t at, float (&v)[CW]) {
-      uint32_t bits[CW];
-      tmem_ld_cols<CW>(at, bits);
-      tmem_wait_ld();
-#pragma unroll
-      for (int k = 0; k < CW; ++k) v[k] = __uint_as_float(bits[k]);
-    };
+    auto load = [&](uint32_t at, float (&v)[CW]) { tmem_ld_cols<CW>(at, *reinterpret_cast<uint32_t(*)[CW]>(&v)); };   // behind it: tmem_wait_ld
     for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
       const Tile t = tile_of(p, i);
       uint32_t acc = lanes + (done & 1) * BN;
@@ -407,12 +432,21 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
         const int64_t block = (row0 >> 5) * ((e.ld_h + 31) >> 5) + (col0 >> 5);
         return reinterpret_cast<float4*>(base_) + (block * 8 + ((col0 & 31) >> 2) + q) * 32 + lane;
       };
-      bool waited = EXACT;
+      // A tile's accumulators are waited for once, and given back as soon as the last of them are in registers.
+      bool waited = EXACT, released = EXACT;
+      auto ready = [&] {
+        if (!waited) wait(f.acc[set], done / 2, W_ACC), waited = true;
+        tc_fence_after();
+      };
 #pragma unroll 1
       for (int c0 = part * MINE; c0 < (part + 1) * MINE; c0 += CW) {
         const int col0 = t.n * S::COLS + c0;
         if (col0 >= p.n) break;
-        const bool in = row0 < p.m;
+        const bool in = row0 < p.m, last = c0 + CW == (part + 1) * MINE || col0 + CW >= p.n;
+        auto taken = [&] {
+          tmem_wait_ld();
+          if (!EXACT && last) release(set), released = true;
+        };
         if constexpr (OUT == Out::GATE || OUT == Out::BACK || OUT == Out::AGAIN) {
           float g[CW], u[CW];
           if constexpr (OUT == Out::BACK) {
@@ -423,12 +457,14 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
               u[4 * q] = uq.x, u[4 * q + 1] = uq.y, u[4 * q + 2] = uq.z, u[4 * q + 3] = uq.w;
             }
           }
-          if (!waited) wait(f.acc[set], done / 2, W_ACC), waited = true;
-          tc_fence_after();
+          ready();
+          float dh[CW], a[CW], da[CW];
           if constexpr (OUT != Out::BACK) {
             load(acc + c0, g);
             load(acc + S::COLS + c0, u);
           }
+          if constexpr (OUT != Out::GATE) load(acc + (OUT == Out::AGAIN ? 128 : 0) + c0, dh);
+          taken();
           if constexpr (OUT == Out::GATE) {
             if (e.g && in)
 #pragma unroll
@@ -436,33 +472,27 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
                 *kept_at(e.g, col0, q) = make_float4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
                 *kept_at(e.u, col0, q) = make_float4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
               }
+            activate<EXACT, false>(e.activation, g, a, da);
 #pragma unroll
-            for (int k = 0; k < CW; ++k) {
-              float a, da;
-              activate<EXACT>(e.activation, g[k], a, da);
-              u[k] *= a;
-            }
+            for (int k = 0; k < CW; ++k) u[k] *= a[k];
             operand_out(e.h, col0, u);
           } else {
-            float dh[CW], h[CW];
-            load(acc + (OUT == Out::AGAIN ? 128 : 0) + c0, dh);
+            activate<EXACT, true>(e.activation, g, a, da);
 #pragma unroll
             for (int k = 0; k < CW; ++k) {
-              float a, da;
-              activate<EXACT>(e.activation, g[k], a, da);
-              h[k] = a * u[k];
-              g[k] = dh[k] * u[k] * da;
-              dh[k] *= a;
+              da[k] *= dh[k] * u[k];   // dg
+              dh[k] *= a[k];           // du
+              a[k] *= u[k];            // h
             }
-            operand_out(e.h, col0, h);
-            operand_out(e.dg, col0, g);
+            operand_out(e.h, col0, a);
+            operand_out(e.dg, col0, da);
             operand_out(e.du, col0, dh);
           }
         } else {
-          if (!waited) wait(f.acc[set], done / 2, W_ACC), waited = true;
-          tc_fence_after();
+          ready();
           float v[CW];
           load(acc + c0, v);
+          taken();
           auto rows_out = [&](auto* to, int64_t ld) {
             using O = std::remove_pointer_t<decltype(to)>;
             const bool wide = ld % (16 / (int)sizeof(O)) == 0;
@@ -476,8 +506,10 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
         }
       }
       if constexpr (!EXACT) {
-        if (!waited) wait(f.acc[set], done / 2, W_ACC);
-        release(set);
+        if (!released) {   // no columns of this warp's part
+          ready();
+          release(set);
+        }
         ++done;
       }
     }
