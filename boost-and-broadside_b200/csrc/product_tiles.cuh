@@ -31,7 +31,6 @@ constexpr int MAX_TERMS = 12;                 // two segments of six
 constexpr int FLUSH = 4;                      // stages of a run
 constexpr int OUT_WARPS = 16, PARTS = OUT_WARPS / 4, CTA = 32 * (2 + OUT_WARPS);
 constexpr uint32_t A_BYTES = BM * BK * 2, SLAB = 64 * BK * 2;   // SLAB: 64 rows or columns by 64
-constexpr uint32_t OUT_BYTES = 2048;          // shared memory of a warp that takes out
 enum : int { W_FULL = 101, W_EMPTY = 102, W_ACC = 103, W_DRAINED = 104 };
 
 // What a tile's results become.
@@ -114,33 +113,28 @@ __device__ __forceinline__ void activate_pair(int kind, F2 g, F2& a, F2& da) {
   a = mul(g, cdf);
   if (SLOPE) da = fma(mul(g, q), f2(0.39894228040143267794f), cdf);
 }
-template <bool EXACT, bool SLOPE, int N>
-__device__ __forceinline__ void activate(int kind, const float (&g)[N], float (&a)[N], float (&da)[N]) {
-  if constexpr (EXACT) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if (kind == BNB_ACT_SILU) {
-        const float s = 1.0f / (1.0f + expf(-g[k]));
-        a[k] = g[k] * s;
-        da[k] = s * fmaf(g[k], 1.0f - s, 1.0f);
-      } else {
-        const float cdf = 0.5f * (1.0f + erff(g[k] * 0.70710678118654752440f));
-        a[k] = g[k] * cdf;
-        da[k] = fmaf(g[k] * 0.39894228040143267794f, expf(-0.5f * g[k] * g[k]), cdf);
-      }
-    }
+__device__ __forceinline__ void activate_exact(int kind, float g, float& a, float& da) {
+  if (kind == BNB_ACT_SILU) {
+    const float s = 1.0f / (1.0f + expf(-g));
+    a = g * s;
+    da = s * fmaf(g, 1.0f - s, 1.0f);
   } else {
-#pragma unroll
-    for (int k = 0; k < N; k += 2) {
-      F2 v, d;
-      activate_pair<SLOPE>(kind, f2(g[k], g[k + 1]), v, d);
-      const float2 vs = halves(v);
-      a[k] = vs.x, a[k + 1] = vs.y;
-      if (SLOPE) {
-        const float2 ds = halves(d);
-        da[k] = ds.x, da[k + 1] = ds.y;
-      }
-    }
+    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678118654752440f));
+    a = g * cdf;
+    da = fmaf(g * 0.39894228040143267794f, expf(-0.5f * g * g), cdf);
+  }
+}
+template <bool EXACT, bool SLOPE>
+__device__ __forceinline__ void activate(int kind, F2 g, F2& a, F2& da) {
+  if constexpr (EXACT) {
+    const float2 gs = halves(g);
+    float2 v, d;
+    activate_exact(kind, gs.x, v.x, d.x);
+    activate_exact(kind, gs.y, v.y, d.y);
+    a = f2(v.x, v.y);
+    da = f2(d.x, d.y);
+  } else {
+    activate_pair<SLOPE>(kind, g, a, da);
   }
 }
 
@@ -148,6 +142,10 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) { r
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename E> __device__ __forceinline__ uint32_t pair_of(F2 v) {
+  const float2 f = halves(v);
+  return pair_of(f.x, f.y, E{});
 }
 __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float up(__half v) { return __half2float(v); }
@@ -179,45 +177,53 @@ template <> struct Format<__nv_bfloat16> { static constexpr uint32_t BITS = (1u 
 template <int BN, Out OUT>
 struct Shape {
   static constexpr uint32_t B_BYTES = BN * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
-  static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_WARPS * OUT_BYTES) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
-  static constexpr uint32_t OUT_AT = STAGES * STAGE, FRAME = OUT_AT + OUT_WARPS * OUT_BYTES, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
   static constexpr int COLS = OUT == Out::GATE ? BN / 2 : OUT == Out::AGAIN ? BN / 3 : BN;   // of the output
+  // a warp that takes out holds CW columns of its rows at a time, the four warps of the same rows 4 CW neighbouring ones
+  static constexpr int CW = COLS / PARTS < 32 || OUT == Out::BACK ? 16 : 32;   // BACK holds four values a column
+  static constexpr uint32_t OUT_BYTES = 4 * 32 * (PARTS * CW * 2) * (OUT == Out::BACK || OUT == Out::AGAIN ? 3 : 1) < OUT_WARPS * 2048
+                                            ? OUT_WARPS * 2048 : 4 * 32 * (PARTS * CW * 2) * (OUT == Out::BACK || OUT == Out::AGAIN ? 3 : 1);
+  static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_BYTES) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
+  static constexpr uint32_t OUT_AT = STAGES * STAGE, FRAME = OUT_AT + OUT_BYTES, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
 };
 
-// 32 rows, a row a lane, of CW values to memory: through shared memory (rows of RB bytes, pieces of 16 bytes swizzled so that neither side
-// meets a bank twice), so that a request writes whole sectors of neighbouring rows.  f(row, first column, the 16 bytes) writes.
+// Results to memory.  A lane has CW neighbouring columns of a row; a request that writes a little of many rows costs the load and store
+// unit as much as one that writes whole lines of each (32 bytes of 16 rows: 16 of its cycles, 4 rows of 128 bytes: 4).
+//
+// 16-bit: the four warps of the same 32 rows put their columns together in shared memory (rows of RB bytes, the 16-byte
+// pieces swizzled so that neither side meets a bank twice), then each writes whole rows: f(row, column, 16 bytes).
+template <int RB>
+__device__ __forceinline__ uint32_t row_piece(int r, int q) { return r * RB + ((q ^ (r & 7)) << 4); }
+template <typename E, int CW>
+__device__ __forceinline__ void put_columns(uint8_t* rows, int part, int lane, const F2 (&v)[CW / 2]) {
+#pragma unroll
+  for (int q = 0; q < CW / 8; ++q)
+    *reinterpret_cast<uint4*>(rows + row_piece<PARTS * CW * 2>(lane, part * (CW / 8) + q)) =
+        make_uint4(pair_of<E>(v[4 * q]), pair_of<E>(v[4 * q + 1]), pair_of<E>(v[4 * q + 2]), pair_of<E>(v[4 * q + 3]));
+}
 template <int RB, class F>
-__device__ __forceinline__ void through(uint8_t* stage, int lane, const uint4 (&v)[RB / 16], F f) {
-  constexpr int PER = RB / 16;
-  auto at = [](int r, int q) { return r * RB + ((RB == 64 ? q ^ ((r >> 1) & 3) : q ^ ((r >> 2) & 1)) << 4); };
-  __syncwarp();
+__device__ __forceinline__ void take_rows(const uint8_t* rows, int part, int lane, F f) {
+  constexpr int PER = RB / 16, AT_ONCE = 32 / PER;   // lanes of a row, rows of a request
 #pragma unroll
-  for (int q = 0; q < PER; ++q) *reinterpret_cast<uint4*>(stage + at(lane, q)) = v[q];
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int r = i * (32 / PER) + lane / PER, q = lane % PER;
-    f(r, q, *reinterpret_cast<const uint4*>(stage + at(r, q)));
+  for (int i = 0; i < 8 / AT_ONCE; ++i) {
+    const int r = 8 * part + i * AT_ONCE + lane / PER, q = lane % PER;
+    f(r, 8 * q, *reinterpret_cast<const uint4*>(rows + row_piece<RB>(r, q)));
   }
 }
-// CW values a lane as elements of type E.
-template <typename E, int CW, class F>
-__device__ __forceinline__ void emit(uint8_t* stage, int lane, const float (&v)[CW], F f) {
-  if constexpr (sizeof(E) == 4) {
+// Float32: a warp for itself, 16 columns at a time.
+template <int CW, class F>
+__device__ __forceinline__ void emit_floats(uint8_t* stage, int lane, const F2 (&v)[CW / 2], F f) {
+  auto at = [](int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); };
 #pragma unroll
-    for (int h = 0; h < CW / 16; ++h) {
-      uint4 c[4];
+  for (int h = 0; h < CW / 16; ++h) {
+    __syncwarp();
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        c[q] = make_uint4(__float_as_uint(v[16 * h + 4 * q]), __float_as_uint(v[16 * h + 4 * q + 1]), __float_as_uint(v[16 * h + 4 * q + 2]), __float_as_uint(v[16 * h + 4 * q + 3]));
-      through<64>(stage, lane, c, [&](int r, int q, uint4 raw) { f(r, 16 * h + 4 * q, raw); });
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<ulonglong2*>(stage + at(lane, q)) = make_ulonglong2(v[8 * h + 2 * q].v, v[8 * h + 2 * q + 1].v);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + lane / 4, q = lane % 4;
+      f(r, 16 * h + 4 * q, *reinterpret_cast<const uint4*>(stage + at(r, q)));
     }
-  } else {
-    uint4 c[CW / 8];
-#pragma unroll
-    for (int q = 0; q < CW / 8; ++q)
-      c[q] = make_uint4(pair_of(v[8 * q], v[8 * q + 1], E{}), pair_of(v[8 * q + 2], v[8 * q + 3], E{}), pair_of(v[8 * q + 4], v[8 * q + 5], E{}), pair_of(v[8 * q + 6], v[8 * q + 7], E{}));
-    through<2 * CW>(stage, lane, c, [&](int r, int q, uint4 raw) { f(r, 8 * q, raw); });
   }
 }
 // The 16 bytes of a row from column `col` on: whole where they may be, else element by element up to `cols`.
@@ -367,10 +373,12 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
     }
   } else {
     // taking out: this warp's 32 rows (a quarter of tensor memory is a warp's by its number) and a part of the columns
-    constexpr int MINE = S::COLS / PARTS, CW = MINE < 32 || OUT == Out::BACK ? 16 : 32;   // BACK holds four values a column
+    constexpr int MINE = S::COLS / PARTS, CW = S::CW, ROW = PARTS * CW * 2;
     static_assert(MINE % CW == 0 && (CW == 16 || CW == 32), "a warp takes 16 or 32 columns at a time");
     const int quarter = warp & 3, part = (warp - 2) >> 2;
-    uint8_t* stage = smem + S::OUT_AT + (warp - 2) * OUT_BYTES;
+    uint8_t* rows = smem + S::OUT_AT + quarter * (S::OUT_BYTES / 4);          // of the four warps
+    uint8_t* stage = smem + S::OUT_AT + (warp - 2) * (S::OUT_BYTES / OUT_WARPS);   // of this one
+    auto meet = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory"); };
     const Epilogue& e = p.e;
     const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
     int done = 0;
@@ -379,7 +387,8 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&f.drained[set]));
     };
-    auto load = [&](uint32_t at, float (&v)[CW]) { tmem_ld_cols<CW>(at, *reinterpret_cast<uint32_t(*)[CW]>(&v)); };   // behind it: tmem_wait_ld
+    struct alignas(16) Cols { uint32_t bits[CW]; __device__ __forceinline__ F2 pair(int k) const { return f2(__uint_as_float(bits[2 * k]), __uint_as_float(bits[2 * k + 1])); } };
+    auto load = [&](uint32_t at, Cols& c) { tmem_ld_cols<CW>(at, c.bits); };   // behind it: tmem_wait_ld
     for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
       const Tile t = tile_of(p, i);
       uint32_t acc = lanes + (done & 1) * BN;
@@ -389,11 +398,11 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
           const int set = done & 1;
           wait(f.acc[set], done / 2, W_ACC);
           tc_fence_after();
-          // its share of the accumulators' columns, in GATE of both halves
+          // the columns that this warp takes out below, in GATE of both halves
 #pragma unroll 1
-          for (int c0 = part * (BN / PARTS); c0 < (part + 1) * (BN / PARTS); c0 += 8) {
+          for (int k0 = 0; k0 < BN / PARTS; k0 += 8) {
             uint32_t v[8], w[8];
-            const int c = OUT == Out::GATE ? (c0 - part * (BN / PARTS) < MINE ? part * MINE + (c0 - part * (BN / PARTS)) : BN / 2 + part * MINE + (c0 - part * (BN / PARTS) - MINE)) : c0;
+            const int in_half = k0 % MINE, c = (k0 / MINE) * S::COLS + (in_half / CW) * (PARTS * CW) + part * CW + in_half % CW;
             tmem_ld8_nowait(lanes + set * BN + c, v);
             if (s > s0) tmem_ld8_nowait(lanes + SUM + c, w);
             tmem_wait_ld();
@@ -410,23 +419,38 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
       }
       const int set = done & 1;
       const int64_t row0 = (int64_t)t.m * BM + 32 * quarter;
-      auto operand_out = [&](void* base_, int col0, float (&v)[CW]) {   // (pieces, m, ld_h)
+      // up to three operands (pieces, m, ld_h) from column `first` of the four warps' columns on
+      auto operands_out = [&](int first, auto&... pairs) {
 #pragma unroll
         for (int piece = 0; piece < PIECES; ++piece) {
-          E* to = static_cast<E*>(base_) + piece * e.piece_stride;
-          emit<E, CW>(stage, lane, v, [&](int r, int c, uint4 raw) {
-            if (row0 + r < p.m && col0 + c < e.ld_h) *reinterpret_cast<uint4*>(to + (row0 + r) * e.ld_h + col0 + c) = raw;
-          });
+          meet();   // what stood there is written
+          int at = 0;
+          (put_columns<E, CW>(rows + (at++) * 32 * ROW, part, lane, pairs.v), ...);
+          meet();
+          at = 0;
+          auto write = [&](void* to_) {
+            E* to = static_cast<E*>(to_) + piece * e.piece_stride;
+            take_rows<ROW>(rows + (at++) * 32 * ROW, part, lane, [&](int r, int c, uint4 raw) {
+              if (row0 + r < p.m && first + c < e.ld_h) *reinterpret_cast<uint4*>(to + (row0 + r) * e.ld_h + first + c) = raw;
+            });
+          };
+          (write(pairs.to), ...);
           if constexpr (PIECES > 1) {
+            auto rest = [](F2 (&v)[CW / 2]) {
 #pragma unroll
-            for (int k = 0; k < CW; ++k) {
-              E r;
-              down(r, v[k]);
-              v[k] -= up(r);
-            }
+              for (int k = 0; k < CW / 2; ++k) {
+                const float2 f = halves(v[k]);
+                E x, y;
+                down(x, f.x);
+                down(y, f.y);
+                v[k] = f2(f.x - up(x), f.y - up(y));
+              }
+            };
+            (rest(pairs.v), ...);
           }
         }
       };
+      struct To { F2 (&v)[CW / 2]; void* to; };
       // kept g and u: a block of 32 x 32 is eight requests of a float4 a lane, its row's
       auto kept_at = [&](float* base_, int col0, int q) {
         const int64_t block = (row0 >> 5) * ((e.ld_h + 31) >> 5) + (col0 >> 5);
@@ -439,70 +463,88 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
         tc_fence_after();
       };
 #pragma unroll 1
-      for (int c0 = part * MINE; c0 < (part + 1) * MINE; c0 += CW) {
-        const int col0 = t.n * S::COLS + c0;
-        if (col0 >= p.n) break;
-        const bool in = row0 < p.m, last = c0 + CW == (part + 1) * MINE || col0 + CW >= p.n;
+      for (int chunk = 0; chunk < MINE / CW; ++chunk) {
+        const int first = t.n * S::COLS + chunk * (PARTS * CW), c0 = chunk * (PARTS * CW) + part * CW, col0 = first + part * CW;
+        if (first >= p.n) break;
+        const bool in = row0 < p.m && col0 < p.n, last = chunk + 1 == MINE / CW || first + PARTS * CW >= p.n;
         auto taken = [&] {
           tmem_wait_ld();
           if (!EXACT && last) release(set), released = true;
         };
         if constexpr (OUT == Out::GATE || OUT == Out::BACK || OUT == Out::AGAIN) {
-          float g[CW], u[CW];
+          Cols g, u;
           if constexpr (OUT == Out::BACK) {
 #pragma unroll
             for (int q = 0; q < CW / 4; ++q) {
-              const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), gq = in ? *kept_at(e.g, col0, q) : zero, uq = in ? *kept_at(e.u, col0, q) : zero;
-              g[4 * q] = gq.x, g[4 * q + 1] = gq.y, g[4 * q + 2] = gq.z, g[4 * q + 3] = gq.w;
-              u[4 * q] = uq.x, u[4 * q + 1] = uq.y, u[4 * q + 2] = uq.z, u[4 * q + 3] = uq.w;
+              const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+              *reinterpret_cast<float4*>(&g.bits[4 * q]) = in ? *kept_at(e.g, col0, q) : zero;
+              *reinterpret_cast<float4*>(&u.bits[4 * q]) = in ? *kept_at(e.u, col0, q) : zero;
             }
           }
           ready();
-          float dh[CW], a[CW], da[CW];
           if constexpr (OUT != Out::BACK) {
             load(acc + c0, g);
             load(acc + S::COLS + c0, u);
           }
-          if constexpr (OUT != Out::GATE) load(acc + (OUT == Out::AGAIN ? 128 : 0) + c0, dh);
-          taken();
+          F2 h[CW / 2];
+          To th{h, e.h};
           if constexpr (OUT == Out::GATE) {
+            taken();
             if (e.g && in)
 #pragma unroll
               for (int q = 0; q < CW / 4; ++q) {
-                *kept_at(e.g, col0, q) = make_float4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
-                *kept_at(e.u, col0, q) = make_float4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
+                *kept_at(e.g, col0, q) = *reinterpret_cast<const float4*>(&g.bits[4 * q]);
+                *kept_at(e.u, col0, q) = *reinterpret_cast<const float4*>(&u.bits[4 * q]);
               }
-            activate<EXACT, false>(e.activation, g, a, da);
 #pragma unroll
-            for (int k = 0; k < CW; ++k) u[k] *= a[k];
-            operand_out(e.h, col0, u);
-          } else {
-            activate<EXACT, true>(e.activation, g, a, da);
-#pragma unroll
-            for (int k = 0; k < CW; ++k) {
-              da[k] *= dh[k] * u[k];   // dg
-              dh[k] *= a[k];           // du
-              a[k] *= u[k];            // h
+            for (int k = 0; k < CW / 2; ++k) {
+              F2 a, da;
+              activate<EXACT, false>(e.activation, g.pair(k), a, da);
+              h[k] = mul(a, u.pair(k));
             }
-            operand_out(e.h, col0, a);
-            operand_out(e.dg, col0, da);
-            operand_out(e.du, col0, dh);
+            operands_out(first, th);
+          } else {
+            Cols dh;
+            load(acc + (OUT == Out::AGAIN ? 128 : 0) + c0, dh);
+            taken();
+            F2 dg[CW / 2], du[CW / 2];
+#pragma unroll
+            for (int k = 0; k < CW / 2; ++k) {
+              F2 a, da;
+              activate<EXACT, true>(e.activation, g.pair(k), a, da);
+              dg[k] = mul(mul(dh.pair(k), u.pair(k)), da);
+              du[k] = mul(dh.pair(k), a);
+              h[k] = mul(a, u.pair(k));
+            }
+            To tg{dg, e.dg}, tu{du, e.du};
+            operands_out(first, th, tg, tu);
           }
         } else {
           ready();
-          float v[CW];
-          load(acc + c0, v);
+          Cols c;
+          load(acc + c0, c);
           taken();
-          auto rows_out = [&](auto* to, int64_t ld) {
-            using O = std::remove_pointer_t<decltype(to)>;
-            const bool wide = ld % (16 / (int)sizeof(O)) == 0;
-            emit<O, CW>(stage, lane, v, [&](int r, int c, uint4 raw) {
-              if (row0 + r < p.m) put16(to + (row0 + r) * ld, col0 + c, p.n, wide, raw);
+          F2 v[CW / 2];
+#pragma unroll
+          for (int k = 0; k < CW / 2; ++k) v[k] = c.pair(k);
+          auto floats_out = [&](float* to, int64_t ld) {
+            emit_floats<CW>(stage, lane, v, [&](int r, int c, uint4 raw) {
+              if (row0 + r < p.m) put16(to + (row0 + r) * ld, col0 + c, p.n, ld % 4 == 0, raw);
             });
           };
-          if constexpr (OUT == Out::PARTIAL) rows_out(e.part + (int64_t)(t.split * p.jobs + t.job) * p.m * p.n, p.n);
-          else if (e.out_kind == 0) rows_out(static_cast<float*>(e.out[t.job]), e.ld_out);
-          else rows_out(static_cast<E*>(e.out[t.job]), e.ld_out);
+          if constexpr (OUT == Out::PARTIAL) {
+            floats_out(e.part + (int64_t)(t.split * p.jobs + t.job) * p.m * p.n, p.n);
+          } else if (e.out_kind == 0) {
+            floats_out(static_cast<float*>(e.out[t.job]), e.ld_out);
+          } else {
+            E* to = static_cast<E*>(e.out[t.job]);
+            meet();
+            put_columns<E, CW>(rows, part, lane, v);
+            meet();
+            take_rows<ROW>(rows, part, lane, [&](int r, int c, uint4 raw) {
+              if (row0 + r < p.m) put16(to + (row0 + r) * e.ld_out, first + c, p.n, e.ld_out % 8 == 0, raw);
+            });
+          }
         }
       }
       if constexpr (!EXACT) {
