@@ -219,10 +219,10 @@ int check(const BnbGatedBlock* c) {
   return BNB_OK;
 }
 
-// Whether the backward computes g and u once more.  Kept in float32 they cost 16 bytes a row and hidden column, forward and backward,
-// which is 4 ps; computed, 28 clocks of a tile's 128 x 64 for each 64 of the width, 0.012 ps for each of it.  So up to a width of 384,
-// in 16 bits; float32 takes six times the products, and keeps.
-bool recomputes(const BnbGatedBlock& c) { return c.element != BNB_ELEM_F32 && c.width <= 384; }
+// Whether the backward computes g and u once more.  Kept in float32 they cost the same at any width, computing them costs with the width: for
+// 33.5 million rows x hidden columns, keeping takes 44 us more forward and 113 for the backward's launch, computing 64 at a width of 128
+// and 230 at 1024.  So up to 512, in 16 bits; float32 takes six times the products, and keeps.
+bool recomputes(const BnbGatedBlock& c) { return c.element != BNB_ELEM_F32 && c.width <= 512; }
 
 int64_t round32(int64_t v) { return (v + 31) / 32 * 32; }
 bool lies_well(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }

@@ -29,7 +29,8 @@ using namespace tensor;
 constexpr int BM = 128, BK = 64;              // tile rows; depth of a stage
 constexpr int MAX_TERMS = 12;                 // two segments of six
 constexpr int FLUSH = 4;                      // stages of a run
-constexpr int OUT_WARPS = 16, PARTS = OUT_WARPS / 4, CTA = 32 * (2 + OUT_WARPS);
+constexpr int OUT_WARPS = 16, CTA = 32 * (2 + OUT_WARPS);
+constexpr uint32_t OUT_BYTES = OUT_WARPS * 2048;   // shared memory of the results on their way out
 constexpr uint32_t A_BYTES = BM * BK * 2, SLAB = 64 * BK * 2;   // SLAB: 64 rows or columns by 64
 enum : int { W_FULL = 101, W_EMPTY = 102, W_ACC = 103, W_DRAINED = 104 };
 
@@ -178,52 +179,41 @@ template <int BN, Out OUT>
 struct Shape {
   static constexpr uint32_t B_BYTES = BN * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
   static constexpr int COLS = OUT == Out::GATE ? BN / 2 : OUT == Out::AGAIN ? BN / 3 : BN;   // of the output
-  // a warp that takes out holds CW columns of its rows at a time, the four warps of the same rows 4 CW neighbouring ones
-  static constexpr int CW = COLS / PARTS < 32 || OUT == Out::BACK ? 16 : 32;   // BACK holds four values a column
-  static constexpr uint32_t OUT_BYTES = 4 * 32 * (PARTS * CW * 2) * (OUT == Out::BACK || OUT == Out::AGAIN ? 3 : 1) < OUT_WARPS * 2048
-                                            ? OUT_WARPS * 2048 : 4 * 32 * (PARTS * CW * 2) * (OUT == Out::BACK || OUT == Out::AGAIN ? 3 : 1);
   static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_BYTES) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
   static constexpr uint32_t OUT_AT = STAGES * STAGE, FRAME = OUT_AT + OUT_BYTES, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
 };
 
-// Results to memory.  A lane has CW neighbouring columns of a row; a request that writes a little of many rows costs the load and store
-// unit as much as one that writes whole lines of each (32 bytes of 16 rows: 16 of its cycles, 4 rows of 128 bytes: 4).
-//
-// 16-bit: the four warps of the same 32 rows put their columns together in shared memory (rows of RB bytes, the 16-byte
-// pieces swizzled so that neither side meets a bank twice), then each writes whole rows: f(row, column, 16 bytes).
-template <int RB>
-__device__ __forceinline__ uint32_t row_piece(int r, int q) { return r * RB + ((q ^ (r & 7)) << 4); }
-template <typename E, int CW>
-__device__ __forceinline__ void put_columns(uint8_t* rows, int part, int lane, const F2 (&v)[CW / 2]) {
+// Results to memory: 32 rows of 64 columns at a time, a row a lane of PARTS warps.  A request that writes a little of many rows costs the load
+// and store unit as much as one that writes whole lines of each (32 bytes of 16 rows: 16 of its cycles, 128 bytes of 4 rows: 4).  So
+// the warps of the same rows put 16-bit results together in shared memory (rows of 128 bytes, the 16-byte pieces swizzled so that
+// neither side meets a bank twice), then each writes whole rows: f(row, column, 16 bytes).
+__device__ __forceinline__ uint32_t row_piece(int r, int q) { return r * 128 + ((q ^ (r & 7)) << 4); }
+template <int PARTS>
+__device__ __forceinline__ void put_columns(uint8_t* rows, int part, int lane, const uint32_t (&v)[32 / PARTS]) {
 #pragma unroll
-  for (int q = 0; q < CW / 8; ++q)
-    *reinterpret_cast<uint4*>(rows + row_piece<PARTS * CW * 2>(lane, part * (CW / 8) + q)) =
-        make_uint4(pair_of<E>(v[4 * q]), pair_of<E>(v[4 * q + 1]), pair_of<E>(v[4 * q + 2]), pair_of<E>(v[4 * q + 3]));
+  for (int q = 0; q < 8 / PARTS; ++q)
+    *reinterpret_cast<uint4*>(rows + row_piece(lane, part * (8 / PARTS) + q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
-template <int RB, class F>
+template <int PARTS, class F>
 __device__ __forceinline__ void take_rows(const uint8_t* rows, int part, int lane, F f) {
-  constexpr int PER = RB / 16, AT_ONCE = 32 / PER;   // lanes of a row, rows of a request
 #pragma unroll
-  for (int i = 0; i < 8 / AT_ONCE; ++i) {
-    const int r = 8 * part + i * AT_ONCE + lane / PER, q = lane % PER;
-    f(r, 8 * q, *reinterpret_cast<const uint4*>(rows + row_piece<RB>(r, q)));
+  for (int i = 0; i < 8 / PARTS; ++i) {
+    const int r = (32 / PARTS) * part + i * 4 + lane / 8, q = lane % 8;
+    f(r, 8 * q, *reinterpret_cast<const uint4*>(rows + row_piece(r, q)));
   }
 }
 // Float32: a warp for itself, 16 columns at a time.
-template <int CW, class F>
-__device__ __forceinline__ void emit_floats(uint8_t* stage, int lane, const F2 (&v)[CW / 2], F f) {
+template <class F>
+__device__ __forceinline__ void emit_floats(uint8_t* stage, int lane, const uint32_t (&v)[16], F f) {
   auto at = [](int r, int q) { return r * 64 + ((q ^ ((r >> 1) & 3)) << 4); };
+  __syncwarp();
 #pragma unroll
-  for (int h = 0; h < CW / 16; ++h) {
-    __syncwarp();
+  for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(stage + at(lane, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  __syncwarp();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) *reinterpret_cast<ulonglong2*>(stage + at(lane, q)) = make_ulonglong2(v[8 * h + 2 * q].v, v[8 * h + 2 * q + 1].v);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + lane / 4, q = lane % 4;
-      f(r, 16 * h + 4 * q, *reinterpret_cast<const uint4*>(stage + at(r, q)));
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + lane / 4, q = lane % 4;
+    f(r, 4 * q, *reinterpret_cast<const uint4*>(stage + at(r, q)));
   }
 }
 // The 16 bytes of a row from column `col` on: whole where they may be, else element by element up to `cols`.
@@ -239,10 +229,15 @@ __device__ __forceinline__ void put16(E* row, int col, int cols, bool wide, uint
   }
 }
 
+// Sixteen warps take out in two groups, tiles in turn: while one group waits for accumulators, for its rows or for memory, the other
+// computes.  (All sixteen on a tile at once wait together: 71 us for dh and its gradients at 65 536 x 128 x 512.)  Float32, whose runs need both
+// sets of accumulators for one tile, has one group, and so has BACK: it waits for g and u from memory most, and 16 columns a warp leave
+// the registers to have all of a segment's on their way at once (128 us against 113 at 8192 x 1024 x 4096).
 template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT>
 __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Product p) {
   using S = Shape<BN, OUT>;
   constexpr bool EXACT = PIECES > 1;
+  constexpr int GROUPS = EXACT || OUT == Out::BACK ? 1 : 2, PARTS = OUT_WARPS / 4 / GROUPS;
   static_assert(!EXACT || 3 * BN <= 512, "two sets of accumulators and their sum");
   constexpr uint32_t SUM = 2 * BN;   // float32: where runs are added
   extern __shared__ uint8_t raw_smem[];
@@ -260,7 +255,7 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&f.acc[i]), 1);
-      mbar_init(smem_u32(&f.drained[i]), OUT_WARPS);
+      mbar_init(smem_u32(&f.drained[i]), OUT_WARPS / GROUPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -372,24 +367,22 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
       }
     }
   } else {
-    // taking out: this warp's 32 rows (a quarter of tensor memory is a warp's by its number) and a part of the columns
-    constexpr int MINE = S::COLS / PARTS, CW = S::CW, ROW = PARTS * CW * 2;
-    static_assert(MINE % CW == 0 && (CW == 16 || CW == 32), "a warp takes 16 or 32 columns at a time");
-    const int quarter = warp & 3, part = (warp - 2) >> 2;
-    uint8_t* rows = smem + S::OUT_AT + quarter * (S::OUT_BYTES / 4);          // of the four warps
-    uint8_t* stage = smem + S::OUT_AT + (warp - 2) * (S::OUT_BYTES / OUT_WARPS);   // of this one
-    auto meet = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory"); };
+    // taking out: this warp's 32 rows (a quarter of tensor memory is a warp's by its number) and a part of every 64 columns
+    constexpr int SEG = 64 / PARTS;   // columns of a warp among 64
+    const int quarter = warp & 3, group = ((warp - 2) >> 2) % GROUPS, part = ((warp - 2) >> 2) / GROUPS;
+    uint8_t* rows = smem + S::OUT_AT + quarter * 8192 + group * 4096;      // of the warps that share rows
+    uint8_t* stage = smem + S::OUT_AT + (warp - 2) * 2048;                  // of this one
+    auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter * GROUPS + group), "n"(32 * PARTS) : "memory"); };
     const Epilogue& e = p.e;
     const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
-    int done = 0;
     auto release = [&](int set) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&f.drained[set]));
     };
-    struct alignas(16) Cols { uint32_t bits[CW]; __device__ __forceinline__ F2 pair(int k) const { return f2(__uint_as_float(bits[2 * k]), __uint_as_float(bits[2 * k + 1])); } };
-    auto load = [&](uint32_t at, Cols& c) { tmem_ld_cols<CW>(at, c.bits); };   // behind it: tmem_wait_ld
-    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+    auto pair = [](const uint32_t (&v)[8], int k) { return f2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])); };
+    int done = group, turn = 0;
+    for (int i = blockIdx.x + group * gridDim.x; i < tiles; i += GROUPS * gridDim.x) {
       const Tile t = tile_of(p, i);
       uint32_t acc = lanes + (done & 1) * BN;
       if constexpr (EXACT) {
@@ -398,11 +391,11 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
           const int set = done & 1;
           wait(f.acc[set], done / 2, W_ACC);
           tc_fence_after();
-          // the columns that this warp takes out below, in GATE of both halves
+          // the columns that this warp takes out below
 #pragma unroll 1
           for (int k0 = 0; k0 < BN / PARTS; k0 += 8) {
             uint32_t v[8], w[8];
-            const int in_half = k0 % MINE, c = (k0 / MINE) * S::COLS + (in_half / CW) * (PARTS * CW) + part * CW + in_half % CW;
+            const int c = (k0 / SEG) * 64 + part * SEG + k0 % SEG;
             tmem_ld8_nowait(lanes + set * BN + c, v);
             if (s > s0) tmem_ld8_nowait(lanes + SUM + c, w);
             tmem_wait_ld();
@@ -419,42 +412,10 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
       }
       const int set = done & 1;
       const int64_t row0 = (int64_t)t.m * BM + 32 * quarter;
-      // up to three operands (pieces, m, ld_h) from column `first` of the four warps' columns on
-      auto operands_out = [&](int first, auto&... pairs) {
-#pragma unroll
-        for (int piece = 0; piece < PIECES; ++piece) {
-          meet();   // what stood there is written
-          int at = 0;
-          (put_columns<E, CW>(rows + (at++) * 32 * ROW, part, lane, pairs.v), ...);
-          meet();
-          at = 0;
-          auto write = [&](void* to_) {
-            E* to = static_cast<E*>(to_) + piece * e.piece_stride;
-            take_rows<ROW>(rows + (at++) * 32 * ROW, part, lane, [&](int r, int c, uint4 raw) {
-              if (row0 + r < p.m && first + c < e.ld_h) *reinterpret_cast<uint4*>(to + (row0 + r) * e.ld_h + first + c) = raw;
-            });
-          };
-          (write(pairs.to), ...);
-          if constexpr (PIECES > 1) {
-            auto rest = [](F2 (&v)[CW / 2]) {
-#pragma unroll
-              for (int k = 0; k < CW / 2; ++k) {
-                const float2 f = halves(v[k]);
-                E x, y;
-                down(x, f.x);
-                down(y, f.y);
-                v[k] = f2(f.x - up(x), f.y - up(y));
-              }
-            };
-            (rest(pairs.v), ...);
-          }
-        }
-      };
-      struct To { F2 (&v)[CW / 2]; void* to; };
       // kept g and u: a block of 32 x 32 is eight requests of a float4 a lane, its row's
-      auto kept_at = [&](float* base_, int col0, int q) {
-        const int64_t block = (row0 >> 5) * ((e.ld_h + 31) >> 5) + (col0 >> 5);
-        return reinterpret_cast<float4*>(base_) + (block * 8 + ((col0 & 31) >> 2) + q) * 32 + lane;
+      auto kept_at = [&](float* base_, int col, int q) {
+        const int64_t block = (row0 >> 5) * ((e.ld_h + 31) >> 5) + (col >> 5);
+        return reinterpret_cast<float4*>(base_) + (block * 8 + ((col & 31) >> 2) + q) * 32 + lane;
       };
       // A tile's accumulators are waited for once, and given back as soon as the last of them are in registers.
       bool waited = EXACT, released = EXACT;
@@ -463,96 +424,133 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
         tc_fence_after();
       };
 #pragma unroll 1
-      for (int chunk = 0; chunk < MINE / CW; ++chunk) {
-        const int first = t.n * S::COLS + chunk * (PARTS * CW), c0 = chunk * (PARTS * CW) + part * CW, col0 = first + part * CW;
+      for (int c64 = 0; c64 < S::COLS; c64 += 64) {
+        const int first = t.n * S::COLS + c64, c0 = c64 + part * SEG, col0 = first + part * SEG;
         if (first >= p.n) break;
-        const bool in = row0 < p.m && col0 < p.n, last = chunk + 1 == MINE / CW || first + PARTS * CW >= p.n;
-        auto taken = [&] {
+        const bool in = row0 < p.m && col0 < p.n, last = c64 + 64 >= S::COLS || first + 64 >= p.n;
+        auto taken = [&](int k) {   // eight columns from k on are in registers
           tmem_wait_ld();
-          if (!EXACT && last) release(set), released = true;
+          if (!EXACT && last && k + 8 == SEG) release(set), released = true;
         };
+        uint4 kept[OUT == Out::BACK ? 2 : 1][SEG / 4];
+        if constexpr (OUT == Out::BACK) {
+#pragma unroll
+          for (int q = 0; q < SEG / 4; ++q) {
+            kept[0][q] = in ? *reinterpret_cast<const uint4*>(kept_at(e.g, col0, q)) : make_uint4(0u, 0u, 0u, 0u);
+            kept[1][q] = in ? *reinterpret_cast<const uint4*>(kept_at(e.u, col0, q)) : make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        ready();
         if constexpr (OUT == Out::GATE || OUT == Out::BACK || OUT == Out::AGAIN) {
-          Cols g, u;
-          if constexpr (OUT == Out::BACK) {
+          constexpr int N = OUT == Out::GATE ? 1 : 3;   // h; dg, du
+          using Held = std::conditional_t<EXACT, F2, uint32_t>;   // 16 bits: rounded at once
+          Held held[N][SEG / 2];
+          auto hold = [](Held& to, F2 v) {
+            if constexpr (EXACT) to = v;
+            else to = pair_of<E>(v);
+          };
 #pragma unroll
-            for (int q = 0; q < CW / 4; ++q) {
-              const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-              *reinterpret_cast<float4*>(&g.bits[4 * q]) = in ? *kept_at(e.g, col0, q) : zero;
-              *reinterpret_cast<float4*>(&u.bits[4 * q]) = in ? *kept_at(e.u, col0, q) : zero;
-            }
-          }
-          ready();
-          if constexpr (OUT != Out::BACK) {
-            load(acc + c0, g);
-            load(acc + S::COLS + c0, u);
-          }
-          F2 h[CW / 2];
-          To th{h, e.h};
-          if constexpr (OUT == Out::GATE) {
-            taken();
-            if (e.g && in)
+          for (int k0 = 0; k0 < SEG; k0 += 8) {
+            uint32_t g[8], u[8], dh[8];
+            if constexpr (OUT == Out::BACK) {
 #pragma unroll
-              for (int q = 0; q < CW / 4; ++q) {
-                *kept_at(e.g, col0, q) = *reinterpret_cast<const float4*>(&g.bits[4 * q]);
-                *kept_at(e.u, col0, q) = *reinterpret_cast<const float4*>(&u.bits[4 * q]);
+              for (int q = 0; q < 2; ++q) {
+                const uint4 gq = kept[0][k0 / 4 + q], uq = kept[1][k0 / 4 + q];
+                g[4 * q] = gq.x, g[4 * q + 1] = gq.y, g[4 * q + 2] = gq.z, g[4 * q + 3] = gq.w;
+                u[4 * q] = uq.x, u[4 * q + 1] = uq.y, u[4 * q + 2] = uq.z, u[4 * q + 3] = uq.w;
               }
-#pragma unroll
-            for (int k = 0; k < CW / 2; ++k) {
-              F2 a, da;
-              activate<EXACT, false>(e.activation, g.pair(k), a, da);
-              h[k] = mul(a, u.pair(k));
+            } else {
+              tmem_ld8_nowait(acc + c0 + k0, g);
+              tmem_ld8_nowait(acc + S::COLS + c0 + k0, u);
             }
-            operands_out(first, th);
-          } else {
-            Cols dh;
-            load(acc + (OUT == Out::AGAIN ? 128 : 0) + c0, dh);
-            taken();
-            F2 dg[CW / 2], du[CW / 2];
+            if constexpr (OUT != Out::GATE) tmem_ld8_nowait(acc + (OUT == Out::AGAIN ? 128 : 0) + c0 + k0, dh);
+            taken(k0);
+            if constexpr (OUT == Out::GATE) {
+              if (e.g && in)
 #pragma unroll
-            for (int k = 0; k < CW / 2; ++k) {
-              F2 a, da;
-              activate<EXACT, true>(e.activation, g.pair(k), a, da);
-              dg[k] = mul(mul(dh.pair(k), u.pair(k)), da);
-              du[k] = mul(dh.pair(k), a);
-              h[k] = mul(a, u.pair(k));
+                for (int q = 0; q < 2; ++q) {
+                  *reinterpret_cast<uint4*>(kept_at(e.g, col0 + k0, q)) = make_uint4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
+                  *reinterpret_cast<uint4*>(kept_at(e.u, col0 + k0, q)) = make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
+                }
             }
-            To tg{dg, e.dg}, tu{du, e.du};
-            operands_out(first, th, tg, tu);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              F2 a, da;
+              activate<EXACT, OUT != Out::GATE>(e.activation, pair(g, k), a, da);
+              hold(held[0][k0 / 2 + k], mul(a, pair(u, k)));
+              if constexpr (OUT != Out::GATE) {
+                hold(held[1][k0 / 2 + k], mul(mul(pair(dh, k), pair(u, k)), da));
+                hold(held[2][k0 / 2 + k], mul(pair(dh, k), a));
+              }
+            }
+          }
+          void* const to[3] = {e.h, e.dg, e.du};
+          // one group has room for two buffers in turn: then a buffer is free again when its warps have met over the other
+#pragma unroll
+          for (int o = 0; o < N; ++o) {
+#pragma unroll
+            for (int piece = 0; piece < PIECES; ++piece) {
+              uint8_t* buf = GROUPS == 1 ? rows + (turn++ & 1) * 4096 : rows;
+              if constexpr (GROUPS == 2) meet();   // what stood there is written
+              if constexpr (EXACT) {
+                uint32_t bits[SEG / 2];
+#pragma unroll
+                for (int k = 0; k < SEG / 2; ++k) {
+                  const float2 v = halves(held[o][k]);
+                  E x, y;
+                  down(x, v.x);
+                  down(y, v.y);
+                  bits[k] = pair_of(v.x, v.y, E{});
+                  held[o][k] = f2(v.x - up(x), v.y - up(y));
+                }
+                put_columns<PARTS>(buf, part, lane, bits);
+              } else {
+                put_columns<PARTS>(buf, part, lane, held[o]);
+              }
+              meet();
+              E* at = static_cast<E*>(to[o]) + piece * e.piece_stride;
+              take_rows<PARTS>(buf, part, lane, [&](int r, int c, uint4 raw) {
+                if (row0 + r < p.m && first + c < e.ld_h) *reinterpret_cast<uint4*>(at + (row0 + r) * e.ld_h + first + c) = raw;
+              });
+            }
           }
         } else {
-          ready();
-          Cols c;
-          load(acc + c0, c);
-          taken();
-          F2 v[CW / 2];
+          const bool floats = OUT == Out::PARTIAL || e.out_kind == 0;
+          uint32_t bits[SEG / 2];   // 16-bit results
 #pragma unroll
-          for (int k = 0; k < CW / 2; ++k) v[k] = c.pair(k);
-          auto floats_out = [&](float* to, int64_t ld) {
-            emit_floats<CW>(stage, lane, v, [&](int r, int c, uint4 raw) {
-              if (row0 + r < p.m) put16(to + (row0 + r) * ld, col0 + c, p.n, ld % 4 == 0, raw);
-            });
-          };
-          if constexpr (OUT == Out::PARTIAL) {
-            floats_out(e.part + (int64_t)(t.split * p.jobs + t.job) * p.m * p.n, p.n);
-          } else if (e.out_kind == 0) {
-            floats_out(static_cast<float*>(e.out[t.job]), e.ld_out);
-          } else {
+          for (int k0 = 0; k0 < SEG; k0 += 16) {
+            uint32_t v[16];
+            tmem_ld16_nowait(acc + c0 + k0, v);
+            tmem_wait_ld();
+            if (!EXACT && last && k0 + 16 == SEG) release(set), released = true;
+            if (floats) {
+              float* to = OUT == Out::PARTIAL ? e.part + (int64_t)(t.split * p.jobs + t.job) * p.m * p.n : static_cast<float*>(e.out[t.job]);
+              const int64_t ld = OUT == Out::PARTIAL ? p.n : e.ld_out;
+              emit_floats(stage, lane, v, [&](int r, int c, uint4 raw) {
+                if (row0 + r < p.m) put16(to + (row0 + r) * ld, col0 + k0 + c, p.n, ld % 4 == 0, raw);
+              });
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) bits[k0 / 2 + k] = pair_of(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]), E{});
+            }
+          }
+          if (!floats) {
             E* to = static_cast<E*>(e.out[t.job]);
             meet();
-            put_columns<E, CW>(rows, part, lane, v);
+            put_columns<PARTS>(rows, part, lane, bits);
             meet();
-            take_rows<ROW>(rows, part, lane, [&](int r, int c, uint4 raw) {
+            take_rows<PARTS>(rows, part, lane, [&](int r, int c, uint4 raw) {
               if (row0 + r < p.m) put16(to + (row0 + r) * e.ld_out, first + c, p.n, e.ld_out % 8 == 0, raw);
             });
           }
         }
       }
       if constexpr (!EXACT) {
-        if (!released) {   // no columns of this warp's part
+        if (!released) {   // no columns here
           ready();
           release(set);
         }
-        ++done;
+        done += GROUPS;
       }
     }
   }

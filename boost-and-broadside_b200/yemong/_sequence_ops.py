@@ -165,7 +165,7 @@ def gated_mlp(x: Tensor, gate_w: Tensor, up_w: Tensor, down_w: Tensor, activatio
 @gated_mlp.register_fake
 def _(x, gate_w, up_w, down_w, activation, keep):
     # as bnb_gated_block_kept_bytes: narrow 16-bit calls compute g and u once more and keep nothing
-    recomputes = x.dtype != torch.float32 and x.shape[-1] <= 384
+    recomputes = x.dtype != torch.float32 and x.shape[-1] <= 512
     rows = x.numel() // x.shape[-1]
     kept = 8 * ((rows + 31) // 32 * 32) * ((gate_w.shape[0] + 31) // 32 * 32)
     return x.new_empty(x.shape), x.new_empty(kept if keep and not recomputes else 0, dtype=torch.uint8)

@@ -146,11 +146,11 @@ def test_gated_block_checks_its_arguments():
     assert lib.bnb_gated_block_scratch_bytes(C.byref(c), 0) >= 100 * 128 * 2
     assert lib.bnb_gated_block_scratch_bytes(C.byref(c), 1) > lib.bnb_gated_block_scratch_bytes(C.byref(c), 0)
     assert lib.bnb_gated_block_kept_bytes(C.byref(c)) == 0                                        # narrow: computed once more
-    assert lib.bnb_gated_block_kept_bytes(C.byref(call(width=400))) == 2 * 128 * 128 * 4          # whole blocks of 32 x 32
+    assert lib.bnb_gated_block_kept_bytes(C.byref(call(width=600))) == 2 * 128 * 128 * 4          # whole blocks of 32 x 32
     g = GatedGrads(fake, 64, fake, fake, None, fake)
     assert lib.bnb_gated_block_bwd(C.byref(call(kept=fake)), C.byref(g), None, 0, None) == 1     # half of the gate's pair
     g = GatedGrads(fake, 64, fake, fake, fake, fake)
-    assert lib.bnb_gated_block_bwd(C.byref(call(width=400)), C.byref(g), None, 0, None) == 1     # nothing kept
+    assert lib.bnb_gated_block_bwd(C.byref(call(width=600)), C.byref(g), None, 0, None) == 1     # nothing kept
     assert lib.bnb_gated_block_bwd(C.byref(call(kept=fake)), C.byref(g), None, 0, None) == 6
 
 
