@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSel
         const float4 b4 = *reinterpret_cast<const float4*>(&b_s[t][NS * lane]);
         const float b[NS] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-        for (int i = 0; i < NS; ++i) h[i] = fmaf(ex2(p * rate[i]), h[i], pu * b[i]);
+        for (int i = 0; i < NS; ++i) h[i] = fmaf(ex2_fast(p * rate[i]), h[i], pu * b[i]);
         if (PASS == LOCAL) {
           sum_p += p;
         } else {
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(256) k_step(const __grid_constant__ BnbSelecti
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const bool has = WIDE ? real : n0 + i < q.states;
-        h[k][i] = fmaf(ex2(p * rate[i]), h[k][i], has ? pu * to_f(b[i]) : 0.f);
+        h[k][i] = fmaf(ex2_fast(p * rate[i]), h[k][i], has ? pu * to_f(b[i]) : 0.f);
         if (has) y = fmaf(to_f(cc[i]), h[k][i], y);
       }
 #pragma unroll

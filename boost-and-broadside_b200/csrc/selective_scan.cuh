@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256) k_join(float* local, const float* sum_p, 
     const int s = REVERSE ? count - 1 - k : k;
     const float left = local[s * cells + i];
     local[s * cells + i] = run;
-    run = (cut[(int64_t)s * rows + r] ? 0.f : ex2(rate * sum_p[s * (int64_t)rows * width + rc]) * run) + left;
+    run = (cut[(int64_t)s * rows + r] ? 0.f : ex2_fast(rate * sum_p[s * (int64_t)rows * width + rc]) * run) + left;
   }
 }
 

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL) k_scan_bwd(const __grid_con
           const float c[NS] = {c4.x, c4.y, c4.z, c4.w};
           sum_p += p;
 #pragma unroll
-          for (int i = 0; i < NS; ++i) carry[i] = (cuts >> t) & 1 ? 0.f : ex2(p * rate[i]) * fmaf(c[i], dy, carry[i]);
+          for (int i = 0; i < NS; ++i) carry[i] = (cuts >> t) & 1 ? 0.f : ex2_fast(p * rate[i]) * fmaf(c[i], dy, carry[i]);
         }
         __syncthreads();
       } else {
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL) k_scan_bwd(const __grid_con
           const float b[NS] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
           for (int i = 0; i < NS; ++i) {
-            e[t][i] = ex2(p * rate[i]);
+            e[t][i] = ex2_fast(p * rate[i]);
             h[t + 1][i] = fmaf(e[t][i], h[t][i], pu * b[i]);
             if (t + 1 < L && ((cuts >> (t + 1)) & 1)) h[t + 1][i] = 0.f;
           }
