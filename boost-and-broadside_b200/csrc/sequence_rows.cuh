@@ -7,8 +7,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "bnb_trunk.h"
-#include "tensor_common.cuh"   // pairs of floats in one instruction, fast exponential and reciprocal
+#include "tensor_common.cuh"   // fast exponential and reciprocal, pairs of floats in one instruction
 
 namespace bnb {
 namespace seq {
@@ -30,42 +32,77 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
-// N neighbouring elements, moved as one access when their bytes are 4, 8 or 16.
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <typename T> __device__ __forceinline__ uint32_t both(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t both<__nv_bfloat16>(float lo, float hi) { return tensor::pack_bf16(lo, hi); }
+template <> __device__ __forceinline__ uint32_t both<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// N neighbouring elements as they lie in memory, moved as one access of 2, 4, 8 or 16 bytes: words until they are used, so that what is on its
+// way takes no more registers than its bytes.
+template <int BYTES> struct Words { uint32_t w[BYTES / 4]; };
+template <> struct Words<2> { unsigned short w[1]; };
+template <typename T, int N> using Raw = Words<sizeof(T) * N>;
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack { T v[N]; };
+__device__ __forceinline__ Raw<T, N> load_raw(const T* at) {
+  Raw<T, N> r;
+  constexpr int B = sizeof(T) * N;
+  if constexpr (B == 2) r.w[0] = *reinterpret_cast<const unsigned short*>(at);
+  else if constexpr (B == 4) r.w[0] = *reinterpret_cast<const uint32_t*>(at);
+  else if constexpr (B == 8) { const uint2 v = *reinterpret_cast<const uint2*>(at); r.w[0] = v.x, r.w[1] = v.y; }
+  else { const uint4 v = *reinterpret_cast<const uint4*>(at); r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w; }
+  return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Raw<T, N>& r, float (&f)[N]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = __uint_as_float(r.w[i]);
+  } else if constexpr (N == 1) {
+    f[0] = to_f(*reinterpret_cast<const T*>(&r.w[0]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[2 * i] = tensor::bf16_lo(r.w[i]), f[2 * i + 1] = tensor::bf16_hi(r.w[i]);
+      } else {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+        f[2 * i] = v.x, f[2 * i + 1] = v.y;
+      }
+    }
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void load(const T* at, float (&f)[N]) { unpack<T, N>(load_raw<T, N>(at), f); }
+template <typename T, int N>
+__device__ __forceinline__ void store(T* at, const float (&f)[N]) {
+  if constexpr (N == 1) {
+    *at = from_f<T>(f[0]);
+  } else {
+    constexpr int W = sizeof(T) * N / 4;
+    uint32_t w[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+      else w[i] = both<T>(f[2 * i], f[2 * i + 1]);
+    }
+    if constexpr (W == 1) *reinterpret_cast<uint32_t*>(at) = w[0];
+    else if constexpr (W == 2) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+    else
+#pragma unroll
+      for (int i = 0; i < W; i += 4) *reinterpret_cast<uint4*>(at + i * 4 / sizeof(T)) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  }
+}
 
 // 1 / (1 + e^-v).  Results of 16-bit calls are rounded to 11 bits or fewer, where the fast exponential and division
 // (2 units in the last place of 24 each, for arguments that matter) are far below the rounding; float32 calls take the exact ones.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float v) {
-  if constexpr (sizeof(T) == 2) return __fdividef(1.0f, 1.0f + __expf(-v));
+  if constexpr (sizeof(T) == 2) return rcp_fast(1.0f + ex2_fast(v * -LOG2E));
   return 1.0f / (1.0f + expf(-v));
-}
-constexpr float LOG2E = 1.4426950408889634f;
-
-// N neighbouring elements as pairs of floats, and back.  One element alone has a partner that is never stored.
-template <int N> constexpr int PAIRS = (N + 1) / 2;
-template <typename T, int N>
-__device__ __forceinline__ void unpack(const Pack<T, N>& p, F2 (&f)[PAIRS<N>]) {
-#pragma unroll
-  for (int i = 0; i < PAIRS<N>; ++i) f[i] = f2(to_f(p.v[2 * i]), 2 * i + 1 < N ? to_f(p.v[2 * i + 1 < N ? 2 * i + 1 : 0]) : 0.f);
-}
-template <int N, typename T>
-__device__ __forceinline__ void store(T* at, const F2 (&f)[PAIRS<N>]) {
-  Pack<T, N> p;
-#pragma unroll
-  for (int i = 0; i < N; ++i) p.v[i] = from_f<T>(i & 1 ? halves(f[i / 2]).y : halves(f[i / 2]).x);
-  *reinterpret_cast<Pack<T, N>*>(at) = p;
-}
-// sigmoid of a pair
-template <typename T>
-__device__ __forceinline__ F2 sigmoid(F2 v) {
-  if constexpr (sizeof(T) == 4) {
-    const float2 s = halves(v);
-    return f2(sigmoid<float>(s.x), sigmoid<float>(s.y));
-  }
-  const float2 m = halves(mul(v, f2(-LOG2E))), den = halves(add(f2(ex2_fast(m.x), ex2_fast(m.y)), f2(1.0f)));
-  return f2(rcp_fast(den.x), rcp_fast(den.y));
 }
 
 // Steps of row r that are looked at.
