@@ -190,54 +190,88 @@ __global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSel
   }
 }
 
-// One token a row.  A thread keeps the constants of its channel's states and goes over rows ROWS at a time, so that their
-// states are in flight together.
+// Four b or c of a lane as they lie: one access where that is on its boundary.
+template <typename T>
+__device__ __forceinline__ Raw<T, NS> load_shared(const T* at, int n0, int states, bool whole) {
+  if (whole) return load_raw<T, NS>(at + n0);
+  Raw<T, NS> r;
+  T* v = reinterpret_cast<T*>(r.w);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) v[i] = n0 + i < states ? at[n0 + i] : from_f<T>(0.f);
+  return r;
+}
+
+// One token a row.  A thread keeps the constants of its channel's states and goes over rows ROWS at a time, whose loads are on their way
+// together.  What is per channel and row (step size, gate, output) is computed by one of the channel's lanes for each row and passed on.
 template <typename T, int KL, int ROWS, bool WIDE>
-__global__ void __launch_bounds__(256) k_step(const __grid_constant__ BnbSelectiveScan q) {
+__global__ void __launch_bounds__(256, 3) k_step(const __grid_constant__ BnbSelectiveScan q, bool whole) {
   constexpr int BITS = KL == 1 ? 0 : KL == 2 ? 1 : KL == 4 ? 2 : KL == 8 ? 3 : 4;
+  constexpr int PER = ROWS > KL ? ROWS / KL : 1, SHARE = KL > ROWS ? KL / ROWS : 1;   // rows of a lane, lanes of a row
   const int lane = threadIdx.x % KL, ch = blockIdx.y * (256 / KL) + threadIdx.x / KL;
   const bool on = ch < q.width;
   const int c = on ? ch : 0, group = c / (q.width / q.groups), n0 = NS * lane;
-  float rate[NS];
-  load_states(rate, q.a + (int64_t)c * q.states, n0, q.states, WIDE);
-#pragma unroll
-  for (int i = 0; i < NS; ++i) rate[i] *= LOG2E;
+  float rate_[NS];
+  load_states(rate_, q.a + (int64_t)c * q.states, n0, q.states, WIDE && n0 < q.states);
+  const F2 rate[2] = {mul(f2(rate_[0], rate_[1]), f2(LOG2E)), mul(f2(rate_[2], rate_[3]), f2(LOG2E))};
   const float bias = q.delta_bias ? q.delta_bias[c] : 0.f, skip = q.d ? q.d[c] : 0.f;
-  const bool real = n0 < q.states;
+  const bool real = on && n0 < q.states;
+  const int first = KL > ROWS ? lane / SHARE : lane * PER;   // this lane's rows among ROWS
   for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < q.rows; r0 += (int64_t)gridDim.x * ROWS) {
     float h[ROWS][NS];
+    Raw<T, NS> b[ROWS], cc[ROWS];
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      const int64_t r = r0 + k;
+      const int64_t r = min(r0 + k, (int64_t)q.rows - 1);
 #pragma unroll
       for (int i = 0; i < NS; ++i) h[k][i] = 0.f;
-      if (r < q.rows && on && real && q.state_in && !(q.reset && q.reset[r])) load_states(h[k], q.state_in + (r * q.width + c) * q.states, n0, q.states, WIDE);
+      if (real && q.state_in && !(q.reset && q.reset[r])) load_states(h[k], q.state_in + (r * q.width + c) * q.states, n0, q.states, WIDE);
+    }
+    float u[PER], p[PER], gate[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int64_t r = min(r0 + first + k, (int64_t)q.rows - 1);
+      u[k] = to_f(static_cast<const T*>(q.u.data)[r * q.u.row + c]);
+      p[k] = to_f(static_cast<const T*>(q.delta.data)[r * q.delta.row + c]);
+      gate[k] = q.z.data ? to_f(static_cast<const T*>(q.z.data)[r * q.z.row + c]) : 0.f;
     }
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      const int64_t r = r0 + k;
-      if (r >= q.rows) break;
-      const float u = to_f(static_cast<const T*>(q.u.data)[r * q.u.row + c]);
-      const float p = step_size(to_f(static_cast<const T*>(q.delta.data)[r * q.delta.row + c]) + bias, q.softplus), pu = p * u;
-      const T* b = static_cast<const T*>(q.b.data) + r * q.b.row + group * q.b.group + n0;
-      const T* cc = static_cast<const T*>(q.c.data) + r * q.c.row + group * q.c.group + n0;
-      float y = 0.f;
+      const int64_t r = min(r0 + k, (int64_t)q.rows - 1);
+      b[k] = load_shared(static_cast<const T*>(q.b.data) + r * q.b.row + group * q.b.group, n0, q.states, whole && n0 < q.states);
+      cc[k] = load_shared(static_cast<const T*>(q.c.data) + r * q.c.row + group * q.c.group, n0, q.states, whole && n0 < q.states);
+    }
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const bool has = WIDE ? real : n0 + i < q.states;
-        h[k][i] = fmaf(ex2_fast(p * rate[i]), h[k][i], has ? pu * to_f(b[i]) : 0.f);
-        if (has) y = fmaf(to_f(cc[i]), h[k][i], y);
+    for (int k = 0; k < PER; ++k) {
+      p[k] = step_size(p[k] + bias, q.softplus);
+      gate[k] = q.z.data ? gate[k] * sigmoid<T>(gate[k]) : 1.f;
+    }
+    float y[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int from = (threadIdx.x & 31 & ~(KL - 1)) + (KL > ROWS ? k * SHARE : k / PER);
+      const float pk = __shfl_sync(0xffffffffu, p[k % PER], from), pu = __shfl_sync(0xffffffffu, p[k % PER] * u[k % PER], from);
+      F2 sum = f2(0.f);
+      float bf[NS], cf[NS];
+      unpack<T, NS>(b[k], bf);
+      unpack<T, NS>(cc[k], cf);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 m = halves(mul(f2(pk), rate[i]));
+        const F2 v = fma(f2(ex2_fast(m.x), ex2_fast(m.y)), f2(h[k][2 * i], h[k][2 * i + 1]), mul(f2(pu), f2(bf[2 * i], bf[2 * i + 1])));
+        sum = fma(f2(cf[2 * i], cf[2 * i + 1]), v, sum);
+        const float2 o = halves(v);
+        h[k][2 * i] = o.x, h[k][2 * i + 1] = o.y;
       }
+      const float2 o = halves(sum);
+      y[k] = o.x + o.y;
+      if (real && r0 + k < q.rows) store_states(q.state_out + ((r0 + k) * q.width + c) * q.states, h[k], n0, q.states, WIDE);
+    }
+    sum_lanes<ROWS, 0, BITS>(y);   // this lane's rows' sums stand in front
+    if (on && writes_sum<ROWS, 0, BITS>()) {
 #pragma unroll
-      for (int o = 1; o < KL; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-      if (on && real) store_states(q.state_out + (r * q.width + c) * q.states, h[k], n0, q.states, WIDE);
-      if (on && lane == 0) {
-        y = fmaf(skip, u, y);
-        if (q.z.data) {
-          const float z = to_f(static_cast<const T*>(q.z.data)[r * q.z.row + c]);
-          y *= z * sigmoid<T>(z);
-        }
-        static_cast<T*>(q.y.data)[r * q.y.row + c] = from_f<T>(y);
+      for (int k = 0; k < PER; ++k) {
+        const int64_t r = r0 + first + k;
+        if (r < q.rows) static_cast<T*>(q.y.data)[r * q.y.row + c] = from_f<T>(fmaf(skip, u[k], y[k]) * gate[k]);
       }
     }
   }
@@ -292,16 +326,18 @@ int launch_step(const BnbSelectiveScan& a, cudaStream_t st) {
   constexpr int ROWS = 4;
   const int tiles = (a.width * KL + 255) / 256;
   if (tiles > 65535) return BNB_ERR_UNSUPPORTED_DIMS;
-  const int64_t groups = (a.rows + ROWS - 1) / ROWS, fit = std::max(1, 148 * 8 / tiles);
+  const int64_t groups = (a.rows + ROWS - 1) / ROWS, fit = std::max(1, 148 * 3 / tiles);
+  auto on = [&](const BnbView& v) { return reinterpret_cast<uintptr_t>(v.data) % (4 * sizeof(T)) == 0 && v.row % 4 == 0 && v.group % 4 == 0; };
+  const bool wide = a.states % NS == 0, whole = wide && on(a.b) && on(a.c);
   count_launch();
   if (groups < fit) {   // fewer rows than it takes to fill the chip: one each
-    const dim3 grid((unsigned)std::min<int64_t>(a.rows, fit), tiles);
-    if (a.states % NS == 0) k_step<T, KL, 1, true><<<grid, 256, 0, st>>>(a);
-    else k_step<T, KL, 1, false><<<grid, 256, 0, st>>>(a);
+    const dim3 grid((unsigned)a.rows, tiles);
+    if (wide) k_step<T, KL, 1, true><<<grid, 256, 0, st>>>(a, whole);
+    else k_step<T, KL, 1, false><<<grid, 256, 0, st>>>(a, whole);
   } else {
     const dim3 grid((unsigned)fit, tiles);
-    if (a.states % NS == 0) k_step<T, KL, ROWS, true><<<grid, 256, 0, st>>>(a);
-    else k_step<T, KL, ROWS, false><<<grid, 256, 0, st>>>(a);
+    if (wide) k_step<T, KL, ROWS, true><<<grid, 256, 0, st>>>(a, whole);
+    else k_step<T, KL, ROWS, false><<<grid, 256, 0, st>>>(a, whole);
   }
   return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;
 }
