@@ -37,14 +37,18 @@ struct Work {
   uint8_t* cut;       // (splits, rows)
   Splits splits;
   int tiles_a_group;
+  bool paired;        // pairs of channels of u, delta, z and y lie on their boundary
 };
 
 template <typename T, int KL, Pass PASS>
-__global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSelectiveScan q, Work w) {
-  constexpr int THREADS = CT * KL, NP = NS * KL, PER = L / KL;   // elements a thread prepares of every (L, CT) array
-  constexpr int BC = (L * NP + THREADS - 1) / THREADS;           // and of b and c
-  __shared__ float p_s[L][CT], pu_s[L][CT], y_s[PASS == LOCAL ? 1 : L][CT];
-  __shared__ __align__(16) float b_s[L][NP], c_s[PASS == LOCAL ? 1 : L][NP];
+__global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSelectiveScan q, const __grid_constant__ Work w) {
+  constexpr int THREADS = CT * KL, NP = NS * KL;
+  constexpr int BC = (L * NP + THREADS - 1) / THREADS;            // elements of b and c that a thread fetches
+  constexpr int PAIRS = CT / 2, AT_ONCE = THREADS / PAIRS < L ? THREADS / PAIRS : L, PER = L / AT_ONCE;   // steps prepared at a time, by a thread
+  constexpr int SUMS = KL < 4 ? KL : 4;                           // parts that y is left in
+  constexpr bool Y = PASS != LOCAL;
+  __shared__ __align__(16) float4 pp_s[L][CT];                    // p, p, p u, p u
+  __shared__ __align__(16) float b_s[L][NP], c_s[Y ? L : 1][NP], y_s[Y ? L : 1][CT][SUMS];
   const int tid = threadIdx.x, cl = tid / KL, lane = tid % KL;
   const int tiles = w.tiles_a_group * q.groups, share = q.width / q.groups;
   const int r = blockIdx.x / tiles, tile = blockIdx.x - r * tiles, group = tile / w.tiles_a_group;
@@ -52,74 +56,92 @@ __global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSel
   const int ch = c0 + cl;
   const bool owns = ch < c_end, wide = q.states % NS == 0;
   const int n = row_steps(q.lengths, r, q.steps);
-  const int split = blockIdx.y, first = split * w.splits.steps, last = min(q.steps, first + w.splits.steps);
+  const int split = blockIdx.y, first = split * w.splits.steps, last = min(q.steps, first + w.splits.steps), live = min(n, last);
   const int64_t rc = (int64_t)r * q.width + ch;
 
-  float rate[NS], h[NS];
-#pragma unroll
-  for (int i = 0; i < NS; ++i) rate[i] = h[i] = 0.f;
+  F2 rate[2] = {f2(0.f), f2(0.f)}, h[2] = {f2(0.f), f2(0.f)};
+  auto state = [&](float (&v)[NS]) {
+    const float2 x = halves(h[0]), z = halves(h[1]);
+    v[0] = x.x, v[1] = x.y, v[2] = z.x, v[3] = z.y;
+  };
   if (owns) {
-    load_states(rate, q.a + (int64_t)ch * q.states, NS * lane, q.states, wide);
-#pragma unroll
-    for (int i = 0; i < NS; ++i) rate[i] *= LOG2E;
+    float v[NS];
+    load_states(v, q.a + (int64_t)ch * q.states, NS * lane, q.states, wide && NS * lane < q.states);
+    rate[0] = mul(f2(v[0], v[1]), f2(LOG2E));
+    rate[1] = mul(f2(v[2], v[3]), f2(LOG2E));
+    clear_states(v);
     if constexpr (PASS == WHOLE) {
-      if (q.state_in) load_states(h, q.state_in + rc * q.states, NS * lane, q.states, wide);
+      if (q.state_in) load_states(v, q.state_in + rc * q.states, NS * lane, q.states, wide && NS * lane < q.states);
     } else if constexpr (PASS == JOINED) {
-      load_states(h, w.local + ((int64_t)split * q.rows * q.width + rc) * NP, NS * lane, NP, true);
+      load_states(v, w.local + ((int64_t)split * q.rows * q.width + rc) * NP, NS * lane, NP, true);
     }
+    h[0] = f2(v[0], v[1]);
+    h[1] = f2(v[2], v[3]);
   }
 
-  // what this thread prepares: steps t0 + tid / CT + k KL of channel c0 + tid % CT
-  const int pc = tid % CT, pt = tid / CT;
-  const bool prepares = c0 + pc < c_end;
-  const float bias = prepares && q.delta_bias ? q.delta_bias[c0 + pc] : 0.f, skip = prepares && q.d ? q.d[c0 + pc] : 0.f;
-  const T* up = static_cast<const T*>(q.u.data) + r * q.u.row + c0 + pc;
-  const T* dp = static_cast<const T*>(q.delta.data) + r * q.delta.row + c0 + pc;
-  const T* zp = static_cast<const T*>(q.z.data) + r * q.z.row + c0 + pc;
-  const T* bp = static_cast<const T*>(q.b.data) + r * q.b.row + group * q.b.group;
-  const T* cp = static_cast<const T*>(q.c.data) + r * q.c.row + group * q.c.group;
-  T* yp = static_cast<T*>(q.y.data) + r * q.y.row + c0 + pc;
+  // what this thread prepares: channels c0 + 2 pair, + 1 of steps t0 + step + k AT_ONCE
+  const int pair = tid % PAIRS, step = tid / PAIRS, count = step < L ? max(0, min(2, c_end - (c0 + 2 * pair))) : 0, pc = c0 + 2 * pair;
+  F2 bias = f2(0.f), skip = f2(0.f);
+  if (q.delta_bias) bias = f2(count > 0 ? q.delta_bias[pc] : 0.f, count > 1 ? q.delta_bias[pc + 1] : 0.f);
+  if (q.d) skip = f2(count > 0 ? q.d[pc] : 0.f, count > 1 ? q.d[pc + 1] : 0.f);
+  const T* up = static_cast<const T*>(q.u.data) + r * q.u.row + pc + (first + step) * q.u.step;
+  const T* dp = static_cast<const T*>(q.delta.data) + r * q.delta.row + pc + (first + step) * q.delta.step;
+  const T* zp = static_cast<const T*>(q.z.data) + r * q.z.row + pc + (first + step) * q.z.step;
+  T* yp = static_cast<T*>(q.y.data) + r * q.y.row + pc + (first + step) * q.y.step;
+  const T* bp = static_cast<const T*>(q.b.data) + r * q.b.row + group * q.b.group + first * q.b.step;
+  const T* cp = static_cast<const T*>(q.c.data) + r * q.c.row + group * q.c.group + first * q.c.step;
+  float* kept = q.kept && owns ? q.kept + ((int64_t)(first / KEEP) * q.rows * q.width + rc) * NP : nullptr;
+  const int64_t kept_step = (int64_t)q.rows * q.width * NP;
   const bool gated = q.z.data != nullptr;
   const T none = from_f<T>(0.f);
-  T u_r[PER], d_r[PER], z_r[PER], b_r[BC], c_r[BC];
-  unsigned cuts = 0, cuts_next = 0;   // bit k: an episode ended before step t0 + k
-  auto fetch = [&](int t0) {
+  Raw<T, 2> u_r[PER], d_r[PER], z_r[PER];
+  T b_r[BC], c_r[BC];
+  unsigned cuts_next = 0;   // bit k: an episode ended before step t0 + k
+  auto fetch = [&](int t0) {   // moves the pointers on
     if (q.done) {
       const int t = t0 + (tid & 31) - 1;
       cuts_next = __ballot_sync(0xffffffffu, (tid & 31) < L && t >= 0 && t + 1 < n && q.done[(int64_t)max(t, 0) * q.rows + r]);
     }
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int t = t0 + pt + k * KL;
-      const bool on = prepares && t < min(n, last);
-      u_r[k] = on ? up[t * q.u.step] : none;
-      d_r[k] = on ? dp[t * q.delta.step] : none;
-      z_r[k] = PASS != LOCAL && gated && on ? zp[t * q.z.step] : none;
+      const int have = t0 + step + k * AT_ONCE < live ? count : 0;
+      u_r[k] = load_pair(up + k * AT_ONCE * q.u.step, have, w.paired);
+      d_r[k] = load_pair(dp + k * AT_ONCE * q.delta.step, have, w.paired);
+      z_r[k] = load_pair(zp + k * AT_ONCE * q.z.step, Y && gated ? have : 0, w.paired);
     }
 #pragma unroll
     for (int k = 0; k < BC; ++k) {
-      const int e = tid + k * THREADS, t = t0 + e / NP, s = e % NP;
-      const bool on = e < L * NP && s < q.states && t < min(n, last);
+      const int e = tid + k * THREADS, t = e / NP, s = e % NP;
+      const bool on = e < L * NP && s < q.states && t0 + t < live;
       b_r[k] = on ? bp[t * q.b.step + s] : none;
-      if (PASS != LOCAL) c_r[k] = on ? cp[t * q.c.step + s] : none;
+      if (Y) c_r[k] = on ? cp[t * q.c.step + s] : none;
     }
+    up += L * q.u.step;
+    dp += L * q.delta.step;
+    zp += L * q.z.step;
+    bp += L * q.b.step;
+    cp += L * q.c.step;
   };
   float sum_p = 0.f;
   bool any_cut = false;
-  const int live = min(n, last);
   if (first < live) fetch(first);
 #pragma unroll 1
   for (int t0 = first; t0 < live; t0 += L) {
-    float u_f[PER], gate[PER];
+    F2 u_f[PER], gate[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      u_f[k] = to_f(u_r[k]);
-      const float p = t0 + pt + k * KL < live ? step_size(to_f(d_r[k]) + bias, q.softplus) : 0.f;
-      p_s[pt + k * KL][pc] = p;
-      pu_s[pt + k * KL][pc] = p * u_f[k];
-      if (PASS != LOCAL) {
-        const float z = to_f(z_r[k]);
-        gate[k] = gated ? z * sigmoid<T>(z) : 1.f;
+      u_f[k] = floats_of<T>(u_r[k]);
+      const int t = step + k * AT_ONCE;
+      F2 p = step_size(add(floats_of<T>(d_r[k]), bias), q.softplus);
+      if (t0 + t >= live) p = f2(0.f);
+      if (Y) {
+        const F2 z = floats_of<T>(z_r[k]);
+        gate[k] = gated ? mul(z, sigmoid_pair<T>(z)) : f2(1.0f);
+      }
+      if (step < L) {
+        const float2 ps = halves(p), pu = halves(mul(p, u_f[k]));
+        pp_s[t][2 * pair] = make_float4(ps.x, ps.x, pu.x, pu.x);
+        pp_s[t][2 * pair + 1] = make_float4(ps.y, ps.y, pu.y, pu.y);
       }
     }
 #pragma unroll
@@ -127,66 +149,73 @@ __global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSel
       const int e = tid + k * THREADS;
       if (e < L * NP) {
         (&b_s[0][0])[e] = to_f(b_r[k]);
-        if (PASS != LOCAL) (&c_s[0][0])[e] = to_f(c_r[k]);
+        if (Y) (&c_s[0][0])[e] = to_f(c_r[k]);
       }
     }
-    cuts = cuts_next;
+    const unsigned cuts = cuts_next;
     any_cut |= cuts != 0;
     __syncthreads();
     if (t0 + L < live) fetch(t0 + L);
-    constexpr int GROUP = KL > 4 ? KL : 4;
 #pragma unroll 1
-    for (int g0 = 0; g0 < L; g0 += GROUP) {
-      float y[GROUP];
-#pragma unroll
-      for (int k = 0; k < GROUP; ++k) {
-        const int t = g0 + k;
-        if (PASS != LOCAL && t % KEEP == 0 && q.kept && owns && t0 + t < live)
-          store_states(q.kept + ((int64_t)((t0 + t) / KEEP) * q.rows * q.width + rc) * NP, h, NS * lane, NP, true);
-        if ((cuts >> t) & 1) {
-#pragma unroll
-          for (int i = 0; i < NS; ++i) h[i] = 0.f;
-        }
-        const float p = p_s[t][cl], pu = pu_s[t][cl];
-        const float4 b4 = *reinterpret_cast<const float4*>(&b_s[t][NS * lane]);
-        const float b[NS] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-        for (int i = 0; i < NS; ++i) h[i] = fmaf(ex2_fast(p * rate[i]), h[i], pu * b[i]);
-        if (PASS == LOCAL) {
-          sum_p += p;
-        } else {
-          const float4 c4 = *reinterpret_cast<const float4*>(&c_s[t][NS * lane]);
-          y[k] = fmaf(c4.x, h[0], c4.y * h[1]) + fmaf(c4.z, h[2], c4.w * h[3]);
-        }
+    for (int g0 = 0; g0 < L; g0 += KEEP) {
+      if (Y && kept && t0 + g0 < live) {
+        float v[NS];
+        state(v);
+        store_states(kept, v, NS * lane, NP, true);
+        kept += kept_step;
       }
-      if constexpr (PASS != LOCAL) {
-        constexpr int BITS = KL == 1 ? 0 : KL == 2 ? 1 : KL == 4 ? 2 : KL == 8 ? 3 : 4;
-        const int at = sum_lanes<GROUP, 0, BITS>(y);
 #pragma unroll
-        for (int k = 0; k < (GROUP >> BITS); ++k) y_s[g0 + at + k][cl] = y[k];
+      for (int k = 0; k < KEEP; ++k) {
+        const int t = g0 + k;
+        if ((cuts >> t) & 1) {
+          h[0] = h[1] = f2(0.f);
+          asm volatile("");   // rare, and the same for all: worth a branch
+        }
+        const ulonglong2 pp = *reinterpret_cast<const ulonglong2*>(&pp_s[t][cl]), b = *reinterpret_cast<const ulonglong2*>(&b_s[t][NS * lane]);
+        const F2 p{pp.x}, pu{pp.y};
+        const float2 m0 = halves(mul(p, rate[0])), m1 = halves(mul(p, rate[1]));
+        h[0] = fma(f2(ex2_fast(m0.x), ex2_fast(m0.y)), h[0], mul(pu, F2{b.x}));
+        h[1] = fma(f2(ex2_fast(m1.x), ex2_fast(m1.y)), h[1], mul(pu, F2{b.y}));
+        if constexpr (!Y) {
+          sum_p += halves(p).x;
+        } else {
+          const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&c_s[t][NS * lane]);
+          const float2 both = halves(fma(F2{c.x}, h[0], mul(F2{c.y}, h[1])));
+          float y = both.x + both.y;
+#pragma unroll
+          for (int o = SUMS; o < KL; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+          if (KL <= SUMS || lane < SUMS) y_s[t][cl][lane % SUMS] = y;
+        }
       }
     }
     __syncthreads();
-    if constexpr (PASS != LOCAL) {
+    if constexpr (Y) {
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int t = t0 + pt + k * KL;
-        if (prepares && t < live) yp[t * q.y.step] = from_f<T>(fmaf(skip, u_f[k], y_s[pt + k * KL][pc]) * gate[k]);
+        const int t = step + k * AT_ONCE;
+        if (t0 + t >= live || step >= L) continue;
+        float2 y = make_float2(y_s[t][2 * pair][0], y_s[t][2 * pair + 1][0]);
+#pragma unroll
+        for (int i = 1; i < SUMS; ++i) y.x += y_s[t][2 * pair][i], y.y += y_s[t][2 * pair + 1][i];
+        store_pair(yp + k * AT_ONCE * q.y.step, mul(fma(skip, u_f[k], f2(y.x, y.y)), gate[k]), count, w.paired);
       }
+      yp += L * q.y.step;
     }
   }
-  if constexpr (PASS == LOCAL) {
+  float v[NS];
+  state(v);
+  if constexpr (!Y) {
     if (owns) {
-      store_states(w.local + ((int64_t)split * q.rows * q.width + rc) * NP, h, NS * lane, NP, true);
+      store_states(w.local + ((int64_t)split * q.rows * q.width + rc) * NP, v, NS * lane, NP, true);
       if (lane == 0) w.sum_p[(int64_t)split * q.rows * q.width + rc] = sum_p;
     }
     if (tid == 0 && tile == 0) w.cut[(int64_t)split * q.rows + r] = any_cut;
   } else {
-    if (prepares)
-      for (int t = max(first, n) + pt; t < last; t += KL) yp[t * q.y.step] = none;
+    yp = static_cast<T*>(q.y.data) + r * q.y.row + pc;
+    for (int t = max(first, n) + step; step < L && t < last; t += AT_ONCE) store_pair(yp + t * q.y.step, f2(0.f), count, w.paired);
     // the split that holds the row's last step has its state; a row without steps, the first one
     if (owns && q.state_out && ((first < n && n <= last) || (n == 0 && split == 0)))
-      store_states(q.state_out + rc * q.states, h, NS * lane, q.states, wide);
+      store_states(q.state_out + rc * q.states, v, NS * lane, q.states, wide && NS * lane < q.states);
   }
 }
 
@@ -300,6 +329,8 @@ int launch(const BnbSelectiveScan& a, uint8_t* scratch, cudaStream_t st) {
   w.tiles_a_group = tiles_a_group(a);
   const int64_t tiles = (int64_t)w.tiles_a_group * a.groups;
   w.splits = splits(a, KL, (int)tiles);
+  w.paired = a.width / a.groups % 2 == 0 && even_view(a.u, a.element) && even_view(a.delta, a.element) && even_view(a.y, a.element) &&
+             (!a.z.data || even_view(a.z, a.element));
   if (tiles * a.rows > INT32_MAX || w.splits.count > 65535) return BNB_ERR_UNSUPPORTED_DIMS;
   const dim3 grid((unsigned)(tiles * a.rows), w.splits.count);
   if (w.splits.count == 1) {

@@ -75,19 +75,67 @@ __device__ __forceinline__ bool writes_sum() {
   return ((threadIdx.x >> LO) & ((1 << (left - halvings)) - 1)) == 0;
 }
 
-// log(1 + e^v) as max(v, 0) + log(1 + x) with x = e^-|v| <= 1, and log(1 + x) = 2 atanh(s), s = x / (2 + x) <= 1/3, by its Taylor series:
-// the first term left out, s^14 / 15, is 1.4e-8 of the sum.  Half the instructions of log1pf(expf(v)), without a branch,
-// and good to some units in the last place, which the gradients of a need: they are long sums.
-__device__ __forceinline__ float step_size(float v, bool with_softplus) {
+// Step sizes of a pair: log(1 + e^v) as max(v, 0) + log(1 + x) with x = e^-|v| <= 1, and log(1 + x) = 2 atanh(s), s = x / (2 + x) <= 1/3, by
+// its Taylor series: the first term left out, s^14 / 15, is 1.4e-8 of the sum.  e^-|v| = 2^-m with the rounding of m = |v| log2(e) put
+// back to first order.  A few units in the last place, which the gradients of a need: they are long sums.
+__device__ __forceinline__ F2 step_size(F2 v, bool with_softplus) {
   if (!with_softplus) return v;
-  const float x = expf(-fabsf(v)), s = __fdividef(x, 2.0f + x), q = s * s;
-  float series = fmaf(q, 1.0f / 13.0f, 1.0f / 11.0f);
-  series = fmaf(q, series, 1.0f / 9.0f);
-  series = fmaf(q, series, 1.0f / 7.0f);
-  series = fmaf(q, series, 1.0f / 5.0f);
-  series = fmaf(q, series, 1.0f / 3.0f);
-  series = fmaf(q, series, 1.0f);
-  return fmaf(2.0f * s, series, fmaxf(v, 0.0f));
+  const float2 vs = halves(v);
+  const F2 mag = f2(fabsf(vs.x), fabsf(vs.y)), m = mul(mag, f2(LOG2E));
+  const F2 rest = fma(mag, f2(-1.925963033e-8f), fma(mag, f2(-LOG2E), m));   // m - |v| log2(e)
+  const float2 ms = halves(m);
+  const F2 x0 = f2(ex2_fast(-ms.x), ex2_fast(-ms.y)), x = fma(x0, mul(rest, f2(0.6931471805599453f)), x0);
+  const float2 den = halves(add(x, f2(2.0f)));
+  const F2 t = mul(x, f2(rcp_fast(den.x), rcp_fast(den.y))), q = mul(t, t);
+  F2 series = fma(q, f2(1.0f / 13.0f), f2(1.0f / 11.0f));
+  series = fma(q, series, f2(1.0f / 9.0f));
+  series = fma(q, series, f2(1.0f / 7.0f));
+  series = fma(q, series, f2(1.0f / 5.0f));
+  series = fma(q, series, f2(1.0f / 3.0f));
+  series = fma(q, series, f2(1.0f));
+  return fma(add(t, t), series, f2(fmaxf(vs.x, 0.0f), fmaxf(vs.y, 0.0f)));
+}
+__device__ __forceinline__ float step_size(float v, bool with_softplus) { return halves(step_size(f2(v), with_softplus)).x; }
+template <typename T>
+__device__ __forceinline__ F2 sigmoid_pair(F2 v) {
+  if constexpr (sizeof(T) == 4) {
+    const float2 s = halves(v);
+    return f2(sigmoid<float>(s.x), sigmoid<float>(s.y));
+  }
+  const float2 m = halves(mul(v, f2(-LOG2E))), den = halves(add(f2(ex2_fast(m.x), ex2_fast(m.y)), f2(1.0f)));
+  return f2(rcp_fast(den.x), rcp_fast(den.y));
+}
+
+// Two neighbouring channels of a step: one access where `paired` says that all are on its boundary, else those of `count` that exist.
+template <typename T>
+__device__ __forceinline__ Raw<T, 2> load_pair(const T* at, int count, bool paired) {
+  if (paired && count == 2) return load_raw<T, 2>(at);
+  Raw<T, 2> r;
+  T* v = reinterpret_cast<T*>(r.w);
+  v[0] = count > 0 ? at[0] : from_f<T>(0.f);
+  v[1] = count > 1 ? at[1] : from_f<T>(0.f);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ F2 floats_of(const Raw<T, 2>& r) {
+  float f[2];
+  unpack<T, 2>(r, f);
+  return f2(f[0], f[1]);
+}
+template <typename T>
+__device__ __forceinline__ void store_pair(T* at, F2 v, int count, bool paired) {
+  const float2 s = halves(v);
+  if (paired && count == 2) {
+    const float f[2] = {s.x, s.y};
+    store(at, f);
+  } else {
+    if (count > 0) at[0] = from_f<T>(s.x);
+    if (count > 1) at[1] = from_f<T>(s.y);
+  }
+}
+// Whether pairs of channels from an even one on lie on their boundary in a view.
+inline bool even_view(const BnbView& v, int element) {
+  return reinterpret_cast<uintptr_t>(v.data) % (2 * elem_bytes(element)) == 0 && v.step % 2 == 0 && v.row % 2 == 0;
 }
 
 // The four states of a lane, n0 .. n0 + 3, of a (.., states) array that may end inside them.
@@ -99,6 +147,10 @@ __device__ __forceinline__ void load_states(float (&h)[NS], const float* at, int
 #pragma unroll
     for (int i = 0; i < NS; ++i) h[i] = n0 + i < states ? at[n0 + i] : 0.f;
   }
+}
+__device__ __forceinline__ void clear_states(float (&h)[NS]) {
+#pragma unroll
+  for (int i = 0; i < NS; ++i) h[i] = 0.f;
 }
 __device__ __forceinline__ void store_states(float* at, const float (&h)[NS], int n0, int states, bool wide) {
   if (wide) {
