@@ -6,12 +6,20 @@
 //   dz = dy (sum_n c_n h_n + d u) silu'(z),   dd = sum dyv u
 //
 // The forward kept the states of every eighth step.  A CTA takes the chunks of eight steps from the last to the first: the states of
-// a chunk are computed forward into registers, with their decays, and the adjoint walks back over them.  Sums over
-// the channels (db, dc) go through the lanes of a warp, the warps of the CTA and, where a group has several tiles of channels, a
+// a chunk are computed forward into registers, and the adjoint walks back over them, with the decays once more.
+//
+// Sums over the channels (db, dc), 2 NS values a thread and step, are the most work of all if they go through shuffles: four instructions for
+// each halving.  They are matrix products instead: D (16 x 8) += A (16 x 8) B (8 x 8) on mma.sync, where a warp's lanes hold four channels as the
+// depth and (state lane, other channels) as the columns of B just as they are, db's values in its upper half and dc's in its lower, and
+// A has ones in the rows of the step, t for db and 8 + t for dc: the accumulators of a chunk's eight steps are filled one row after
+// the other.  The operands have 11 bits: 16-bit calls round to them (a sum of many terms then is good to 2^-12 or so of its size), float32
+// calls add the products of the bits that remain.
+//
+// What is left of the sums over channels goes through the warps of the CTA and, where a group has several tiles of channels, a
 // short kernel over the tiles; sums over rows and time (da, dd, d bias) stay in registers while a CTA goes over its rows.  No
 // atomics, so a result does not depend on timing.
 //
-// About 35 instructions a state and step bound it, the exponential among them; memory moves some 24 bytes a channel and step.
+// About 25 instructions a state and step bound it, two exponentials among them; memory moves some 24 bytes a channel and step.
 #include "selective_scan.cuh"
 
 namespace bnb {
@@ -30,21 +38,43 @@ struct Work {
   Splits splits;     // steps of a split: a multiple of 16, so of a chunk
   int tiles_a_group;
   int row_blocks;
+  bool paired;       // pairs of channels of u, delta, z, dy and their gradients lie on their boundary
 };
 
 template <int KL> constexpr int CHANNELS = KL <= 4 ? 64 : 256 / KL;   // of a CTA
 
+// d += a b, 11 bits of every operand; see above for what is where.
+__device__ __forceinline__ void mma_rows(float (&d)[4], uint32_t one, float upper, float lower) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%5,%4}, {%6,%7}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(one), "r"(0u), "r"(__float_as_uint(upper)), "r"(__float_as_uint(lower)));
+}
+template <typename T>
+__device__ __forceinline__ void add_rows(float (&d)[4], uint32_t one, float upper, float lower) {
+  if constexpr (sizeof(T) == 2) {   // the product drops 13 bits: rounded to the nearest before
+    mma_rows(d, one, __uint_as_float(__float_as_uint(upper) + 0x1000u), __uint_as_float(__float_as_uint(lower) + 0x1000u));
+  } else {
+    const float u = __uint_as_float(__float_as_uint(upper) & 0xffffe000u), l = __uint_as_float(__float_as_uint(lower) & 0xffffe000u);
+    mma_rows(d, one, upper - u, lower - l);
+    mma_rows(d, one, u, l);
+  }
+}
+
 // LOCAL: only what a split leaves of a zero adjoint behind it, see selective_scan.cuh.
 template <typename T, int KL, bool LOCAL>
-__global__ void __launch_bounds__(CHANNELS<KL> * KL) k_scan_bwd(const __grid_constant__ BnbSelectiveScan q, const __grid_constant__ BnbSelectiveScanGrads g, Work w) {
-  constexpr int CT = CHANNELS<KL>, THREADS = CT * KL, NP = NS * KL, PER = (L + KL - 1) / KL, WARPS = THREADS / 32;
-  constexpr int BITS = KL == 1 ? 0 : KL == 2 ? 1 : KL == 4 ? 2 : KL == 8 ? 3 : 4;
+__global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<KL> * KL) : 2) k_scan_bwd(const __grid_constant__ BnbSelectiveScan q, const __grid_constant__ BnbSelectiveScanGrads g, const __grid_constant__ Work w) {
+  constexpr int CT = CHANNELS<KL>, THREADS = CT * KL, NP = NS * KL, WARPS = THREADS / 32;
+  constexpr int BITS = KL == 1 ? 0 : KL == 2 ? 1 : KL == 4 ? 2 : KL == 8 ? 3 : 4, CB = 5 - BITS;   // lane: channel in the low CB bits, state lane above
   constexpr int BC = (L * NP + THREADS - 1) / THREADS;
-  constexpr int GROUP = 4;   // steps whose sums over a channel's lanes are taken together
-  __shared__ float p_s[L][CT], pu_s[LOCAL ? 1 : L][CT], dy_s[L][CT], sum_s[LOCAL ? 1 : L][3][CT];
+  constexpr int PAIRS = CT / 2, AT_ONCE = THREADS / PAIRS < L ? THREADS / PAIRS : L, PER = L / AT_ONCE;   // steps prepared at a time, by a thread
+  constexpr int GROUP = 4;         // steps whose sums over a channel's lanes are taken together
+  constexpr bool MMA = KL <= 8;    // with 16 lanes a channel, four neighbouring lanes are not four channels
+  __shared__ __align__(16) float4 pp_s[L][CT];                        // p, p, p u, p u
+  __shared__ __align__(16) float2 dy_s[L][CT];                        // dyv twice
   __shared__ __align__(16) float b_s[LOCAL ? 1 : L][NP], c_s[L][NP];
-  extern __shared__ float red[];   // (L, WARPS, 2 NP): sums over a warp's channels
-  const int tid = threadIdx.x, cl = tid / KL, lane = tid % KL, warp = tid / 32;
+  __shared__ __align__(16) float held_s[LOCAL ? 1 : L][3][CT];        // u, softplus', dy silu'(z)
+  __shared__ __align__(16) float sum_s[LOCAL ? 1 : L][3][CT];
+  extern __shared__ __align__(16) float red[];   // (L, WARPS, 2 NP): sums over a warp's channels
+  const int tid = threadIdx.x, warp = tid / 32, wl = tid & 31, lane = wl >> CB, cl = warp * (32 / KL) + (wl & ((1 << CB) - 1));
   const int tiles = w.tiles_a_group * q.groups, share = q.width / q.groups;
   const int row_block = blockIdx.x / tiles, tile = blockIdx.x - row_block * tiles, group = tile / w.tiles_a_group, tile_in = tile - group * w.tiles_a_group;
   const int c0 = group * share + tile_in * CT, c_end = min((group + 1) * share, c0 + CT);
@@ -52,110 +82,107 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL) k_scan_bwd(const __grid_con
   const bool owns = ch < c_end, wide = q.states % NS == 0;
   const int split = blockIdx.y, first = split * w.splits.steps, last = min(q.steps, first + w.splits.steps);
 
-  float rate[NS], da[NS];
-#pragma unroll
-  for (int i = 0; i < NS; ++i) rate[i] = da[i] = 0.f;
-  if (owns) load_states(rate, q.a + (int64_t)ch * q.states, NS * lane, q.states, wide);
-#pragma unroll
-  for (int i = 0; i < NS; ++i) rate[i] *= LOG2E;
-  const int pc = tid % CT, pt = tid / CT;   // prepares steps pt + k KL of channel c0 + pc
-  const bool prepares = c0 + pc < c_end;
-  const float bias = prepares && q.delta_bias ? q.delta_bias[c0 + pc] : 0.f, skip = prepares && q.d ? q.d[c0 + pc] : 0.f;
+  F2 rate[2] = {f2(0.f), f2(0.f)}, da[2] = {f2(0.f), f2(0.f)};
+  auto put = [](float (&v)[NS], const F2 (&x)[2]) {
+    const float2 a = halves(x[0]), b = halves(x[1]);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  };
+  auto get = [](F2 (&x)[2], const float (&v)[NS]) {
+    x[0] = f2(v[0], v[1]);
+    x[1] = f2(v[2], v[3]);
+  };
+  if (owns) {
+    float v[NS];
+    load_states(v, q.a + (int64_t)ch * q.states, NS * lane, q.states, wide && NS * lane < q.states);
+    get(rate, v);
+    rate[0] = mul(rate[0], f2(LOG2E));
+    rate[1] = mul(rate[1], f2(LOG2E));
+  }
+  // what this thread prepares: channels c0 + 2 pair, + 1 of steps t0 + step + k AT_ONCE
+  const int pair = tid % PAIRS, step = tid / PAIRS, pc = c0 + 2 * pair, count = step < L ? max(0, min(2, c_end - pc)) : 0;
+  F2 bias = f2(0.f), skip = f2(0.f), dd = f2(0.f), dbias = f2(0.f);
+  if (q.delta_bias) bias = f2(count > 0 ? q.delta_bias[pc] : 0.f, count > 1 ? q.delta_bias[pc + 1] : 0.f);
+  if (q.d) skip = f2(count > 0 ? q.d[pc] : 0.f, count > 1 ? q.d[pc + 1] : 0.f);
   const bool gated = q.z.data != nullptr;
   const T none = from_f<T>(0.f);
-  float dd = 0.f, dbias = 0.f;
 
   for (int r = row_block; r < q.rows; r += w.row_blocks) {
     const int n = row_steps(q.lengths, r, q.steps), live = min(n, last);
     const int64_t rc = (int64_t)r * q.width + ch;
-    const T* up = static_cast<const T*>(q.u.data) + r * q.u.row + c0 + pc;
-    const T* dp = static_cast<const T*>(q.delta.data) + r * q.delta.row + c0 + pc;
-    const T* zp = static_cast<const T*>(q.z.data) + r * q.z.row + c0 + pc;
-    const T* yp = static_cast<const T*>(g.dy.data) + r * g.dy.row + c0 + pc;
-    const T* bp = static_cast<const T*>(q.b.data) + r * q.b.row + group * q.b.group;
-    const T* cp = static_cast<const T*>(q.c.data) + r * q.c.row + group * q.c.group;
-    T* dup = static_cast<T*>(g.du.data) + r * g.du.row + c0 + pc;
-    T* ddp = static_cast<T*>(g.ddelta.data) + r * g.ddelta.row + c0 + pc;
-    T* dzp = static_cast<T*>(g.dz.data) + r * g.dz.row + c0 + pc;
-    T* dbp = static_cast<T*>(g.db.data) + r * g.db.row + group * g.db.group;
-    T* dcp = static_cast<T*>(g.dc.data) + r * g.dc.row + group * g.dc.group;
+    const int begin = live > first ? (live - 1) / L * L : first - L;   // the last chunk; first is a multiple of L
+    // a step of a row; what is the same for the CTA is computed once for it
+    auto at = [&](const BnbView& v, int t) { return static_cast<T*>(v.data) + r * v.row + t * v.step; };
+    auto db_at = [&](int t) { return at(g.db, t) + group * g.db.group; };
+    auto dc_at = [&](int t) { return at(g.dc, t) + group * g.dc.group; };
     float* part_bc = w.part_bc ? w.part_bc + (((int64_t)tile_in * q.steps * q.rows + r) * q.groups + group) * 2 * NP : nullptr;
     const int64_t part_step = (int64_t)q.rows * q.groups * 2 * NP;
 
     // steps behind the row's end
     if constexpr (!LOCAL) {
-      if (prepares)
-        for (int t = max(first, n) + pt; t < last; t += KL) {
-          dup[t * g.du.step] = none;
-          ddp[t * g.ddelta.step] = none;
-          if (gated) dzp[t * g.dz.step] = none;
-        }
+      for (int t = max(first, n) + step; step < L && t < last; t += AT_ONCE) {
+        store_pair(at(g.du, t) + pc, f2(0.f), count, w.paired);
+        store_pair(at(g.ddelta, t) + pc, f2(0.f), count, w.paired);
+        if (gated) store_pair(at(g.dz, t) + pc, f2(0.f), count, w.paired);
+      }
       for (int64_t e = tid; e < (int64_t)(last - max(first, n)) * 2 * NP; e += THREADS) {
         const int t = max(first, n) + (int)(e / (2 * NP)), s = (int)(e % (2 * NP));
         if (part_bc) part_bc[t * part_step + s] = 0.f;
-        else if (s < NP) { if (s < q.states) dbp[t * g.db.step + s] = none; }
-        else if (s - NP < q.states) dcp[t * g.dc.step + s - NP] = none;
+        else if (s < NP) { if (s < q.states) db_at(t)[s] = none; }
+        else if (s - NP < q.states) dc_at(t)[s - NP] = none;
       }
     }
 
-    float carry[NS];
-#pragma unroll
-    for (int i = 0; i < NS; ++i) carry[i] = 0.f;
+    F2 carry[2] = {f2(0.f), f2(0.f)};
     if (!LOCAL && owns) {
-      if (w.splits.count > 1) load_states(carry, w.carry + ((int64_t)split * q.rows * q.width + rc) * NP, NS * lane, NP, true);
-      else if (g.dstate_out) load_states(carry, g.dstate_out + rc * q.states, NS * lane, q.states, wide);
+      float v[NS];
+      clear_states(v);
+      if (w.splits.count > 1) load_states(v, w.carry + ((int64_t)split * q.rows * q.width + rc) * NP, NS * lane, NP, true);
+      else if (g.dstate_out) load_states(v, g.dstate_out + rc * q.states, NS * lane, q.states, wide && NS * lane < q.states);
+      get(carry, v);
     }
-    T u_r[PER], d_r[PER], z_r[PER], y_r[PER], b_r[BC], c_r[BC];
-    float4 h_r = make_float4(0.f, 0.f, 0.f, 0.f);
-    unsigned cuts_next = 0;
-    auto fetch = [&](int t0) {
+    float sum_p = 0.f;
+    bool any_cut = false;
+#pragma unroll 1
+    for (int t0 = begin; t0 >= first; t0 -= L) {
+      unsigned cuts = 0;   // bit k: an episode ended before step t0 + k
       if (q.done) {
-        const int t = t0 + (tid & 31) - 1;
-        cuts_next = __ballot_sync(0xffffffffu, (tid & 31) < L && t >= 0 && t + 1 < live && q.done[(int64_t)max(t, 0) * q.rows + r]);
+        const int t = t0 + wl - 1;
+        cuts = __ballot_sync(0xffffffffu, wl < L && t >= 0 && t + 1 < live && q.done[(int64_t)max(t, 0) * q.rows + r]);
       }
-#pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        const int t = t0 + pt + k * KL;
-        const bool on = prepares && t < live && pt + k * KL < L;
-        u_r[k] = on ? up[t * q.u.step] : none;
-        d_r[k] = on ? dp[t * q.delta.step] : none;
-        z_r[k] = gated && on ? zp[t * q.z.step] : none;
-        y_r[k] = on ? yp[t * g.dy.step] : none;
-      }
+      float4 h_r = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (!LOCAL && owns) h_r = *reinterpret_cast<const float4*>(q.kept + ((int64_t)(t0 / KEEP) * q.rows * q.width + rc) * NP + NS * lane);
+      T b_r[BC], c_r[BC];
 #pragma unroll
       for (int k = 0; k < BC; ++k) {
         const int e = tid + k * THREADS, t = t0 + e / NP, s = e % NP;
         const bool on = e < L * NP && s < q.states && t < live;
-        if (!LOCAL) b_r[k] = on ? bp[t * q.b.step + s] : none;
-        c_r[k] = on ? cp[t * q.c.step + s] : none;
+        if (!LOCAL) b_r[k] = on ? at(q.b, t)[group * q.b.group + s] : none;
+        c_r[k] = on ? at(q.c, t)[group * q.c.group + s] : none;
       }
-      if (!LOCAL && owns) h_r = *reinterpret_cast<const float4*>(q.kept + ((int64_t)(t0 / KEEP) * q.rows * q.width + rc) * NP + NS * lane);
-    };
-    float sum_p = 0.f;
-    bool any_cut = false;
-    const int begin = live > first ? (live - 1) / L * L : first - L;   // first is a multiple of L
-    if (begin >= first) fetch(begin);
-#pragma unroll 1
-    for (int t0 = begin; t0 >= first; t0 -= L) {
-      float u_f[PER], p_f[PER], dyv[PER], raw[PER], dgate[PER];   // dgate: dy silu'(z)
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int t = pt + k * KL;
-        u_f[k] = to_f(u_r[k]);
-        raw[k] = to_f(d_r[k]) + bias;
-        p_f[k] = t0 + t < live ? step_size(raw[k], q.softplus) : 0.f;
-        const float dy = to_f(y_r[k]);
-        dyv[k] = dy;
-        dgate[k] = 0.f;
+        const int ts = step + k * AT_ONCE, t = t0 + ts, have = t < live ? count : 0;
+        const Raw<T, 2> u_r = load_pair<T>(at(q.u, t) + pc, LOCAL ? 0 : have, w.paired), d_r = load_pair<T>(at(q.delta, t) + pc, have, w.paired);
+        const Raw<T, 2> z_r = load_pair<T>(at(q.z, t) + pc, gated ? have : 0, w.paired), y_r = load_pair<T>(at(g.dy, t) + pc, have, w.paired);
+        const F2 u = floats_of<T>(u_r), raw = add(floats_of<T>(d_r), bias), dy = floats_of<T>(y_r);
+        const F2 p = t < live ? step_size(raw, q.softplus) : f2(0.f);
+        F2 dyv = dy, dgate = f2(0.f);   // dgate: dy silu'(z)
         if (gated) {
-          const float z = to_f(z_r[k]), sg = sigmoid<T>(z);
-          dyv[k] = dy * (z * sg);
-          dgate[k] = dy * (sg * fmaf(z, 1.f - sg, 1.f));
+          const F2 z = floats_of<T>(z_r), sg = sigmoid_pair<T>(z);
+          dyv = mul(dy, mul(z, sg));
+          dgate = mul(dy, mul(sg, fma(z, fma(sg, f2(-1.0f), f2(1.0f)), f2(1.0f))));
         }
-        if (t < L) {
-          p_s[t][pc] = p_f[k];
-          dy_s[t][pc] = dyv[k];
-          if (!LOCAL) pu_s[t][pc] = p_f[k] * u_f[k];
+        if (step < L) {
+          const float2 ps = halves(p), pu = halves(mul(p, u)), ds = halves(dyv);
+          pp_s[ts][2 * pair] = make_float4(ps.x, ps.x, pu.x, pu.x);
+          pp_s[ts][2 * pair + 1] = make_float4(ps.y, ps.y, pu.y, pu.y);
+          *reinterpret_cast<float4*>(&dy_s[ts][2 * pair]) = make_float4(ds.x, ds.x, ds.y, ds.y);
+          if (!LOCAL) {   // for this thread's own use behind the walk
+            const F2 slope = q.softplus ? sigmoid_pair<T>(raw) : f2(1.0f);
+            *reinterpret_cast<float2*>(&held_s[ts][0][2 * pair]) = halves(u);
+            *reinterpret_cast<float2*>(&held_s[ts][1][2 * pair]) = halves(slope);
+            *reinterpret_cast<float2*>(&held_s[ts][2][2 * pair]) = halves(dgate);
+          }
         }
       }
 #pragma unroll
@@ -166,67 +193,88 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL) k_scan_bwd(const __grid_con
           (&c_s[0][0])[e] = to_f(c_r[k]);
         }
       }
-      const float h0[NS] = {h_r.x, h_r.y, h_r.z, h_r.w};
-      const unsigned cuts = cuts_next;
+      const F2 h0[2] = {f2(h_r.x, h_r.y), f2(h_r.z, h_r.w)};
       any_cut |= cuts != 0;
       __syncthreads();
-      if (t0 - L >= first) fetch(t0 - L);
       if constexpr (LOCAL) {
 #pragma unroll
         for (int t = L - 1; t >= 0; --t) {
-          const float p = p_s[t][cl], dy = dy_s[t][cl];
-          const float4 c4 = *reinterpret_cast<const float4*>(&c_s[t][NS * lane]);
-          const float c[NS] = {c4.x, c4.y, c4.z, c4.w};
-          sum_p += p;
-#pragma unroll
-          for (int i = 0; i < NS; ++i) carry[i] = (cuts >> t) & 1 ? 0.f : ex2_fast(p * rate[i]) * fmaf(c[i], dy, carry[i]);
+          const F2 p{*reinterpret_cast<const unsigned long long*>(&pp_s[t][cl])}, dy{*reinterpret_cast<const unsigned long long*>(&dy_s[t][cl])};
+          const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&c_s[t][NS * lane]);
+          sum_p += halves(p).x;
+          const float2 m0 = halves(mul(p, rate[0])), m1 = halves(mul(p, rate[1]));
+          carry[0] = mul(f2(ex2_fast(m0.x), ex2_fast(m0.y)), fma(F2{c.x}, dy, carry[0]));
+          carry[1] = mul(f2(ex2_fast(m1.x), ex2_fast(m1.y)), fma(F2{c.y}, dy, carry[1]));
+          if ((cuts >> t) & 1) carry[0] = carry[1] = f2(0.f);
         }
         __syncthreads();
       } else {
-        float h[L + 1][NS], e[L][NS];   // h[t]: before step t, episode ends applied; h[t + 1] behind it unless one follows
-#pragma unroll
-        for (int i = 0; i < NS; ++i) h[0][i] = cuts & 1 ? 0.f : h0[i];
+        F2 h[L + 1][2];   // h[t]: before step t, episode ends applied; h[t + 1] behind it unless one follows
+        h[0][0] = cuts & 1 ? f2(0.f) : h0[0];
+        h[0][1] = cuts & 1 ? f2(0.f) : h0[1];
 #pragma unroll
         for (int t = 0; t < L; ++t) {
-          const float p = p_s[t][cl], pu = pu_s[t][cl];
-          const float4 b4 = *reinterpret_cast<const float4*>(&b_s[t][NS * lane]);
-          const float b[NS] = {b4.x, b4.y, b4.z, b4.w};
+          const ulonglong2 pp = *reinterpret_cast<const ulonglong2*>(&pp_s[t][cl]), b = *reinterpret_cast<const ulonglong2*>(&b_s[t][NS * lane]);
+          const F2 bs[2] = {F2{b.x}, F2{b.y}};
 #pragma unroll
-          for (int i = 0; i < NS; ++i) {
-            e[t][i] = ex2_fast(p * rate[i]);
-            h[t + 1][i] = fmaf(e[t][i], h[t][i], pu * b[i]);
-            if (t + 1 < L && ((cuts >> (t + 1)) & 1)) h[t + 1][i] = 0.f;
+          for (int i = 0; i < 2; ++i) {
+            const float2 m = halves(mul(F2{pp.x}, rate[i]));
+            h[t + 1][i] = fma(f2(ex2_fast(m.x), ex2_fast(m.y)), h[t][i], mul(F2{pp.y}, bs[i]));
+          }
+          if (t + 1 < L && ((cuts >> (t + 1)) & 1)) {
+            h[t + 1][0] = h[t + 1][1] = f2(0.f);
+            asm volatile("");   // rare, and the same for all: worth a branch
           }
         }
         float sums[GROUP][3];   // over the states: c h, g b, g e h- a
+        float rows[MMA ? NS : 1][4];
+#pragma unroll
+        for (int i = 0; i < (MMA ? NS : 1); ++i) rows[i][0] = rows[i][1] = rows[i][2] = rows[i][3] = 0.f;
 #pragma unroll
         for (int t = L - 1; t >= 0; --t) {
-          const float p = p_s[t][cl], pu = pu_s[t][cl], dy = dy_s[t][cl];
-          const float4 b4 = *reinterpret_cast<const float4*>(&b_s[t][NS * lane]), c4 = *reinterpret_cast<const float4*>(&c_s[t][NS * lane]);
-          const float b[NS] = {b4.x, b4.y, b4.z, b4.w}, c[NS] = {c4.x, c4.y, c4.z, c4.w};
-          const bool ends = t + 1 < L && ((cuts >> (t + 1)) & 1);   // h[t + 1] was cleared for the next step
-          float bc[2 * NS], sy = 0.f, sb = 0.f, sa = 0.f;
+          const ulonglong2 pp = *reinterpret_cast<const ulonglong2*>(&pp_s[t][cl]);
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&b_s[t][NS * lane]), c = *reinterpret_cast<const ulonglong2*>(&c_s[t][NS * lane]);
+          const F2 p{pp.x}, pu{pp.y}, dy{*reinterpret_cast<const unsigned long long*>(&dy_s[t][cl])};
+          const F2 bs[2] = {F2{b.x}, F2{b.y}}, cs[2] = {F2{c.x}, F2{c.y}};
+          F2 sy = f2(0.f), sb = f2(0.f), sa = f2(0.f);
+          F2 of_b[2], of_c[2];
 #pragma unroll
-          for (int i = 0; i < NS; ++i) {
-            const float eh = e[t][i] * h[t][i];
-            const float behind = ends ? fmaf(pu, b[i], eh) : h[t + 1][i];
-            const float gh = fmaf(c[i], dy, carry[i]);
-            sy = fmaf(c[i], behind, sy);
-            sb = fmaf(gh, b[i], sb);
-            const float ge = gh * eh;
-            sa = fmaf(ge, rate[i], sa);
-            da[i] = fmaf(ge, p, da[i]);
-            bc[i] = gh * pu;
-            bc[NS + i] = behind * dy;
-            carry[i] = (cuts >> t) & 1 ? 0.f : gh * e[t][i];
+          for (int i = 0; i < 2; ++i) {
+            const float2 m = halves(mul(p, rate[i]));
+            const F2 e = f2(ex2_fast(m.x), ex2_fast(m.y)), eh = mul(e, h[t][i]);
+            F2 behind = h[t + 1][i];
+            if (t + 1 < L && ((cuts >> (t + 1)) & 1)) {   // cleared for the next step
+              behind = fma(pu, bs[i], eh);
+              asm volatile("");
+            }
+            const F2 gh = fma(cs[i], dy, carry[i]), ge = mul(gh, eh);
+            sy = i ? fma(cs[i], behind, sy) : mul(cs[i], behind);
+            sb = i ? fma(gh, bs[i], sb) : mul(gh, bs[i]);
+            sa = i ? fma(ge, rate[i], sa) : mul(ge, rate[i]);
+            da[i] = fma(ge, p, da[i]);
+            of_b[i] = mul(gh, pu);
+            of_c[i] = mul(behind, dy);
+            carry[i] = mul(gh, e);
           }
-          sums[t % GROUP][0] = sy;
-          sums[t % GROUP][1] = sb;
-          sums[t % GROUP][2] = sa;
-          {   // over the warp's channels
-            const int at = sum_lanes<2 * NS, BITS, 5>(bc);
-            constexpr int LEFT = (2 * NS) >> (5 - BITS) ? (2 * NS) >> (5 - BITS) : 1;
-            if (writes_sum<2 * NS, BITS, 5>()) {
+          if ((cuts >> t) & 1) {
+            carry[0] = carry[1] = f2(0.f);
+            asm volatile("");
+          }
+          const float2 y2 = halves(sy), b2 = halves(sb), a2 = halves(sa);
+          sums[t % GROUP][0] = y2.x + y2.y;
+          sums[t % GROUP][1] = b2.x + b2.y;
+          sums[t % GROUP][2] = a2.x + a2.y;
+          float bc[2 * NS];
+          put(*reinterpret_cast<float(*)[NS]>(&bc[0]), of_b);
+          put(*reinterpret_cast<float(*)[NS]>(&bc[NS]), of_c);
+          if constexpr (MMA) {
+            const uint32_t one = (wl >> 2) == t ? 0x3f800000u : 0u;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) add_rows<T>(rows[i], one, bc[i], bc[NS + i]);
+          } else {   // over the warp's channels by shuffles
+            const int at = sum_lanes<2 * NS, 0, CB>(bc);
+            constexpr int LEFT = (2 * NS) >> CB ? (2 * NS) >> CB : 1;
+            if (writes_sum<2 * NS, 0, CB>()) {
 #pragma unroll
               for (int k = 0; k < LEFT; ++k) {
                 const int v = at + k;   // 0 .. 3: b, 4 .. 7: c
@@ -240,28 +288,59 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL) k_scan_bwd(const __grid_con
               float v[GROUP];
 #pragma unroll
               for (int k = 0; k < GROUP; ++k) v[k] = sums[k][s];
-              const int at = sum_lanes<GROUP, 0, BITS>(v);
+              const int at = sum_lanes<GROUP, CB, 5>(v);
               constexpr int LEFT = GROUP >> BITS ? GROUP >> BITS : 1;
-              if (writes_sum<GROUP, 0, BITS>()) {
+              if (writes_sum<GROUP, CB, 5>()) {
 #pragma unroll
                 for (int k = 0; k < LEFT; ++k) sum_s[t + at + k][s][cl] = v[k];
               }
             }
           }
         }
+        if constexpr (MMA) {
+          // this lane's row is step wl / 4 (db in rows[i][0..1], dc in [2..3]), its columns 2 (wl % 4), + 1: column = state lane times
+          // 8 / KL + the channels' upper bits, over which the rest of the sum goes
+          const int t = wl >> 2, m = wl & 3;
+          float v[2][KL == 8 ? 2 : 1][NS];
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+              if constexpr (KL == 8) {
+                v[s][0][i] = rows[i][2 * s];
+                v[s][1][i] = rows[i][2 * s + 1];
+              } else {
+                v[s][0][i] = rows[i][2 * s] + rows[i][2 * s + 1];
+                if (KL <= 2) v[s][0][i] += __shfl_xor_sync(0xffffffffu, v[s][0][i], 1);
+                if (KL == 1) v[s][0][i] += __shfl_xor_sync(0xffffffffu, v[s][0][i], 2);
+              }
+            }
+          const bool writes = KL >= 4 || (KL == 2 ? (m & 1) == 0 : m == 0);
+          if (writes) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int x = 0; x < (KL == 8 ? 2 : 1); ++x) {
+                const int of = KL == 8 ? 2 * m + x : KL == 4 ? m : KL == 2 ? m >> 1 : 0;   // state lane
+                *reinterpret_cast<float4*>(&red[(t * WARPS + warp) * 2 * NP + s * NP + NS * of]) = make_float4(v[s][x][0], v[s][x][1], v[s][x][2], v[s][x][3]);
+              }
+          }
+        }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const int t = pt + k * KL;
-          if (t >= L || !prepares || t0 + t >= live) continue;
-          const float sy = sum_s[t][0][pc], sb = sum_s[t][1][pc], sa = sum_s[t][2][pc];
-          const float dpt = fmaf(sa, 1.0f / LOG2E, sb * u_f[k]);
-          const float draw = q.softplus ? dpt * sigmoid<T>(raw[k]) : dpt;
-          dup[(t0 + t) * g.du.step] = from_f<T>(fmaf(sb, p_f[k], skip * dyv[k]));
-          ddp[(t0 + t) * g.ddelta.step] = from_f<T>(draw);
-          if (gated) dzp[(t0 + t) * g.dz.step] = from_f<T>(dgate[k] * fmaf(skip, u_f[k], sy));
-          dd = fmaf(dyv[k], u_f[k], dd);
-          dbias += draw;
+          const int t = step + k * AT_ONCE;
+          if (step >= L || t0 + t >= live) continue;
+          auto pair_of = [&](const float* at) { const float2 v = *reinterpret_cast<const float2*>(at); return f2(v.x, v.y); };
+          const F2 sy = pair_of(&sum_s[t][0][2 * pair]), sb = pair_of(&sum_s[t][1][2 * pair]), sa = pair_of(&sum_s[t][2][2 * pair]);
+          const F2 u = pair_of(&held_s[t][0][2 * pair]), slope = pair_of(&held_s[t][1][2 * pair]), dgate = pair_of(&held_s[t][2][2 * pair]);
+          const F2 p = f2(pp_s[t][2 * pair].x, pp_s[t][2 * pair + 1].x), dyv = f2(dy_s[t][2 * pair].x, dy_s[t][2 * pair + 1].x);
+          const F2 draw = mul(fma(sa, f2(1.0f / LOG2E), mul(sb, u)), slope);
+          store_pair(at(g.du, t0 + t) + pc, fma(sb, p, mul(skip, dyv)), count, w.paired);
+          store_pair(at(g.ddelta, t0 + t) + pc, draw, count, w.paired);
+          if (gated) store_pair(at(g.dz, t0 + t) + pc, mul(dgate, fma(skip, u, sy)), count, w.paired);
+          dd = fma(dyv, u, dd);
+          dbias = add(dbias, draw);
         }
         for (int x = tid; x < L * 2 * NP; x += THREADS) {
           const int t = x / (2 * NP), s = x % (2 * NP);
@@ -270,41 +349,43 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL) k_scan_bwd(const __grid_con
 #pragma unroll
           for (int k = 0; k < WARPS; ++k) v += red[(t * WARPS + k) * 2 * NP + s];
           if (part_bc) part_bc[(t0 + t) * part_step + s] = v;
-          else if (s < NP) { if (s < q.states) dbp[(t0 + t) * g.db.step + s] = from_f<T>(v); }
-          else if (s - NP < q.states) dcp[(t0 + t) * g.dc.step + s - NP] = from_f<T>(v);
+          else if (s < NP) { if (s < q.states) db_at(t0 + t)[s] = from_f<T>(v); }
+          else if (s - NP < q.states) dc_at(t0 + t)[s - NP] = from_f<T>(v);
         }
-        // the next chunk's sums are written behind its first barrier
+        // the next chunk's sums are written behind its first barrier; what a thread prepared it reads itself
       }
     }
+    float v[NS];
+    put(v, carry);
     if constexpr (LOCAL) {
       if (owns) {
-        store_states(w.carry + ((int64_t)split * q.rows * q.width + rc) * NP, carry, NS * lane, NP, true);
+        store_states(w.carry + ((int64_t)split * q.rows * q.width + rc) * NP, v, NS * lane, NP, true);
         if (lane == 0) w.sum_p[(int64_t)split * q.rows * q.width + rc] = sum_p;
       }
       if (tid == 0 && tile == 0) w.cut[(int64_t)split * q.rows + r] = any_cut;
     } else if (owns && split == 0 && g.dstate_in) {
-      store_states(g.dstate_in + rc * q.states, carry, NS * lane, q.states, wide);
+      store_states(g.dstate_in + rc * q.states, v, NS * lane, q.states, wide && NS * lane < q.states);
     }
   }
   if constexpr (!LOCAL) {
     const int64_t part = (int64_t)blockIdx.y * w.row_blocks + row_block;
-    if (owns) store_states(w.part_a + (part * q.width + ch) * NP, da, NS * lane, NP, true);
+    float v[NS];
+    put(v, da);
+    if (owns) store_states(w.part_a + (part * q.width + ch) * NP, v, NS * lane, NP, true);
     __syncthreads();
-    float* both = &sum_s[0][0][0];   // (KL, 2, CT) of the threads that prepared a channel
-    constexpr int HELD = KL > L ? L : KL;   // threads behind the eighth prepared nothing
-    static_assert(sizeof(sum_s) >= HELD * 2 * CT * 4, "room for the sums of a channel");
-    if (pt < HELD) {
-      both[(pt * 2 + 0) * CT + pc] = dd;
-      both[(pt * 2 + 1) * CT + pc] = dbias;
+    float* both = &sum_s[0][0][0];   // (AT_ONCE, 2, CT) of the threads that prepared a pair
+    static_assert(sizeof(sum_s) >= AT_ONCE * 2 * CT * 4, "room for the sums of a channel");
+    if (step < AT_ONCE) {
+      *reinterpret_cast<float2*>(&both[(step * 2 + 0) * CT + 2 * pair]) = halves(dd);
+      *reinterpret_cast<float2*>(&both[(step * 2 + 1) * CT + 2 * pair]) = halves(dbias);
     }
     __syncthreads();
-    if (pt < 2 || KL == 1) {
-      for (int s = pt; s < 2; s += KL) {
-        float v = 0.f;
+    for (int x = tid; x < 2 * CT; x += THREADS) {
+      const int s = x / CT, c = x % CT;
+      float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < HELD; ++k) v += both[(k * 2 + s) * CT + pc];
-        if (prepares) w.part_d[(part * 2 + s) * q.width + c0 + pc] = v;
-      }
+      for (int k = 0; k < AT_ONCE; ++k) sum += both[(k * 2 + s) * CT + c];
+      if (c0 + c < c_end) w.part_d[(part * 2 + s) * q.width + c0 + c] = sum;
     }
   }
 }
@@ -389,6 +470,8 @@ int launch(const BnbSelectiveScan& a, const BnbSelectiveScanGrads& g, const Plan
   w.splits = p.splits;
   w.tiles_a_group = p.tiles_a_group;
   w.row_blocks = p.row_blocks;
+  w.paired = a.width / a.groups % 2 == 0 && even_view(a.u, a.element) && even_view(a.delta, a.element) && even_view(g.dy, a.element) &&
+             even_view(g.du, a.element) && even_view(g.ddelta, a.element) && (!a.z.data || (even_view(a.z, a.element) && even_view(g.dz, a.element)));
   w.carry = reinterpret_cast<float*>(scratch);
   w.sum_p = reinterpret_cast<float*>(scratch + p.sum_p);
   w.cut = scratch + p.cut;
