@@ -7,6 +7,9 @@ reference's own ``nn.Module`` signatures.
 The modules mirror ``boost_and_broadside.models.yemong.{attention,griffin}`` of the
 reference (same constructor arguments, parameter names and forward signatures) and call
 the C-ABI library ``libbnb_trunk.so`` (include/bnb_trunk.h).  There is no CPU path.
+
+Beside them stand operators for layers of other shapes: ``causal_conv``, ``selective_scan`` and their
+single-token forms, ``gated_mlp``, and ``SelectiveTemporalBlock``, a temporal sublayer made of them.
 """
 
 from .config import ModelConfig
@@ -16,7 +19,7 @@ from .yemong.gated import gated_mlp
 from .yemong.heads import HeadMLP, NextStateHead, TeamPMA, evaluate_action, sample_action
 from .yemong.griffin import CONV_KERNEL, RGLRU, GriffinTemporalBlock, YemongBlock
 from .yemong.policy import YemongPolicy
-from .yemong.selective import causal_conv, causal_conv_step, selective_scan, selective_step
+from .yemong.selective import SelectiveTemporalBlock, causal_conv, causal_conv_step, selective_scan, selective_step
 from .yemong.trunk import YemongTrunk, RaggedBatch
 
 __all__ = [
@@ -29,6 +32,7 @@ __all__ = [
     "NextStateHead",
     "RGLRU",
     "RaggedBatch",
+    "SelectiveTemporalBlock",
     "ShipEncoder",
     "TeamPMA",
     "TransformerBlock",

@@ -13,6 +13,15 @@ from torch import Tensor
 from .. import _capi
 
 
+_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
+
+
+def activation_code(fn: str, name: Optional[str], allowed: tuple) -> int:
+    if name not in allowed:
+        raise ValueError(f"{fn}: activation must be one of {allowed}, got {name!r}")
+    return _ACTIVATIONS[name]
+
+
 def _rows_like(x: Tensor) -> Tensor:
     """As the native code lays out a result of x's shape: step by step, or row by row where x is."""
     if x.dim() < 3 or x.stride(0) >= x.stride(1):

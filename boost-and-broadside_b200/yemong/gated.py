@@ -10,7 +10,7 @@ import torch
 
 from .. import _capi
 from . import _ops, _sequence_ops
-from .selective import activation_code
+from ._sequence_ops import activation_code
 
 
 def gated_mlp(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor, down_w: torch.Tensor, *, activation: str = "gelu") -> torch.Tensor:

@@ -15,18 +15,19 @@ once on the way out.
 
 from __future__ import annotations
 
+import math
+
 import torch
+import torch.nn as nn
+import torch.nn.functional as F
 
 from .. import _capi
 from . import _ops, _sequence_ops
+from ._sequence_ops import activation_code
+from .attention import GatedMLP
+from .gated import gated_mlp
 
-_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
-
-
-def activation_code(fn: str, name: str | None, allowed: tuple) -> int:
-    if name not in allowed:
-        raise ValueError(f"{fn}: activation must be one of {allowed}, got {name!r}")
-    return _ACTIVATIONS[name]
+TAPS: int = 4  # of the block's convolution, as CONV_KERNEL of the Griffin sublayer (griffin.py:22)
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, state: torch.Tensor | None = None,
@@ -116,3 +117,95 @@ def selective_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     B, C = _grouped("selective_step", "B", B, 2), _grouped("selective_step", "C", C, 2)
     run = _capi.host if _ops.direct(u) else _sequence_ops
     return run.selective_step(u, delta, A, B, C, D, state, z, delta_bias, reset, softplus)
+
+
+class SelectiveTemporalBlock(nn.Module):
+    """A temporal sublayer on these operators, in the place and with the signatures of ``GriffinTemporalBlock``
+    (griffin.py:222-286): norm -> in_proj -> (causal conv -> selective scan) gated -> out_proj -> residual
+    -> gated feed-forward (norm) -> residual, per row across time.
+
+    Its state is wider than the Griffin sublayer's: (R, E, N) and the taps (R, 3, E), E = expand * d_model channels of N
+    states, whose decay depends on the input.  Whole sequences are differentiable; ``step`` moves the state on in
+    place for rollouts.  Any d_model; float32, or bfloat16 activations inside ``torch.autocast``.
+
+    Args:
+        d_model: width of the tokens.
+        d_state: N, states a channel (1 to 64).
+        expand: E / d_model.
+        dt_rank: rank of the step sizes' projection, d_model / 16 rounded up by default.
+    """
+
+    def __init__(self, d_model: int, d_state: int = 16, expand: int = 2, dt_rank: int | None = None) -> None:
+        super().__init__()
+        if not 1 <= d_state <= 64:
+            raise ValueError(f"d_state must be between 1 and 64, got {d_state}")
+        E = expand * d_model
+        self.d_model, self.d_state, self.d_inner = d_model, d_state, E
+        self.dt_rank = (d_model + 15) // 16 if dt_rank is None else dt_rank
+        self.norm1 = nn.RMSNorm(d_model)
+        self.in_proj = nn.Linear(d_model, 2 * E, bias=False)
+        self.conv = nn.Conv1d(E, E, kernel_size=TAPS, groups=E, bias=True)
+        self.x_proj = nn.Linear(E, self.dt_rank + 2 * d_state, bias=False)
+        self.dt_proj = nn.Linear(self.dt_rank, E, bias=True)
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, d_state + 1, dtype=torch.float32)).repeat(E, 1))
+        self.D = nn.Parameter(torch.ones(E))
+        self.out_proj = nn.Linear(E, d_model, bias=False)
+        self.norm2 = nn.RMSNorm(d_model)
+        self.gated_mlp = GatedMLP(d_model)
+        with torch.no_grad():   # step sizes of 0.001 to 0.1 at a zero input
+            rate = torch.exp(torch.rand(E) * (math.log(0.1) - math.log(0.001)) + math.log(0.001))
+            self.dt_proj.bias.copy_(rate + torch.log(-torch.expm1(-rate)))
+
+    def initial_state(self, rows: int, device=None) -> tuple[torch.Tensor, torch.Tensor]:
+        """(h (R, E, N), conv_buf (R, 3, E)), zeros."""
+        return (torch.zeros(rows, self.d_inner, self.d_state, device=device), torch.zeros(rows, TAPS - 1, self.d_inner, device=device))
+
+    def _projected(self, u: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """delta, B and C of the conv's output."""
+        dt, B, C = self.x_proj(u).split([self.dt_rank, self.d_state, self.d_state], dim=-1)
+        return F.linear(dt, self.dt_proj.weight), B, C
+
+    def _feed_forward(self, x: torch.Tensor) -> torch.Tensor:
+        mlp, n = self.gated_mlp, self.norm2(x)
+        if _capi.current_precision(x.device) == _capi.BNB_BF16:
+            n = n.to(torch.bfloat16)
+        return x + gated_mlp(n, mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight).to(x.dtype)
+
+    def _check(self, x: torch.Tensor, dims: int, h: torch.Tensor, conv_buf: torch.Tensor) -> None:
+        if x.dim() != dims or x.shape[-1] != self.d_model:
+            raise RuntimeError(f"expected an input of {dims} dims ending in {self.d_model}, got {tuple(x.shape)}")
+        R = x.shape[0]
+        if tuple(h.shape) != (R, self.d_inner, self.d_state) or tuple(conv_buf.shape) != (R, TAPS - 1, self.d_inner):
+            raise RuntimeError("h / conv_buf shapes do not match the input")
+        _capi.require_cuda(x, "x")
+
+    def forward_sequence(
+        self,
+        x_seq: torch.Tensor,  # (R, T, D)
+        h0: torch.Tensor,  # (R, E, N)
+        conv_buf: torch.Tensor,  # (R, 3, E)
+        done_mask: torch.Tensor | None = None,  # (R, T) bool
+        lengths: torch.Tensor | None = None,  # (R,) int
+    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Returns (out (R, T, D), new_h (R, E, N), new_conv_buf (R, 3, E)).  Outputs behind a row's length are those of the
+        feed-forward half alone."""
+        self._check(x_seq, 3, h0, conv_buf)
+        x = x_seq.transpose(0, 1)   # time-major, as it lies
+        done = None if done_mask is None else done_mask.transpose(0, 1)
+        u, z = self.in_proj(self.norm1(x)).split(self.d_inner, dim=-1)
+        u, taps = causal_conv(u, self.conv.weight[:, 0], self.conv.bias, state=conv_buf, done=done, lengths=lengths, activation="silu")
+        delta, B, C = self._projected(u)
+        y, h = selective_scan(u, delta, -torch.exp(self.A_log), B, C, self.D, z=z, delta_bias=self.dt_proj.bias, softplus=True,
+                              state=h0, done=done, lengths=lengths)
+        return self._feed_forward(x + self.out_proj(y).to(x.dtype)).transpose(0, 1), h, taps
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, h: torch.Tensor, conv_buf: torch.Tensor, reset: torch.Tensor | None = None) -> torch.Tensor:
+        """One token a row, without gradients: x (R, D) -> (R, D).  ``h`` (R, E, N) and ``conv_buf`` (R, 3, E) move on in
+        place; rows of ``reset`` (R,) bool start from zeros."""
+        self._check(x, 2, h, conv_buf)
+        u, z = self.in_proj(self.norm1(x)).split(self.d_inner, dim=-1)
+        u = causal_conv_step(u, conv_buf, self.conv.weight[:, 0], self.conv.bias, reset=reset, activation="silu")
+        delta, B, C = self._projected(u)
+        y = selective_step(u, delta, -torch.exp(self.A_log), B, C, self.D, h, z=z, delta_bias=self.dt_proj.bias, softplus=True, reset=reset)
+        return self._feed_forward(x + self.out_proj(y).to(x.dtype))
