@@ -164,13 +164,12 @@ __global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSel
         store_states(kept, v, NS * lane, NP, true);
         kept += kept_step;
       }
+auto walk = [&](auto with_cuts) {
+      constexpr bool cutting = decltype(with_cuts)::value;
 #pragma unroll
       for (int k = 0; k < KEEP; ++k) {
         const int t = g0 + k;
-        if ((cuts >> t) & 1) {
-          h[0] = h[1] = f2(0.f);
-          asm volatile("");   // rare, and the same for all: worth a branch
-        }
+        if (cutting && ((cuts >> t) & 1)) h[0] = h[1] = f2(0.f);
         const ulonglong2 pp = *reinterpret_cast<const ulonglong2*>(&pp_s[t][cl]), b = *reinterpret_cast<const ulonglong2*>(&b_s[t][NS * lane]);
         const F2 p{pp.x}, pu{pp.y};
         const float2 m0 = halves(mul(p, rate[0])), m1 = halves(mul(p, rate[1]));
@@ -187,6 +186,10 @@ __global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSel
           if (KL <= SUMS || lane < SUMS) y_s[t][cl][lane % SUMS] = y;
         }
       }
+      };
+      // ends of episodes are rare: without any, the steps are one run of instructions
+      if ((cuts >> g0) & ((1u << KEEP) - 1)) walk(std::true_type{});
+      else walk(std::false_type{});
     }
     __syncthreads();
     if constexpr (Y) {

@@ -12,8 +12,8 @@
 // each halving.  They are matrix products instead: D (16 x 8) += A (16 x 8) B (8 x 8) on mma.sync, where a warp's lanes hold four channels as the
 // depth and (state lane, other channels) as the columns of B just as they are, db's values in its upper half and dc's in its lower, and
 // A has ones in the rows of the step, t for db and 8 + t for dc: the accumulators of a chunk's eight steps are filled one row after
-// the other.  The operands have 11 bits: 16-bit calls round to them (a sum of many terms then is good to 2^-12 or so of its size), float32
-// calls add the products of the bits that remain.
+// the other.  The operands have 11 bits: bfloat16 calls round to them (a sum of many terms is then good to 2^-12 or so of its size, against
+// 2^-9 of the result), others add the products of the bits that remain.
 //
 // What is left of the sums over channels goes through the warps of the CTA and, where a group has several tiles of channels, a
 // short kernel over the tiles; sums over rows and time (da, dd, d bias) stay in registers while a CTA goes over its rows.  No
@@ -45,12 +45,12 @@ template <int KL> constexpr int CHANNELS = KL <= 4 ? 64 : 256 / KL;   // of a CT
 
 // d += a b, 11 bits of every operand; see above for what is where.
 __device__ __forceinline__ void mma_rows(float (&d)[4], uint32_t one, float upper, float lower) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%5,%4}, {%6,%7}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%5,%4}, {%6,%7}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(one), "r"(0u), "r"(__float_as_uint(upper)), "r"(__float_as_uint(lower)));
 }
 template <typename T>
 __device__ __forceinline__ void add_rows(float (&d)[4], uint32_t one, float upper, float lower) {
-  if constexpr (sizeof(T) == 2) {   // the product drops 13 bits: rounded to the nearest before
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {   // the product drops 13 bits: rounded to the nearest before
     mma_rows(d, one, __uint_as_float(__float_as_uint(upper) + 0x1000u), __uint_as_float(__float_as_uint(lower) + 0x1000u));
   } else {
     const float u = __uint_as_float(__float_as_uint(upper) & 0xffffe000u), l = __uint_as_float(__float_as_uint(lower) & 0xffffe000u);
@@ -209,11 +209,15 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
         }
         __syncthreads();
       } else {
+        auto walk = [&](auto with_cuts) {
+      constexpr bool cutting = decltype(with_cuts)::value;
         F2 h[L + 1][2];   // h[t]: before step t, episode ends applied; h[t + 1] behind it unless one follows
-        h[0][0] = cuts & 1 ? f2(0.f) : h0[0];
-        h[0][1] = cuts & 1 ? f2(0.f) : h0[1];
+        const bool start = cutting && (cuts & 1);
+        h[0][0] = start ? f2(0.f) : h0[0];
+        h[0][1] = start ? f2(0.f) : h0[1];
 #pragma unroll
         for (int t = 0; t < L; ++t) {
+          asm volatile("" ::: "memory");   // a step's loads stay in their step: with all in front, registers spill
           const ulonglong2 pp = *reinterpret_cast<const ulonglong2*>(&pp_s[t][cl]), b = *reinterpret_cast<const ulonglong2*>(&b_s[t][NS * lane]);
           const F2 bs[2] = {F2{b.x}, F2{b.y}};
 #pragma unroll
@@ -221,17 +225,16 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
             const float2 m = halves(mul(F2{pp.x}, rate[i]));
             h[t + 1][i] = fma(f2(ex2_fast(m.x), ex2_fast(m.y)), h[t][i], mul(F2{pp.y}, bs[i]));
           }
-          if (t + 1 < L && ((cuts >> (t + 1)) & 1)) {
-            h[t + 1][0] = h[t + 1][1] = f2(0.f);
-            asm volatile("");   // rare, and the same for all: worth a branch
-          }
+          if (cutting && t + 1 < L && ((cuts >> (t + 1)) & 1)) h[t + 1][0] = h[t + 1][1] = f2(0.f);
         }
         float sums[GROUP][3];   // over the states: c h, g b, g e h- a
+        F2 da_chunk[2];         // summed by chunks first: one long sum of float32 loses a digit
         float rows[MMA ? NS : 1][4];
 #pragma unroll
         for (int i = 0; i < (MMA ? NS : 1); ++i) rows[i][0] = rows[i][1] = rows[i][2] = rows[i][3] = 0.f;
 #pragma unroll
         for (int t = L - 1; t >= 0; --t) {
+          asm volatile("" ::: "memory");
           const ulonglong2 pp = *reinterpret_cast<const ulonglong2*>(&pp_s[t][cl]);
           const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&b_s[t][NS * lane]), c = *reinterpret_cast<const ulonglong2*>(&c_s[t][NS * lane]);
           const F2 p{pp.x}, pu{pp.y}, dy{*reinterpret_cast<const unsigned long long*>(&dy_s[t][cl])};
@@ -243,23 +246,17 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
             const float2 m = halves(mul(p, rate[i]));
             const F2 e = f2(ex2_fast(m.x), ex2_fast(m.y)), eh = mul(e, h[t][i]);
             F2 behind = h[t + 1][i];
-            if (t + 1 < L && ((cuts >> (t + 1)) & 1)) {   // cleared for the next step
-              behind = fma(pu, bs[i], eh);
-              asm volatile("");
-            }
+            if (cutting && t + 1 < L && ((cuts >> (t + 1)) & 1)) behind = fma(pu, bs[i], eh);   // cleared for the next step
             const F2 gh = fma(cs[i], dy, carry[i]), ge = mul(gh, eh);
             sy = i ? fma(cs[i], behind, sy) : mul(cs[i], behind);
             sb = i ? fma(gh, bs[i], sb) : mul(gh, bs[i]);
             sa = i ? fma(ge, rate[i], sa) : mul(ge, rate[i]);
-            da[i] = fma(ge, p, da[i]);
+            da_chunk[i] = t == L - 1 ? mul(ge, p) : fma(ge, p, da_chunk[i]);
             of_b[i] = mul(gh, pu);
             of_c[i] = mul(behind, dy);
             carry[i] = mul(gh, e);
           }
-          if ((cuts >> t) & 1) {
-            carry[0] = carry[1] = f2(0.f);
-            asm volatile("");
-          }
+          if (cutting && ((cuts >> t) & 1)) carry[0] = carry[1] = f2(0.f);
           const float2 y2 = halves(sy), b2 = halves(sb), a2 = halves(sa);
           sums[t % GROUP][0] = y2.x + y2.y;
           sums[t % GROUP][1] = b2.x + b2.y;
@@ -297,6 +294,8 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
             }
           }
         }
+        da[0] = add(da[0], da_chunk[0]);
+        da[1] = add(da[1], da_chunk[1]);
         if constexpr (MMA) {
           // this lane's row is step wl / 4 (db in rows[i][0..1], dc in [2..3]), its columns 2 (wl % 4), + 1: column = state lane times
           // 8 / KL + the channels' upper bits, over which the rest of the sum goes
@@ -326,6 +325,10 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
               }
           }
         }
+        };
+        // ends of episodes are rare: without any, the steps are one run of instructions
+        if (cuts) walk(std::true_type{});
+        else walk(std::false_type{});
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
