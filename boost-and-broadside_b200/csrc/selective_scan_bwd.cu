@@ -105,12 +105,13 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
   if (q.d) skip = f2(count > 0 ? q.d[pc] : 0.f, count > 1 ? q.d[pc + 1] : 0.f);
   const bool gated = q.z.data != nullptr;
   const T none = from_f<T>(0.f);
+  auto place = [&](const BnbView& v) { return step * v.step + pc; };
 
   for (int r = row_block; r < q.rows; r += w.row_blocks) {
     const int n = row_steps(q.lengths, r, q.steps), live = min(n, last);
     const int64_t rc = (int64_t)r * q.width + ch;
     const int begin = live > first ? (live - 1) / L * L : first - L;   // the last chunk; first is a multiple of L
-    // a step of a row; what is the same for the CTA is computed once for it
+    // A row's step: the same address for the whole CTA.  A thread's place from there is the same for every chunk.
     auto at = [&](const BnbView& v, int t) { return static_cast<T*>(v.data) + r * v.row + t * v.step; };
     auto db_at = [&](int t) { return at(g.db, t) + group * g.db.group; };
     auto dc_at = [&](int t) { return at(g.dc, t) + group * g.dc.group; };
@@ -156,14 +157,15 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
       for (int k = 0; k < BC; ++k) {
         const int e = tid + k * THREADS, t = t0 + e / NP, s = e % NP;
         const bool on = e < L * NP && s < q.states && t < live;
-        if (!LOCAL) b_r[k] = on ? at(q.b, t)[group * q.b.group + s] : none;
-        c_r[k] = on ? at(q.c, t)[group * q.c.group + s] : none;
+        if (!LOCAL) b_r[k] = on ? at(q.b, t0 + k * (THREADS / NP))[tid / NP * q.b.step + group * q.b.group + s] : none;
+        c_r[k] = on ? at(q.c, t0 + k * (THREADS / NP))[tid / NP * q.c.step + group * q.c.group + s] : none;
       }
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
         const int ts = step + k * AT_ONCE, t = t0 + ts, have = t < live ? count : 0;
-        const Raw<T, 2> u_r = load_pair<T>(at(q.u, t) + pc, LOCAL ? 0 : have, w.paired), d_r = load_pair<T>(at(q.delta, t) + pc, have, w.paired);
-        const Raw<T, 2> z_r = load_pair<T>(at(q.z, t) + pc, gated ? have : 0, w.paired), y_r = load_pair<T>(at(g.dy, t) + pc, have, w.paired);
+        const int tu = t0 + k * AT_ONCE;
+        const Raw<T, 2> u_r = load_pair<T>(at(q.u, tu) + place(q.u), LOCAL ? 0 : have, w.paired), d_r = load_pair<T>(at(q.delta, tu) + place(q.delta), have, w.paired);
+        const Raw<T, 2> z_r = load_pair<T>(at(q.z, tu) + place(q.z), gated ? have : 0, w.paired), y_r = load_pair<T>(at(g.dy, tu) + place(g.dy), have, w.paired);
         const F2 u = floats_of<T>(u_r), raw = add(floats_of<T>(d_r), bias), dy = floats_of<T>(y_r);
         const F2 p = t < live ? step_size(raw, q.softplus) : f2(0.f);
         F2 dyv = dy, dgate = f2(0.f);   // dgate: dy silu'(z)
@@ -339,9 +341,9 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
           const F2 u = pair_of(&held_s[t][0][2 * pair]), slope = pair_of(&held_s[t][1][2 * pair]), dgate = pair_of(&held_s[t][2][2 * pair]);
           const F2 p = f2(pp_s[t][2 * pair].x, pp_s[t][2 * pair + 1].x), dyv = f2(dy_s[t][2 * pair].x, dy_s[t][2 * pair + 1].x);
           const F2 draw = mul(fma(sa, f2(1.0f / LOG2E), mul(sb, u)), slope);
-          store_pair(at(g.du, t0 + t) + pc, fma(sb, p, mul(skip, dyv)), count, w.paired);
-          store_pair(at(g.ddelta, t0 + t) + pc, draw, count, w.paired);
-          if (gated) store_pair(at(g.dz, t0 + t) + pc, mul(dgate, fma(skip, u, sy)), count, w.paired);
+          store_pair(at(g.du, t0 + k * AT_ONCE) + place(g.du), fma(sb, p, mul(skip, dyv)), count, w.paired);
+          store_pair(at(g.ddelta, t0 + k * AT_ONCE) + place(g.ddelta), draw, count, w.paired);
+          if (gated) store_pair(at(g.dz, t0 + k * AT_ONCE) + place(g.dz), mul(dgate, fma(skip, u, sy)), count, w.paired);
           dd = fma(dyv, u, dd);
           dbias = add(dbias, draw);
         }
