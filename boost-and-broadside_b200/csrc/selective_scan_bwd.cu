@@ -39,6 +39,7 @@ struct Work {
   int tiles_a_group;
   int row_blocks;
   bool paired;       // pairs of channels of u, delta, z, dy and their gradients lie on their boundary
+  bool paired_bc;    // and pairs of states of b and c
 };
 
 template <int KL> constexpr int CHANNELS = KL <= 4 ? 64 : 256 / KL;   // of a CTA
@@ -59,12 +60,22 @@ __device__ __forceinline__ void add_rows(float (&d)[4], uint32_t one, float uppe
   }
 }
 
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
+}
+// Two neighbouring elements, or those of `count` that exist and zeros: under way with one access where they lie on their boundary.
+template <typename T>
+__device__ __forceinline__ void copy_pair(Raw<T, 2>* to, const T* from, int count, bool paired) {
+  if (paired && count == 2) copy_async<2 * sizeof(T)>(to, from);
+  else *to = load_pair<T>(from, count, false);
+}
+
 // LOCAL: only what a split leaves of a zero adjoint behind it, see selective_scan.cuh.
 template <typename T, int KL, bool LOCAL>
 __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<KL> * KL) : 2) k_scan_bwd(const __grid_constant__ BnbSelectiveScan q, const __grid_constant__ BnbSelectiveScanGrads g, const __grid_constant__ Work w) {
   constexpr int CT = CHANNELS<KL>, THREADS = CT * KL, NP = NS * KL, WARPS = THREADS / 32;
   constexpr int BITS = KL == 1 ? 0 : KL == 2 ? 1 : KL == 4 ? 2 : KL == 8 ? 3 : 4, CB = 5 - BITS;   // lane: channel in the low CB bits, state lane above
-  constexpr int BC = (L * NP + THREADS - 1) / THREADS;
   constexpr int PAIRS = CT / 2, AT_ONCE = THREADS / PAIRS < L ? THREADS / PAIRS : L, PER = L / AT_ONCE;   // steps prepared at a time, by a thread
   constexpr int GROUP = 4;         // steps whose sums over a channel's lanes are taken together
   constexpr bool MMA = KL <= 8;    // with 16 lanes a channel, four neighbouring lanes are not four channels
@@ -73,6 +84,10 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
   __shared__ __align__(16) float b_s[LOCAL ? 1 : L][NP], c_s[L][NP];
   __shared__ __align__(16) float held_s[LOCAL ? 1 : L][3][CT];        // u, softplus', dy silu'(z)
   __shared__ __align__(16) float sum_s[LOCAL ? 1 : L][3][CT];
+  // the next chunk, on its way while this one is computed: a thread copies what it reads itself
+  constexpr int PREPARE = PAIRS * AT_ONCE, BC = (LOCAL ? 1 : 2) * L * NP / 2, BC_PER = (BC + THREADS - 1) / THREADS;
+  __shared__ __align__(16) Raw<T, 2> next_s[PER][4][PREPARE], next_bc_s[BC_PER][THREADS];   // u, delta, z, dy; pairs of c, then of b
+  __shared__ __align__(16) float4 next_h_s[LOCAL ? 1 : THREADS];
   extern __shared__ __align__(16) float red[];   // (L, WARPS, 2 NP): sums over a warp's channels
   const int tid = threadIdx.x, warp = tid / 32, wl = tid & 31, lane = wl >> CB, cl = warp * (32 / KL) + (wl & ((1 << CB) - 1));
   const int tiles = w.tiles_a_group * q.groups, share = q.width / q.groups;
@@ -106,11 +121,44 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
   const bool gated = q.z.data != nullptr;
   const T none = from_f<T>(0.f);
   auto place = [&](const BnbView& v) { return step * v.step + pc; };
+  // starts the copies of row r's chunk at t0, of which the steps before `live` exist
+  auto fetch = [&](int r, int t0, int live) {
+    auto at = [&](const BnbView& v, int t) { return static_cast<const T*>(v.data) + r * v.row + t * v.step; };
+    if (step < AT_ONCE) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int tu = t0 + k * AT_ONCE, have = tu + step < live ? count : 0;
+        if (!LOCAL) copy_pair(&next_s[k][0][tid], at(q.u, tu) + place(q.u), have, w.paired);
+        copy_pair(&next_s[k][1][tid], at(q.delta, tu) + place(q.delta), have, w.paired);
+        copy_pair(&next_s[k][2][tid], at(q.z, tu) + place(q.z), gated ? have : 0, w.paired);
+        copy_pair(&next_s[k][3][tid], at(g.dy, tu) + place(g.dy), have, w.paired);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < BC_PER; ++k) {
+      const int x = tid + k * THREADS, e = x % (L * NP / 2), t = e / (NP / 2), s = e % (NP / 2) * 2;
+      const BnbView& v = x < L * NP / 2 ? q.c : q.b;
+      if (x < BC) copy_pair(&next_bc_s[k][tid], at(v, t0 + t) + group * v.group + s, t0 + t < live ? max(0, min(2, q.states - s)) : 0, w.paired_bc);
+    }
+    if (!LOCAL && owns) copy_async<16>(&next_h_s[tid], q.kept + ((int64_t)(t0 / KEEP) * q.rows * q.width + (int64_t)r * q.width + ch) * NP + NS * lane);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // whether an episode ended before this lane's step of a chunk
+  auto ended = [&](int r, int t0, int live) -> uint8_t {
+    const int t = t0 + wl - 1;
+    return q.done && wl < L && t >= 0 && t + 1 < live ? q.done[(int64_t)t * q.rows + r] : 0;
+  };
+  auto last_chunk = [&](int live) { return live > first ? (live - 1) / L * L : first - L; };   // first is a multiple of L
+  if (!LOCAL && !owns) next_h_s[tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool fetched = false;
+  uint8_t ended_next = 0;
+  int n_next = row_block < q.rows ? row_steps(q.lengths, row_block, q.steps) : 0;
 
   for (int r = row_block; r < q.rows; r += w.row_blocks) {
-    const int n = row_steps(q.lengths, r, q.steps), live = min(n, last);
+    const int n = n_next, live = min(n, last), r_next = r + w.row_blocks;
+    if (r_next < q.rows) n_next = row_steps(q.lengths, r_next, q.steps);
     const int64_t rc = (int64_t)r * q.width + ch;
-    const int begin = live > first ? (live - 1) / L * L : first - L;   // the last chunk; first is a multiple of L
+    const int begin = last_chunk(live);
     // A row's step: the same address for the whole CTA.  A thread's place from there is the same for every chunk.
     auto at = [&](const BnbView& v, int t) { return static_cast<T*>(v.data) + r * v.row + t * v.step; };
     auto db_at = [&](int t) { return at(g.db, t) + group * g.db.group; };
@@ -143,29 +191,21 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
     }
     float sum_p = 0.f;
     bool any_cut = false;
+    if (!fetched && begin >= first) {
+      fetch(r, begin, live);
+      ended_next = ended(r, begin, live);
+    }
+    fetched = false;
 #pragma unroll 1
     for (int t0 = begin; t0 >= first; t0 -= L) {
-      unsigned cuts = 0;   // bit k: an episode ended before step t0 + k
-      if (q.done) {
-        const int t = t0 + wl - 1;
-        cuts = __ballot_sync(0xffffffffu, wl < L && t >= 0 && t + 1 < live && q.done[(int64_t)max(t, 0) * q.rows + r]);
-      }
-      float4 h_r = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (!LOCAL && owns) h_r = *reinterpret_cast<const float4*>(q.kept + ((int64_t)(t0 / KEEP) * q.rows * q.width + rc) * NP + NS * lane);
-      T b_r[BC], c_r[BC];
-#pragma unroll
-      for (int k = 0; k < BC; ++k) {
-        const int e = tid + k * THREADS, t = t0 + e / NP, s = e % NP;
-        const bool on = e < L * NP && s < q.states && t < live;
-        if (!LOCAL) b_r[k] = on ? at(q.b, t0 + k * (THREADS / NP))[tid / NP * q.b.step + group * q.b.group + s] : none;
-        c_r[k] = on ? at(q.c, t0 + k * (THREADS / NP))[tid / NP * q.c.step + group * q.c.group + s] : none;
-      }
+      const unsigned cuts = __ballot_sync(0xffffffffu, ended_next != 0);   // bit k: an episode ended before step t0 + k
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      const float4 h_r = LOCAL ? make_float4(0.f, 0.f, 0.f, 0.f) : next_h_s[LOCAL ? 0 : tid];
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int ts = step + k * AT_ONCE, t = t0 + ts, have = t < live ? count : 0;
-        const int tu = t0 + k * AT_ONCE;
-        const Raw<T, 2> u_r = load_pair<T>(at(q.u, tu) + place(q.u), LOCAL ? 0 : have, w.paired), d_r = load_pair<T>(at(q.delta, tu) + place(q.delta), have, w.paired);
-        const Raw<T, 2> z_r = load_pair<T>(at(q.z, tu) + place(q.z), gated ? have : 0, w.paired), y_r = load_pair<T>(at(g.dy, tu) + place(g.dy), have, w.paired);
+        if (step >= AT_ONCE) continue;
+        const int ts = step + k * AT_ONCE, t = t0 + ts;
+        const Raw<T, 2> u_r = next_s[k][0][tid], d_r = next_s[k][1][tid], z_r = next_s[k][2][tid], y_r = next_s[k][3][tid];
         const F2 u = floats_of<T>(u_r), raw = add(floats_of<T>(d_r), bias), dy = floats_of<T>(y_r);
         const F2 p = t < live ? step_size(raw, q.softplus) : f2(0.f);
         F2 dyv = dy, dgate = f2(0.f);   // dgate: dy silu'(z)
@@ -174,7 +214,7 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
           dyv = mul(dy, mul(z, sg));
           dgate = mul(dy, mul(sg, fma(z, fma(sg, f2(-1.0f), f2(1.0f)), f2(1.0f))));
         }
-        if (step < L) {
+        {
           const float2 ps = halves(p), pu = halves(mul(p, u)), ds = halves(dyv);
           pp_s[ts][2 * pair] = make_float4(ps.x, ps.x, pu.x, pu.x);
           pp_s[ts][2 * pair + 1] = make_float4(ps.y, ps.y, pu.y, pu.y);
@@ -188,16 +228,24 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
         }
       }
 #pragma unroll
-      for (int k = 0; k < BC; ++k) {
-        const int e = tid + k * THREADS;
-        if (e < L * NP) {
-          if (!LOCAL) (&b_s[0][0])[e] = to_f(b_r[k]);
-          (&c_s[0][0])[e] = to_f(c_r[k]);
-        }
+      for (int k = 0; k < BC_PER; ++k) {
+        const int x = tid + k * THREADS;
+        if (x < BC) *reinterpret_cast<float2*>(x < L * NP / 2 ? &c_s[0][0] + 2 * x : &b_s[0][0] + 2 * x - L * NP) = halves(floats_of<T>(next_bc_s[k][tid]));
       }
       const F2 h0[2] = {f2(h_r.x, h_r.y), f2(h_r.z, h_r.w)};
       any_cut |= cuts != 0;
       __syncthreads();
+      if (t0 > first) {
+        fetch(r, t0 - L, live);
+        ended_next = ended(r, t0 - L, live);
+      } else if (r_next < q.rows) {
+        const int of = min(n_next, last), begins = last_chunk(of);
+        fetched = begins >= first;
+        if (fetched) {
+          fetch(r_next, begins, of);
+          ended_next = ended(r_next, begins, of);
+        }
+      }
       if constexpr (LOCAL) {
 #pragma unroll
         for (int t = L - 1; t >= 0; --t) {
@@ -477,6 +525,7 @@ int launch(const BnbSelectiveScan& a, const BnbSelectiveScanGrads& g, const Plan
   w.row_blocks = p.row_blocks;
   w.paired = a.width / a.groups % 2 == 0 && even_view(a.u, a.element) && even_view(a.delta, a.element) && even_view(g.dy, a.element) &&
              even_view(g.du, a.element) && even_view(g.ddelta, a.element) && (!a.z.data || (even_view(a.z, a.element) && even_view(g.dz, a.element)));
+  w.paired_bc = even_view(a.b, a.element) && even_view(a.c, a.element) && a.b.group % 2 == 0 && a.c.group % 2 == 0;
   w.carry = reinterpret_cast<float*>(scratch);
   w.sum_p = reinterpret_cast<float*>(scratch + p.sum_p);
   w.cut = scratch + p.cut;
