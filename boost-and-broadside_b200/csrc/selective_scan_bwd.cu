@@ -10,16 +10,22 @@
 //
 // Sums over the channels (db, dc), 2 NS values a thread and step, are the most work of all if they go through shuffles: four instructions for
 // each halving.  They are matrix products instead: D (16 x 8) += A (16 x 8) B (8 x 8) on mma.sync, where a warp's lanes hold four channels as the
-// depth and (state lane, other channels) as the columns of B just as they are, db's values in its upper half and dc's in its lower, and
-// A has ones in the rows of the step, t for db and 8 + t for dc: the accumulators of a chunk's eight steps are filled one row after
-// the other.  The operands have 11 bits: bfloat16 calls round to them (a sum of many terms is then good to 2^-12 or so of its size, against
+// depth and (state lane, other channels) as the rows of A just as they are, db's values in its upper half and dc's in its lower, one
+// state in the depths 0 .. 3 and a second one in 4 .. 7.  B has ones in a step's two columns, so that the accumulators of four steps are
+// filled two columns after two.  (With the values in B, which holds half of what A does, twice the products were needed: 2030 us against
+// 2020 at 32 steps x 8192 rows x 256 channels x 16 states in bfloat16, and more in float32, where there are twice as many.)
+// The operands have 11 bits: bfloat16 calls round to them (a sum of many terms is then good to 2^-12 or so of its size, against
 // 2^-9 of the result), others add the products of the bits that remain.
 //
 // What is left of the sums over channels goes through the warps of the CTA and, where a group has several tiles of channels, a
 // short kernel over the tiles; sums over rows and time (da, dd, d bias) stay in registers while a CTA goes over its rows.  No
 // atomics, so a result does not depend on timing.
 //
-// About 25 instructions a state and step bound it, two exponentials among them; memory moves some 24 bytes a channel and step.
+// Some 140 instructions for a warp's step of 8 channels x 16 states bound it (8 exponentials, 60 for the recurrence and its adjoint, 14 for db
+// and dc, 12 for the sums over a channel's lanes, the rest per chunk), issued in 55 % of the cycles: at 128 registers a thread 16 warps fit on an
+// SM.  Registers decide what else may be tried: a version with 20 more values alive in the walk spilled, and took 2460 us, not 2020.
+// Memory moves some 24 bytes a channel and step, 20 % of what it could.  The next chunk's operands therefore come by asynchronous
+// copies into shared memory, which hold no register (2220 -> 2150 us).
 #include "selective_scan.cuh"
 
 namespace bnb {
@@ -45,19 +51,25 @@ struct Work {
 template <int KL> constexpr int CHANNELS = KL <= 4 ? 64 : 256 / KL;   // of a CTA
 
 // d += a b, 11 bits of every operand; see above for what is where.
-__device__ __forceinline__ void mma_rows(float (&d)[4], uint32_t one, float upper, float lower) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%5,%4}, {%6,%7}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(one), "r"(0u), "r"(__float_as_uint(upper)), "r"(__float_as_uint(lower)));
+__device__ __forceinline__ void mma_rows(float (&d)[4], const float (&a)[4], const uint32_t (&one)[2]) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])), "r"(one[0]), "r"(one[1]));
 }
 template <typename T>
-__device__ __forceinline__ void add_rows(float (&d)[4], uint32_t one, float upper, float lower) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {   // the product drops 13 bits: rounded to the nearest before
-    mma_rows(d, one, __uint_as_float(__float_as_uint(upper) + 0x1000u), __uint_as_float(__float_as_uint(lower) + 0x1000u));
-  } else {
-    const float u = __uint_as_float(__float_as_uint(upper) & 0xffffe000u), l = __uint_as_float(__float_as_uint(lower) & 0xffffe000u);
-    mma_rows(d, one, upper - u, lower - l);
-    mma_rows(d, one, u, l);
+__device__ __forceinline__ void add_rows(float (&d)[4], const float (&a)[4], const uint32_t (&one)[2]) {
+  float high[4], low[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {   // the product drops 13 bits: rounded to the nearest before
+      high[i] = __uint_as_float(__float_as_uint(a[i]) + 0x1000u);
+    } else {
+      high[i] = __uint_as_float(__float_as_uint(a[i]) & 0xffffe000u);
+      low[i] = a[i] - high[i];
+    }
   }
+  if constexpr (!std::is_same<T, __nv_bfloat16>::value) mma_rows(d, low, one);
+  mma_rows(d, high, one);
 }
 
 template <int BYTES>
@@ -77,18 +89,19 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
   constexpr int CT = CHANNELS<KL>, THREADS = CT * KL, NP = NS * KL, WARPS = THREADS / 32;
   constexpr int BITS = KL == 1 ? 0 : KL == 2 ? 1 : KL == 4 ? 2 : KL == 8 ? 3 : 4, CB = 5 - BITS;   // lane: channel in the low CB bits, state lane above
   constexpr int PAIRS = CT / 2, AT_ONCE = THREADS / PAIRS < L ? THREADS / PAIRS : L, PER = L / AT_ONCE;   // steps prepared at a time, by a thread
-  constexpr int GROUP = 4;         // steps whose sums over a channel's lanes are taken together
+  constexpr int GROUP = 2;         // steps whose sums over a channel's lanes are taken together: with 4, 6 more values live and spill
   constexpr bool MMA = KL <= 8;    // with 16 lanes a channel, four neighbouring lanes are not four channels
+  constexpr int PARTS = MMA ? 8 / KL : 1, RED = PARTS * 2 * NP;   // sums over a part of a warp's channels, a step's of a warp
   __shared__ __align__(16) float4 pp_s[L][CT];                        // p, p, p u, p u
   __shared__ __align__(16) float2 dy_s[L][CT];                        // dyv twice
   __shared__ __align__(16) float b_s[LOCAL ? 1 : L][NP], c_s[L][NP];
-  __shared__ __align__(16) float held_s[LOCAL ? 1 : L][3][CT];        // u, softplus', dy silu'(z)
   __shared__ __align__(16) float sum_s[LOCAL ? 1 : L][3][CT];
+  __shared__ __align__(16) float held_s[LOCAL ? 1 : L][3][CT];        // u, softplus', dy silu'(z)
   // the next chunk, on its way while this one is computed: a thread copies what it reads itself
   constexpr int PREPARE = PAIRS * AT_ONCE, BC = (LOCAL ? 1 : 2) * L * NP / 2, BC_PER = (BC + THREADS - 1) / THREADS;
   __shared__ __align__(16) Raw<T, 2> next_s[PER][4][PREPARE], next_bc_s[BC_PER][THREADS];   // u, delta, z, dy; pairs of c, then of b
   __shared__ __align__(16) float4 next_h_s[LOCAL ? 1 : THREADS];
-  extern __shared__ __align__(16) float red[];   // (L, WARPS, 2 NP): sums over a warp's channels
+  extern __shared__ __align__(16) float red[];   // (L, WARPS, 2, PARTS, NP): sums over channels
   const int tid = threadIdx.x, warp = tid / 32, wl = tid & 31, lane = wl >> CB, cl = warp * (32 / KL) + (wl & ((1 << CB) - 1));
   const int tiles = w.tiles_a_group * q.groups, share = q.width / q.groups;
   const int row_block = blockIdx.x / tiles, tile = blockIdx.x - row_block * tiles, group = tile / w.tiles_a_group, tile_in = tile - group * w.tiles_a_group;
@@ -261,10 +274,9 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
       } else {
         auto walk = [&](auto with_cuts) {
       constexpr bool cutting = decltype(with_cuts)::value;
-        F2 h[L + 1][2];   // h[t]: before step t, episode ends applied; h[t + 1] behind it unless one follows
-        const bool start = cutting && (cuts & 1);
-        h[0][0] = start ? f2(0.f) : h0[0];
-        h[0][1] = start ? f2(0.f) : h0[1];
+        F2 h[L + 1][2];   // behind step t - 1
+        h[0][0] = h0[0];
+        h[0][1] = h0[1];
 #pragma unroll
         for (int t = 0; t < L; ++t) {
           asm volatile("" ::: "memory");   // a step's loads stay in their step: with all in front, registers spill
@@ -273,30 +285,30 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float2 m = halves(mul(F2{pp.x}, rate[i]));
-            h[t + 1][i] = fma(f2(ex2_fast(m.x), ex2_fast(m.y)), h[t][i], mul(F2{pp.y}, bs[i]));
+            h[t + 1][i] = fma(f2(ex2_fast(m.x), ex2_fast(m.y)), cutting && ((cuts >> t) & 1) ? f2(0.f) : h[t][i], mul(F2{pp.y}, bs[i]));
           }
-          if (cutting && t + 1 < L && ((cuts >> (t + 1)) & 1)) h[t + 1][0] = h[t + 1][1] = f2(0.f);
         }
-        float sums[GROUP][3];   // over the states: c h, g b, g e h- a
+        struct Step { ulonglong2 pp, b, c; unsigned long long dy; };
+        auto operands = [&](int t) -> Step {
+          return {*reinterpret_cast<const ulonglong2*>(&pp_s[t][cl]), *reinterpret_cast<const ulonglong2*>(&b_s[t][NS * lane]),
+                  *reinterpret_cast<const ulonglong2*>(&c_s[t][NS * lane]), *reinterpret_cast<const unsigned long long*>(&dy_s[t][cl])};
+        };
+        Step next = operands(L - 1);
         F2 da_chunk[2];         // summed by chunks first: one long sum of float32 loses a digit
-        float rows[MMA ? NS : 1][4];
-#pragma unroll
-        for (int i = 0; i < (MMA ? NS : 1); ++i) rows[i][0] = rows[i][1] = rows[i][2] = rows[i][3] = 0.f;
+        float rows[2][4], sums[GROUP][3];   // over the states: c h, g b, g e h- a
 #pragma unroll
         for (int t = L - 1; t >= 0; --t) {
           asm volatile("" ::: "memory");
-          const ulonglong2 pp = *reinterpret_cast<const ulonglong2*>(&pp_s[t][cl]);
-          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&b_s[t][NS * lane]), c = *reinterpret_cast<const ulonglong2*>(&c_s[t][NS * lane]);
-          const F2 p{pp.x}, pu{pp.y}, dy{*reinterpret_cast<const unsigned long long*>(&dy_s[t][cl])};
-          const F2 bs[2] = {F2{b.x}, F2{b.y}}, cs[2] = {F2{c.x}, F2{c.y}};
+          const Step now = next;   // the step's operands came while the one behind it was computed
+          if (t) next = operands(t - 1);
+          const F2 p{now.pp.x}, pu{now.pp.y}, dy{now.dy};
+          const F2 bs[2] = {F2{now.b.x}, F2{now.b.y}}, cs[2] = {F2{now.c.x}, F2{now.c.y}};
           F2 sy = f2(0.f), sb = f2(0.f), sa = f2(0.f);
           F2 of_b[2], of_c[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float2 m = halves(mul(p, rate[i]));
-            const F2 e = f2(ex2_fast(m.x), ex2_fast(m.y)), eh = mul(e, h[t][i]);
-            F2 behind = h[t + 1][i];
-            if (cutting && t + 1 < L && ((cuts >> (t + 1)) & 1)) behind = fma(pu, bs[i], eh);   // cleared for the next step
+            const F2 e = f2(ex2_fast(m.x), ex2_fast(m.y)), eh = mul(e, cutting && ((cuts >> t) & 1) ? f2(0.f) : h[t][i]), behind = h[t + 1][i];
             const F2 gh = fma(cs[i], dy, carry[i]), ge = mul(gh, eh);
             sy = i ? fma(cs[i], behind, sy) : mul(cs[i], behind);
             sb = i ? fma(gh, bs[i], sb) : mul(gh, bs[i]);
@@ -311,24 +323,6 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
           sums[t % GROUP][0] = y2.x + y2.y;
           sums[t % GROUP][1] = b2.x + b2.y;
           sums[t % GROUP][2] = a2.x + a2.y;
-          float bc[2 * NS];
-          put(*reinterpret_cast<float(*)[NS]>(&bc[0]), of_b);
-          put(*reinterpret_cast<float(*)[NS]>(&bc[NS]), of_c);
-          if constexpr (MMA) {
-            const uint32_t one = (wl >> 2) == t ? 0x3f800000u : 0u;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) add_rows<T>(rows[i], one, bc[i], bc[NS + i]);
-          } else {   // over the warp's channels by shuffles
-            const int at = sum_lanes<2 * NS, 0, CB>(bc);
-            constexpr int LEFT = (2 * NS) >> CB ? (2 * NS) >> CB : 1;
-            if (writes_sum<2 * NS, 0, CB>()) {
-#pragma unroll
-              for (int k = 0; k < LEFT; ++k) {
-                const int v = at + k;   // 0 .. 3: b, 4 .. 7: c
-                red[(t * WARPS + warp) * 2 * NP + (v / NS) * NP + NS * lane + v % NS] = bc[k];
-              }
-            }
-          }
           if (t % GROUP == 0) {   // over the channel's lanes
 #pragma unroll
             for (int s = 0; s < 3; ++s) {
@@ -343,38 +337,40 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
               }
             }
           }
+          if constexpr (MMA) {
+            const uint32_t one[2] = {(wl >> 2) == 2 * (t % 4) ? 0x3f800000u : 0u, (wl >> 2) == 2 * (t % 4) + 1 ? 0x3f800000u : 0u};
+            if (t % 4 == 3)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) rows[i][0] = rows[i][1] = rows[i][2] = rows[i][3] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 fb = halves(of_b[i]), fc = halves(of_c[i]);
+              const float a[4] = {fb.x, fc.x, fb.y, fc.y};
+              add_rows<T>(rows[i], a, one);
+            }
+            if (t % 4 == 0) {   // this lane's sums are of step t + wl % 4 and of all four states of the state lane of row wl / 4
+              const int g8 = wl >> 2;
+              float* to = &red[((t + (wl & 3)) * WARPS + warp) * RED + (g8 % PARTS) * NP + g8 / PARTS * NS];
+              *reinterpret_cast<float4*>(to) = make_float4(rows[0][0], rows[0][1], rows[1][0], rows[1][1]);
+              *reinterpret_cast<float4*>(to + PARTS * NP) = make_float4(rows[0][2], rows[0][3], rows[1][2], rows[1][3]);
+            }
+          } else {   // over the warp's channels by shuffles
+            float bc[2 * NS];
+            put(*reinterpret_cast<float(*)[NS]>(&bc[0]), of_b);
+            put(*reinterpret_cast<float(*)[NS]>(&bc[NS]), of_c);
+            const int at = sum_lanes<2 * NS, 0, CB>(bc);
+            constexpr int LEFT = (2 * NS) >> CB ? (2 * NS) >> CB : 1;
+            if (writes_sum<2 * NS, 0, CB>()) {
+#pragma unroll
+              for (int k = 0; k < LEFT; ++k) {
+                const int v = at + k;   // 0 .. 3: b, 4 .. 7: c
+                red[(t * WARPS + warp) * RED + (v / NS) * NP + NS * lane + v % NS] = bc[k];
+              }
+            }
+          }
         }
         da[0] = add(da[0], da_chunk[0]);
         da[1] = add(da[1], da_chunk[1]);
-        if constexpr (MMA) {
-          // this lane's row is step wl / 4 (db in rows[i][0..1], dc in [2..3]), its columns 2 (wl % 4), + 1: column = state lane times
-          // 8 / KL + the channels' upper bits, over which the rest of the sum goes
-          const int t = wl >> 2, m = wl & 3;
-          float v[2][KL == 8 ? 2 : 1][NS];
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < NS; ++i) {
-              if constexpr (KL == 8) {
-                v[s][0][i] = rows[i][2 * s];
-                v[s][1][i] = rows[i][2 * s + 1];
-              } else {
-                v[s][0][i] = rows[i][2 * s] + rows[i][2 * s + 1];
-                if (KL <= 2) v[s][0][i] += __shfl_xor_sync(0xffffffffu, v[s][0][i], 1);
-                if (KL == 1) v[s][0][i] += __shfl_xor_sync(0xffffffffu, v[s][0][i], 2);
-              }
-            }
-          const bool writes = KL >= 4 || (KL == 2 ? (m & 1) == 0 : m == 0);
-          if (writes) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int x = 0; x < (KL == 8 ? 2 : 1); ++x) {
-                const int of = KL == 8 ? 2 * m + x : KL == 4 ? m : KL == 2 ? m >> 1 : 0;   // state lane
-                *reinterpret_cast<float4*>(&red[(t * WARPS + warp) * 2 * NP + s * NP + NS * of]) = make_float4(v[s][x][0], v[s][x][1], v[s][x][2], v[s][x][3]);
-              }
-          }
-        }
         };
         // ends of episodes are rare: without any, the steps are one run of instructions
         if (cuts) walk(std::true_type{});
@@ -400,7 +396,8 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
           if (t0 + t >= live) break;
           float v = 0.f;
 #pragma unroll
-          for (int k = 0; k < WARPS; ++k) v += red[(t * WARPS + k) * 2 * NP + s];
+          for (int k = 0; k < WARPS * PARTS; ++k)   // dc's parts in another order than db's, for the banks
+            v += red[(t * WARPS + k / PARTS) * RED + (s < NP ? 0 : PARTS * NP) + ((k % PARTS) ^ (s < NP || PARTS == 1 ? 0 : 1)) * NP + s % NP];
           if (part_bc) part_bc[(t0 + t) * part_step + s] = v;
           else if (s < NP) { if (s < q.states) db_at(t0 + t)[s] = from_f<T>(v); }
           else if (s - NP < q.states) dc_at(t0 + t)[s - NP] = from_f<T>(v);
@@ -518,7 +515,7 @@ Plan plan_of(const BnbSelectiveScan& a) {
 template <typename T, int KL>
 int launch(const BnbSelectiveScan& a, const BnbSelectiveScanGrads& g, const Plan& p, uint8_t* scratch, cudaStream_t st) {
   constexpr int CT = CHANNELS<KL>, NP = NS * KL, WARPS = CT * KL / 32;
-  constexpr size_t RED = (size_t)L * WARPS * 2 * NP * 4;   // at most 32 KB beside 17 KB of static shared memory
+  constexpr size_t RED = (size_t)L * WARPS * 2 * (NP < 32 ? 32 : NP) * 4;   // at most 32 KB, beside 40 KB of static shared memory
   Work w{};
   w.splits = p.splits;
   w.tiles_a_group = p.tiles_a_group;
