@@ -175,11 +175,24 @@ __global__ void __launch_bounds__(256) k_join(float* local, const float* sum_p, 
   const bool real = n < states;
   const float rate = real ? a[(int64_t)c * states + n] * LOG2E : 0.f;
   float run = real && start ? start[rc * states + n] : 0.f;
-  for (int k = 0; k < count; ++k) {
-    const int s = REVERSE ? count - 1 - k : k;
-    const float left = local[s * cells + i];
-    local[s * cells + i] = run;
-    run = (cut[(int64_t)s * rows + r] ? 0.f : ex2_fast(rate * sum_p[s * (int64_t)rows * width + rc]) * run) + left;
+  constexpr int AT_ONCE = 4;   // splits whose loads are on their way together
+  for (int k0 = 0; k0 < count; k0 += AT_ONCE) {
+    float left[AT_ONCE], sums[AT_ONCE];
+    bool passes[AT_ONCE];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int64_t s = REVERSE ? max(count - 1 - k0 - k, 0) : min(k0 + k, count - 1);
+      left[k] = local[s * cells + i];
+      sums[k] = sum_p[s * rows * width + rc];
+      passes[k] = !cut[s * rows + r];
+    }
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      if (k0 + k >= count) break;
+      const int64_t s = REVERSE ? count - 1 - k0 - k : k0 + k;
+      local[s * cells + i] = run;
+      run = (passes[k] ? ex2_fast(rate * sums[k]) * run : 0.f) + left[k];
+    }
   }
 }
 
