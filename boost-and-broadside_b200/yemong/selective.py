@@ -98,6 +98,9 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
 
     Returns:
         y (T, R, C) in u's type and the state (R, C, N) behind the last step.
+
+    An infinity or NaN among an episode's values stays in it, with one exception: the gradients of B and C may show it in
+    the row's other episodes too, up to eight steps away.
     """
     B, C = _grouped("selective_scan", "B", B, 3), _grouped("selective_scan", "C", C, 3)
     if _ops.direct(u):

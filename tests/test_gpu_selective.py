@@ -239,6 +239,9 @@ SCAN = [
     (200, 2, 40, 16, 1, torch.float32, "batch", "done ragged"),      # several splits of time
     (333, 1, 70, 5, 1, torch.bfloat16, "dense", ""),
     (261, 3, 12, 64, 1, torch.float32, "dense", "done ragged"),
+    (20, 700, 8, 16, 1, torch.bfloat16, "dense", "done ragged"),     # more rows than are worked on at once, some without steps
+    (11, 650, 3, 3, 1, torch.float32, "columns", "ragged"),
+    (9, 610, 16, 64, 1, torch.float16, "batch", "done ragged"),
 ]
 
 
@@ -300,6 +303,50 @@ def test_selective_scan(T, R, W, N, G, dtype, layout, masks, full):
     again = torch.autograd.grad(bnb.selective_scan(u, delta, A, B, C, D, **kwargs), [t for t in leaves if t is not None],
                                 [_layout(_nan_behind(dy, lengths), layout), ds.to(DEV)])
     assert all(torch.equal(a, b) for a, b in zip(again, got))   # sums in a fixed order
+
+
+@pytest.mark.parametrize("first,behind", [(8, 16), (6, 18)])
+def test_an_ended_episode_keeps_its_values(first, behind):
+    """Infinities and NaN of an episode, its gradients' too, do not reach the next or the last one's values.  The gradients of B and C
+    are the exception that is documented: they may within eight steps."""
+    import boost_and_broadside_b200 as bnb
+
+    g = torch.Generator().manual_seed(21)
+    T, R, W, N = 24, 3, 40, 16
+    u, delta, A, B, C, D, z, bias, state = [t.to(DEV) for t in _scan_inputs(g, T, R, W, N, 1, torch.float32)]
+    done = torch.zeros(T, R, dtype=torch.bool, device=DEV)
+    done[first - 1] = done[behind - 1] = True
+    dy = _r(g, T, R, W).to(DEV)
+    runs = []
+    for value in (0.0, float("nan"), float("inf")):
+        v, gy = u.clone(), dy.clone()
+        v[10, :, 3] = value
+        gy[12, :, 5] = value
+        leaves = [t.clone().requires_grad_(True) for t in (v, delta, z, B, C, state)]
+        y, st = bnb.selective_scan(leaves[0], leaves[1], A, leaves[3], leaves[4], D, z=leaves[2], delta_bias=bias, softplus=True, state=leaves[5], done=done)
+        runs.append([y, *torch.autograd.grad([y, st], leaves, [gy, torch.ones_like(st)]), st])
+    for other in runs[1:]:
+        for a, b in zip(runs[0][:4], other[:4]):   # per step: y and the gradients of u, delta, z
+            assert torch.equal(a[:first], b[:first]) and torch.equal(a[behind:], b[behind:])
+        for a, b in zip(runs[0][4:6], other[4:6]):
+            lo, hi = first // 8 * 8, (behind + 7) // 8 * 8
+            assert torch.equal(a[:lo], b[:lo]) and torch.equal(a[hi:], b[hi:])
+        assert torch.equal(runs[0][6], other[6]) and torch.equal(runs[0][7], other[7])
+
+
+def test_the_same_tensor_twice():
+    """u as step sizes too, B as C too: the gradients add up."""
+    import boost_and_broadside_b200 as bnb
+
+    g = torch.Generator().manual_seed(22)
+    T, R, W, N = 13, 4, 24, 8
+    u, _, A, B, *_ = _scan_inputs(g, T, R, W, N, 1, torch.float32)
+    dy = _r(g, T, R, W)
+    ud, Bd = u.to(DEV).requires_grad_(True), B.to(DEV).requires_grad_(True)
+    got = torch.autograd.grad(bnb.selective_scan(ud, ud, A.to(DEV), Bd, Bd, softplus=True)[0], [ud, Bd], dy.to(DEV))
+    one, two, b, c = [t.to(DEV).requires_grad_(True) for t in (u, u, B, B)]
+    apart = torch.autograd.grad(bnb.selective_scan(one, two, A.to(DEV), b, c, softplus=True)[0], [one, two, b, c], dy.to(DEV))
+    assert torch.equal(got[0], apart[0] + apart[1]) and torch.equal(got[1], apart[2] + apart[3])
 
 
 def test_scan_gradient_against_differences():
