@@ -40,8 +40,11 @@ struct Work {
   bool paired;        // pairs of channels of u, delta, z and y lie on their boundary
 };
 
+// 64 registers a thread, so that 32 warps fit on an SM, and the splits that are aimed at all at once: 665 -> 647 us at 32 steps x 8192 rows x 256
+// channels x 16 states of bfloat16, 1669 -> 1170 at 128 channels x 64 states, 120 -> 112 for the joined pass over 2 rows x 4093 steps x 1536
+// channels; what spills costs a launch of few warps 4 us.  Fewer lanes a channel prepare more steps a thread and are left their registers.
 template <typename T, int KL, Pass PASS>
-__global__ void __launch_bounds__(CT * KL) k_scan(const __grid_constant__ BnbSelectiveScan q, const __grid_constant__ Work w) {
+__global__ void __launch_bounds__(CT * KL, KL >= 4 ? 1024 / (CT * KL) : 1) k_scan(const __grid_constant__ BnbSelectiveScan q, const __grid_constant__ Work w) {
   constexpr int THREADS = CT * KL, NP = NS * KL;
   constexpr int BC = (L * NP + THREADS - 1) / THREADS;            // elements of b and c that a thread fetches
   constexpr int PAIRS = CT / 2, AT_ONCE = THREADS / PAIRS < L ? THREADS / PAIRS : L, PER = L / AT_ONCE;   // steps prepared at a time, by a thread
@@ -309,7 +312,7 @@ __global__ void __launch_bounds__(256, 3) k_step(const __grid_constant__ BnbSele
   }
 }
 
-// Sixteen warps of each SM with two CTAs to spare: what the splits aim at.
+// 32 warps of each SM: what the splits aim at.
 Splits splits(const BnbSelectiveScan& a, int kl, int tiles) {
   return splits_of(a.steps, (int64_t)tiles * a.rows, 148 * std::max(1, 1024 / (CT * kl)));
 }
