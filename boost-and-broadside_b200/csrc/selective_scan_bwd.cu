@@ -501,7 +501,9 @@ Plan plan_of(const BnbSelectiveScan& a) {
   p.ct = p.kl <= 4 ? 64 : 256 / p.kl;   // CHANNELS
   p.tiles_a_group = (a.width / a.groups + p.ct - 1) / p.ct;
   p.tiles = p.tiles_a_group * a.groups;
-  const int fit = 148 * 2;   // CTAs of 256 threads that the chip holds at 128 registers a thread
+  // CTAs that the chip holds: at 128 registers a thread 512 threads of an SM, with one lane a channel as many as shared memory has room for. (With two
+  // of every size on an SM, 32 steps x 4096 rows x 256 channels of bfloat16 took 947 us backward at 4 states and 738 at 8, now 561 and 589.)
+  const int fit = 148 * (p.kl == 1 ? 5 : p.kl == 2 ? 4 : 2);
   p.splits = splits_of(a.steps, (int64_t)p.tiles * a.rows, fit);
   p.row_blocks = (int)std::min<int64_t>(a.rows, std::max<int64_t>(1, fit / ((int64_t)p.tiles * p.splits.count)));
   const size_t cells = (size_t)a.rows * a.width, np = (size_t)NS * p.kl, parts = (size_t)p.splits.count * p.row_blocks;
