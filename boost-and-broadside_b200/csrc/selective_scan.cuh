@@ -75,13 +75,20 @@ __device__ __forceinline__ bool writes_sum() {
   return ((threadIdx.x >> LO) & ((1 << (left - halvings)) - 1)) == 0;
 }
 
+// |v| up to 128, from where on e^-|v| is 0 in float32; a NaN stays one.
+__device__ __forceinline__ float bounded_size(float v) {
+  float m;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(v)), "f"(128.0f));
+  return m;
+}
 // Step sizes of a pair: log(1 + e^v) as max(v, 0) + log(1 + x) with x = e^-|v| <= 1, and log(1 + x) = 2 atanh(s), s = x / (2 + x) <= 1/3, by
 // its Taylor series: the first term left out, s^14 / 15, is 1.4e-8 of the sum.  e^-|v| = 2^-m with the rounding of m = |v| log2(e) put
-// back to first order.  A few units in the last place, which the gradients of a need: they are long sums.
+// back to first order.  A few units in the last place, which the gradients of a need: they are long sums.  The size of v is
+// bounded first: -inf and a type's lowest value, which mask a step, give the step size 0 and not inf - inf.
 __device__ __forceinline__ F2 step_size(F2 v, bool with_softplus) {
   if (!with_softplus) return v;
   const float2 vs = halves(v);
-  const F2 mag = f2(fabsf(vs.x), fabsf(vs.y)), m = mul(mag, f2(LOG2E));
+  const F2 mag = f2(bounded_size(vs.x), bounded_size(vs.y)), m = mul(mag, f2(LOG2E));
   const F2 rest = fma(mag, f2(-1.925963033e-8f), fma(mag, f2(-LOG2E), m));   // m - |v| log2(e)
   const float2 ms = halves(m);
   const F2 x0 = f2(ex2_fast(-ms.x), ex2_fast(-ms.y)), x = fma(x0, mul(rest, f2(0.6931471805599453f)), x0);
