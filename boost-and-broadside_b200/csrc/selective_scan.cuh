@@ -168,6 +168,14 @@ __device__ __forceinline__ void store_states(float* at, const float (&h)[NS], in
   }
 }
 
+// A state (or adjoint) behind a split's steps whose decays multiply to 2^m.  No step's decay need be beyond float32 where the product is: zero and
+// infinity stay what they are, as they do step by step, and the decay is taken in two halves, whose range holds whatever the result's does.
+__device__ __forceinline__ float across(float h, float m) {
+  if (h == 0.f || isinf(h)) return h;
+  const float half = ex2_fast(0.5f * m);
+  return h * half * half;
+}
+
 // Starting states of the splits from what each leaves of a zero start: local (count, rows, width, 4 KL) holds that on the way in and the
 // starting state on the way out.  REVERSE: the same for the adjoint, from the last split to the first.
 //   sum_p (count, rows, width); cut (count, rows): the split does not pass on what it starts with
@@ -198,7 +206,7 @@ __global__ void __launch_bounds__(256) k_join(float* local, const float* sum_p, 
       if (k0 + k >= count) break;
       const int64_t s = REVERSE ? count - 1 - k0 - k : k0 + k;
       local[s * cells + i] = run;
-      run = (passes[k] ? ex2_fast(rate * sums[k]) * run : 0.f) + left[k];
+      run = (passes[k] ? across(run, rate * sums[k]) : 0.f) + left[k];
     }
   }
 }
