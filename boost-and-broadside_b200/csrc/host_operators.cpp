@@ -92,11 +92,12 @@ OptTensor done_bytes(const char* fn, const OptTensor& done, int64_t T, int64_t R
   expect(fn, "done", *done, {T, R}, dev);
   return bytes_of(done);
 }
-OptTensor row_lengths(const char* fn, const OptTensor& lengths, int64_t R, const c10::Device& dev) {
+// As the kernels read them, which clamp to 0 .. T themselves: values of 64 bits are clamped before they lose their upper half.
+OptTensor row_lengths(const char* fn, const OptTensor& lengths, int64_t T, int64_t R, const c10::Device& dev) {
   if (!lengths.has_value()) return c10::nullopt;
   expect(fn, "lengths", *lengths, {R}, dev);
   if (lengths->scalar_type() != at::kInt && lengths->scalar_type() != at::kLong) refuse(std::string(fn) + ": lengths must be int32 or int64");
-  return contiguous(lengths->to(at::kInt));
+  return contiguous(lengths->scalar_type() == at::kLong ? lengths->clamp(0, T).to(at::kInt) : *lengths);
 }
 OptTensor reset_bytes(const char* fn, const OptTensor& reset, int64_t R, const c10::Device& dev) {
   if (!reset.has_value()) return c10::nullopt;
@@ -200,7 +201,7 @@ ConvCall conv_call(const char* fn, const Tensor& x, const Tensor& weight, const 
     expect_type(fn, "state", *state, at::kFloat);
   }
   k.done = done_bytes(fn, done, T, R, dev);
-  k.lengths = row_lengths(fn, lengths, R, dev);
+  k.lengths = row_lengths(fn, lengths, T, R, dev);
   c.steps = fits_int(fn, T);
   c.rows = fits_int(fn, R);
   c.width = fits_int(fn, C);
@@ -351,7 +352,7 @@ ScanCall scan_sequence(const Tensor& u, const Tensor& delta, const Tensor& a, co
     k.q.state_in = floats(*state, k.held);
   }
   k.done = done_bytes(fn, done, u.size(0), u.size(1), u.device());
-  k.lengths = row_lengths(fn, lengths, u.size(1), u.device());
+  k.lengths = row_lengths(fn, lengths, u.size(0), u.size(1), u.device());
   k.q.done = data<uint8_t>(k.done);
   k.q.lengths = data<int32_t>(k.lengths);
   return k;
