@@ -80,12 +80,11 @@ BnbView shared_view(const Tensor& t, std::vector<Tensor>& held) {
   o.group = v.stride(-2);
   return o;
 }
-// A new dense tensor of x's shape that lies in memory as x does: step by step, or row by row (batch-major programs).
+// A new dense tensor of x's shape that lies in memory as x does: step by step, or row by row (batch-major programs).  It is no view
+// of another: a differentiated call's result could not be changed in place then.
 Tensor rows_like(const Tensor& x) {
-  std::vector<int64_t> sizes = x.sizes().vec();
-  if (x.dim() < 3 || x.stride(0) >= x.stride(1)) return at::empty(sizes, x.options());
-  std::swap(sizes[0], sizes[1]);
-  return at::empty(sizes, x.options()).transpose(0, 1);
+  if (x.dim() < 3 || x.stride(0) >= x.stride(1)) return at::empty(x.sizes(), x.options());
+  return at::empty_strided(x.sizes(), {x.size(2), x.size(0) * x.size(2), 1}, x.options());
 }
 OptTensor done_bytes(const char* fn, const OptTensor& done, int64_t T, int64_t R, const c10::Device& dev) {
   if (!done.has_value()) return c10::nullopt;

@@ -26,7 +26,7 @@ def _rows_like(x: Tensor) -> Tensor:
     """As the native code lays out a result of x's shape: step by step, or row by row where x is."""
     if x.dim() < 3 or x.stride(0) >= x.stride(1):
         return x.new_empty(x.shape)
-    return x.new_empty((x.shape[1], x.shape[0], x.shape[2])).transpose(0, 1)
+    return x.new_empty_strided(x.shape, (x.shape[2], x.shape[0] * x.shape[2], 1))
 
 
 def _given(grads: List[Tensor], has: List[bool]) -> list:
