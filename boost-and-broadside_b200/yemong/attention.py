@@ -22,8 +22,8 @@ class GatedMLP(nn.Module):
     """down_proj(gelu(gate_proj(x)) * up_proj(x)), no biases (attention.py:21-37).
 
     Inside a sublayer the product runs fused in the sublayer kernels; ``forward`` serves callers
-    that use the module on its own (the reference's tests do) through ``bnb_gated_mlp_fwd``, or, for an
-    input that requires grad, through ``gated_mlp``, which has a backward.
+    that use the module on its own (the reference's tests do) through ``bnb_gated_mlp_fwd``, or, where the
+    input or a weight requires grad, through ``gated_mlp``, which has a backward.
     """
 
     def __init__(self, d_model: int, expand: int = 4) -> None:
@@ -45,13 +45,12 @@ class GatedMLP(nn.Module):
         _capi.require_cuda(x, "x")
         dev = x.device
         precision = _capi.current_precision(dev)
-        if torch.is_grad_enabled() and x.requires_grad:
-            return gated_mlp(x.to(torch.bfloat16 if precision == _capi.BNB_BF16 else torch.float32), self.gate_proj.weight,
-                             self.up_proj.weight, self.down_proj.weight)
+        ws = [self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight]
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *ws)):
+            return gated_mlp(x.to(torch.bfloat16 if precision == _capi.BNB_BF16 else torch.float32), *ws)
         with torch.cuda.device(dev):
             flat = _capi.f32c(x).reshape(-1, D)
             y = torch.empty_like(flat)
-            ws = [self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight]
             for w in ws:
                 if w.device != dev or w.dtype != torch.float32 or not w.is_contiguous():
                     raise RuntimeError("GatedMLP parameters must be contiguous float32 on the input's device")
