@@ -181,6 +181,15 @@ class SelectiveTemporalBlock(nn.Module):
         if tuple(h.shape) != (R, self.d_inner, self.d_state) or tuple(conv_buf.shape) != (R, TAPS - 1, self.d_inner):
             raise RuntimeError("h / conv_buf shapes do not match the input")
         _capi.require_cuda(x, "x")
+        _capi.current_precision(x.device)   # refuses what the feed-forward half would refuse behind the state's update
+
+    def _check_in_place(self, x: torch.Tensor, **states: torch.Tensor) -> None:
+        """What the operators ask of a state that they move on, of both before either is."""
+        for name, t in states.items():
+            if t.device != x.device or t.dtype != torch.float32:
+                raise RuntimeError(f"{name} must be float32 on the input's device {x.device}, got {t.dtype} on {t.device}")
+            if not t.is_contiguous() or (not torch.compiler.is_compiling() and t.data_ptr() % 16):
+                raise RuntimeError(f"{name} is updated in place and must be contiguous, on a 16-byte boundary")
 
     def forward_sequence(
         self,
@@ -205,8 +214,9 @@ class SelectiveTemporalBlock(nn.Module):
     @torch.no_grad()
     def step(self, x: torch.Tensor, h: torch.Tensor, conv_buf: torch.Tensor, reset: torch.Tensor | None = None) -> torch.Tensor:
         """One token a row, without gradients: x (R, D) -> (R, D).  ``h`` (R, E, N) and ``conv_buf`` (R, 3, E) move on in
-        place; rows of ``reset`` (R,) bool start from zeros."""
+        place; rows of ``reset`` (R,) bool start from zeros.  A call that is refused leaves both as they were."""
         self._check(x, 2, h, conv_buf)
+        self._check_in_place(x, h=h, conv_buf=conv_buf)
         u, z = self.in_proj(self.norm1(x)).split(self.d_inner, dim=-1)
         u = causal_conv_step(u, conv_buf, self.conv.weight[:, 0], self.conv.bias, reset=reset, activation="silu")
         delta, B, C = self._projected(u)
