@@ -389,7 +389,10 @@ std::vector<Tensor> scan_backward(const Tensor& u, const Tensor& delta, const Te
   const Tensor gy = dy.has_value() ? dy->to(u.scalar_type()) : at::zeros_like(u);
   expect("selective_scan", "the gradient of y", gy, u.sizes(), u.device());
   const Tensor du = rows_like(u), dd = rows_like(delta), dz = z.has_value() ? rows_like(*z) : Tensor();
-  const Tensor db = at::empty(b.sizes(), b.options()), dc = at::empty(c.sizes(), c.options());
+  // without channels nothing is launched, and b and c, whose shapes do not have them, get sums over nothing
+  const bool none = u.size(2) == 0;
+  const Tensor db = none ? at::zeros(b.sizes(), b.options()) : at::empty(b.sizes(), b.options()),
+               dc = none ? at::zeros(c.sizes(), c.options()) : at::empty(c.sizes(), c.options());
   const Tensor da = at::empty(a.sizes(), a.options());
   const Tensor dskip = d.has_value() ? at::empty({u.size(2)}, a.options()) : Tensor(), dbias = bias.has_value() ? at::empty({u.size(2)}, a.options()) : Tensor();
   const Tensor ds = state.has_value() ? at::empty(state->sizes(), state->options()) : Tensor();
