@@ -30,7 +30,7 @@ int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
 // (pieces, rows, cols) 16-bit elements.
 struct Operand { const void* data; int64_t rows, cols, ld, piece_stride; };
 
-// What the products cannot read as it lies (float32, strides or addresses off 16 bytes): copied as operand pieces.
+// What the products cannot read as it lies (float32, strides or addresses off 16 bytes, overlapping rows): copied as operand pieces.
 struct PackJob { const void* src; void* dst; int64_t rows, src_ld, piece_stride; int cols, dst_ld, kind; };   // kind: 0 float32, else the operands' type
 constexpr int MAX_JOBS = 5;
 struct PackJobs { PackJob job[MAX_JOBS]; };
@@ -225,7 +225,8 @@ int check(const BnbGatedBlock* c) {
 bool recomputes(const BnbGatedBlock& c) { return c.element != BNB_ELEM_F32 && c.width <= 512; }
 
 int64_t round32(int64_t v) { return (v + 31) / 32 * 32; }
-bool lies_well(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
+// Whether a tensor map can describe rows as they lie: no rows that share memory (a gradient expanded from one row) among them.
+bool lies_well(const void* p, int64_t cols, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld >= cols; }
 
 // Where everything of a call stands in its scratch; sizes alone with base = null.
 struct Layout {
@@ -245,7 +246,7 @@ struct Layout {
       return at;
     };
     auto operand = [&](const void* p, int64_t rows, int64_t cols, int64_t ld, int element) {
-      if (pieces == 1 && element == c.element && lies_well(p, ld)) return Operand{p, rows, cols, ld, 0};
+      if (pieces == 1 && element == c.element && lies_well(p, cols, ld)) return Operand{p, rows, cols, ld, 0};
       const int64_t to = round8(cols), stride = rows * to;
       void* at = take((size_t)pieces * stride * 2);
       jobs.job[n_jobs++] = {p, at, rows, ld, stride, (int)cols, (int)to, element == BNB_ELEM_F32 ? 0 : 1};
