@@ -116,6 +116,8 @@ void expect_state(const char* fn, const Tensor& s, at::IntArrayRef sizes, const 
   expect_type(fn, "state", s, at::kFloat);
   if (!s.is_contiguous() || reinterpret_cast<uintptr_t>(s.data_ptr()) % 16)
     refuse(std::string(fn) + ": the state is updated in place and must be contiguous, on a 16-byte boundary");
+  if (s.is_inference() && !c10::InferenceMode::is_enabled())   // as autograd does, but before the kernel has run
+    refuse(std::string(fn) + ": the state is updated in place and was made in inference mode, outside of which it must not be changed");
 }
 
 // The autograd node of an eager call: saved inputs (and what the forward kept), and the backward as a function of them.

@@ -188,8 +188,14 @@ class SelectiveTemporalBlock(nn.Module):
         for name, t in states.items():
             if t.device != x.device or t.dtype != torch.float32:
                 raise RuntimeError(f"{name} must be float32 on the input's device {x.device}, got {t.dtype} on {t.device}")
-            if not t.is_contiguous() or (not torch.compiler.is_compiling() and t.data_ptr() % 16):
-                raise RuntimeError(f"{name} is updated in place and must be contiguous, on a 16-byte boundary")
+            if not t.is_contiguous():
+                raise RuntimeError(f"{name} is updated in place and must be contiguous")
+            if not _ops.direct(t):   # what cannot be traced the operators ask themselves
+                continue
+            if t.data_ptr() % 16:
+                raise RuntimeError(f"{name} is updated in place and must lie on a 16-byte boundary")
+            if t.is_inference() and not torch.is_inference_mode_enabled():
+                raise RuntimeError(f"{name} is updated in place and was made in inference mode, outside of which it must not be changed")
 
     def forward_sequence(
         self,
