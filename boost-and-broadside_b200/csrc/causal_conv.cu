@@ -4,11 +4,12 @@
 //   pre[t] = b + sum_j w[K-1-j] x[t-j],  y = pre or silu(pre);  x[t-j] of an earlier episode counts as 0, before step 0 it is the state
 //   dpre = dy act'(pre),  dx[t] = sum_j w[K-1-j] dpre[t+j],  dw[K-1-j] = sum dpre[t] x[t-j],  db = sum dpre
 //
-// Memory bounds it: x is read and y written once, with some 15 instructions an element in between.  So a thread takes a few
-// neighbouring channels of a span of steps of a row, all of whose loads are on their way at once, and goes over them with the taps in
-// registers; the K - 1 steps before (and behind, for gradients) are read by the neighbour too, and come from the caches.  Threads that walked along
-// a whole row had a third of the loads in flight: 32 x 8192 x 256 of bfloat16 took 121 us forward and 301 backward, now 90 (368 MB) and 217
-// (502 MB).
+// x is read and y written once, so memory is what it could be bound by: 319 MB forward and 478 backward at 32 x 8192 x 256 of bfloat16.
+// What it spends beside that are instructions, some 29 a thread and element forward and 63 backward (SiLU and its slope, the taps,
+// unpacking), so that neither is full: issue slots 55 and 53 %, DRAM 36 and 25 %.  A thread takes a few neighbouring channels of a
+// span of steps of a row, all of whose loads are on their way at once, and goes over them with the taps in registers; the K - 1 steps before (and behind,
+// for gradients) are read by the neighbour too, and come from the caches.  Threads that walked along a whole row had a third of the loads in
+// flight: 121 us forward and 301 backward, now 91 and 218.
 #include <algorithm>
 
 #include "launch_count.h"
@@ -403,8 +404,10 @@ Plan plan(const BnbCausalConv& a, int vec, int span, int resident) {
   return p;
 }
 
-// Channels of a thread, and CTAs of an SM: what leaves a span's loads, weights and sums in registers.  Measured with the spans: forward 4 channels, 8
-// steps, 4 CTAs 90 us, 3 CTAs 95, 16 steps 112; backward 2 channels, 16 steps, 2 CTAs 217 us, 4 channels, 8 steps 233, 3 CTAs 261.
+// Channels of a thread, and CTAs of an SM: what was fastest in bfloat16, with the spans: forward 4 channels, 8 steps, 4 CTAs 90 us, 3 CTAs 95, 16 steps
+// 112; backward 2 channels, 16 steps, 2 CTAs 217 us, 4 channels, 8 steps 233, 3 CTAs 261.  With four taps not all of a span's loads, weights
+// and sums stay in registers: 16-bit calls spill 52 bytes a thread forward and up to 40 backward, float32 ones, whose loads take
+// twice the registers, up to 276 and 64.
 constexpr int FWD_VEC = 4, FWD_RESIDENT = 4, BWD_VEC = 2, BWD_RESIDENT = 2;
 
 template <typename T, int VEC, int K>
@@ -431,7 +434,7 @@ size_t part_bytes(const BnbCausalConv& a, const Plan& p) { return round256((size
 template <typename T, int VEC, int K>
 int launch_bwd(const BnbCausalConv& a, const BnbCausalConvGrads& g, float* part, cudaStream_t st) {
   const Plan p = plan(a, VEC, BWD_SPAN, BWD_RESIDENT);
-  const size_t smem = (size_t)p.by * (K + 1) * p.bx * VEC * 4;   // at most 256 threads x 4 x 5 floats = 20 KB
+  const size_t smem = (size_t)p.by * (K + 1) * p.bx * VEC * 4;   // at most 256 threads x 2 channels x 5 floats = 10 KB
   const dim3 grid(p.blocks, p.tiles), block(p.bx, p.by);
   count_launch();
   if (a.activation == BNB_ACT_SILU) k_conv_bwd<T, VEC, K, true><<<grid, block, smem, st>>>(a, g, p.units, p.spans, part);

@@ -48,8 +48,8 @@ void expect_type(const char* fn, const char* name, const Tensor& t, at::ScalarTy
 void expect_cuda(const char* fn, const Tensor& t) {
   if (!t.is_cuda()) refuse(std::string(fn) + ": the input is on " + t.device().str() + "; the kernels run on CUDA only (sm_100a) and have no CPU path");
 }
-// A float32 parameter or state as the kernels read it: contiguous, on a 16-byte boundary (32 bytes for states of the conv, whose accesses are
-// narrower otherwise).  A copy is put into `held` until the call is queued.
+// A float32 parameter or state as the kernels read it: contiguous, on a 16-byte boundary.  A copy is put into `held` until the call is
+// queued.
 const float* floats(const Tensor& t, std::vector<Tensor>& held) {
   Tensor v = t.is_contiguous() ? t : t.contiguous();
   if (reinterpret_cast<uintptr_t>(v.data_ptr()) % 16) v = v.clone();

@@ -2,7 +2,7 @@
 // selective_scan_bwd.cu).
 //
 // Layout of the work.  KL neighbouring lanes own a channel of a row, four states each (KL = states / 4 rounded up to a power of two;
-// states behind the last have a = 0 and b = c = 0, so they stay 0).  A CTA walks along time in chunks with a tile of channels of one
+// states behind the last have a = 0 and b = c = 0, so they stay 0, or become NaN where p u is infinite, and y with them).  A CTA walks along time in chunks with a tile of channels of one
 // row: what is per channel and step (softplus, gate, p u) is computed once by the CTA's threads together and stands in shared memory,
 // and so do the chunk's b and c, which the tile's channels share.  Steps at and behind a row's length get p = 0 and b = c = 0, which
 // makes them the identity.

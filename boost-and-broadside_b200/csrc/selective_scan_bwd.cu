@@ -15,15 +15,17 @@
 // filled two columns after two.  (With the values in B, which holds half of what A does, twice the products were needed: 2030 us against
 // 2020 at 32 steps x 8192 rows x 256 channels x 16 states in bfloat16, and more in float32, where there are twice as many.)
 // The operands have 11 bits: bfloat16 calls round to them (a sum of many terms is then good to 2^-12 or so of its size, against
-// 2^-9 of the result), others add the products of the bits that remain.
+// 2^-9 of the result), others add the products of the bits that remain.  An infinity times the zeros of the other columns is NaN in them, and in
+// float32 and float16 calls in its own too, where nothing remains of it but inf - inf.
 //
 // What is left of the sums over channels goes through the warps of the CTA and, where a group has several tiles of channels, a
 // short kernel over the tiles; sums over rows and time (da, dd, d bias) stay in registers while a CTA goes over its rows.  No
 // atomics, so a result does not depend on timing.
 //
-// Some 140 instructions for a warp's step of 8 channels x 16 states bound it (8 exponentials, 60 for the recurrence and its adjoint, 14 for db
-// and dc, 12 for the sums over a channel's lanes, the rest per chunk), issued in 55 % of the cycles: at 128 registers a thread 16 warps fit on an
-// SM.  Registers decide what else may be tried: a version with 20 more values alive in the walk spilled, and took 2460 us, not 2020.
+// Some 150 instructions for a warp's step of 8 channels x 16 states bound it (8 exponentials, 60 for the recurrence and its adjoint, 22 for db
+// and dc, 12 for the sums over a channel's lanes, the rest per chunk), issued in 57 % of the cycles: at 128 registers a thread 16 warps fit on an
+// SM.  2070 us at 32 steps x 8192 rows x 256 channels of bfloat16; 2020 without the 8 instructions that keep NaN (add_rows).  Registers decide
+// what else may be tried: a version with 20 more values alive in the walk spilled, and took 2460 us when this one took 2020.
 // Memory moves some 24 bytes a channel and step, 20 % of what it could.  The next chunk's operands therefore come by asynchronous
 // copies into shared memory, which hold no register (2220 -> 2150 us).
 #include "selective_scan.cuh"

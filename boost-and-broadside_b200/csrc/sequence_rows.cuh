@@ -98,7 +98,8 @@ __device__ __forceinline__ void store(T* at, const float (&f)[N]) {
 }
 
 // 1 / (1 + e^-v).  Results of 16-bit calls are rounded to 11 bits or fewer, where the fast exponential and division
-// (2 units in the last place of 24 each, for arguments that matter) are far below the rounding; float32 calls take the exact ones.
+// (2 units in the last place of 24 each, for arguments that matter) are far below the rounding; float32 calls take the exact ones here.  The decays
+// and step sizes of the scan (selective_scan.cuh) take the fast ones in every type.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float v) {
   if constexpr (sizeof(T) == 2) return rcp_fast(1.0f + ex2_fast(v * -LOG2E));

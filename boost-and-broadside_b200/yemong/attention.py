@@ -23,7 +23,8 @@ class GatedMLP(nn.Module):
 
     Inside a sublayer the product runs fused in the sublayer kernels; ``forward`` serves callers
     that use the module on its own (the reference's tests do) through ``bnb_gated_mlp_fwd``, or, where the
-    input or a weight requires grad, through ``gated_mlp``, which has a backward.
+    input or a weight requires grad, through ``gated_mlp``, which has a backward.  The two are different
+    kernels: their values agree to rounding, not in every bit.
     """
 
     def __init__(self, d_model: int, expand: int = 4) -> None:

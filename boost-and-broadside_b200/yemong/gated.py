@@ -24,7 +24,8 @@ def gated_mlp(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor, down_w:
 
     Returns:
         (.., D) in x's type.  16-bit calls: products of 16-bit operands summed in float32, the hidden activations and their
-        gradients rounded to x's type as operands of the next product.  float32 calls: float32 products.
+        gradients rounded to x's type as operands of the next product.  float32 calls: float32 products, of numbers in pieces, so that
+        an infinity, or a number above 3.39e38, comes out as NaN.
     """
     act = activation_code("gated_mlp", activation, ("gelu", "silu"))
     if _ops.direct(x):

@@ -10,7 +10,8 @@ single-token forms does).
 
 Activations may be float32, bfloat16 or float16 and strided (columns of a projection's output, batch-major
 tensors transposed), innermost stride 1; parameters and states are float32.  All arithmetic is float32, rounded
-once on the way out.
+once on the way out, with one exception: the terms of the sums over channels that are the gradients of B and C are
+rounded to 11 bits in bfloat16 calls of up to 32 states.  Decays and step sizes are good to a few units of 2^-23 in every type.
 """
 
 from __future__ import annotations
@@ -99,8 +100,11 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     Returns:
         y (T, R, C) in u's type and the state (R, C, N) behind the last step.
 
+    A step is masked by delta = -inf or its type's lowest value where ``softplus`` is asked for: its size is 0, the state stays.
+
     An infinity or NaN among an episode's values stays in it, with one exception: the gradients of B and C may show it in
-    the row's other episodes too, up to eight steps away.
+    the row's other episodes too, up to eight steps away.  An infinity may come out as NaN: in those gradients, and in y
+    where N is not 4, 8, 16, 32 or 64.
     """
     B, C = _grouped("selective_scan", "B", B, 3), _grouped("selective_scan", "C", C, 3)
     if _ops.direct(u):
@@ -124,7 +128,8 @@ def selective_step(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
 
 class SelectiveTemporalBlock(nn.Module):
     """A temporal sublayer on these operators, in the place and with the signatures of ``GriffinTemporalBlock``
-    (griffin.py:222-286): norm -> in_proj -> (causal conv -> selective scan) gated -> out_proj -> residual
+    (griffin.py:222-286).  Projections, parameters' names and starting values are those of the selective state space layer that
+    Gu and Dao published (2023, arXiv:2312.00752), inside that sublayer's frame: norm -> in_proj -> (causal conv -> selective scan) gated -> out_proj -> residual
     -> gated feed-forward (norm) -> residual, per row across time.
 
     Its state is wider than the Griffin sublayer's: (R, E, N) and the taps (R, 3, E), E = expand * d_model channels of N
