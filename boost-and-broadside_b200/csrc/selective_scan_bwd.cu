@@ -14,18 +14,19 @@
 // state in the depths 0 .. 3 and a second one in 4 .. 7.  B has ones in a step's two columns, so that the accumulators of four steps are
 // filled two columns after two.  (With the values in B, which holds half of what A does, twice the products were needed: 2030 us against
 // 2020 at 32 steps x 8192 rows x 256 channels x 16 states in bfloat16, and more in float32, where there are twice as many.)
-// The operands have 11 bits: bfloat16 calls round to them (a sum of many terms is then good to 2^-12 or so of its size, against
-// 2^-9 of the result), others add the products of the bits that remain.  An infinity times the zeros of the other columns is NaN in them, and in
-// float32 and float16 calls in its own too, where nothing remains of it but inf - inf.
+// The operands are pieces of the float32 values.  bfloat16 calls: two bfloat16 pieces, 2^-15 of a value at most from it, side by side in the depth of
+// a 16 x 8 x 16 product.  Others: 11 bits and, in a product of its own, the 11 that follow.  (Rounded to 11 bits alone, a bfloat16 call
+// took 2020 us, lost NaN, and was off by 2^-11 of a term where few channels share b and c; two products of 11 bits took 2190.)  An infinity
+// becomes NaN: inf - inf remains of it, and it meets the zeros of the other columns.
 //
 // What is left of the sums over channels goes through the warps of the CTA and, where a group has several tiles of channels, a
 // short kernel over the tiles; sums over rows and time (da, dd, d bias) stay in registers while a CTA goes over its rows.  No
 // atomics, so a result does not depend on timing.
 //
-// Some 150 instructions for a warp's step of 8 channels x 16 states bound it (8 exponentials, 60 for the recurrence and its adjoint, 22 for db
+// Some 156 instructions for a warp's step of 8 channels x 16 states bound it (8 exponentials, 60 for the recurrence and its adjoint, 30 for db
 // and dc, 12 for the sums over a channel's lanes, the rest per chunk), issued in 57 % of the cycles: at 128 registers a thread 16 warps fit on an
-// SM.  2070 us at 32 steps x 8192 rows x 256 channels of bfloat16; 2020 without the 8 instructions that keep NaN (add_rows).  Registers decide
-// what else may be tried: a version with 20 more values alive in the walk spilled, and took 2460 us when this one took 2020.
+// SM.  2117 us at 32 steps x 8192 rows x 256 channels of bfloat16.  Registers decide what else may be tried: a version with 20 more values alive in
+// the walk spilled, and took 2460 us when this one took 2020.
 // Memory moves some 24 bytes a channel and step, 20 % of what it could.  The next chunk's operands therefore come by asynchronous
 // copies into shared memory, which hold no register (2220 -> 2150 us).
 #include "selective_scan.cuh"
@@ -52,28 +53,36 @@ struct Work {
 
 template <int KL> constexpr int CHANNELS = KL <= 4 ? 64 : 256 / KL;   // of a CTA
 
-// d += a b, 11 bits of every operand; see above for what is where.
-__device__ __forceinline__ void mma_rows(float (&d)[4], const float (&a)[4], const uint32_t (&one)[2]) {
+// d += what a lane holds of two states for db and for dc, in a step's columns; see above for what is where.  KEPT: the bits of a float's first piece.
+template <uint32_t KEPT>
+__device__ __forceinline__ F2 first_piece(F2 v) {
+  const float2 s = halves(v);
+  return f2(__uint_as_float(__float_as_uint(s.x) & KEPT), __uint_as_float(__float_as_uint(s.y) & KEPT));
+}
+__device__ __forceinline__ uint32_t pieces(float first, float rest) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(first), "f"(rest));
+  return r;
+}
+__device__ __forceinline__ void mma_rows(float (&d)[4], float2 b, float2 c, const uint32_t (&one)[2]) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])), "r"(one[0]), "r"(one[1]));
+      : "r"(__float_as_uint(b.x)), "r"(__float_as_uint(c.x)), "r"(__float_as_uint(b.y)), "r"(__float_as_uint(c.y)), "r"(one[0]), "r"(one[1]));
 }
 template <typename T>
-__device__ __forceinline__ void add_rows(float (&d)[4], const float (&a)[4], const uint32_t (&one)[2]) {
-  float high[4], low[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      // The product drops 13 bits: rounded to the nearest before.  The NaN of arithmetic, 0x7fffffff, would be carried over into the sign and
-      // vanish as -0, so it is made one that leaves room.  (2 % of a call; the conversion instruction, which keeps NaN too, takes 5 %.)
-      high[i] = __int_as_float(min(__float_as_int(a[i]), 0x7fffefff) + 0x1000);
-    } else {
-      high[i] = __uint_as_float(__float_as_uint(a[i]) & 0xffffe000u);
-      low[i] = a[i] - high[i];
-    }
+__device__ __forceinline__ void add_rows(float (&d)[4], F2 b, F2 c, const uint32_t (&one)[2]) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t KEPT = BF16 ? 0xffff0000u : 0xffffe000u;
+  const F2 bh = first_piece<KEPT>(b), ch = first_piece<KEPT>(c);
+  const float2 b1 = halves(bh), c1 = halves(ch), b2 = halves(fma(bh, f2(-1.0f), b)), c2 = halves(fma(ch, f2(-1.0f), c));
+  if constexpr (BF16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(pieces(b1.x, b2.x)), "r"(pieces(c1.x, c2.x)), "r"(pieces(b1.y, b2.y)), "r"(pieces(c1.y, c2.y)), "r"(one[0]), "r"(one[1]));
+  } else {
+    mma_rows(d, b2, c2, one);
+    mma_rows(d, b1, c1, one);
   }
-  if constexpr (!std::is_same<T, __nv_bfloat16>::value) mma_rows(d, low, one);
-  mma_rows(d, high, one);
 }
 
 template <int BYTES>
@@ -342,16 +351,13 @@ __global__ void __launch_bounds__(CHANNELS<KL> * KL, KL <= 4 ? 512 / (CHANNELS<K
             }
           }
           if constexpr (MMA) {
-            const uint32_t one[2] = {(wl >> 2) == 2 * (t % 4) ? 0x3f800000u : 0u, (wl >> 2) == 2 * (t % 4) + 1 ? 0x3f800000u : 0u};
+            constexpr uint32_t ONE = std::is_same<T, __nv_bfloat16>::value ? 0x3f803f80u : 0x3f800000u;   // for both pieces, or the one
+            const uint32_t one[2] = {(wl >> 2) == 2 * (t % 4) ? ONE : 0u, (wl >> 2) == 2 * (t % 4) + 1 ? ONE : 0u};
             if (t % 4 == 3)
 #pragma unroll
               for (int i = 0; i < 2; ++i) rows[i][0] = rows[i][1] = rows[i][2] = rows[i][3] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float2 fb = halves(of_b[i]), fc = halves(of_c[i]);
-              const float a[4] = {fb.x, fc.x, fb.y, fc.y};
-              add_rows<T>(rows[i], a, one);
-            }
+            for (int i = 0; i < 2; ++i) add_rows<T>(rows[i], of_b[i], of_c[i], one);
             if (t % 4 == 0) {   // this lane's sums are of step t + wl % 4 and of all four states of the state lane of row wl / 4
               const int g8 = wl >> 2;
               float* to = &red[((t + (wl & 3)) * WARPS + warp) * RED + (g8 % PARTS) * NP + g8 / PARTS * NS];

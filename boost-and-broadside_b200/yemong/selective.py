@@ -10,8 +10,8 @@ single-token forms does).
 
 Activations may be float32, bfloat16 or float16 and strided (columns of a projection's output, batch-major
 tensors transposed), innermost stride 1; parameters and states are float32.  All arithmetic is float32, rounded
-once on the way out, with one exception: the terms of the sums over channels that are the gradients of B and C are
-rounded to 11 bits in bfloat16 calls of up to 32 states.  Decays and step sizes are good to a few units of 2^-23 in every type.
+once on the way out; the terms of the sums over channels that are the gradients of B and C enter them with 16 bits
+(bfloat16) or 22 (others), up to 32 states.  Decays and step sizes are good to a few units of 2^-23 in every type.
 """
 
 from __future__ import annotations
