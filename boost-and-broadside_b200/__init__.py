@@ -19,6 +19,7 @@ from .yemong.gated import gated_mlp
 from .yemong.heads import HeadMLP, NextStateHead, TeamPMA, evaluate_action, sample_action
 from .yemong.griffin import CONV_KERNEL, RGLRU, GriffinTemporalBlock, YemongBlock
 from .yemong.policy import YemongPolicy
+from .yemong.policy_loss import policy_loss
 from .yemong.selective import SelectiveTemporalBlock, causal_conv, causal_conv_step, selective_scan, selective_step
 from .yemong.trunk import YemongTrunk, RaggedBatch
 
@@ -43,6 +44,7 @@ __all__ = [
     "causal_conv_step",
     "evaluate_action",
     "gated_mlp",
+    "policy_loss",
     "sample_action",
     "selective_scan",
     "selective_step",

@@ -824,6 +824,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_tail(const Tensor& x_in, const
 
 PYBIND11_MODULE(_host_path, m) {
   bnb::host::bind_operators(m);
+  bnb::host::bind_update(m);
   m.def("trunk_params", &trunk_params);
   m.def("keep_activations", [](const c10::Device& dev, const std::vector<int64_t>& geom, int64_t d_model, int64_t n_bullets) {
     return keep_activations(dev, Geometry(geom), d_model, n_bullets);

@@ -69,8 +69,9 @@ struct NoSecondOrder : public torch::autograd::Node {
   }
 };
 
-// The operators outside the trunk (host_operators.cpp).
+// The operators outside the trunk (host_operators.cpp) and those behind it in an update (host_update.cpp).
 void bind_operators(py::module& m);
+void bind_update(py::module& m);
 
 }  // namespace host
 }  // namespace bnb

@@ -604,6 +604,47 @@ typedef struct {
 int bnb_gated_block_bwd(const BnbGatedBlock* call, const BnbGatedBlockGrads* grads, void* scratch, size_t scratch_bytes,
                         void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The end of a policy update: the loss behind a head's logits.
+ *
+ * Replaces: the policy part of _compute_minibatch_loss (ppo.py:1351) behind _evaluate_action (policy.py:578-602), with its
+ * gradient.  A row's logits are n_slices distributions of their own, side by side (the policy's actions: 3 | 7 | 2).
+ *   l = sum over slices of log softmax(logits)[action], H = sum of their entropies, ratio = exp(l - old_logprob)
+ *   surrogate = min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A),  k = exp(ref - l) - (ref - l) - 1
+ *   loss = sum of w (-surrogate + kl_coef k - entropy_coef H) / sum of w;  0 where no row has weight
+ *   element: type of the logits (rows, sum of sizes), logits_row elements between rows
+ *   actions (rows, n_slices), contiguous; one outside of its slice makes the row's results NaN
+ *   old_logprob, advantages (rows); ref_logprob (rows) or NULL: k is 0
+ *   weights (rows) float32, or mask (rows) bytes, or neither: 1.  Rows of weight 0 are not looked at: logprob is 0, their gradient too
+ *   loss (1); stats (4): means of surrogate, k, H and of whether the ratio is beyond its clipping; logprob (rows)
+ *   kept: bnb_policy_loss_kept_bytes bytes that the backward reads; scratch 16-byte aligned */
+#define BNB_MAX_SLICES 16
+typedef struct {
+  int64_t rows;
+  int32_t element, n_slices;
+  int32_t sizes[BNB_MAX_SLICES];
+  const void* logits;
+  int64_t logits_row;
+  const int64_t* actions;
+  const float* old_logprob;
+  const float* advantages;
+  const float* ref_logprob;
+  const float* weights;
+  const uint8_t* mask;
+  float clip_low, clip_high, kl_coef, entropy_coef;
+  float* loss;
+  float* stats;
+  float* logprob;
+  float* kept;
+} BnbPolicyLoss;
+size_t bnb_policy_loss_kept_bytes(const BnbPolicyLoss* call);
+size_t bnb_policy_loss_scratch_bytes(const BnbPolicyLoss* call);
+int bnb_policy_loss_fwd(const BnbPolicyLoss* call, void* scratch, size_t scratch_bytes, void* stream);
+
+/* dlogits (rows, sum of sizes), contiguous, of the logits' type, for the loss's gradient dloss (1, on the device).  The call's `kept`
+ * as the forward left it; its loss, stats and logprob are not read. */
+int bnb_policy_loss_bwd(const BnbPolicyLoss* call, const float* dloss, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

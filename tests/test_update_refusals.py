@@ -1,0 +1,74 @@
+"""What the operators of an update's end refuse, on the host and before anything is launched; their operators' shapes."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+
+def _policy(**over):
+    import boost_and_broadside_b200 as bnb
+
+    a = dict(logits=torch.zeros(4, 12), actions=torch.zeros(4, 3, dtype=torch.int64), old=torch.zeros(4), adv=torch.zeros(4), sizes=(3, 7, 2))
+    a.update(over)
+    return bnb.policy_loss(a.pop("logits"), a.pop("actions"), a.pop("old"), a.pop("adv"), **a)
+
+
+def test_policy_loss_has_no_cpu_path_and_checks_its_numbers():
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        _policy()
+    for clip in (-0.1, (0.2, -1.0), float("nan")):
+        with pytest.raises(ValueError, match="clip"):
+            _policy(clip=clip)
+    with pytest.raises(ValueError, match="sizes"):
+        _policy(sizes=())
+    for name, over in (("old_logprob", dict(old=torch.zeros(4, requires_grad=True))), ("advantages", dict(adv=torch.zeros(4, requires_grad=True))),
+                       ("ref_logprob", dict(ref_logprob=torch.zeros(4, requires_grad=True))), ("weights", dict(weights=torch.ones(4, requires_grad=True)))):
+        with pytest.raises(NotImplementedError, match=name):
+            _policy(**over)
+
+
+class Policy(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("element", C.c_int32), ("n_slices", C.c_int32), ("sizes", C.c_int32 * 16), ("logits", C.c_void_p),
+                ("logits_row", C.c_int64)] + [(n, C.c_void_p) for n in ("actions", "old", "adv", "ref", "weights", "mask")] + [
+                    (n, C.c_float) for n in ("low", "high", "kl", "entropy")] + [(n, C.c_void_p) for n in ("loss", "stats", "logprob", "kept")]
+
+
+def test_policy_entry_points_check_their_arguments():
+    from boost_and_broadside_b200 import _capi
+
+    lib, fake = _capi.lib, 0x1000
+
+    def call(**over):
+        c = Policy(100, 1, 3, (C.c_int32 * 16)(3, 7, 2), fake, 12, fake, fake, fake, None, None, None, 0.2, 0.2, 0.0, 0.0, fake, fake, fake, fake)
+        for k, v in over.items():
+            setattr(c, k, v)
+        return c
+
+    fwd = lambda scratch=None, bytes_=0, **over: lib.bnb_policy_loss_fwd(C.byref(call(**over)), scratch, bytes_, None)  # noqa: E731
+    assert fwd() == 6 and fwd(scratch=fake + 4, bytes_=1 << 20) == 2
+    assert fwd(n_slices=0) == 3 and fwd(n_slices=17) == 3 and fwd(sizes=(C.c_int32 * 16)(3, 0, 2)) == 3
+    assert fwd(sizes=(C.c_int32 * 16)(1 << 28, 7, 2)) == 3
+    assert fwd(rows=-1) == 5 and fwd(element=3) == 5 and fwd(low=-0.1) == 5 and fwd(high=float("nan")) == 5
+    assert fwd(weights=fake, mask=fake) == 5
+    for name in ("logits", "actions", "old", "adv", "loss", "stats", "logprob", "kept"):
+        assert fwd(**{name: None}) == 1, name
+    assert lib.bnb_policy_loss_fwd(None, None, 0, None) == 1
+    bwd = lambda dloss, out, **over: lib.bnb_policy_loss_bwd(C.byref(call(**over)), dloss, out, None)  # noqa: E731
+    assert bwd(None, fake) == 1 and bwd(fake, None) == 1 and bwd(fake, fake + 2) == 2 and bwd(fake, fake, n_slices=99) == 3
+    assert bwd(None, None, rows=0, logits=None) == 0
+    assert lib.bnb_policy_loss_kept_bytes(C.byref(call())) == 4 * (4 + 100 * 7)
+    assert lib.bnb_policy_loss_scratch_bytes(C.byref(call())) > 0
+
+
+def test_operators_have_shape_only_fakes():
+    import boost_and_broadside_b200  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    ops = torch.ops.bnb_b200
+    with FakeTensorMode():
+        z = torch.empty(5, 3, 12, device="cuda", dtype=torch.bfloat16)
+        a, v = torch.empty(5, 3, 3, device="cuda", dtype=torch.int64), torch.empty(5, 3, device="cuda")
+        loss, l, stats, kept = ops.policy_loss(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0)
+        assert loss.shape == () and loss.dtype == torch.float32 and l.shape == (5, 3) and stats.shape == (4,) and kept.numel() == 4 + 15 * 7
+        assert ops.policy_loss_backward(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0, kept, loss).shape == z.shape
