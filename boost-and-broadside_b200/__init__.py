@@ -18,12 +18,14 @@ from .yemong.encoder import BulletEncoder, ShipEncoder
 from .yemong.gated import gated_mlp
 from .yemong.heads import HeadMLP, NextStateHead, TeamPMA, evaluate_action, sample_action
 from .yemong.griffin import CONV_KERNEL, RGLRU, GriffinTemporalBlock, YemongBlock
+from .yemong.optimizer import AdamW
 from .yemong.policy import YemongPolicy
 from .yemong.policy_loss import policy_loss
 from .yemong.selective import SelectiveTemporalBlock, causal_conv, causal_conv_step, selective_scan, selective_step
 from .yemong.trunk import YemongTrunk, RaggedBatch
 
 __all__ = [
+    "AdamW",
     "BulletEncoder",
     "CONV_KERNEL",
     "GatedMLP",

@@ -1,6 +1,8 @@
-// The host side of the operators behind the trunk in an update (yemong/policy_loss.py): checks, outputs and scratch from torch's
+// The host side of the operators behind the trunk in an update (yemong/policy_loss.py, yemong/optimizer.py): checks, outputs and scratch from torch's
 // allocator, the launch, the autograd nodes of eager calls.
 #include "host_nodes.h"
+
+#include <torch/csrc/autograd/python_variable.h>
 
 #include <tuple>
 
@@ -128,9 +130,138 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
   return {loss, logprob, stats};
 }
 
+// ------------------------------------------------------------------ AdamW
+
+constexpr int64_t STATE_BLOCK = 256;   // elements that share a scale of 8-bit states
+
+bool laid_out_as(const Tensor& t, const Tensor& p) { return t.sizes() == p.sizes() && (t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous())); }
+Tensor state_of(const py::dict& state, const char* name) {
+  PyObject* v = PyDict_GetItemString(state.ptr(), name);
+  if (!v || !THPVariable_Check(v)) refuse(std::string("AdamW: a parameter's state has no tensor '") + name + "'");
+  return THPVariable_Unpack(v);
+}
+void expect_kept(const char* name, const Tensor& t, const Tensor& like, at::ScalarType type, const c10::Device& dev) {
+  if (t.scalar_type() != type || t.device() != dev || !laid_out_as(t, like))
+    refuse(std::string("AdamW: the state '") + name + "' must be " + c10::toString(type) + " of shape " + shape_text(like.sizes()) + " on " + dev.str() +
+           ", laid out as its parameter; got " + c10::toString(t.scalar_type()) + " of shape " + shape_text(t.sizes()) + " on " + t.device().str());
+}
+void expect_changeable(const char* name, const Tensor& t) {
+  if (t.is_inference() && !c10::InferenceMode::is_enabled())
+    refuse(std::string("AdamW: ") + name + " was made in inference mode, outside of which it must not be changed");
+}
+
+// One step of the parameters of all groups that have a gradient.  groups: (parameters, states: dicts of tensors, positions, lr, beta1, beta2, eps, weight decay)
+// each.  Everything is checked before the first launch.  Returns the gradients' norm where they are clipped.
+using Group = std::tuple<py::list, py::list, std::vector<int64_t>, py::object, double, double, double, double>;
+OptTensor adamw_step(const std::vector<Group>& groups, const py::object& max_norm, int state_bits, uint32_t seed, const Tensor& control) {
+  const bool eight = state_bits == 8;
+  std::vector<Tensor> held, changed;
+  std::vector<std::vector<BnbAdamTensor>> lists;
+  std::vector<BnbAdamW> calls;
+  c10::optional<c10::Device> dev;
+  for (const Group& group : groups) {
+    const auto& [params, states, positions, lr, beta1, beta2, eps, decay] = group;
+    std::vector<BnbAdamTensor> list;
+    for (size_t i = 0; i < params.size(); ++i) {
+      const Tensor p = THPVariable_Unpack(params[i].ptr());
+      Tensor g = p.grad();
+      if (!g.defined()) continue;
+      if (!p.is_cuda()) refuse("AdamW: a parameter is on " + p.device().str() + "; the kernels run on CUDA only (sm_100a) and have no CPU path");
+      if (!dev) dev = p.device();
+      if (p.device() != *dev) refuse("AdamW: parameters on " + p.device().str() + " and " + dev->str() + "; one optimizer serves one device");
+      if (g.layout() != at::kStrided) refuse("AdamW: sparse gradients are not taken");
+      if (g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() || g.device() != *dev) refuse("AdamW: a gradient has another type, shape or device than its parameter");
+      if (!p.is_non_overlapping_and_dense()) throw py::value_error("AdamW: a parameter's elements must lie densely in memory, each in a place of its own");
+      const c10::cuda::CUDAGuard guard(*dev);
+      BnbAdamTensor t{};
+      t.element = element_of("AdamW", p);
+      t.n = p.numel();
+      t.position = positions[i];
+      const py::dict state = py::reinterpret_borrow<py::dict>(states[i]);
+      const Tensor step = state_of(state, "step"), m = state_of(state, "exp_avg"), v = state_of(state, eight ? "exp_avg_sq_root" : "exp_avg_sq");
+      if (step.scalar_type() != at::kFloat || step.numel() != 1 || step.device() != *dev) refuse("AdamW: the state 'step' must be one float32 number on " + dev->str());
+      const at::ScalarType type = eight ? at::kFloat8_e4m3fn : at::kFloat;
+      expect_kept("exp_avg", m, p, type, *dev);
+      expect_kept(eight ? "exp_avg_sq_root" : "exp_avg_sq", v, p, type, *dev);
+      if (eight) {
+        const int64_t blocks = (t.n + STATE_BLOCK - 1) / STATE_BLOCK;
+        for (const auto& [name, to] : {std::pair<const char*, float**>{"exp_avg_scale", &t.m_scale}, {"exp_avg_sq_root_scale", &t.v_scale}}) {
+          const Tensor s = state_of(state, name);
+          if (s.scalar_type() != at::kFloat || s.dim() != 1 || s.size(0) != blocks || !s.is_contiguous() || s.device() != *dev)
+            refuse(std::string("AdamW: the state '") + name + "' must be float32 of shape " + shape_text({blocks}) + ", contiguous, on " + dev->str());
+          *to = static_cast<float*>(s.data_ptr());
+          changed.push_back(s);
+        }
+      }
+      if (!laid_out_as(g, p)) {
+        g = at::empty_like(p).copy_(g);
+        held.push_back(g);
+      }
+      t.p = p.data_ptr();
+      t.g = g.data_ptr();
+      t.m = m.data_ptr();
+      t.v = v.data_ptr();
+      t.step = static_cast<float*>(step.data_ptr());
+      list.push_back(t);
+      changed.insert(changed.end(), {p, m, v, step});
+    }
+    BnbAdamW c{};
+    c.state_bits = state_bits;
+    c.seed = seed;
+    if (THPVariable_Check(lr.ptr())) {
+      const Tensor rate = THPVariable_Unpack(lr.ptr());
+      if (rate.numel() != 1) refuse("AdamW: lr must be a number or a tensor of one");
+      if (rate.is_cuda()) {
+        if (dev && rate.device() != *dev) refuse("AdamW: lr is on " + rate.device().str() + ", the parameters on " + dev->str());
+        held.push_back(rate.to(at::kFloat));
+        c.lr_device = static_cast<const float*>(held.back().data_ptr());
+      } else {
+        c.lr = rate.item<float>();
+      }
+    } else {
+      c.lr = (float)lr.cast<double>();
+    }
+    c.beta1 = beta1;
+    c.beta2 = beta2;
+    c.eps = (float)eps;
+    c.weight_decay = (float)decay;
+    c.control = static_cast<int32_t*>(control.data_ptr());
+    calls.push_back(c);
+    lists.push_back(std::move(list));
+  }
+  if (!dev) return c10::nullopt;
+  expect("AdamW", "the control word", control, {1}, *dev);
+  for (const Tensor& t : changed) expect_changeable("a parameter or its state", t);
+  const c10::cuda::CUDAGuard guard(*dev);
+  void* stream = stream_of(*dev);
+  OptTensor norm;
+  Tensor parts;
+  if (!max_norm.is_none()) {
+    const auto options = at::TensorOptions().device(*dev);
+    parts = at::empty({BNB_GRAD_NORM_PARTS}, options.dtype(at::kDouble));
+    norm = at::empty({}, options.dtype(at::kFloat));
+    std::vector<BnbAdamTensor> all;
+    for (const auto& list : lists) all.insert(all.end(), list.begin(), list.end());
+    check("bnb_grad_norm", bnb_grad_norm(all.data(), (int)all.size(), static_cast<double*>(parts.data_ptr()), stream));
+  }
+  for (size_t i = 0; i < lists.size(); ++i) {
+    if (norm.has_value()) {
+      calls[i].norm_parts = static_cast<const double*>(parts.data_ptr());
+      calls[i].n_norm_parts = BNB_GRAD_NORM_PARTS;
+      calls[i].max_norm = (float)max_norm.cast<double>();
+      calls[i].norm = static_cast<float*>(norm->data_ptr());
+    }
+    check("bnb_adamw_step", bnb_adamw_step(lists[i].data(), (int)lists[i].size(), &calls[i], stream));
+  }
+  for (const Tensor& t : changed)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 }  // namespace
 
 void bind_update(py::module& m) {
+  m.def("adamw_step", &adamw_step);
   m.def("policy_loss_forward", &policy_forward);
   m.def("policy_loss_backward", &policy_backward);
   m.def("policy_loss", torch::wrap_pybind_function(policy_loss));

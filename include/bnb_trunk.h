@@ -645,6 +645,48 @@ int bnb_policy_loss_fwd(const BnbPolicyLoss* call, void* scratch, size_t scratch
  * as the forward left it; its loss, stats and logprob are not read. */
 int bnb_policy_loss_bwd(const BnbPolicyLoss* call, const float* dloss, void* dlogits, void* stream);
 
+/* One AdamW step over many tensors at once.
+ *
+ * Replaces: clip_grad_norm_ and optim.step of the update (ppo.py:2011-2051, which skips an update whose gradients are not finite).
+ *   c = min(1, max_norm / (norm + 1e-6)) where the gradients are clipped, g = c grad
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  t = step + 1
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * A tensor is n elements in whatever order p, g, m and v share.  States of 32 bits are m and v in float32.  States of 8 bits are m and sqrt(v)
+ * in e4m3 with a float32 scale for each 256 elements, a power of two that takes the largest to 128 .. 256: m rounded to
+ * nearest, sqrt(v) up or down at random, unbiased, by 20 bits hashed from seed, t and position + the element's index; a sqrt(v) below the
+ * least normal number is held there, so that only 0 is taken for 0. */
+typedef struct {
+  void* p;                  /* element type below, updated in place */
+  const void* g;            /* of p's type */
+  void* m;
+  void* v;                  /* 8 bits: sqrt(v) */
+  float* m_scale;           /* 8 bits: (n + 255) / 256 */
+  float* v_scale;
+  float* step;              /* 1: steps made; moves on by one */
+  int64_t n;
+  int64_t position;
+  int32_t element;
+} BnbAdamTensor;
+
+typedef struct {
+  int32_t state_bits;       /* 32 or 8 */
+  uint32_t seed;
+  float lr;
+  const float* lr_device;   /* NULL, or the learning rate (1) on the device, in lr's place */
+  double beta1, beta2;
+  float eps, weight_decay, max_norm;
+  const double* norm_parts; /* NULL: no clipping; else the sums of squares that bnb_grad_norm left: a norm that is not finite skips the step */
+  int32_t n_norm_parts;
+  float* norm;              /* NULL, or where the norm goes (1) */
+  int32_t* control;         /* 1: zero before the first call, left so by every call */
+} BnbAdamW;
+#define BNB_GRAD_NORM_PARTS 1184
+
+/* Sums of squares of all tensors' g (the other fields but n and element are not read): BNB_GRAD_NORM_PARTS 64-bit sums in parts, all of them
+ * written.  The list is host memory and free again when the call returns. */
+int bnb_grad_norm(const BnbAdamTensor* tensors_host, int n_tensors, double* parts, void* stream);
+int bnb_adamw_step(const BnbAdamTensor* tensors_host, int n_tensors, const BnbAdamW* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -95,3 +95,40 @@ def policy_bounds(logits, actions, old, adv, weights=None, ref=None, sizes=None,
         hit = torch.zeros_like(p).scatter_(1, act, 1.0)
         ez[:, at:at + n] = v + hit * (edl + U * dl.abs())[:, None]
     return eloss, torch.where(on, el, 0.0), estats, torch.where(on[:, None], ez, 0.0)
+
+
+def adamw(p, g, m, v, step, lr, betas, eps, decay, clip=1.0):
+    """One step in 64 bits, m and v as they stand (the square of the root of 8-bit states): (p, m, v) behind it."""
+    p, g, m, v = (t.double() for t in (p, g, m, v))
+    t = step + 1
+    g = g * clip
+    m = betas[0] * m + (1 - betas[0]) * g
+    v = betas[1] * v + (1 - betas[1]) * g * g
+    p = p * (1 - lr * decay) - lr / (1 - betas[0] ** t) * m / (v.sqrt() / (1 - betas[1] ** t) ** 0.5 + eps)
+    return p, m, v
+
+
+def adamw_bounds(p, g, m, v, step, lr, betas, eps, decay, clip=1.0):
+    """What float32 results of the above may be off by: (p, m, v).  The factors count roundings: of the betas, of products and sums, of the clipping's
+    factor (8, from a norm), of the bias corrections (6 each)."""
+    p, g, m, v = (t.double() for t in (p, g, m, v))
+    p1, m1, v1 = adamw(p, g, m, v, step, lr, betas, eps, decay, clip)
+    t = step + 1
+    em = U * (3 * (betas[0] * m).abs() + 12 * ((1 - betas[0]) * g * clip).abs())
+    ev = U * (3 * betas[1] * v + 24 * (1 - betas[1]) * (g * clip) ** 2)
+    r, root, rate = v1.sqrt(), (1 - betas[1] ** t) ** -0.5, lr / (1 - betas[0] ** t)
+    er = torch.where(r > 0, ev / (2 * r.clamp(min=1e-300)), 0.0) + U * r
+    d = r * root + eps
+    ed = er * root + 8 * U * d
+    q = rate * m1.abs() / d
+    eq = rate * em / d + q * (ed / d + 12 * U)
+    return eq + U * (4 * p.abs() + 2 * q + 2 * p1.abs()), em, ev
+
+
+def noise(positions: torch.Tensor, seed: int, step: int) -> torch.Tensor:
+    """The 20 random bits of 8-bit states: products and shifts of 32 bits."""
+    low = lambda v: v & 0xFFFFFFFF  # noqa: E731
+    h = low(low(positions + (positions >> 32) * 0x632BE5AB) * 0x9E3779B1 + seed * 0x5D2F63B9 + step * 0x3C6EF36B)
+    h = low((h ^ (h >> 15)) * 0x6C8E944D)
+    h = low((h ^ (h >> 13)) * 0x5B297A4D)
+    return (h ^ (h >> 16)) >> 12

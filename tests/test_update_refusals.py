@@ -72,3 +72,71 @@ def test_operators_have_shape_only_fakes():
         loss, l, stats, kept = ops.policy_loss(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0)
         assert loss.shape == () and loss.dtype == torch.float32 and l.shape == (5, 3) and stats.shape == (4,) and kept.numel() == 4 + 15 * 7
         assert ops.policy_loss_backward(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0, kept, loss).shape == z.shape
+
+
+class AdamTensor(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale", "step")] + [("n", C.c_int64), ("position", C.c_int64), ("element", C.c_int32)]
+
+
+class AdamCall(C.Structure):
+    _fields_ = [("state_bits", C.c_int32), ("seed", C.c_uint32), ("lr", C.c_float), ("lr_device", C.c_void_p), ("beta1", C.c_double), ("beta2", C.c_double)] + [
+        (n, C.c_float) for n in ("eps", "weight_decay", "max_norm")] + [("norm_parts", C.c_void_p), ("n_norm_parts", C.c_int32), ("norm", C.c_void_p), ("control", C.c_void_p)]
+
+
+def test_adamw_entry_points_check_their_arguments():
+    from boost_and_broadside_b200 import _capi
+
+    lib, fake = _capi.lib, 0x1000
+
+    def step(tensor=None, **over):
+        t = AdamTensor(fake, fake, fake, fake, None, None, fake, 10, 0, 0)
+        for k, v in (tensor or {}).items():
+            setattr(t, k, v)
+        c = AdamCall(32, 0, 1e-3, None, 0.9, 0.999, 1e-8, 0.0, 0.0, None, 0, None, fake)
+        for k, v in over.items():
+            setattr(c, k, v)
+        return lib.bnb_adamw_step(C.byref(t), 1, C.byref(c), None)
+
+    assert step(state_bits=16) == 5 and step(beta1=1.0) == 5 and step(beta2=-0.1) == 5 and step(eps=float("nan")) == 5
+    assert step(control=None) == 1 and step(norm_parts=fake) == 5 and step(norm_parts=fake, n_norm_parts=3, max_norm=-1.0) == 5
+    assert step(state_bits=8) == 1                            # scales missing
+    for name in ("p", "g", "m", "v", "step"):
+        assert step(tensor={name: None}) == 1, name
+    assert step(tensor={"n": -1}) == 5 and step(tensor={"element": 3}) == 5
+    c = AdamCall(32, 0, 1e-3, None, 0.9, 0.999, 1e-8, 0.0, 0.0, None, 0, None, fake)
+    assert lib.bnb_adamw_step(None, 1, C.byref(c), None) == 1 and lib.bnb_adamw_step(None, -1, C.byref(c), None) == 5
+    assert lib.bnb_adamw_step(None, 0, C.byref(c), None) == 0 and lib.bnb_adamw_step(None, 0, None, None) == 1
+    assert lib.bnb_grad_norm(None, 0, None, None) == 1
+
+
+def test_adamw_checks_its_numbers():
+    import boost_and_broadside_b200 as bnb
+
+    p = torch.nn.Parameter(torch.zeros(3))
+    for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(max_norm=-1.0), dict(state_bits=16),
+                dict(lr=torch.zeros(2))):
+        with pytest.raises(ValueError, match="AdamW"):
+            bnb.AdamW([p], **bad)
+    with pytest.raises(ValueError, match="float64"):
+        bnb.AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float64))])
+    opt = bnb.AdamW([p])
+    opt.step()                                                # no gradient, nothing to do
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2))], lr=-1.0))
+    assert len(opt.param_groups) == 1
+    p.grad = torch.zeros(3)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        opt.step()
+
+
+def test_random_bits_are_even_and_of_their_own():
+    """The 20 bits behind a rounding at random: means, neighbours, steps and seeds, within five standard errors."""
+    from oracle import update_oracle as O
+
+    n = 1 << 18
+    at = torch.arange(n)
+    a = O.noise(at, 3, 7).double() / 2 ** 20
+    for other in (O.noise(at, 3, 8), O.noise(at, 4, 7), O.noise(at + 256, 3, 7), O.noise(at + 1, 3, 7), O.noise(at + (1 << 32), 3, 7)):
+        b = other.double() / 2 ** 20
+        assert abs(float(b.mean()) - 0.5) <= 5 * (1 / 12 / n) ** 0.5
+        assert abs(float(((a - 0.5) * (b - 0.5)).mean())) <= 5 / 12 / n ** 0.5
