@@ -18,6 +18,7 @@ from .yemong.encoder import BulletEncoder, ShipEncoder
 from .yemong.gated import gated_mlp
 from .yemong.heads import HeadMLP, NextStateHead, TeamPMA, evaluate_action, sample_action
 from .yemong.griffin import CONV_KERNEL, RGLRU, GriffinTemporalBlock, YemongBlock
+from .yemong.linear import linear
 from .yemong.optimizer import AdamW
 from .yemong.policy import YemongPolicy
 from .yemong.policy_loss import policy_loss
@@ -46,6 +47,7 @@ __all__ = [
     "causal_conv_step",
     "evaluate_action",
     "gated_mlp",
+    "linear",
     "policy_loss",
     "sample_action",
     "selective_scan",

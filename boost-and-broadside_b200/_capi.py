@@ -147,6 +147,10 @@ EXPORTS = {
     "bnb_gated_block_fwd": (C.c_int, [_fp, _fp, C.c_size_t, _fp]),
     "bnb_gated_block_bwd": (C.c_int, [_fp, _fp, _fp, C.c_size_t, _fp]),
     # the end of an update (csrc/host_update.cpp)
+    "bnb_linear_kept_bytes": (C.c_size_t, [_fp]),
+    "bnb_linear_scratch_bytes": (C.c_size_t, [_fp, C.c_int]),
+    "bnb_linear_fwd": (C.c_int, [_fp, _fp, C.c_size_t, _fp]),
+    "bnb_linear_bwd": (C.c_int, [_fp, _fp, _fp, C.c_size_t, _fp]),
     "bnb_policy_loss_kept_bytes": (C.c_size_t, [_fp]),
     "bnb_policy_loss_scratch_bytes": (C.c_size_t, [_fp]),
     "bnb_policy_loss_fwd": (C.c_int, [_fp, _fp, C.c_size_t, _fp]),

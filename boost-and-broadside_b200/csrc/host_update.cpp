@@ -1,4 +1,4 @@
-// The host side of the operators behind the trunk in an update (yemong/policy_loss.py, yemong/optimizer.py): checks, outputs and scratch from torch's
+// The host side of the operators behind the trunk in an update (yemong/linear.py, yemong/policy_loss.py, yemong/optimizer.py): checks, outputs and scratch from torch's
 // allocator, the launch, the autograd nodes of eager calls.
 #include "host_nodes.h"
 
@@ -9,6 +9,123 @@
 namespace bnb {
 namespace host {
 namespace {
+
+// ------------------------------------------------------------------ linear layer
+
+struct LinearCall {
+  BnbLinear c{};
+  std::vector<Tensor> held;
+};
+std::vector<int64_t> out_sizes(const Tensor& x, const Tensor& weight) {
+  std::vector<int64_t> s = x.sizes().vec();
+  s.back() = weight.size(0);
+  return s;
+}
+LinearCall linear_call(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int activation) {
+  const char* fn = "linear";
+  expect_cuda(fn, x);
+  if (x.dim() < 1) refuse("linear: x must have shape (.., width)");
+  const int64_t K = x.size(-1);
+  const c10::Device dev = x.device();
+  LinearCall k;
+  BnbLinear& c = k.c;
+  c.element = element_of(fn, x);
+  if (weight.dim() != 2) refuse("linear: weight must have shape (out, " + std::to_string(K) + "), got " + shape_text(weight.sizes()));
+  const int64_t N = weight.size(0);
+  if (K < 1 || N < 1) throw py::value_error("linear: width and outputs must be at least 1");
+  expect(fn, "weight", weight, {N, K}, dev);
+  if (weight.scalar_type() != x.scalar_type() && weight.scalar_type() != at::kFloat)
+    refuse(std::string("linear: weight must be float32 or of the input's type ") + c10::toString(x.scalar_type()));
+  c.weight_element = element_of(fn, weight);
+  c.bias_element = c.element;
+  if (bias.has_value()) {
+    expect(fn, "bias", *bias, {N}, dev);
+    if (bias->scalar_type() != x.scalar_type() && bias->scalar_type() != at::kFloat)
+      refuse(std::string("linear: bias must be float32 or of the input's type ") + c10::toString(x.scalar_type()));
+    c.bias_element = element_of(fn, *bias);
+    k.held.push_back(contiguous(*bias));
+    c.bias = k.held.back().data_ptr();
+  }
+  const Tensor flat = rows_of(x);
+  k.held.push_back(flat);
+  c.rows = flat.size(0);
+  c.width = fits_int(fn, K);
+  c.out = fits_int(fn, N);
+  c.activation = activation;
+  c.x = flat.data_ptr();
+  c.x_row = row_stride(flat);
+  k.held.push_back(contiguous(weight));
+  c.weight = k.held.back().data_ptr();
+  if (residual.has_value()) {
+    expect(fn, "residual", *residual, out_sizes(x, weight), dev);
+    expect_type(fn, "residual", *residual, x.scalar_type());
+    const Tensor r = rows_of(*residual);
+    k.held.push_back(r);
+    c.residual = r.data_ptr();
+    c.residual_row = row_stride(r);
+  }
+  return k;
+}
+
+// (y, what the backward reads: empty unless asked for)
+std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int activation, bool keep) {
+  const c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
+  LinearCall k = linear_call(x, weight, bias, residual, activation);
+  raise_pending_status(x.device());
+  const Tensor y = at::empty(out_sizes(x, weight), x.options());
+  const Tensor kept = at::empty({keep ? (int64_t)bnb_linear_kept_bytes(&k.c) : 0}, x.options().dtype(at::kByte));
+  k.c.y = y.data_ptr();
+  k.c.kept = keep && kept.numel() ? kept.data_ptr() : nullptr;
+  const Tensor scratch = scratch_of(bnb_linear_scratch_bytes(&k.c, 0), x);
+  check("bnb_linear_fwd", bnb_linear_fwd(&k.c, scratch.data_ptr(), (size_t)scratch.numel(), stream_of(x.device())));
+  return {y, kept};
+}
+
+// Gradients of x, weight and bias, those that are wanted.
+std::vector<Tensor> linear_backward(const Tensor& x, const Tensor& weight, const OptTensor& bias, int activation, const Tensor& kept, const Tensor& dy,
+                                    bool want_x, bool want_weight, bool want_bias) {
+  if (!want_x && !want_weight && !(want_bias && bias.has_value())) return std::vector<Tensor>(3);
+  const c10::cuda::CUDAGuard guard(x.device());
+  LinearCall k = linear_call(x, weight, bias, c10::nullopt, activation);
+  Tensor held = contiguous(kept).to(x.device());
+  if (held.scalar_type() != at::kByte || (size_t)held.numel() != bnb_linear_kept_bytes(&k.c))
+    refuse("linear: the kept activations came back as another tensor: saved-tensor hooks have to return type and shape as they were");
+  if (reinterpret_cast<uintptr_t>(held.data_ptr()) % 16) held = held.clone();
+  expect("linear", "the gradient of y", dy, out_sizes(x, weight), x.device());
+  const Tensor gy = rows_of(dy.to(x.scalar_type()));
+  const Tensor dx = want_x ? at::empty(x.sizes(), x.options()) : Tensor(), dw = want_weight ? at::empty(weight.sizes(), weight.options()) : Tensor(),
+               db = want_bias && bias.has_value() ? at::empty(bias->sizes(), bias->options()) : Tensor();
+  auto at_ = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  k.c.kept = held.numel() ? held.data_ptr() : nullptr;
+  const BnbLinearGrads g{gy.data_ptr(), row_stride(gy), at_(dx), at_(dw), at_(db)};
+  const Tensor scratch = scratch_of(bnb_linear_scratch_bytes(&k.c, 1), x);
+  check("bnb_linear_bwd", bnb_linear_bwd(&k.c, &g, scratch.data_ptr(), (size_t)scratch.numel(), stream_of(x.device())));
+  return {dx, dw, db};
+}
+
+Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int activation) {
+  const variable_list inputs{x, weight, value(bias), value(residual)};
+  if (!wants_grad(inputs)) return std::get<0>(linear_forward(x, weight, bias, residual, activation, false));
+  Tensor y, kept;
+  {
+    const at::NoGradGuard no_grad;
+    std::tie(y, kept) = linear_forward(x, weight, bias, residual, activation, true);
+  }
+  // the residual's values are not needed again: an undefined tensor in its place
+  auto node = node_of({x, weight, value(bias)}, {kept}, {});
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs));
+  const bool has_residual = residual.has_value();
+  OpNode* const self = node.get();
+  node->backward = [activation, has_residual, self](const std::vector<Tensor>& s, const variable_list& g) -> variable_list {
+    if (!g[0].defined()) return variable_list(4);
+    variable_list out = linear_backward(s[0], s[1], opt(s[2]), activation, s[3], g[0], self->task_should_compute_output(0), self->task_should_compute_output(1),
+                                        s[2].defined() && self->task_should_compute_output(2));
+    out.push_back(has_residual ? g[0].to(s[0].scalar_type()) : Tensor());
+    return out;
+  };
+  torch::autograd::create_gradient_edge(y, node);
+  return y;
+}
 
 // ------------------------------------------------------------------ policy loss
 
@@ -261,6 +378,9 @@ OptTensor adamw_step(const std::vector<Group>& groups, const py::object& max_nor
 }  // namespace
 
 void bind_update(py::module& m) {
+  m.def("linear_forward", &linear_forward);
+  m.def("linear_backward", &linear_backward);
+  m.def("linear", torch::wrap_pybind_function(linear));
   m.def("adamw_step", &adamw_step);
   m.def("policy_loss_forward", &policy_forward);
   m.def("policy_loss_backward", &policy_backward);

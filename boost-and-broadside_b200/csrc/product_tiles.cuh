@@ -1,5 +1,5 @@
-// Matrix products on tcgen05 tiles for operands of any size, with the epilogues of the gated feed-forward block fused
-// into them (gated_mlp.cu).
+// Matrix products on tcgen05 tiles for operands of any size, with the epilogues of the gated feed-forward block (gated_mlp.cu) and of the
+// linear layer (linear.cu) fused into them.
 //
 // out (m, n) = sum over terms of A_t (m, k) B_t (n, k)^T.  One persistent CTA per SM walks over tiles of 128 x BN; a warp fetches (TMA
 // boxes of 64 elements by 64 to 256, 128-byte swizzle, zeros outside the tensors, so that no size has to be a multiple of a
@@ -40,7 +40,10 @@ enum : int { W_FULL = 101, W_EMPTY = 102, W_ACC = 103, W_DRAINED = 104 };
 //   GATE     columns come in pairs of tiles, g and u: h = act(g) u as operand pieces; g and u themselves where they are kept
 //   BACK     columns are dh: dg = dh u act'(g), du = dh act(g), h = act(g) u as operand pieces, from the kept g and u
 //   AGAIN    the same with g and u computed once more: a stage holds x and dy, and 64 columns of all three weights
-enum class Out : int { VALUES, PARTIAL, GATE, BACK, AGAIN };
+//   LINEAR   z = sum + bias, out[0] = act(z) + other (m, n); z itself where it is kept
+//   SLOPE    the same z: other act'(z) as operand pieces (16 bits)
+enum class Out : int { VALUES, PARTIAL, GATE, BACK, AGAIN, LINEAR, SLOPE };
+template <Out OUT> constexpr bool is_linear = OUT == Out::LINEAR || OUT == Out::SLOPE;
 
 struct Epilogue {
   void* out[2];
@@ -52,7 +55,11 @@ struct Epilogue {
   float* u;
   int64_t ld_out, ld_h, piece_stride;
   int out_kind;         // 0: float32, 1: the operands' type
-  int activation;       // BNB_ACT_SILU or BNB_ACT_GELU
+  int activation;       // BNB_ACT_SILU or BNB_ACT_GELU; a linear layer's also BNB_ACT_NONE
+  const void* bias;     // (n), or null
+  const void* other;    // LINEAR: (m, n) of the results' type to be added, or null; SLOPE: dy
+  int64_t ld_other;
+  int bias_kind, other_wide;   // bias_kind: 0 float32, 1 the operands' type; other_wide: rows of `other` start on 16 bytes
 };
 
 struct Product {
@@ -139,6 +146,11 @@ __device__ __forceinline__ void activate(int kind, F2 g, F2& a, F2& da) {
   }
 }
 
+// Where float32 values are kept for a backward: blocks of 32 rows by 32 columns, each eight requests of a float4 a lane, its row's.
+__device__ __forceinline__ int64_t kept_index(int64_t r, int c, int64_t ld) {
+  return ((((r >> 5) * ((ld + 31) >> 5) + (c >> 5)) * 8 + ((c & 31) >> 2)) * 32 + (r & 31)) * 4 + (c & 3);
+}
+
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -179,8 +191,9 @@ template <int BN, Out OUT>
 struct Shape {
   static constexpr uint32_t B_BYTES = BN * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
   static constexpr int COLS = OUT == Out::GATE ? BN / 2 : OUT == Out::AGAIN ? BN / 3 : BN;   // of the output
-  static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_BYTES) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
-  static constexpr uint32_t OUT_AT = STAGES * STAGE, FRAME = OUT_AT + OUT_BYTES, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
+  static constexpr uint32_t BIAS = is_linear<OUT> ? OUT_WARPS * 128 : 0;   // a warp's bias of a segment
+  static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_BYTES - BIAS) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
+  static constexpr uint32_t OUT_AT = STAGES * STAGE, BIAS_AT = OUT_AT + OUT_BYTES, FRAME = BIAS_AT + BIAS, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
 };
 
 // Results to memory: 32 rows of 64 columns at a time, a row a lane of PARTS warps.  A request that writes a little of many rows costs the load
@@ -229,12 +242,29 @@ __device__ __forceinline__ void put16(E* row, int col, int cols, bool wide, uint
   }
 }
 
+// The reverse: what is not there is 0.
+template <typename E>
+__device__ __forceinline__ uint4 get16(const E* row, int col, int cols, bool wide) {
+  constexpr int N = 16 / sizeof(E);
+  if (wide && col + N <= cols) return *reinterpret_cast<const uint4*>(row + col);
+  uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+  E* e = reinterpret_cast<E*>(&raw);
+#pragma unroll
+  for (int i = 0; i < N; ++i) if (col + i < cols) e[i] = row[col + i];
+  return raw;
+}
+__device__ __forceinline__ F2 pair_up(uint32_t v, __nv_bfloat16) { return unpack_bf16(v); }
+__device__ __forceinline__ F2 pair_up(uint32_t v, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return f2(f.x, f.y);
+}
+
 // Sixteen warps take out in two groups, tiles in turn: while one group waits for accumulators, for its rows or for memory, the other
 // computes.  (All sixteen on a tile at once wait together: 71 us for dh and its gradients at 65 536 x 128 x 512.)  Float32, whose runs need both
 // sets of accumulators for one tile, has one group, and so has BACK: it waits for g and u from memory most, and 16 columns a warp leave
 // the registers to have all of a segment's on their way at once (128 us against 113 at 8192 x 1024 x 4096).
 template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT>
-__global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Product p) {
+static __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Product p) {
   using S = Shape<BN, OUT>;
   constexpr bool EXACT = PIECES > 1;
   constexpr int GROUPS = EXACT || OUT == Out::BACK ? 1 : 2, PARTS = OUT_WARPS / 4 / GROUPS;
@@ -432,6 +462,26 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
           tmem_wait_ld();
           if (!EXACT && last && k + 8 == SEG) release(set), released = true;
         };
+        // a linear layer: the rows of `other` as whole rows and the bias, on their way before the accumulators are waited for
+        uint4 others[is_linear<OUT> && !EXACT ? 8 / PARTS : 1];
+        float* bias = reinterpret_cast<float*>(smem + S::BIAS_AT + (warp - 2) * 128);
+        if constexpr (is_linear<OUT>) {
+          float b = 0.f;
+          if (e.bias && lane < SEG && col0 + lane < p.n)
+            b = e.bias_kind == 0 ? static_cast<const float*>(e.bias)[col0 + lane] : up(static_cast<const E*>(e.bias)[col0 + lane]);
+          if constexpr (!EXACT) {
+            if (e.other)
+#pragma unroll
+              for (int i = 0; i < 8 / PARTS; ++i) {
+                const int r = (32 / PARTS) * part + i * 4 + lane / 8;
+                others[i] = row0 + r < p.m ? get16(static_cast<const E*>(e.other) + (row0 + r) * e.ld_other, first + 8 * (lane % 8), p.n, e.other_wide)
+                                           : make_uint4(0u, 0u, 0u, 0u);
+              }
+          }
+          __syncwarp();
+          bias[lane] = b;
+          __syncwarp();
+        }
         uint4 kept[OUT == Out::BACK ? 2 : 1][SEG / 4];
         if constexpr (OUT == Out::BACK) {
 #pragma unroll
@@ -513,6 +563,85 @@ __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Prod
                 if (row0 + r < p.m && first + c < e.ld_h) *reinterpret_cast<uint4*>(at + (row0 + r) * e.ld_h + first + c) = raw;
               });
             }
+          }
+        } else if constexpr (is_linear<OUT> && !EXACT) {
+          meet();   // what stood there is written
+          if (e.other) {
+#pragma unroll
+            for (int i = 0; i < 8 / PARTS; ++i) *reinterpret_cast<uint4*>(rows + row_piece((32 / PARTS) * part + i * 4 + lane / 8, lane % 8)) = others[i];
+            meet();
+          }
+#pragma unroll
+          for (int k0 = 0; k0 < SEG; k0 += 8) {
+            uint32_t z[8], bits[4], o[4] = {0u, 0u, 0u, 0u};
+            tmem_ld8_nowait(acc + c0 + k0, z);
+            uint4* at = reinterpret_cast<uint4*>(rows + row_piece(lane, (part * SEG + k0) / 8));   // this lane's own
+            const float4 b0 = *reinterpret_cast<const float4*>(bias + k0), b1 = *reinterpret_cast<const float4*>(bias + k0 + 4);
+            if (e.other) {
+              const uint4 raw = *at;
+              o[0] = raw.x, o[1] = raw.y, o[2] = raw.z, o[3] = raw.w;
+            }
+            taken(k0);
+            const F2 b[4] = {f2(b0.x, b0.y), f2(b0.z, b0.w), f2(b1.x, b1.y), f2(b1.z, b1.w)};
+            F2 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = add(pair(z, k), b[k]);
+            if constexpr (OUT == Out::LINEAR) {
+              if (e.g && in)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  const float2 x = halves(v[2 * q]), y = halves(v[2 * q + 1]);
+                  *kept_at(e.g, col0 + k0, q) = make_float4(x.x, x.y, y.x, y.y);
+                }
+            }
+            F2 a[4], da[4];
+            if (e.activation == BNB_ACT_NONE) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) a[k] = v[k], da[k] = f2(1.f);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) activate<false, OUT == Out::SLOPE>(e.activation, v[k], a[k], da[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) bits[k] = pair_of<E>(OUT == Out::SLOPE ? mul(pair_up(o[k], E{}), da[k]) : e.other ? add(a[k], pair_up(o[k], E{})) : a[k]);
+            *at = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+          }
+          meet();
+          E* to = static_cast<E*>(OUT == Out::SLOPE ? e.h : e.out[0]);
+          const int64_t ld = OUT == Out::SLOPE ? e.ld_h : e.ld_out;
+          const int cols = OUT == Out::SLOPE ? (int)e.ld_h : p.n;   // an operand's rows are padded with zeros
+          take_rows<PARTS>(rows, part, lane, [&](int r, int c, uint4 raw) {
+            if (row0 + r < p.m) put16(to + (row0 + r) * ld, first + c, cols, ld % 8 == 0, raw);
+          });
+        } else if constexpr (is_linear<OUT>) {
+          // float32: 16 columns at a time
+#pragma unroll
+          for (int k0 = 0; k0 < SEG; k0 += 16) {
+            uint32_t v[16];
+            tmem_ld16_nowait(acc + c0 + k0, v);
+            tmem_wait_ld();
+            float o[16];
+            const float* row = static_cast<const float*>(e.other) + (row0 + lane) * e.ld_other;
+#pragma unroll
+            for (int q = 0; q < 16; q += 4) {
+              const uint4 raw = e.other && row0 + lane < p.m ? get16(row, col0 + k0 + q, p.n, e.other_wide) : make_uint4(0u, 0u, 0u, 0u);
+              o[q] = __uint_as_float(raw.x), o[q + 1] = __uint_as_float(raw.y), o[q + 2] = __uint_as_float(raw.z), o[q + 3] = __uint_as_float(raw.w);
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) + bias[k0 + k]);
+            if (e.g && in)
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<uint4*>(kept_at(e.g, col0 + k0, q)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float a = __uint_as_float(v[k]), da;
+              if (e.activation != BNB_ACT_NONE) activate_exact(e.activation, a, a, da);
+              v[k] = __float_as_uint(e.other ? a + o[k] : a);
+            }
+            emit_floats(stage, lane, v, [&](int r, int c, uint4 raw) {
+              if (row0 + r < p.m) put16(static_cast<float*>(e.out[0]) + (row0 + r) * e.ld_out, col0 + k0 + c, p.n, e.ld_out % 4 == 0, raw);
+            });
           }
         } else {
           const bool floats = OUT == Out::PARTIAL || e.out_kind == 0;

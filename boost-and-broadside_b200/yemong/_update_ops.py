@@ -1,4 +1,4 @@
-"""Opaque ``torch.library`` operators of an update's end (``policy_loss.py``), for callers that have to see them: a compiler, a
+"""Opaque ``torch.library`` operators of an update's end (``linear.py``, ``policy_loss.py``), for callers that have to see them: a compiler, a
 tracer, a dispatch mode.  Same reason and same form as ``_ops.py``; eager calls go to the native code (csrc/host_update.cpp)
 directly, autograd nodes included.
 """
@@ -11,6 +11,64 @@ import torch
 from torch import Tensor
 
 from .. import _capi
+
+
+# ----------------------------------------------------------------------------- linear layer
+
+
+@torch.library.custom_op("bnb_b200::linear", mutates_args=(), device_types="cuda")
+def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional[Tensor], activation: int, keep: bool) -> Tuple[Tensor, Tensor]:
+    """``bnb_linear_fwd``: x (.., K), weight (N, K) -> (y (.., N), what the backward reads: empty without ``keep``)."""
+    return _capi.host.linear_forward(x, weight, bias, residual, activation, keep)
+
+
+@linear.register_fake
+def _(x, weight, bias, residual, activation, keep):
+    # as bnb_linear_kept_bytes: without an activation nothing is kept, and narrow 16-bit calls compute z once more
+    recomputes = activation == 0 or (x.dtype != torch.float32 and x.shape[-1] <= 512)
+    rows = x.numel() // x.shape[-1]
+    kept = 4 * ((rows + 31) // 32 * 32) * ((weight.shape[0] + 31) // 32 * 32)
+    return x.new_empty((*x.shape[:-1], weight.shape[0])), x.new_empty(kept if keep and not recomputes else 0, dtype=torch.uint8)
+
+
+@torch.library.custom_op("bnb_b200::linear_backward", mutates_args=(), device_types="cuda")
+def linear_backward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: int, kept: Tensor, dy: Tensor, want_x: bool, want_weight: bool,
+                    want_bias: bool) -> List[Tensor]:
+    """Gradients of x, weight and bias; an empty tensor for one that is not wanted or was not given."""
+    out = _capi.host.linear_backward(x, weight, bias, activation, kept, dy, want_x, want_weight, want_bias)
+    return [x.new_empty(0) if g is None else g for g in out]
+
+
+@linear_backward.register_fake
+def _(x, weight, bias, activation, kept, dy, want_x, want_weight, want_bias):
+    like = lambda t, wanted: x.new_empty(0) if t is None or not wanted else t.new_empty(t.shape)  # noqa: E731
+    return [like(x, want_x), like(weight, want_weight), like(bias, want_bias)]
+
+
+def _linear_context(ctx, inputs, output):
+    x, weight, bias, residual, activation, keep = inputs
+    ctx.activation, ctx.keep, ctx.has_residual = activation, keep, residual is not None
+    ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, weight, bias, output[1])
+
+
+def _linear_formula(ctx, dy, _dkept):
+    if not ctx.keep:
+        raise RuntimeError("linear was called without keeping what its backward reads")
+    x, weight, bias, kept = ctx.saved_tensors
+    if dy is None:
+        return (None,) * 6
+    want = ctx.needs_input_grad
+    wants = (want[0], want[1], want[2] and bias is not None)
+    grads = linear_backward(x, weight, bias, ctx.activation, kept, dy, *wants)
+    return (*(g if w else None for g, w in zip(grads, wants)), dy if ctx.has_residual else None, None, None)
+
+
+linear.register_autograd(_linear_formula, setup_context=_linear_context)
+
+
+# ----------------------------------------------------------------------------- policy loss
 
 
 @torch.library.custom_op("bnb_b200::policy_loss", mutates_args=(), device_types="cuda")

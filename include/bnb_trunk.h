@@ -604,6 +604,40 @@ typedef struct {
 int bnb_gated_block_bwd(const BnbGatedBlock* call, const BnbGatedBlockGrads* grads, void* scratch, size_t scratch_bytes,
                         void* stream);
 
+/* y = act(x weight^T + bias) + residual on tensor-core tiles, any width and number of outputs.
+ *   element: type of x, residual and y; 16-bit ones are the operands of the products, float32 ones go through exact pieces
+ *   weight_element, bias_element: element, or BNB_ELEM_F32; weights a call of 16-bit elements rounds as autocast does, a bias not
+ *   weight (out, width) contiguous, bias (out) or NULL; x (rows, width), residual (rows, out) or NULL, x_row and residual_row elements
+ *   between rows; y (rows, out) contiguous; activation BNB_ACT_NONE, BNB_ACT_SILU or BNB_ACT_GELU
+ *   kept: NULL, or bnb_linear_kept_bytes bytes that the backward reads
+ *   y, kept, scratch 16-byte aligned.  Waits are bounded, as in bnb_gated_block_fwd. */
+typedef struct {
+  int64_t rows;
+  int32_t width, out, element, weight_element, bias_element, activation;
+  const void* x;
+  int64_t x_row;
+  const void* weight;
+  const void* bias;
+  const void* residual;
+  int64_t residual_row;
+  void* y;
+  void* kept;
+} BnbLinear;
+size_t bnb_linear_kept_bytes(const BnbLinear* call);
+size_t bnb_linear_scratch_bytes(const BnbLinear* call, int backward);
+int bnb_linear_fwd(const BnbLinear* call, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Gradients of given dy (rows, out), dy_row elements between rows: dx (rows, width) of x's type, dweight of the weights', dbias of the
+ * bias's.  Any may be NULL and is left out.  The residual's gradient is dy.  The call's `kept` as the forward left it; its y is not read. */
+typedef struct {
+  const void* dy;
+  int64_t dy_row;
+  void* dx;
+  void* dweight;
+  void* dbias;
+} BnbLinearGrads;
+int bnb_linear_bwd(const BnbLinear* call, const BnbLinearGrads* grads, void* scratch, size_t scratch_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------------
  * The end of a policy update: the loss behind a head's logits.
  *

@@ -132,3 +132,12 @@ def noise(positions: torch.Tensor, seed: int, step: int) -> torch.Tensor:
     h = low((h ^ (h >> 15)) * 0x6C8E944D)
     h = low((h ^ (h >> 13)) * 0x5B297A4D)
     return (h ^ (h >> 16)) >> 12
+
+
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """act(x weight^T + bias) + residual; act is none, SiLU or erf GELU."""
+    f = torch.nn.functional
+    z = x.double() @ weight.double().t()
+    z = z if bias is None else z + bias.double()
+    y = {None: lambda v: v, "silu": f.silu, "gelu": f.gelu}[activation](z)
+    return y if residual is None else y + residual.double()

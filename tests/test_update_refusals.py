@@ -71,6 +71,9 @@ def test_operators_have_shape_only_fakes():
         a, v = torch.empty(5, 3, 3, device="cuda", dtype=torch.int64), torch.empty(5, 3, device="cuda")
         loss, l, stats, kept = ops.policy_loss(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0)
         assert loss.shape == () and loss.dtype == torch.float32 and l.shape == (5, 3) and stats.shape == (4,) and kept.numel() == 4 + 15 * 7
+        y, kept_z = ops.linear(z, torch.empty(20, 12, device="cuda"), None, None, 2, True)
+        assert y.shape == (5, 3, 20) and y.dtype == z.dtype and kept_z.numel() == 0
+        assert ops.linear(z.float(), torch.empty(20, 12, device="cuda"), None, None, 2, True)[1].numel() == 4 * 32 * 32
         assert ops.policy_loss_backward(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0, kept, loss).shape == z.shape
 
 
@@ -140,3 +143,45 @@ def test_random_bits_are_even_and_of_their_own():
         b = other.double() / 2 ** 20
         assert abs(float(b.mean()) - 0.5) <= 5 * (1 / 12 / n) ** 0.5
         assert abs(float(((a - 0.5) * (b - 0.5)).mean())) <= 5 / 12 / n ** 0.5
+
+
+class Linear(C.Structure):
+    _fields_ = [("rows", C.c_int64)] + [(n, C.c_int32) for n in ("width", "out", "element", "weight_element", "bias_element", "activation")] + [
+        ("x", C.c_void_p), ("x_row", C.c_int64), ("weight", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("residual_row", C.c_int64),
+        ("y", C.c_void_p), ("kept", C.c_void_p)]
+
+
+class LinearGrads(C.Structure):
+    _fields_ = [("dy", C.c_void_p), ("dy_row", C.c_int64)] + [(n, C.c_void_p) for n in ("dx", "dweight", "dbias")]
+
+
+def test_linear_checks_its_arguments():
+    import boost_and_broadside_b200 as bnb
+    from boost_and_broadside_b200 import _capi
+
+    x, w = torch.zeros(3, 8), torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        bnb.linear(x, w)
+    with pytest.raises(ValueError, match="activation"):
+        bnb.linear(x, w, activation="relu")
+    lib, fake = _capi.lib, 0x1000
+
+    def call(**over):
+        c = Linear(100, 64, 128, 1, 1, 1, 2, fake, 64, fake, fake, None, 0, fake, None)
+        for k, v in over.items():
+            setattr(c, k, v)
+        return c
+
+    fwd = lambda **over: lib.bnb_linear_fwd(C.byref(call(**over)), None, 0, None)  # noqa: E731
+    assert fwd(width=0) == 3 and fwd(out=0) == 3 and fwd(weight_element=2) == 3 and fwd(bias_element=2) == 3
+    assert fwd(activation=3) == 5 and fwd(element=3) == 5 and fwd(rows=-1) == 5
+    assert fwd(weight=None) == 1 and fwd(x=None) == 1 and fwd(y=None) == 1
+    assert fwd(y=fake + 4) == 2 and fwd() == 6 and fwd(rows=0) == 0
+    kept = lambda **over: lib.bnb_linear_kept_bytes(C.byref(call(**over)))  # noqa: E731
+    assert kept() == 0 and kept(width=600, activation=0) == 0                # computed once more; no activation
+    assert kept(width=600) == 128 * 128 * 4 and kept(element=0, weight_element=0, bias_element=0) == 128 * 128 * 4
+    assert lib.bnb_linear_scratch_bytes(C.byref(call()), 1) > lib.bnb_linear_scratch_bytes(C.byref(call()), 0)
+    bwd = lambda g, **over: lib.bnb_linear_bwd(C.byref(call(**over)), C.byref(g) if g else None, None, 0, None)  # noqa: E731
+    assert bwd(None) == 1 and bwd(LinearGrads(None, 128, fake, fake, fake)) == 1
+    assert bwd(LinearGrads(fake, 128, fake, fake, fake), width=600) == 1     # nothing kept
+    assert bwd(LinearGrads(fake, 128, fake + 8, fake, fake)) == 2 and bwd(LinearGrads(fake, 128, fake, fake, fake)) == 6
