@@ -26,24 +26,24 @@ constexpr int SMS = 148, THREADS = 256, CHUNK = THREADS * 8, BLOCK = 256;
 constexpr int CTAS = SMS * 8;
 static_assert(CTAS == BNB_GRAD_NORM_PARTS, "a part a CTA");
 
-// Arguments of a kernel end at 32 764 bytes.
+// Arguments of a kernel end at 32 764 bytes, and a longer list takes longer to launch.
 template <int MOST> struct Tensors {
   int n;
-  int64_t chunks;
-  int64_t first[MOST + 1];   // chunks before each tensor
+  uint32_t chunks;
+  uint32_t first[MOST + 1];   // chunks before each tensor; all of them behind the last
   BnbAdamTensor t[MOST];
 };
-constexpr int FEW = 32, MANY = 320;
+constexpr int FEW = 32, SOME = 128, MANY = 360;
 
+// The tensor of a chunk, by all lanes of a warp: two steps where halving takes nine, each of which waits for memory.
 template <int MOST>
-__device__ __forceinline__ int tensor_of(const Tensors<MOST>& l, int64_t chunk) {
-  int lo = 0, hi = l.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (l.first[mid] <= chunk) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+__device__ __forceinline__ int tensor_of(const Tensors<MOST>& l, uint32_t chunk) {
+  constexpr int STRIDE = (MOST + 31) / 32;
+  const int lane = threadIdx.x & 31;
+  const int part = __popc(__ballot_sync(0xffffffffu, l.first[min(lane * STRIDE, MOST)] <= chunk)) - 1;
+  const int i = part * STRIDE + lane;
+  const unsigned in = __ballot_sync(0xffffffffu, lane < STRIDE && i < l.n && l.first[min(i, MOST)] <= chunk);
+  return part * STRIDE + __popc(in) - 1;
 }
 
 // Eight neighbouring elements from `at` on of `n`; `wide`: all there, on their natural boundary of eight.
@@ -122,6 +122,12 @@ __device__ __forceinline__ float warp_max(float v) {
   for (int by = 16; by; by >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, by));
   return v;
 }
+// Square root by the instruction, within a unit in the last place; numbers below the normal ones are not taken for 0.
+__device__ __forceinline__ float root_of(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 // The exponent (in place) of the scale that takes `most` to 128 .. 256.
 __device__ __forceinline__ uint32_t scale_exponent(float most) { return (uint32_t)max((int)(__float_as_uint(most) >> 23) - 7, 1); }
 __device__ __forceinline__ float power(uint32_t exponent) { return __uint_as_float(exponent << 23); }
@@ -143,13 +149,13 @@ __global__ void __launch_bounds__(THREADS) k_norm(const __grid_constant__ Tensor
   let_next_start();
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c0 = l.chunks * blockIdx.x / gridDim.x, c1 = l.chunks * (blockIdx.x + 1) / gridDim.x;
+  const uint32_t c0 = (uint64_t)l.chunks * blockIdx.x / gridDim.x, c1 = (uint64_t)l.chunks * (blockIdx.x + 1) / gridDim.x;
   double sum = 0;
   int i = c0 < c1 ? tensor_of(l, c0) : 0;
-  for (int64_t c = c0; c < c1; ++c) {
+  for (uint32_t c = c0; c < c1; ++c) {
     while (l.first[i + 1] <= c) ++i;
     const BnbAdamTensor& t = l.t[i];
-    const int64_t at = (c - l.first[i]) * CHUNK + threadIdx.x * 8;
+    const int64_t at = (int64_t)(c - l.first[i]) * CHUNK + threadIdx.x * 8;
     if (at >= t.n) continue;
     float g[8];
     take_any(t.element, t.g, at, t.n, values_lie_well(t.element, t.g) && at + 8 <= t.n, g);
@@ -180,6 +186,19 @@ struct Hyper {
   float log1, log2_;                  // natural logarithms of the betas
 };
 
+// Eight elements of a lane as they come from memory.
+template <bool EIGHT>
+struct Piece {
+  float p[8], g[8];
+  float m[EIGHT ? 1 : 8], v[EIGHT ? 1 : 8];
+  uint2 codes_m, codes_v;
+  float scale_m, scale_v;
+  int64_t at;       // of the lane's first element, behind the tensor's end where the warp has nothing
+  int tensor;
+  bool whole;
+};
+
+// With 8-bit states a chunk's loads are on their way while the one before is rounded and written.
 template <int MOST, bool EIGHT>
 __global__ void __launch_bounds__(THREADS) k_step(const __grid_constant__ Tensors<MOST> l, const __grid_constant__ Hyper h) {
   __shared__ double sums[THREADS / 32];
@@ -187,11 +206,35 @@ __global__ void __launch_bounds__(THREADS) k_step(const __grid_constant__ Tensor
   let_next_start();
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t c0 = (uint64_t)l.chunks * blockIdx.x / gridDim.x, c1 = (uint64_t)l.chunks * (blockIdx.x + 1) / gridDim.x;
+  int i = c0 < c1 ? tensor_of(l, c0) : 0;
+  auto fetch = [&](uint32_t c, Piece<EIGHT>& x) {
+    while (l.first[i + 1] <= c) ++i;
+    const BnbAdamTensor& t = l.t[i];
+    const int64_t start = (int64_t)(c - l.first[i]) * CHUNK + warp * BLOCK;
+    x.at = start + lane * 8;
+    x.tensor = i;
+    x.whole = x.at + 8 <= t.n;
+    if (start >= t.n) return;
+    take_any(t.element, t.p, x.at, t.n, x.whole && values_lie_well(t.element, t.p), x.p);
+    take_any(t.element, t.g, x.at, t.n, x.whole && values_lie_well(t.element, t.g), x.g);
+    if constexpr (EIGHT) {
+      x.codes_m = take_codes(static_cast<const uint8_t*>(t.m), x.at, t.n, x.whole && on(t.m, 8));
+      x.codes_v = take_codes(static_cast<const uint8_t*>(t.v), x.at, t.n, x.whole && on(t.v, 8));
+      x.scale_m = t.m_scale[start / BLOCK];
+      x.scale_v = t.v_scale[start / BLOCK];
+    } else {
+      take(static_cast<const float*>(t.m), x.at, t.n, x.whole && on(t.m, 32), x.m);
+      take(static_cast<const float*>(t.v), x.at, t.n, x.whole && on(t.v, 32), x.v);
+    }
+  };
+  Piece<EIGHT> x;
+  if (c0 < c1) fetch(c0, x);
+  const float lr = h.c.lr_device ? *h.c.lr_device : h.c.lr, decay = lr * h.c.weight_decay;
   float clip = 1.f;
-  bool skip = false;
   if (h.c.norm_parts) {
     double sum = 0;
-    for (int i = threadIdx.x; i < h.c.n_norm_parts; i += THREADS) sum += h.c.norm_parts[i];
+    for (int k = threadIdx.x; k < h.c.n_norm_parts; k += THREADS) sum += h.c.norm_parts[k];
 #pragma unroll
     for (int by = 16; by; by >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, by);
     if (lane == 0) sums[warp] = sum;
@@ -199,54 +242,52 @@ __global__ void __launch_bounds__(THREADS) k_step(const __grid_constant__ Tensor
     sum = sums[0];
     for (int w = 1; w < THREADS / 32; ++w) sum += sums[w];
     const float norm = (float)sqrt(sum);
-    clip = fminf(1.f, h.c.max_norm / (norm + 1e-6f));
-    skip = !isfinite(norm);
     if (h.c.norm && blockIdx.x == 0 && threadIdx.x == 0) *h.c.norm = norm;
+    if (!isfinite(norm)) return;   // all CTAs do: nobody counts
+    clip = fminf(1.f, h.c.max_norm / (norm + 1e-6f));
   }
-  if (skip) return;   // all CTAs do: nobody counts
-  const float lr = h.c.lr_device ? *h.c.lr_device : h.c.lr, decay = lr * h.c.weight_decay;
-  const int64_t c0 = l.chunks * blockIdx.x / gridDim.x, c1 = l.chunks * (blockIdx.x + 1) / gridDim.x;
-  int i = c0 < c1 ? tensor_of(l, c0) : 0, known = -1;
+  int known = -1;
   float rate = 0.f, root = 0.f;
   uint32_t key = 0;
-  for (int64_t c = c0; c < c1; ++c) {
-    while (l.first[i + 1] <= c) ++i;
-    const BnbAdamTensor& t = l.t[i];
-    const int64_t start = (c - l.first[i]) * CHUNK + warp * BLOCK, at = start + lane * 8;
-    if (start >= t.n) continue;   // the warp's
-    const bool whole = at + 8 <= t.n;
-    const bool wide_p = whole && values_lie_well(t.element, t.p), wide_g = whole && values_lie_well(t.element, t.g);
-    float p[8], g[8], m[8], v[8];
-    take_any(t.element, t.p, at, t.n, wide_p, p);
-    take_any(t.element, t.g, at, t.n, wide_g, g);
-    const bool wide_m = whole && on(t.m, EIGHT ? 8 : 32), wide_v = whole && on(t.v, EIGHT ? 8 : 32);
-    if constexpr (EIGHT) {
-      const int64_t block = start / BLOCK;
-      decode(take_codes(static_cast<const uint8_t*>(t.m), at, t.n, wide_m), t.m_scale[block], m);
-      decode(take_codes(static_cast<const uint8_t*>(t.v), at, t.n, wide_v), t.v_scale[block], v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= v[k];
-    } else {
-      take(static_cast<const float*>(t.m), at, t.n, wide_m, m);
-      take(static_cast<const float*>(t.v), at, t.n, wide_v, v);
+  for (uint32_t c = c0; c < c1; ++c) {
+    const BnbAdamTensor& t = l.t[x.tensor];
+    if (x.at - lane * 8 >= t.n) {   // the warp's
+      if (c + 1 < c1) fetch(c + 1, x);
+      continue;
     }
-    if (known != i) {
-      known = i;
+    if (known != x.tensor) {
+      known = x.tensor;
       const float steps = *t.step + 1.f;
       rate = lr / -expm1f(steps * h.log1);
       root = 1.f / sqrtf(-expm1f(steps * h.log2_));
       key = h.c.seed * 0x5D2F63B9u + (uint32_t)steps * 0x3C6EF36Bu;
     }
+    float m[8], v[8];
+    if constexpr (EIGHT) {
+      decode(x.codes_m, x.scale_m, m);
+      decode(x.codes_v, x.scale_v, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m[k] = x.m[k], v[k] = x.v[k];
+    }
+    float p[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float gk = g[k] * clip;
+      const float gk = x.g[k] * clip;
       m[k] = fmaf(m[k], h.beta1, gk * h.rest1);
       v[k] = fmaf(v[k], h.beta2, gk * gk * h.rest2);
-      const float r = sqrtf(v[k]);
-      p[k] = fmaf(-p[k], decay, p[k]) - rate * (m[k] / fmaf(r, root, h.c.eps));
+      const float r = root_of(v[k]);
+      // the quotient by a reciprocal, 2 units in the last place of a change that is a small part of p; 0 for a divisor above 2^126
+      p[k] = fmaf(-x.p[k], decay, x.p[k]) - rate * __fdividef(m[k], fmaf(r, root, h.c.eps));
       if constexpr (EIGHT) v[k] = r;
     }
-    put_any(t.element, t.p, at, t.n, wide_p, p);
+    const int64_t at = x.at;
+    const bool whole = x.whole;
+    if constexpr (EIGHT)
+      if (c + 1 < c1) fetch(c + 1, x);
+    put_any(t.element, t.p, at, t.n, whole && values_lie_well(t.element, t.p), p);
     if constexpr (EIGHT) {
       float most_m = 0.f, most_r = 0.f;
 #pragma unroll
@@ -264,23 +305,25 @@ __global__ void __launch_bounds__(THREADS) k_step(const __grid_constant__ Tensor
         const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(fmaf(a, 0.f, a), fmaf(b, 0.f, b)), __NV_SATFINITE, __NV_E4M3);
         cm[k / 4] |= two << (8 * (k % 4));
       }
+      const uint64_t position = (uint64_t)(t.position + at);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float x = v[k] * by_r;
+        const float r = v[k] * by_r;
         // three bits of the mantissa are kept, exponents start at 2^-6; NaN and infinities end beyond the largest code
-        const int q = (int)((__float_as_uint(x) + noise((uint64_t)(t.position + at + k), key)) >> 20) - ((127 - 7) << 3);
-        const int code = x == 0.f ? 0 : min(max(q, 8), 0x7F);
+        const int q = (int)((__float_as_uint(r) + noise(position + k, key)) >> 20) - ((127 - 7) << 3);
+        const int code = r == 0.f ? 0 : min(max(q, 8), 0x7F);
         cr[k / 4] |= (uint32_t)code << (8 * (k % 4));
       }
-      put_codes(static_cast<uint8_t*>(t.m), at, t.n, wide_m, make_uint2(cm[0], cm[1]));
-      put_codes(static_cast<uint8_t*>(t.v), at, t.n, wide_v, make_uint2(cr[0], cr[1]));
+      put_codes(static_cast<uint8_t*>(t.m), at, t.n, whole && on(t.m, 8), make_uint2(cm[0], cm[1]));
+      put_codes(static_cast<uint8_t*>(t.v), at, t.n, whole && on(t.v, 8), make_uint2(cr[0], cr[1]));
       if (lane == 0) {
-        t.m_scale[start / BLOCK] = power(em);
-        t.v_scale[start / BLOCK] = power(er);
+        t.m_scale[at / BLOCK] = power(em);
+        t.v_scale[at / BLOCK] = power(er);
       }
     } else {
-      put(static_cast<float*>(t.m), at, t.n, wide_m, m);
-      put(static_cast<float*>(t.v), at, t.n, wide_v, v);
+      put(static_cast<float*>(t.m), at, t.n, whole && on(t.m, 32), m);
+      put(static_cast<float*>(t.v), at, t.n, whole && on(t.v, 32), v);
+      if (c + 1 < c1) fetch(c + 1, x);
     }
   }
   // the last CTA counts: every other one has read what it needs
@@ -302,6 +345,7 @@ int check(const BnbAdamTensor* t, int n) {
   if (n && !t) return BNB_ERR_NULL_POINTER;
   for (int i = 0; i < n; ++i) {
     if (t[i].n < 0 || t[i].element < 0 || t[i].element > 2) return BNB_ERR_BAD_ARGUMENT;
+    if (t[i].n > (int64_t)1 << 40) return BNB_ERR_UNSUPPORTED_DIMS;   // chunks of all tensors of a launch in 32 bits
     if (t[i].n && !t[i].g) return BNB_ERR_NULL_POINTER;
   }
   return BNB_OK;
@@ -314,12 +358,12 @@ Tensors<MOST> list_of(const BnbAdamTensor* t, int n) {
   for (int i = 0; i < n; ++i) {
     l.t[i] = t[i];
     l.first[i] = l.chunks;
-    l.chunks += (t[i].n + CHUNK - 1) / CHUNK;
+    l.chunks += (uint32_t)((t[i].n + CHUNK - 1) / CHUNK);
   }
   for (int i = n; i <= MOST; ++i) l.first[i] = l.chunks;
   return l;
 }
-unsigned ctas_of(int64_t chunks) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(chunks, CTAS)); }
+unsigned ctas_of(uint32_t chunks) { return std::max(1u, std::min(chunks, (uint32_t)CTAS)); }
 
 template <int MOST>
 int norm(const BnbAdamTensor* t, int n, double* parts, bool add, cudaStream_t st) {
@@ -347,7 +391,7 @@ extern "C" int bnb_grad_norm(const BnbAdamTensor* t, int n, double* parts, void*
   int i = 0;
   do {
     const int k = std::min(n - i, MANY);
-    if (const int r = k <= FEW ? norm<FEW>(t + i, k, parts, i > 0, s) : norm<MANY>(t + i, k, parts, i > 0, s)) return r;
+    if (const int r = k <= FEW ? norm<FEW>(t + i, k, parts, i > 0, s) : k <= SOME ? norm<SOME>(t + i, k, parts, i > 0, s) : norm<MANY>(t + i, k, parts, i > 0, s)) return r;
     i += k;
   } while (i < n);
   return BNB_OK;
@@ -370,7 +414,7 @@ extern "C" int bnb_adamw_step(const BnbAdamTensor* t, int n, const BnbAdamW* c, 
   const auto s = static_cast<cudaStream_t>(stream);
   for (int i = 0; i < n;) {
     const int k = std::min(n - i, MANY);
-    if (const int r = k <= FEW ? step<FEW>(t + i, k, h, s) : step<MANY>(t + i, k, h, s)) return r;
+    if (const int r = k <= FEW ? step<FEW>(t + i, k, h, s) : k <= SOME ? step<SOME>(t + i, k, h, s) : step<MANY>(t + i, k, h, s)) return r;
     i += k;
   }
   return BNB_OK;

@@ -252,84 +252,184 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tenso
 constexpr int64_t STATE_BLOCK = 256;   // elements that share a scale of 8-bit states
 
 bool laid_out_as(const Tensor& t, const Tensor& p) { return t.sizes() == p.sizes() && (t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous())); }
-Tensor state_of(const py::dict& state, const char* name) {
-  PyObject* v = PyDict_GetItemString(state.ptr(), name);
-  if (!v || !THPVariable_Check(v)) refuse(std::string("AdamW: a parameter's state has no tensor '") + name + "'");
-  return THPVariable_Unpack(v);
-}
 void expect_kept(const char* name, const Tensor& t, const Tensor& like, at::ScalarType type, const c10::Device& dev) {
   if (t.scalar_type() != type || t.device() != dev || !laid_out_as(t, like))
     refuse(std::string("AdamW: the state '") + name + "' must be " + c10::toString(type) + " of shape " + shape_text(like.sizes()) + " on " + dev.str() +
            ", laid out as its parameter; got " + c10::toString(t.scalar_type()) + " of shape " + shape_text(t.sizes()) + " on " + t.device().str());
 }
-void expect_changeable(const char* name, const Tensor& t) {
+void expect_changeable(const Tensor& t) {
   if (t.is_inference() && !c10::InferenceMode::is_enabled())
-    refuse(std::string("AdamW: ") + name + " was made in inference mode, outside of which it must not be changed");
+    refuse("AdamW: a parameter or its state was made in inference mode, outside of which it must not be changed");
 }
 
-// One step of the parameters of all groups that have a gradient.  groups: (parameters, states: dicts of tensors, positions, lr, beta1, beta2, eps, weight decay)
-// each.  Everything is checked before the first launch.  Returns the gradients' norm where they are clipped.
-using Group = std::tuple<py::list, py::list, std::vector<int64_t>, py::object, double, double, double, double>;
-OptTensor adamw_step(const std::vector<Group>& groups, const py::object& max_norm, int state_bits, uint32_t seed, const Tensor& control) {
-  const bool eight = state_bits == 8;
-  std::vector<Tensor> held, changed;
-  std::vector<std::vector<BnbAdamTensor>> lists;
-  std::vector<BnbAdamW> calls;
-  c10::optional<c10::Device> dev;
-  for (const Group& group : groups) {
-    const auto& [params, states, positions, lr, beta1, beta2, eps, decay] = group;
-    std::vector<BnbAdamTensor> list;
-    for (size_t i = 0; i < params.size(); ++i) {
-      const Tensor p = THPVariable_Unpack(params[i].ptr());
-      Tensor g = p.grad();
-      if (!g.defined()) continue;
-      if (!p.is_cuda()) refuse("AdamW: a parameter is on " + p.device().str() + "; the kernels run on CUDA only (sm_100a) and have no CPU path");
-      if (!dev) dev = p.device();
-      if (p.device() != *dev) refuse("AdamW: parameters on " + p.device().str() + " and " + dev->str() + "; one optimizer serves one device");
-      if (g.layout() != at::kStrided) refuse("AdamW: sparse gradients are not taken");
-      if (g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() || g.device() != *dev) refuse("AdamW: a gradient has another type, shape or device than its parameter");
-      if (!p.is_non_overlapping_and_dense()) throw py::value_error("AdamW: a parameter's elements must lie densely in memory, each in a place of its own");
-      const c10::cuda::CUDAGuard guard(*dev);
-      BnbAdamTensor t{};
-      t.element = element_of("AdamW", p);
-      t.n = p.numel();
-      t.position = positions[i];
-      const py::dict state = py::reinterpret_borrow<py::dict>(states[i]);
-      const Tensor step = state_of(state, "step"), m = state_of(state, "exp_avg"), v = state_of(state, eight ? "exp_avg_sq_root" : "exp_avg_sq");
-      if (step.scalar_type() != at::kFloat || step.numel() != 1 || step.device() != *dev) refuse("AdamW: the state 'step' must be one float32 number on " + dev->str());
-      const at::ScalarType type = eight ? at::kFloat8_e4m3fn : at::kFloat;
-      expect_kept("exp_avg", m, p, type, *dev);
-      expect_kept(eight ? "exp_avg_sq_root" : "exp_avg_sq", v, p, type, *dev);
-      if (eight) {
-        const int64_t blocks = (t.n + STATE_BLOCK - 1) / STATE_BLOCK;
-        for (const auto& [name, to] : {std::pair<const char*, float**>{"exp_avg_scale", &t.m_scale}, {"exp_avg_sq_root_scale", &t.v_scale}}) {
-          const Tensor s = state_of(state, name);
-          if (s.scalar_type() != at::kFloat || s.dim() != 1 || s.size(0) != blocks || !s.is_contiguous() || s.device() != *dev)
-            refuse(std::string("AdamW: the state '") + name + "' must be float32 of shape " + shape_text({blocks}) + ", contiguous, on " + dev->str());
-          *to = static_cast<float*>(s.data_ptr());
-          changed.push_back(s);
+// The parameters and states of an optimizer as tensors, looked up once: a hundred of them cost more in Python than their update on the GPU.  A step
+// compares the optimizer's lists and dicts with those that the plan was made of, object by object, so what was replaced in them is seen; what
+// may change in place (data, types, gradients) is read anew.
+class AdamWPlan {
+ public:
+  AdamWPlan(const py::list& groups, const py::dict& state, int state_bits) : eight_(state_bits == 8) {
+    names_ = eight_ ? std::vector<const char*>{"step", "exp_avg", "exp_avg_sq_root", "exp_avg_scale", "exp_avg_sq_root_scale"}
+                    : std::vector<const char*>{"step", "exp_avg", "exp_avg_sq"};
+    for (const char* name : names_) keys_.push_back(py::reinterpret_steal<py::object>(PyUnicode_InternFromString(name)));
+    int64_t at = 0;
+    for (const py::handle& group : groups) {
+      std::vector<Entry> entries;
+      for (const py::handle& param : py::list(group["params"])) {
+        Entry e;
+        e.object = py::reinterpret_borrow<py::object>(param);
+        e.p = THPVariable_Unpack(param.ptr());
+        e.position = at;
+        at += (e.p.numel() + STATE_BLOCK - 1) / STATE_BLOCK * STATE_BLOCK;
+        PyObject* of = PyDict_GetItemWithError(state.ptr(), param.ptr());
+        if (!of && PyErr_Occurred()) throw py::error_already_set();
+        if (of && PyDict_Check(of) && PyDict_Size(of)) {
+          e.state = py::reinterpret_borrow<py::object>(of);
+          for (size_t i = 0; i < names_.size(); ++i) {
+            PyObject* v = PyDict_GetItemWithError(of, keys_[i].ptr());
+            if (!v || !THPVariable_Check(v)) refuse(std::string("AdamW: a parameter's state has no tensor '") + names_[i] + "'");
+            e.objects.push_back(py::reinterpret_borrow<py::object>(v));
+            e.kept.push_back(THPVariable_Unpack(v));
+          }
         }
+        entries.push_back(std::move(e));
       }
-      if (!laid_out_as(g, p)) {
-        g = at::empty_like(p).copy_(g);
-        held.push_back(g);
-      }
-      t.p = p.data_ptr();
-      t.g = g.data_ptr();
-      t.m = m.data_ptr();
-      t.v = v.data_ptr();
-      t.step = static_cast<float*>(step.data_ptr());
-      list.push_back(t);
-      changed.insert(changed.end(), {p, m, v, step});
+      groups_.push_back(std::move(entries));
     }
+    PyObject *key, *value;
+    for (Py_ssize_t i = 0; PyDict_Next(state.ptr(), &i, &key, &value);) states_.emplace_back(py::reinterpret_borrow<py::object>(key), py::reinterpret_borrow<py::object>(value));
+  }
+
+  // One step of the parameters that have a gradient.  False where the plan is of other lists, dicts or states than these; else the gradients' norm where
+  // they are clipped, or None.  Everything is checked before the first launch.
+  py::object step(const py::list& groups, const py::dict& state, const py::object& max_norm, uint32_t seed, const Tensor& control) {
+    if (!is_of(groups, state)) return py::bool_(false);
+    std::vector<Tensor> held;
+    std::vector<const Tensor*> changed;
+    std::vector<std::vector<BnbAdamTensor>> lists(groups_.size());
+    std::vector<BnbAdamW> calls(groups_.size());
+    const c10::Device dev = control.device();
+    const c10::cuda::OptionalCUDAGuard guard(control.is_cuda() ? c10::optional<c10::Device>(dev) : c10::nullopt);
+    size_t total = 0;
+    for (size_t i = 0; i < groups_.size(); ++i) {
+      const py::dict group = groups[i];
+      for (const Entry& e : groups_[i])
+        if (const Tensor& g = e.p.grad(); g.defined()) lists[i].push_back(tensor_of(e, g, dev, held, changed));
+      calls[i] = call_of(group, seed, control, held);
+      total += lists[i].size();
+    }
+    if (!total) return py::none();
+    expect("AdamW", "the control word", control, {1}, dev);
+    for (const Tensor* t : changed) expect_changeable(*t);
+    void* stream = stream_of(dev);
+    py::object out = py::none();
+    Tensor parts, norm;
+    if (!max_norm.is_none()) {
+      parts = at::empty({BNB_GRAD_NORM_PARTS}, control.options().dtype(at::kDouble));
+      norm = at::empty({}, control.options().dtype(at::kFloat));
+      std::vector<BnbAdamTensor> all;
+      if (lists.size() > 1)
+        for (const auto& list : lists) all.insert(all.end(), list.begin(), list.end());
+      const std::vector<BnbAdamTensor>& of = lists.size() > 1 ? all : lists[0];
+      check("bnb_grad_norm", bnb_grad_norm(of.data(), (int)of.size(), static_cast<double*>(parts.data_ptr()), stream));
+      out = py::cast(norm);
+    }
+    for (size_t i = 0; i < lists.size(); ++i) {
+      if (norm.defined()) {
+        calls[i].norm_parts = static_cast<const double*>(parts.data_ptr());
+        calls[i].n_norm_parts = BNB_GRAD_NORM_PARTS;
+        calls[i].max_norm = (float)max_norm.cast<double>();
+        calls[i].norm = static_cast<float*>(norm.data_ptr());
+      }
+      check("bnb_adamw_step", bnb_adamw_step(lists[i].data(), (int)lists[i].size(), &calls[i], stream));
+    }
+    for (const Tensor* t : changed)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    return out;
+  }
+
+ private:
+  struct Entry {
+    py::object object, state;            // the parameter; its state's dict, or null
+    Tensor p;
+    std::vector<py::object> objects;     // the state's tensors, in the order of names_
+    std::vector<Tensor> kept;
+    int64_t position;
+  };
+
+  bool is_of(const py::list& groups, const py::dict& state) const {
+    if (groups.size() != groups_.size() || (size_t)PyDict_Size(state.ptr()) != states_.size()) return false;
+    PyObject *key, *value;
+    size_t k = 0;
+    for (Py_ssize_t i = 0; PyDict_Next(state.ptr(), &i, &key, &value); ++k)
+      if (key != states_[k].first.ptr() || value != states_[k].second.ptr()) return false;
+    for (size_t i = 0; i < groups_.size(); ++i) {
+      const py::object params = groups[i]["params"];
+      if (!PyList_Check(params.ptr()) || (size_t)PyList_GET_SIZE(params.ptr()) != groups_[i].size()) return false;
+      for (size_t j = 0; j < groups_[i].size(); ++j) {
+        const Entry& e = groups_[i][j];
+        if (PyList_GET_ITEM(params.ptr(), j) != e.object.ptr()) return false;
+        if (!e.state.ptr()) {
+          if (e.p.grad().defined()) return false;   // its first
+          continue;
+        }
+        for (size_t n = 0; n < names_.size(); ++n)
+          if (PyDict_GetItemWithError(e.state.ptr(), keys_[n].ptr()) != e.objects[n].ptr()) return false;
+      }
+    }
+    return true;
+  }
+
+  BnbAdamTensor tensor_of(const Entry& e, const Tensor& grad, const c10::Device& dev, std::vector<Tensor>& held, std::vector<const Tensor*>& changed) const {
+    const Tensor& p = e.p;
+    if (!p.is_cuda()) refuse("AdamW: a parameter is on " + p.device().str() + "; the kernels run on CUDA only (sm_100a) and have no CPU path");
+    if (p.device() != dev) refuse("AdamW: parameters on " + p.device().str() + " and " + dev.str() + "; one optimizer serves one device");
+    if (grad.layout() != at::kStrided) refuse("AdamW: sparse gradients are not taken");
+    if (grad.scalar_type() != p.scalar_type() || grad.sizes() != p.sizes() || grad.device() != dev)
+      refuse("AdamW: a gradient has another type, shape or device than its parameter");
+    if (!p.is_contiguous() && !p.is_non_overlapping_and_dense())
+      throw py::value_error("AdamW: a parameter's elements must lie densely in memory, each in a place of its own");
+    BnbAdamTensor t{};
+    t.element = element_of("AdamW", p);
+    t.n = p.numel();
+    t.position = e.position;
+    const Tensor &step = e.kept[0], &m = e.kept[1], &v = e.kept[2];
+    if (step.scalar_type() != at::kFloat || step.numel() != 1 || step.device() != dev) refuse("AdamW: the state 'step' must be one float32 number on " + dev.str());
+    const at::ScalarType type = eight_ ? at::kFloat8_e4m3fn : at::kFloat;
+    expect_kept(names_[1], m, p, type, dev);
+    expect_kept(names_[2], v, p, type, dev);
+    if (eight_) {
+      const int64_t blocks = (t.n + STATE_BLOCK - 1) / STATE_BLOCK;
+      for (int i : {3, 4}) {
+        const Tensor& s = e.kept[i];
+        if (s.scalar_type() != at::kFloat || s.dim() != 1 || s.size(0) != blocks || !s.is_contiguous() || s.device() != dev)
+          refuse(std::string("AdamW: the state '") + names_[i] + "' must be float32 of shape " + shape_text({blocks}) + ", contiguous, on " + dev.str());
+        (i == 3 ? t.m_scale : t.v_scale) = static_cast<float*>(s.data_ptr());
+      }
+    }
+    t.g = grad.data_ptr();
+    if (!laid_out_as(grad, p)) {
+      held.push_back(at::empty_like(p).copy_(grad));
+      t.g = held.back().data_ptr();
+    }
+    t.p = p.data_ptr();
+    t.m = m.data_ptr();
+    t.v = v.data_ptr();
+    t.step = static_cast<float*>(step.data_ptr());
+    changed.push_back(&p);
+    for (const Tensor& s : e.kept) changed.push_back(&s);
+    return t;
+  }
+
+  BnbAdamW call_of(const py::dict& group, uint32_t seed, const Tensor& control, std::vector<Tensor>& held) const {
     BnbAdamW c{};
-    c.state_bits = state_bits;
+    c.state_bits = eight_ ? 8 : 32;
     c.seed = seed;
+    const py::object lr = group["lr"];
     if (THPVariable_Check(lr.ptr())) {
       const Tensor rate = THPVariable_Unpack(lr.ptr());
       if (rate.numel() != 1) refuse("AdamW: lr must be a number or a tensor of one");
       if (rate.is_cuda()) {
-        if (dev && rate.device() != *dev) refuse("AdamW: lr is on " + rate.device().str() + ", the parameters on " + dev->str());
+        if (rate.device() != control.device()) refuse("AdamW: lr is on " + rate.device().str() + ", the parameters on " + control.device().str());
         held.push_back(rate.to(at::kFloat));
         c.lr_device = static_cast<const float*>(held.back().data_ptr());
       } else {
@@ -338,42 +438,21 @@ OptTensor adamw_step(const std::vector<Group>& groups, const py::object& max_nor
     } else {
       c.lr = (float)lr.cast<double>();
     }
-    c.beta1 = beta1;
-    c.beta2 = beta2;
-    c.eps = (float)eps;
-    c.weight_decay = (float)decay;
+    const py::tuple betas = py::tuple(group["betas"]);
+    c.beta1 = betas[0].cast<double>();
+    c.beta2 = betas[1].cast<double>();
+    c.eps = (float)group["eps"].cast<double>();
+    c.weight_decay = (float)group["weight_decay"].cast<double>();
     c.control = static_cast<int32_t*>(control.data_ptr());
-    calls.push_back(c);
-    lists.push_back(std::move(list));
+    return c;
   }
-  if (!dev) return c10::nullopt;
-  expect("AdamW", "the control word", control, {1}, *dev);
-  for (const Tensor& t : changed) expect_changeable("a parameter or its state", t);
-  const c10::cuda::CUDAGuard guard(*dev);
-  void* stream = stream_of(*dev);
-  OptTensor norm;
-  Tensor parts;
-  if (!max_norm.is_none()) {
-    const auto options = at::TensorOptions().device(*dev);
-    parts = at::empty({BNB_GRAD_NORM_PARTS}, options.dtype(at::kDouble));
-    norm = at::empty({}, options.dtype(at::kFloat));
-    std::vector<BnbAdamTensor> all;
-    for (const auto& list : lists) all.insert(all.end(), list.begin(), list.end());
-    check("bnb_grad_norm", bnb_grad_norm(all.data(), (int)all.size(), static_cast<double*>(parts.data_ptr()), stream));
-  }
-  for (size_t i = 0; i < lists.size(); ++i) {
-    if (norm.has_value()) {
-      calls[i].norm_parts = static_cast<const double*>(parts.data_ptr());
-      calls[i].n_norm_parts = BNB_GRAD_NORM_PARTS;
-      calls[i].max_norm = (float)max_norm.cast<double>();
-      calls[i].norm = static_cast<float*>(norm->data_ptr());
-    }
-    check("bnb_adamw_step", bnb_adamw_step(lists[i].data(), (int)lists[i].size(), &calls[i], stream));
-  }
-  for (const Tensor& t : changed)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  return norm;
-}
+
+  const bool eight_;
+  std::vector<const char*> names_;
+  std::vector<py::object> keys_;
+  std::vector<std::vector<Entry>> groups_;
+  std::vector<std::pair<py::object, py::object>> states_;
+};
 
 }  // namespace
 
@@ -381,7 +460,7 @@ void bind_update(py::module& m) {
   m.def("linear_forward", &linear_forward);
   m.def("linear_backward", &linear_backward);
   m.def("linear", torch::wrap_pybind_function(linear));
-  m.def("adamw_step", &adamw_step);
+  py::class_<AdamWPlan>(m, "AdamWPlan").def(py::init<const py::list&, const py::dict&, int>()).def("step", &AdamWPlan::step);
   m.def("policy_loss_forward", &policy_forward);
   m.def("policy_loss_backward", &policy_backward);
   m.def("policy_loss", torch::wrap_pybind_function(policy_loss));

@@ -49,6 +49,7 @@ class AdamW(torch.optim.Optimizer):
         self._max_norm, self._state_bits, self._seed = max_norm, state_bits, int(seed) & 0xFFFFFFFF
         self.grad_norm: Optional[torch.Tensor] = None
         self._control: Optional[torch.Tensor] = None
+        self._plan = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group: dict) -> None:
@@ -78,6 +79,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)
+        self._plan = None
         self.__dict__.setdefault("grad_norm", None)
         self.__dict__.setdefault("_control", None)
 
@@ -125,23 +127,32 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        groups, at = [], 0
+        norm = False if self._plan is None else self._launch()
+        if norm is False:
+            if not self._prepare():
+                self.grad_norm = None
+                return loss
+            norm = self._launch()
+        self.grad_norm = norm
+        return loss
+
+    def _launch(self):
+        return self._plan.step(self.param_groups, self.state, self._max_norm, self._seed, self._control)
+
+    def _prepare(self) -> bool:
+        """States for the parameters that have a gradient and none yet, and a plan of all; whether there is anything to do."""
+        some = None
         for group in self.param_groups:
-            params, states, positions = [], [], []
             for p in group["params"]:
                 if p.grad is not None:
-                    state = self.state[p]
-                    if not state:
-                        state.update(self._new_state(p))
-                    if self._control is None or self._control.device != p.device:
-                        if torch.cuda.is_current_stream_capturing():
-                            raise RuntimeError("AdamW: make a step before the capture")
-                        self._control = torch.zeros(1, dtype=torch.int32, device=p.device)
-                    params.append(p)
-                    states.append(state)
-                    positions.append(at)
-                at += (p.numel() + _BLOCK - 1) // _BLOCK * _BLOCK
-            groups.append((params, states, positions, group["lr"], *group["betas"], group["eps"], group["weight_decay"]))
-        if self._control is not None:
-            self.grad_norm = _capi.host.adamw_step(groups, self._max_norm, self._state_bits, self._seed, self._control)
-        return loss
+                    some = p if some is None else some
+                    if not self.state[p]:
+                        self.state[p].update(self._new_state(p))
+        if some is None:
+            return False
+        if self._control is None or self._control.device != some.device:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a captured step needs a word of its own that outlives it; make a step before the capture")
+            self._control = torch.zeros(1, dtype=torch.int32, device=some.device)
+        self._plan = _capi.host.AdamWPlan(self.param_groups, self.state, self._state_bits)
+        return True
