@@ -33,7 +33,7 @@ template <int MOST> struct Tensors {
   uint32_t first[MOST + 1];   // chunks before each tensor; all of them behind the last
   BnbAdamTensor t[MOST];
 };
-constexpr int FEW = 32, SOME = 128, MANY = 360;
+constexpr int MANY = 360;
 
 // The tensor of a chunk, by all lanes of a warp: two steps where halving takes nine, each of which waits for memory.
 template <int MOST>
@@ -107,40 +107,70 @@ __device__ __forceinline__ void put_codes(uint8_t* to, int64_t at, int64_t n, bo
       if (at + i < n) to[at + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
   }
 }
-__device__ __forceinline__ void decode(uint2 codes, float scale, float (&f)[8]) {
+__device__ __forceinline__ void decode(uint2 codes, F2 (&f)[4]) {
   const uint32_t w[2] = {codes.x, codes.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 h(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (16 * (i % 2))), __NV_E4M3));
-    const float2 v = __half22float2(h);
-    f[2 * i] = v.x * scale;
-    f[2 * i + 1] = v.y * scale;
+    const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (16 * (i % 2))), __NV_E4M3)));
+    f[i] = f2(v.x, v.y);
   }
+}
+// Maxima over a warp, NaN where any is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int by = 16; by; by >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, by));
+  for (int by = 16; by; by >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, by));
   return v;
 }
-// Square root by the instruction, within a unit in the last place; numbers below the normal ones are not taken for 0.
+// Square root by the instruction, within a unit in the last place.  For 8-bit states, which are bound by their arithmetic, numbers below 2^-126 are 0;
+// taking them as they are is three instructions more.
+template <bool FLUSH>
 __device__ __forceinline__ float root_of(float v) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  if constexpr (FLUSH) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  else asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 // The exponent (in place) of the scale that takes `most` to 128 .. 256.
 __device__ __forceinline__ uint32_t scale_exponent(float most) { return (uint32_t)max((int)(__float_as_uint(most) >> 23) - 7, 1); }
 __device__ __forceinline__ float power(uint32_t exponent) { return __uint_as_float(exponent << 23); }
-// 20 random bits.
-__device__ __forceinline__ uint32_t noise(uint64_t position, uint32_t key) {
-  uint32_t h = ((uint32_t)position + (uint32_t)(position >> 32) * 0x632BE5ABu) * 0x9E3779B1u + key;
+// 20 random bits of a position: its product with a constant and the key, mixed.  Eight neighbours from a multiple of eight on share the upper half.
+__device__ __forceinline__ uint32_t spread(uint64_t position, uint32_t key) {
+  return ((uint32_t)position + (uint32_t)(position >> 32) * 0x632BE5ABu) * 0x9E3779B1u + key;
+}
+__device__ __forceinline__ uint32_t noise(uint32_t h) {
   h ^= h >> 15;
   h *= 0x6C8E944Du;
   h ^= h >> 13;
   h *= 0x5B297A4Du;
   return (h ^ (h >> 16)) >> 12;
 }
-
+// The codes of eight values within 0 .. 256, whose block has no others: m to nearest; r, not negative, at random, 0 alone to 0.  Added to the bits that
+// e4m3 has not, the noise carries into the last that it has in proportion; what is left converts exactly.
+__device__ __forceinline__ uint2 codes_of(const F2 (&m)[4], F2 by) {
+  uint32_t c[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) c[k] = __nv_cvt_float2_to_fp8x2(halves(mul(m[k], by)), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
+}
+__device__ __forceinline__ uint2 random_codes_of(const F2 (&r)[4], F2 by, uint32_t h) {
+  uint32_t c[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const F2 x = mul(r[k], by);
+    const float2 v = halves(x), up = halves(mul(x, f2(0x1p100f)));
+    float2 y;
+    // no smaller than the least normal number, except 0
+    y.x = __uint_as_float((__float_as_uint(fmaxf(v.x, fminf(up.x, 0x1p-6f))) + noise(h + (2 * k) * 0x9E3779B1u)) & 0xFFF00000u);
+    y.y = __uint_as_float((__float_as_uint(fmaxf(v.y, fminf(up.y, 0x1p-6f))) + noise(h + (2 * k + 1) * 0x9E3779B1u)) & 0xFFF00000u);
+    c[k] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
+}
 // ------------------------------------------------------------------ norm
 
 template <int MOST>
@@ -186,6 +216,69 @@ struct Hyper {
   float log1, log2_;                  // natural logarithms of the betas
 };
 
+// What a CTA of a step knows before its first chunk: the clipping of the gradients (false: their norm is not finite, and nobody counts).
+__device__ __forceinline__ bool clipping(const Hyper& h, double (&sums)[THREADS / 32], float& clip) {
+  clip = 1.f;
+  if (!h.c.norm_parts) return true;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double sum = 0;
+  for (int k = threadIdx.x; k < h.c.n_norm_parts; k += THREADS) sum += h.c.norm_parts[k];
+#pragma unroll
+  for (int by = 16; by; by >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, by);
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  sum = sums[0];
+  for (int w = 1; w < THREADS / 32; ++w) sum += sums[w];
+  const float norm = (float)sqrt(sum);
+  if (h.c.norm && blockIdx.x == 0 && threadIdx.x == 0) *h.c.norm = norm;
+  clip = fminf(1.f, h.c.max_norm / (norm + 1e-6f));
+  return isfinite(norm);
+}
+// A tensor's step: the learning rate and the root's factor with their corrections, the key of its random numbers.
+struct Rates { float rate, root; uint32_t key; };
+__device__ __forceinline__ Rates rates_of(const Hyper& h, float lr, const float* step) {
+  const float steps = *step + 1.f;
+  return {lr / -expm1f(steps * h.log1), 1.f / sqrtf(-expm1f(steps * h.log2_)), h.c.seed * 0x5D2F63B9u + (uint32_t)steps * 0x3C6EF36Bu};
+}
+// Eight elements: m and v come multiplied by their betas; with EIGHT, v goes back as its root.
+template <bool EIGHT>
+__device__ __forceinline__ void update(const Hyper& h, const Rates& k, float clip, float decay, const float (&g)[8], float (&p)[8], F2 (&m)[4], F2 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const F2 gi = mul(f2(g[2 * i], g[2 * i + 1]), f2(clip)), old = f2(p[2 * i], p[2 * i + 1]);
+    m[i] = fma(gi, f2(h.rest1), m[i]);
+    v[i] = fma(mul(gi, gi), f2(h.rest2), v[i]);
+    const float2 vs = halves(v[i]);
+    const F2 r = f2(root_of<EIGHT>(vs.x), root_of<EIGHT>(vs.y));
+    // the quotient by a reciprocal, 2 units in the last place of a change that is a small part of p
+    const float2 d = halves(fma(r, f2(k.root), f2(h.c.eps)));
+    const float2 q = halves(add(fma(old, f2(-decay), old), mul(mul(m[i], f2(-k.rate)), f2(rcp_fast(d.x), rcp_fast(d.y)))));
+    p[2 * i] = q.x, p[2 * i + 1] = q.y;
+    if constexpr (EIGHT) v[i] = r;
+  }
+}
+__device__ __forceinline__ void flat(const F2 (&f)[4], float (&o)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 s = halves(f[k]);
+    o[2 * k] = s.x, o[2 * k + 1] = s.y;
+  }
+}
+// The last CTA counts: every other one has read what it needs.
+template <int MOST>
+__device__ __forceinline__ void count(const Tensors<MOST>& l, int32_t* control) {
+  __shared__ bool last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(control, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  for (int k = threadIdx.x; k < l.n; k += THREADS) *l.t[k].step += 1.f;
+  if (threadIdx.x == 0) *control = 0;
+}
+
 // Eight elements of a lane as they come from memory.
 template <bool EIGHT>
 struct Piece {
@@ -193,149 +286,124 @@ struct Piece {
   float m[EIGHT ? 1 : 8], v[EIGHT ? 1 : 8];
   uint2 codes_m, codes_v;
   float scale_m, scale_v;
-  int64_t at;       // of the lane's first element, behind the tensor's end where the warp has nothing
+  int64_t at;       // of the lane's first element
   int tensor;
-  bool whole;
 };
 
-// With 8-bit states a chunk's loads are on their way while the one before is rounded and written.
+// With 8-bit states a chunk's loads are on their way while the one before is rounded and written.  These are bound by their arithmetic and its latency, 66
+// instructions an element at 56 % of the issue slots with 24 warps an SM: one wave of CTAs, 149 us for 40 M elements (eight CTAs an SM 157; four an SM at
+// 64 registers 159, two 168).  States of 32 bits are bound by memory, 98 % of the measured copy rate with float32 parameters; 16-bit ones leave fewer bytes
+// on their way, 79 % (two CTAs an SM 69 %; four 89 %, but float32 92 %).
+constexpr int RESIDENT = 3;
 template <int MOST, bool EIGHT>
-__global__ void __launch_bounds__(THREADS) k_step(const __grid_constant__ Tensors<MOST> l, const __grid_constant__ Hyper h) {
+__global__ void __launch_bounds__(THREADS, RESIDENT) k_step(const __grid_constant__ Tensors<MOST> l, const __grid_constant__ Hyper h) {
   __shared__ double sums[THREADS / 32];
-  __shared__ bool last;
   let_next_start();
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t c0 = (uint64_t)l.chunks * blockIdx.x / gridDim.x, c1 = (uint64_t)l.chunks * (blockIdx.x + 1) / gridDim.x;
-  int i = c0 < c1 ? tensor_of(l, c0) : 0;
+  int i = c0 < c1 ? tensor_of(l, c0) : 0, known = -1;
   auto fetch = [&](uint32_t c, Piece<EIGHT>& x) {
     while (l.first[i + 1] <= c) ++i;
     const BnbAdamTensor& t = l.t[i];
-    const int64_t start = (int64_t)(c - l.first[i]) * CHUNK + warp * BLOCK;
-    x.at = start + lane * 8;
+    const int64_t start = (int64_t)(c - l.first[i]) * CHUNK + warp * BLOCK, at = start + lane * 8;
+    x.at = at;
     x.tensor = i;
-    x.whole = x.at + 8 <= t.n;
-    if (start >= t.n) return;
-    take_any(t.element, t.p, x.at, t.n, x.whole && values_lie_well(t.element, t.p), x.p);
-    take_any(t.element, t.g, x.at, t.n, x.whole && values_lie_well(t.element, t.g), x.g);
+    if (start >= t.n) return;   // the warp's
+    const bool whole = at + 8 <= t.n;
+    take_any(t.element, t.p, at, t.n, whole && values_lie_well(t.element, t.p), x.p);
+    take_any(t.element, t.g, at, t.n, whole && values_lie_well(t.element, t.g), x.g);
     if constexpr (EIGHT) {
-      x.codes_m = take_codes(static_cast<const uint8_t*>(t.m), x.at, t.n, x.whole && on(t.m, 8));
-      x.codes_v = take_codes(static_cast<const uint8_t*>(t.v), x.at, t.n, x.whole && on(t.v, 8));
+      x.codes_m = take_codes(static_cast<const uint8_t*>(t.m), at, t.n, whole && on(t.m, 8));
+      x.codes_v = take_codes(static_cast<const uint8_t*>(t.v), at, t.n, whole && on(t.v, 8));
       x.scale_m = t.m_scale[start / BLOCK];
       x.scale_v = t.v_scale[start / BLOCK];
     } else {
-      take(static_cast<const float*>(t.m), x.at, t.n, x.whole && on(t.m, 32), x.m);
-      take(static_cast<const float*>(t.v), x.at, t.n, x.whole && on(t.v, 32), x.v);
+      take(static_cast<const float*>(t.m), at, t.n, whole && on(t.m, 32), x.m);
+      take(static_cast<const float*>(t.v), at, t.n, whole && on(t.v, 32), x.v);
     }
   };
   Piece<EIGHT> x;
   if (c0 < c1) fetch(c0, x);
   const float lr = h.c.lr_device ? *h.c.lr_device : h.c.lr, decay = lr * h.c.weight_decay;
-  float clip = 1.f;
-  if (h.c.norm_parts) {
-    double sum = 0;
-    for (int k = threadIdx.x; k < h.c.n_norm_parts; k += THREADS) sum += h.c.norm_parts[k];
-#pragma unroll
-    for (int by = 16; by; by >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, by);
-    if (lane == 0) sums[warp] = sum;
-    __syncthreads();
-    sum = sums[0];
-    for (int w = 1; w < THREADS / 32; ++w) sum += sums[w];
-    const float norm = (float)sqrt(sum);
-    if (h.c.norm && blockIdx.x == 0 && threadIdx.x == 0) *h.c.norm = norm;
-    if (!isfinite(norm)) return;   // all CTAs do: nobody counts
-    clip = fminf(1.f, h.c.max_norm / (norm + 1e-6f));
-  }
-  int known = -1;
-  float rate = 0.f, root = 0.f;
-  uint32_t key = 0;
+  float clip;
+  if (!clipping(h, sums, clip)) return;   // while the first loads are on their way; all CTAs do: nobody counts
+  Rates k{};
   for (uint32_t c = c0; c < c1; ++c) {
     const BnbAdamTensor& t = l.t[x.tensor];
-    if (x.at - lane * 8 >= t.n) {   // the warp's
+    const int64_t at = x.at, start = at - lane * 8;
+    if (start >= t.n) {   // the warp's
       if (c + 1 < c1) fetch(c + 1, x);
       continue;
     }
     if (known != x.tensor) {
       known = x.tensor;
-      const float steps = *t.step + 1.f;
-      rate = lr / -expm1f(steps * h.log1);
-      root = 1.f / sqrtf(-expm1f(steps * h.log2_));
-      key = h.c.seed * 0x5D2F63B9u + (uint32_t)steps * 0x3C6EF36Bu;
+      k = rates_of(h, lr, t.step);
     }
-    float m[8], v[8];
+    const bool whole = at + 8 <= t.n;
+    F2 m[4], v[4];
     if constexpr (EIGHT) {
-      decode(x.codes_m, x.scale_m, m);
-      decode(x.codes_v, x.scale_v, v);
+      decode(x.codes_m, m);
+      decode(x.codes_v, v);
+      // scales are powers of two: beta times a scale is exact
+      const F2 bm = f2(h.beta1 * x.scale_m), bv = f2(h.beta2 * fminf(x.scale_v * x.scale_v, 3.4e38f));
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= v[k];
+      for (int j = 0; j < 4; ++j) m[j] = mul(m[j], bm), v[j] = mul(mul(v[j], v[j]), bv);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m[k] = x.m[k], v[k] = x.v[k];
+      for (int j = 0; j < 4; ++j) m[j] = mul(f2(x.m[2 * j], x.m[2 * j + 1]), f2(h.beta1)), v[j] = mul(f2(x.v[2 * j], x.v[2 * j + 1]), f2(h.beta2));
     }
-    float p[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float gk = x.g[k] * clip;
-      m[k] = fmaf(m[k], h.beta1, gk * h.rest1);
-      v[k] = fmaf(v[k], h.beta2, gk * gk * h.rest2);
-      const float r = root_of(v[k]);
-      // the quotient by a reciprocal, 2 units in the last place of a change that is a small part of p; 0 for a divisor above 2^126
-      p[k] = fmaf(-x.p[k], decay, x.p[k]) - rate * __fdividef(m[k], fmaf(r, root, h.c.eps));
-      if constexpr (EIGHT) v[k] = r;
-    }
-    const int64_t at = x.at;
-    const bool whole = x.whole;
-    if constexpr (EIGHT)
-      if (c + 1 < c1) fetch(c + 1, x);
-    put_any(t.element, t.p, at, t.n, whole && values_lie_well(t.element, t.p), p);
+    update<EIGHT>(h, k, clip, decay, x.g, x.p, m, v);
+    put_any(t.element, t.p, at, t.n, whole && values_lie_well(t.element, t.p), x.p);
+    float ms[8], vs[8];
+    flat(m, ms);
+    flat(v, vs);
     if constexpr (EIGHT) {
+      if (c + 1 < c1) fetch(c + 1, x);
       float most_m = 0.f, most_r = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        most_m = fmaxf(most_m, fabsf(m[k]));
-        most_r = fmaxf(most_r, v[k]);
+      for (int j = 0; j < 8; ++j) {
+        most_m = max_nan(most_m, fabsf(ms[j]));
+        most_r = max_nan(most_r, vs[j]);
       }
-      const uint32_t em = scale_exponent(warp_max(most_m)), er = scale_exponent(warp_max(most_r));
-      const float by_m = power(254 - em), by_r = power(254 - er);   // exact
-      uint32_t cm[2] = {0, 0}, cr[2] = {0, 0};
+      most_m = warp_max(most_m);
+      most_r = warp_max(most_r);
+      const bool broken = !(isfinite(most_m) && isfinite(most_r));   // the warp's
+      if (broken) {   // the scales are those of what is finite
+        most_m = most_r = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; k += 2) {
-        const float a = m[k] * by_m, b = m[k + 1] * by_m;
-        // an infinity saturates in the conversion: NaN instead
-        const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(fmaf(a, 0.f, a), fmaf(b, 0.f, b)), __NV_SATFINITE, __NV_E4M3);
-        cm[k / 4] |= two << (8 * (k % 4));
+        for (int j = 0; j < 8; ++j) {
+          if (isfinite(ms[j])) most_m = fmaxf(most_m, fabsf(ms[j]));
+          if (isfinite(vs[j])) most_r = fmaxf(most_r, vs[j]);
+        }
+        most_m = warp_max(most_m);
+        most_r = warp_max(most_r);
       }
-      const uint64_t position = (uint64_t)(t.position + at);
+      const uint32_t em = scale_exponent(most_m), er = scale_exponent(most_r);
+      uint2 codes_m = codes_of(m, f2(power(254 - em)));   // by powers of two: exact
+      uint2 codes_r = random_codes_of(v, f2(power(254 - er)), spread((uint64_t)(t.position + at), k.key));
+      if (broken) {   // what is not is NaN
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float r = v[k] * by_r;
-        // three bits of the mantissa are kept, exponents start at 2^-6; NaN and infinities end beyond the largest code
-        const int q = (int)((__float_as_uint(r) + noise(position + k, key)) >> 20) - ((127 - 7) << 3);
-        const int code = r == 0.f ? 0 : min(max(q, 8), 0x7F);
-        cr[k / 4] |= (uint32_t)code << (8 * (k % 4));
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t nan = 0x7Fu << (8 * (j % 4)), all = 0xFFu << (8 * (j % 4));
+          uint32_t &a = j < 4 ? codes_m.x : codes_m.y, &b = j < 4 ? codes_r.x : codes_r.y;
+          if (!isfinite(ms[j])) a = (a & ~all) | nan;
+          if (!isfinite(vs[j])) b = (b & ~all) | nan;
+        }
       }
-      put_codes(static_cast<uint8_t*>(t.m), at, t.n, whole && on(t.m, 8), make_uint2(cm[0], cm[1]));
-      put_codes(static_cast<uint8_t*>(t.v), at, t.n, whole && on(t.v, 8), make_uint2(cr[0], cr[1]));
+      put_codes(static_cast<uint8_t*>(t.m), at, t.n, whole && on(t.m, 8), codes_m);
+      put_codes(static_cast<uint8_t*>(t.v), at, t.n, whole && on(t.v, 8), codes_r);
       if (lane == 0) {
-        t.m_scale[at / BLOCK] = power(em);
-        t.v_scale[at / BLOCK] = power(er);
+        t.m_scale[start / BLOCK] = power(em);
+        t.v_scale[start / BLOCK] = power(er);
       }
     } else {
-      put(static_cast<float*>(t.m), at, t.n, whole && on(t.m, 32), m);
-      put(static_cast<float*>(t.v), at, t.n, whole && on(t.v, 32), v);
+      put(static_cast<float*>(t.m), at, t.n, whole && on(t.m, 32), ms);
+      put(static_cast<float*>(t.v), at, t.n, whole && on(t.v, 32), vs);
       if (c + 1 < c1) fetch(c + 1, x);
     }
   }
-  // the last CTA counts: every other one has read what it needs
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    last = atomicAdd(h.c.control, 1) == (int)gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!last) return;
-  for (int k = threadIdx.x; k < l.n; k += THREADS) *l.t[k].step += 1.f;
-  if (threadIdx.x == 0) *h.c.control = 0;
+  count(l, h.c.control);
 }
 
 // ------------------------------------------------------------------ the calls
@@ -345,6 +413,7 @@ int check(const BnbAdamTensor* t, int n) {
   if (n && !t) return BNB_ERR_NULL_POINTER;
   for (int i = 0; i < n; ++i) {
     if (t[i].n < 0 || t[i].element < 0 || t[i].element > 2) return BNB_ERR_BAD_ARGUMENT;
+    if (t[i].position & (BLOCK - 1)) return BNB_ERR_BAD_ARGUMENT;
     if (t[i].n > (int64_t)1 << 40) return BNB_ERR_UNSUPPORTED_DIMS;   // chunks of all tensors of a launch in 32 bits
     if (t[i].n && !t[i].g) return BNB_ERR_NULL_POINTER;
   }
@@ -365,6 +434,14 @@ Tensors<MOST> list_of(const BnbAdamTensor* t, int n) {
 }
 unsigned ctas_of(uint32_t chunks) { return std::max(1u, std::min(chunks, (uint32_t)CTAS)); }
 
+// f of the shortest list that holds n tensors.
+template <class F>
+int with_list(int n, F f) {
+  if (n <= 32) return f(std::integral_constant<int, 32>());
+  if (n <= 112) return f(std::integral_constant<int, 112>());
+  if (n <= 192) return f(std::integral_constant<int, 192>());
+  return f(std::integral_constant<int, MANY>());
+}
 template <int MOST>
 int norm(const BnbAdamTensor* t, int n, double* parts, bool add, cudaStream_t st) {
   const Tensors<MOST> l = list_of<MOST>(t, n);
@@ -373,7 +450,7 @@ int norm(const BnbAdamTensor* t, int n, double* parts, bool add, cudaStream_t st
 template <int MOST>
 int step(const BnbAdamTensor* t, int n, const Hyper& h, cudaStream_t st) {
   const Tensors<MOST> l = list_of<MOST>(t, n);
-  return h.c.state_bits == 8 ? launch_after(k_step<MOST, true>, dim3(ctas_of(l.chunks)), THREADS, 0, st, l, h)
+  return h.c.state_bits == 8 ? launch_after(k_step<MOST, true>, dim3(std::min(ctas_of(l.chunks), (unsigned)(SMS * RESIDENT))), THREADS, 0, st, l, h)
                              : launch_after(k_step<MOST, false>, dim3(ctas_of(l.chunks)), THREADS, 0, st, l, h);
 }
 
@@ -391,7 +468,7 @@ extern "C" int bnb_grad_norm(const BnbAdamTensor* t, int n, double* parts, void*
   int i = 0;
   do {
     const int k = std::min(n - i, MANY);
-    if (const int r = k <= FEW ? norm<FEW>(t + i, k, parts, i > 0, s) : k <= SOME ? norm<SOME>(t + i, k, parts, i > 0, s) : norm<MANY>(t + i, k, parts, i > 0, s)) return r;
+    if (const int r = with_list(k, [&](auto most) { return norm<decltype(most)::value>(t + i, k, parts, i > 0, s); })) return r;
     i += k;
   } while (i < n);
   return BNB_OK;
@@ -414,7 +491,7 @@ extern "C" int bnb_adamw_step(const BnbAdamTensor* t, int n, const BnbAdamW* c, 
   const auto s = static_cast<cudaStream_t>(stream);
   for (int i = 0; i < n;) {
     const int k = std::min(n - i, MANY);
-    if (const int r = k <= FEW ? step<FEW>(t + i, k, h, s) : k <= SOME ? step<SOME>(t + i, k, h, s) : step<MANY>(t + i, k, h, s)) return r;
+    if (const int r = with_list(k, [&](auto most) { return step<decltype(most)::value>(t + i, k, h, s); })) return r;
     i += k;
   }
   return BNB_OK;

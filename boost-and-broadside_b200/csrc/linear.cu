@@ -31,39 +31,76 @@ int check(const BnbLinear* c) {
 bool recomputes(const BnbLinear& c) { return c.activation == BNB_ACT_NONE || (c.element != BNB_ELEM_F32 && c.width <= 512); }
 bool keeps(const BnbLinear& c) { return !recomputes(c); }
 
-// dz from the kept z, eight neighbouring columns a thread, a row a lane.
+// dz from the kept z.  A warp takes blocks of 32 x 32: z as it was kept, a row a lane, dy and dz as whole pieces of rows through shared memory (a
+// lane's own row straight from memory is 32 lines a request).
 template <typename E, int PIECES>
 __global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, int64_t ld_dy, int wide, int activation, int64_t m, int n, void* dz, int64_t ld, int64_t piece_stride) {
-  using T = std::conditional_t<(PIECES > 1), float, E>;
+  constexpr bool EXACT = PIECES > 1;
+  using T = std::conditional_t<EXACT, float, E>;
+  constexpr int N = 16 / sizeof(T), ROW = 32 / N;   // pieces of a block's row: 4, float32 8
+  __shared__ uint4 staged[8][32 * ROW];
   let_next_start();
   wait_for_previous();
-  const int64_t groups = ld / 8, blocks = (m + 31) / 32, total = blocks * groups * 32;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t block = i / (groups * 32), rest = i - block * groups * 32, r = block * 32 + rest % 32;
-    const int c = (int)(rest / 32) * 8;
-    if (r >= m) continue;
-    float v[8];
-    const float4 z0 = *reinterpret_cast<const float4*>(z + kept_index(r, c, ld)), z1 = *reinterpret_cast<const float4*>(z + kept_index(r, c + 4, ld));
-    const float zs[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
-    const T* row = static_cast<const T*>(dy) + r * ld_dy;
-    constexpr int N = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint4* const mine = staged[warp];
+  auto spot = [](int r, int q) { return r * ROW + (q ^ ((r / (8 / ROW)) % ROW)); };
+  const int64_t columns = (ld + 31) / 32, blocks = (m + 31) / 32 * columns;
+  for (int64_t b = (int64_t)blockIdx.x * 8 + warp; b < blocks; b += (int64_t)gridDim.x * 8) {
+    const int64_t r0 = b / columns * 32;
+    const int c0 = (int)(b % columns) * 32;
+    const float4* kept = reinterpret_cast<const float4*>(z) + b * 256 + lane;
+    float4 zs[8];
+    uint4 in[ROW];
 #pragma unroll
-    for (int k = 0; k < 8; k += N) {
-      const uint4 raw = get16(row, c + k, n, wide);
-      const T* e = reinterpret_cast<const T*>(&raw);
+    for (int q = 0; q < 8; ++q) zs[q] = kept[q * 32];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if constexpr (PIECES > 1) v[k + j] = e[j];
-        else v[k + j] = up(e[j]);
+    for (int q = 0; q < ROW; ++q) {
+      const int r = q * (32 / ROW) + lane / ROW, c = c0 + lane % ROW * N;
+      in[q] = r0 + r < m && c < n ? get16(static_cast<const T*>(dy) + (r0 + r) * ld_dy, c, n, wide) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < ROW; ++q) mine[spot(q * (32 / ROW) + lane / ROW, lane % ROW)] = in[q];
+    __syncwarp();
+    F2 v[16];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const bool there[4] = {c0 + 4 * q < n, c0 + 4 * q + 1 < n, c0 + 4 * q + 2 < n, c0 + 4 * q + 3 < n};   // nothing was kept behind the last column
+      F2 a, d0, d1;
+      activate<EXACT, true>(activation, f2(there[0] ? zs[q].x : 0.f, there[1] ? zs[q].y : 0.f), a, d0);
+      activate<EXACT, true>(activation, f2(there[2] ? zs[q].z : 0.f, there[3] ? zs[q].w : 0.f), a, d1);
+      if constexpr (EXACT) {
+        const uint4 raw = mine[spot(lane, q)];
+        v[2 * q] = mul(d0, f2(__uint_as_float(raw.x), __uint_as_float(raw.y)));
+        v[2 * q + 1] = mul(d1, f2(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+      } else {
+        const uint2 raw = reinterpret_cast<const uint2*>(&mine[spot(lane, q / 2)])[q % 2];
+        v[2 * q] = mul(d0, pair_up(raw.x, E{}));
+        v[2 * q + 1] = mul(d1, pair_up(raw.y, E{}));
       }
     }
+    // the results: four pieces of a row, whatever dy was
+    auto out = [](int r, int q) { return r * 4 + (q ^ ((r / 2) % 4)); };
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float a, da;
-      activate_exact(activation, c + k < n ? zs[k] : 0.f, a, da);
-      v[k] *= da;
+    for (int piece = 0; piece < PIECES; ++piece) {
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t bits[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          bits[k] = pair_of<E>(v[4 * q + k]);
+          if constexpr (EXACT) v[4 * q + k] = add(v[4 * q + k], mul(pair_up(bits[k], E{}), f2(-1.f)));
+        }
+        mine[out(lane, q)] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = q * 8 + lane / 4, c = c0 + lane % 4 * 8;
+        if (r0 + r < m && c < ld) *reinterpret_cast<uint4*>(static_cast<E*>(dz) + piece * piece_stride + (r0 + r) * ld + c) = mine[out(r, lane % 4)];
+      }
     }
-    put_operand<E, PIECES>(dz, piece_stride, r * ld + c, v);
   }
 }
 
@@ -77,14 +114,31 @@ __global__ void __launch_bounds__(256) k_column_sums(const Operand o, float* par
   const int64_t r0 = o.rows * blockIdx.y / gridDim.y, r1 = o.rows * (blockIdx.y + 1) / gridDim.y;
   float v[8] = {};
   if (col < o.ld) {
-    for (int64_t r = r0 + t; r < r1; r += 32) {
+    constexpr int UNROLL = 4;   // rows whose loads are on their way together
+    const E* from = static_cast<const E*>(o.data) + col;
+    auto add_row = [&](const uint4 (&raw)[PIECES]) {
 #pragma unroll
       for (int p = PIECES - 1; p >= 0; --p) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const E*>(o.data) + p * o.piece_stride + r * o.ld + col);
-        const E* e = reinterpret_cast<const E*>(&raw);
+        const E* e = reinterpret_cast<const E*>(&raw[p]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] += up(e[k]);
       }
+    };
+    int64_t r = r0 + t;
+    for (; r + (UNROLL - 1) * 32 < r1; r += UNROLL * 32) {
+      uint4 raw[UNROLL][PIECES];
+#pragma unroll
+      for (int i = 0; i < UNROLL; ++i)
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) raw[i][p] = *reinterpret_cast<const uint4*>(from + p * o.piece_stride + (r + 32 * i) * o.ld);
+#pragma unroll
+      for (int i = 0; i < UNROLL; ++i) add_row(raw[i]);
+    }
+    for (; r < r1; r += 32) {
+      uint4 raw[PIECES];
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) raw[p] = *reinterpret_cast<const uint4*>(from + p * o.piece_stride + r * o.ld);
+      add_row(raw);
     }
   }
 #pragma unroll
@@ -97,8 +151,8 @@ __global__ void __launch_bounds__(256) k_column_sums(const Operand o, float* par
   const int c = blockIdx.x * 64 + threadIdx.x;
   if (c < n) part[(int64_t)blockIdx.y * n + c] = s;
 }
-// How many CTAs share the rows: enough for every SM, no fewer than 128 rows each.
-int row_shares(int64_t rows, int n) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 127) / 128, SMS * 4 / ((n + 63) / 64))); }
+// How many CTAs share the rows: six an SM, no fewer than 128 rows each.
+int row_shares(int64_t rows, int n) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 127) / 128, SMS * 6 / ((n + 63) / 64))); }
 
 // Where everything of a call stands in its scratch; sizes alone with base = null.
 struct Layout {
@@ -165,8 +219,8 @@ int backward(const BnbLinear& c, const BnbLinearGrads& g, const Layout& l, cudaS
   if (c.activation != BNB_ACT_NONE) {
     const int wide = reinterpret_cast<uintptr_t>(g.dy) % 16 == 0 && g.dy_row % (PIECES > 1 ? 4 : 8) == 0;
     if (keeps(c)) {
-      const int64_t work = (l.M + 31) / 32 * 32 * (l.ld / 8);
-      r = launch_after(k_slope<E, PIECES>, dim3((unsigned)std::min<int64_t>((work + 255) / 256, SMS * 32)), 256, 0, st, static_cast<const float*>(c.kept), g.dy, g.dy_row, wide,
+      const int64_t blocks = (l.M + 31) / 32 * ((l.ld + 31) / 32);
+      r = launch_after(k_slope<E, PIECES>, dim3((unsigned)std::min<int64_t>((blocks + 7) / 8, SMS * 8)), 256, 0, st, static_cast<const float*>(c.kept), g.dy, g.dy_row, wide,
                        (int)c.activation, l.M, (int)l.N, const_cast<void*>(l.dz.data), l.ld, l.dz.piece_stride);
     } else if constexpr (PIECES == 1) {
       Epilogue e{};

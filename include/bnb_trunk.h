@@ -698,7 +698,7 @@ typedef struct {
   float* v_scale;
   float* step;              /* 1: steps made; moves on by one */
   int64_t n;
-  int64_t position;
+  int64_t position;         /* a multiple of 256 */
   int32_t element;
 } BnbAdamTensor;
 
