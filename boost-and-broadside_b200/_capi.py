@@ -154,7 +154,8 @@ EXPORTS = {
     "bnb_policy_loss_kept_bytes": (C.c_size_t, [_fp]),
     "bnb_policy_loss_scratch_bytes": (C.c_size_t, [_fp]),
     "bnb_policy_loss_fwd": (C.c_int, [_fp, _fp, C.c_size_t, _fp]),
-    "bnb_policy_loss_bwd": (C.c_int, [_fp, _fp, _fp, _fp]),
+    "bnb_policy_loss_takes_gradients": (C.c_int, [_fp]),
+    "bnb_policy_loss_bwd": (C.c_int, [_fp, _fp, _fp, C.c_int, _fp]),
     "bnb_grad_norm": (C.c_int, [_fp, C.c_int, _fp, _fp]),
     "bnb_adamw_step": (C.c_int, [_fp, C.c_int, _fp, _fp]),
 }

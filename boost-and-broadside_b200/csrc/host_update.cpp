@@ -193,10 +193,11 @@ PolicyCall policy_call(const Tensor& logits, const Tensor& actions, const Tensor
   return k;
 }
 
-// (loss, log-probability of each row's actions, means, what the backward reads)
-std::tuple<Tensor, Tensor, Tensor, Tensor> policy_forward(const Tensor& logits, const Tensor& actions, const Tensor& old_logprob, const Tensor& advantages,
-                                                          const OptTensor& ref_logprob, const OptTensor& weights, const std::vector<int64_t>& sizes,
-                                                          double clip_low, double clip_high, double kl_coef, double entropy_coef) {
+struct PolicyResults { Tensor loss, logprob, stats, kept, dlogits; };
+// gradients: the logits' for dloss = 1 are written too, where the call takes them.
+PolicyResults policy_results(const Tensor& logits, const Tensor& actions, const Tensor& old_logprob, const Tensor& advantages,
+                             const OptTensor& ref_logprob, const OptTensor& weights, const std::vector<int64_t>& sizes, double clip_low, double clip_high,
+                             double kl_coef, double entropy_coef, bool gradients) {
   const c10::cuda::OptionalCUDAGuard guard(logits.is_cuda() ? c10::optional<c10::Device>(logits.device()) : c10::nullopt);
   PolicyCall k = policy_call(logits, actions, old_logprob, advantages, ref_logprob, weights, sizes, clip_low, clip_high, kl_coef, entropy_coef);
   const auto floats_of = logits.options().dtype(at::kFloat);
@@ -206,14 +207,23 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_forward(const Tensor& logits, 
   k.c.stats = static_cast<float*>(stats.data_ptr());
   k.c.logprob = static_cast<float*>(logprob.data_ptr());
   k.c.kept = static_cast<float*>(kept.data_ptr());
+  const Tensor dlogits = gradients && bnb_policy_loss_takes_gradients(&k.c) ? at::empty(logits.sizes(), logits.options()) : Tensor();
+  k.c.dlogits = dlogits.defined() && dlogits.numel() ? dlogits.data_ptr() : nullptr;
   const Tensor scratch = scratch_of(bnb_policy_loss_scratch_bytes(&k.c), logits);
   check("bnb_policy_loss_fwd", bnb_policy_loss_fwd(&k.c, scratch.data_ptr(), (size_t)scratch.numel(), stream_of(logits.device())));
-  return {loss, logprob, stats, kept};
+  return {loss, logprob, stats, kept, dlogits};
+}
+// (loss, log-probability of each row's actions, means, what the backward reads)
+std::tuple<Tensor, Tensor, Tensor, Tensor> policy_forward(const Tensor& logits, const Tensor& actions, const Tensor& old_logprob, const Tensor& advantages,
+                                                          const OptTensor& ref_logprob, const OptTensor& weights, const std::vector<int64_t>& sizes,
+                                                          double clip_low, double clip_high, double kl_coef, double entropy_coef) {
+  const PolicyResults r = policy_results(logits, actions, old_logprob, advantages, ref_logprob, weights, sizes, clip_low, clip_high, kl_coef, entropy_coef, false);
+  return {r.loss, r.logprob, r.stats, r.kept};
 }
 
 Tensor policy_backward(const Tensor& logits, const Tensor& actions, const Tensor& old_logprob, const Tensor& advantages, const OptTensor& ref_logprob,
                        const OptTensor& weights, const std::vector<int64_t>& sizes, double clip_low, double clip_high, double kl_coef, double entropy_coef,
-                       const Tensor& kept, const Tensor& dloss) {
+                       const Tensor& kept, const Tensor& dloss, const Tensor& unit) {
   const c10::cuda::CUDAGuard guard(logits.device());
   PolicyCall k = policy_call(logits, actions, old_logprob, advantages, ref_logprob, weights, sizes, clip_low, clip_high, kl_coef, entropy_coef);
   const Tensor rows = contiguous(kept).to(logits.device());
@@ -221,30 +231,55 @@ Tensor policy_backward(const Tensor& logits, const Tensor& actions, const Tensor
     refuse("policy_loss: what the forward kept came back as another tensor: saved-tensor hooks have to return type and shape as they were");
   expect("policy_loss", "the gradient of the loss", dloss, {}, logits.device());
   const Tensor slope = dloss.to(at::kFloat);
-  const Tensor out = at::empty(logits.sizes(), logits.options());
+  // the gradient that the forward wrote, if it is as it was
+  const bool holds = unit.defined() && unit.sizes() == logits.sizes() && unit.scalar_type() == logits.scalar_type() && unit.device() == logits.device() &&
+                     unit.is_contiguous() && reinterpret_cast<uintptr_t>(unit.data_ptr()) % 16 == 0;
+  const Tensor out = holds ? unit : at::empty(logits.sizes(), logits.options());
   k.c.kept = static_cast<float*>(rows.data_ptr());
-  check("bnb_policy_loss_bwd", bnb_policy_loss_bwd(&k.c, static_cast<const float*>(slope.data_ptr()), out.data_ptr(), stream_of(logits.device())));
+  check("bnb_policy_loss_bwd", bnb_policy_loss_bwd(&k.c, static_cast<const float*>(slope.data_ptr()), out.data_ptr(), holds ? 1 : 0, stream_of(logits.device())));
   return out;
+}
+Tensor policy_backward_alone(const Tensor& logits, const Tensor& actions, const Tensor& old_logprob, const Tensor& advantages, const OptTensor& ref_logprob,
+                             const OptTensor& weights, const std::vector<int64_t>& sizes, double clip_low, double clip_high, double kl_coef, double entropy_coef,
+                             const Tensor& kept, const Tensor& dloss) {
+  return policy_backward(logits, actions, old_logprob, advantages, ref_logprob, weights, sizes, clip_low, clip_high, kl_coef, entropy_coef, kept, dloss, Tensor());
+}
+// The capture that a device's current stream is in, or 0.
+unsigned long long capture_of(const c10::Device& dev) {
+  cudaStreamCaptureStatus status;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream(dev.index()).stream(), &status, &id) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
 }
 
 std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& actions, const Tensor& old_logprob, const Tensor& advantages,
                                                const OptTensor& ref_logprob, const OptTensor& weights, const std::vector<int64_t>& sizes, double clip_low,
-                                               double clip_high, double kl_coef, double entropy_coef) {
+                                               double clip_high, double kl_coef, double entropy_coef, bool grad_in_forward) {
   const variable_list inputs{logits};
-  Tensor loss, logprob, stats, kept;
+  const bool differentiable = wants_grad(inputs);
+  PolicyResults r;
   {
     const at::NoGradGuard no_grad;
-    std::tie(loss, logprob, stats, kept) =
-        policy_forward(logits, actions, old_logprob, advantages, ref_logprob, weights, sizes, clip_low, clip_high, kl_coef, entropy_coef);
+    r = policy_results(logits, actions, old_logprob, advantages, ref_logprob, weights, sizes, clip_low, clip_high, kl_coef, entropy_coef,
+                       differentiable && grad_in_forward);
   }
-  if (!wants_grad(inputs)) return {loss, logprob, stats};
-  auto node = node_of(inputs, {actions, old_logprob, advantages, value(ref_logprob), value(weights), kept},
-                      [=](const std::vector<Tensor>& s, const variable_list& g) -> variable_list {
-                        if (!g[0].defined()) return variable_list(1);
-                        return {policy_backward(s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), sizes, clip_low, clip_high, kl_coef, entropy_coef, s[6], g[0])};
-                      });
-  torch::autograd::create_gradient_edge(loss, node);
-  return {loss, logprob, stats};
+  if (!differentiable) return {r.loss, r.logprob, r.stats};
+  auto node = node_of(inputs, {actions, old_logprob, advantages, value(ref_logprob), value(weights), r.kept, r.dlogits}, {});
+  OpNode* const self = node.get();
+  // The gradient that the forward wrote goes out once: a second backward of the same graph, or one whose forward is not part of its
+  // capture (a replay has to repeat it), computes it.
+  const unsigned long long capture = capture_of(logits.device());
+  node->backward = [=](const std::vector<Tensor>& s, const variable_list& g) -> variable_list {
+    if (!g[0].defined()) return variable_list(1);
+    self->saved[7] = SavedVariable();
+    const Tensor unit = s[7].defined() && capture_of(s[0].device()) == capture ? s[7] : Tensor();
+    return {policy_backward(s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), sizes, clip_low, clip_high, kl_coef, entropy_coef, s[6], g[0], unit)};
+  };
+  torch::autograd::create_gradient_edge(r.loss, node);
+  return {r.loss, r.logprob, r.stats};
 }
 
 // ------------------------------------------------------------------ AdamW
@@ -462,7 +497,7 @@ void bind_update(py::module& m) {
   m.def("linear", torch::wrap_pybind_function(linear));
   py::class_<AdamWPlan>(m, "AdamWPlan").def(py::init<const py::list&, const py::dict&, int>()).def("step", &AdamWPlan::step);
   m.def("policy_loss_forward", &policy_forward);
-  m.def("policy_loss_backward", &policy_backward);
+  m.def("policy_loss_backward", &policy_backward_alone);
   m.def("policy_loss", torch::wrap_pybind_function(policy_loss));
 }
 

@@ -12,8 +12,7 @@
 // NaN, while NaN passes.  A row's terms are float32, their sums over rows 64 bits: thousands of terms of either sign leave a small mean.
 // Sums of CTAs are added in a fixed order by a last launch.
 //
-// Slices of up to 64 logits: a thread takes a slice, from a tile of rows in shared memory.  Wider ones: a warp takes a row, and from 1024 logits
-// on a CTA.
+// Slices of up to 64 logits: a thread takes a slice, from a tile of rows in shared memory.  Wider ones: 8 to 512 threads take a row.
 #include <algorithm>
 
 #include "launch_after.h"
@@ -29,9 +28,8 @@ using tensor::wait_for_previous;
 
 constexpr int SMS = 148, HEAD = 4;          // floats before the rows of `kept`: 1 / W
 constexpr int NARROW = 64;                  // logits of a slice that a thread takes
-constexpr int WARP_ROW = 1024;              // logits of a row that a warp takes
 constexpr int TERMS = 5;                    // w surrogate, w k, w H, w clipped, w
-constexpr int MAX_CTAS = SMS * 8;
+constexpr int MAX_CTAS = SMS * 16;
 
 // The larger of two, NaN where either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -61,28 +59,49 @@ struct Soft {
     if (z > m) raise(z);
     term(z, base());
   }
+  // N values, two an instruction where there is one; their sums apart until all are there.
   template <int N>
   __device__ __forceinline__ void add(const float (&z)[N]) {
     float top = z[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
     if (top > m) raise(top);
-    const float b = base();
+    const F2 b = f2(-base());
+    F2 ss = f2(0.f), us = f2(0.f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) term(z[i], b);
-  }
-  __device__ __forceinline__ void join(Soft o) {
-    const float to = fmaxf(m, o.m);
-    if (to > m) raise(to);
-    if (to > o.m) o.raise(to);
-    s += o.s;
-    u += o.u;
+    for (int i = 0; i < N; i += 2) {
+      const float2 d = halves(seq::add(f2(z[i], z[i + 1]), b));
+      const F2 t = f2(max_nan(d.x, -1e4f), max_nan(d.y, -1e4f));
+      const float2 x = halves(mul(t, f2(LOG2E)));
+      const F2 e = f2(ex2_fast(x.x), ex2_fast(x.y));
+      ss = seq::add(ss, e);
+      us = fma(e, t, us);
+    }
+    const float2 a = halves(ss), c = halves(us);
+    s += a.x + a.y;
+    u += c.x + c.y;
   }
   __device__ __forceinline__ float lse() const { return m == -INFINITY ? NAN : m + logf(s); }
   __device__ __forceinline__ float entropy() const { return m == -INFINITY ? NAN : logf(s) - u / s; }
 };
-__device__ __forceinline__ Soft shuffle(const Soft& v, int by) {
-  return {__shfl_xor_sync(0xffffffffu, v.m, by), __shfl_xor_sync(0xffffffffu, v.s, by), __shfl_xor_sync(0xffffffffu, v.u, by)};
+// The sums of N neighbouring lanes together, in all of them: first to one maximum, so that the sums are plain ones.  ALL: the whole warp holds the
+// same N values over and over, and one instruction has their maximum.
+template <int N, bool ALL>
+__device__ __forceinline__ Soft joined_lanes(Soft v) {
+  float top = v.m;
+  if constexpr (ALL) {
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(v.m));
+  } else {
+#pragma unroll
+    for (int by = N / 2; by; by >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, by));
+  }
+  if (top > v.m) v.raise(top);
+#pragma unroll
+  for (int by = N / 2; by; by >>= 1) {
+    v.s += __shfl_xor_sync(0xffffffffu, v.s, by);
+    v.u += __shfl_xor_sync(0xffffffffu, v.u, by);
+  }
+  return v;
 }
 
 struct Args {
@@ -90,8 +109,11 @@ struct Args {
   int width;
   int first[BNB_MAX_SLICES + 1];
   double* part;      // (CTAs, TERMS)
-  const float* dloss;
+  double* weights;   // sums of weights, n_weights of them; null where there are none
+  int n_weights;
+  const float* dloss;   // null: 1
   void* dlogits;
+  int holds_unit;    // dlogits has the gradient for dloss = 1
 };
 
 __device__ __forceinline__ float weight_of(const BnbPolicyLoss& c, int64_t r) {
@@ -102,11 +124,16 @@ __device__ __forceinline__ int action_of(const BnbPolicyLoss& c, int64_t r, int 
   const int64_t a = c.actions[r * c.n_slices + s];
   return a >= 0 && a < c.sizes[s] ? (int)a : -1;
 }
-// A row's terms and, where wanted, the loss's slope in l.
+// What a row has besides its logits.
+struct RowIn { float w, old, advantage, ref; };
+__device__ __forceinline__ RowIn row_in(const BnbPolicyLoss& c, int64_t r) {
+  return {weight_of(c, r), c.old_logprob[r], c.advantages[r], c.ref_logprob ? c.ref_logprob[r] : 0.f};
+}
+// A row's terms and the loss's slope in l.
 struct RowTerms { float surrogate, kl, clipped, slope; };
-__device__ __forceinline__ RowTerms row_terms(const BnbPolicyLoss& c, int64_t r, float l) {
+__device__ __forceinline__ RowTerms row_terms(const BnbPolicyLoss& c, const RowIn& x, float l) {
   RowTerms v;
-  const float a = c.advantages[r], ratio = expf(l - c.old_logprob[r]);
+  const float a = x.advantage, ratio = expf(l - x.old);
   const float lo = 1.f - c.clip_low, hi = 1.f + c.clip_high, held = ratio < lo ? lo : ratio > hi ? hi : ratio;
   const float free_ = ratio * a, bound = held * a;
   v.surrogate = free_ <= bound ? free_ : bound != bound || free_ == free_ ? bound : free_;   // NaN stays NaN
@@ -114,7 +141,7 @@ __device__ __forceinline__ RowTerms row_terms(const BnbPolicyLoss& c, int64_t r,
   v.clipped = ratio < lo || ratio > hi ? 1.f : 0.f;
   v.kl = 0.f;
   if (c.ref_logprob) {
-    const float d = c.ref_logprob[r] - l, grown = expm1f(d);
+    const float d = x.ref - l, grown = expm1f(d);
     v.kl = grown - d;
     if (c.kl_coef != 0.f) v.slope = fmaf(-c.kl_coef, grown, v.slope);
   }
@@ -136,20 +163,12 @@ struct Sums {
     v[4] += d;
   }
 };
-// Sums over a CTA's warps, lane 0 of each holding its own, to the CTA's place.
-__device__ __forceinline__ void put_sums(const Args& a, Sums s, double (*shared)[TERMS]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-#pragma unroll
-  for (int i = 0; i < TERMS; ++i)
-#pragma unroll
-    for (int by = 16; by; by >>= 1) s.v[i] += __shfl_xor_sync(0xffffffffu, s.v[i], by);
-  if (lane == 0)
-#pragma unroll
-    for (int i = 0; i < TERMS; ++i) shared[warp][i] = s.v[i];
+// `parts` sums of a CTA, to the CTA's place.
+__device__ __forceinline__ void put_sums(const Args& a, const double (*shared)[TERMS], int parts) {
   __syncthreads();
   if (threadIdx.x < TERMS) {
     double v = 0;
-    for (int w = 0; w < warps; ++w) v += shared[w][threadIdx.x];
+    for (int w = 0; w < parts; ++w) v += shared[w][threadIdx.x];
     a.part[(int64_t)blockIdx.x * TERMS + threadIdx.x] = v;
   }
 }
@@ -161,6 +180,7 @@ __global__ void __launch_bounds__(32 * TERMS) k_finish(const __grid_constant__ A
   let_next_start();
   wait_for_previous();
   double v = 0;
+#pragma unroll 8
   for (int i = lane; i < ctas; i += 32) v += a.part[(int64_t)i * TERMS + term];
 #pragma unroll
   for (int by = 16; by; by >>= 1) v += __shfl_xor_sync(0xffffffffu, v, by);
@@ -173,6 +193,35 @@ __global__ void __launch_bounds__(32 * TERMS) k_finish(const __grid_constant__ A
 #pragma unroll
   for (int i = 0; i < 4; ++i) a.c.stats[i] = (float)mean[i];
   a.c.kept[0] = (float)by;
+}
+
+// Sums of weights, for a forward that writes gradients: they need 1 / W.
+constexpr int WEIGHT_ROWS = 4096;   // of a CTA, at most SMS of them
+__global__ void __launch_bounds__(256) k_weights(const __grid_constant__ Args a) {
+  __shared__ double sums[8];
+  let_next_start();
+  wait_for_previous();
+  double v = 0;
+  for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.c.rows; r += (int64_t)gridDim.x * 256) v += weight_of(a.c, r);
+#pragma unroll
+  for (int by = 16; by; by >>= 1) v += __shfl_xor_sync(0xffffffffu, v, by);
+  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = v;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < 8; ++w) v += sums[w];
+  a.weights[blockIdx.x] = v;
+}
+// 1 / W, by every warp for itself.
+__device__ __forceinline__ float share_of_rows(const Args& a) {
+  double v = 0;
+  if (a.weights) {
+    for (int i = threadIdx.x & 31; i < a.n_weights; i += 32) v += a.weights[i];
+#pragma unroll
+    for (int by = 16; by; by >>= 1) v += __shfl_xor_sync(0xffffffffu, v, by);
+  } else {
+    v = (double)a.c.rows;
+  }
+  return v != 0 ? (float)(1 / v) : 0.f;
 }
 
 // ------------------------------------------------------------------ narrow slices
@@ -251,13 +300,20 @@ __global__ void __launch_bounds__(512) k_narrow(const __grid_constant__ Args a, 
           l += v.x;
           h += v.y;
         }
-        s.add(w, row_terms(c, r, l), h);
+        s.add(w, row_terms(c, row_in(c, r), l), h);
         kept[2 * S] = l;
       }
       c.logprob[r] = l;
     }
   }
-  put_sums(a, s, sums);
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i)
+#pragma unroll
+    for (int by = 16; by; by >>= 1) s.v[i] += __shfl_xor_sync(0xffffffffu, s.v[i], by);
+  if ((tid & 31) == 0)
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) sums[tid >> 5][i] = s.v[i];
+  put_sums(a, sums, threads / 32);
 }
 
 // ------------------------------------------------------------------ wide slices
@@ -274,36 +330,123 @@ __device__ __forceinline__ Span span_of(const E* at, int n) {
   return s;
 }
 
-// T threads a row, of CTAs of THREADS.
-template <typename E, int T, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_wide(const __grid_constant__ Args a) {
-  constexpr int N = 16 / sizeof(E), ROWS = THREADS / T, UNROLL = 4;
-  __shared__ double sums[THREADS / 32][TERMS];
+// What a row's gradients need: dl, and c2 (c1 with each slice's H).
+struct Slope { float dl, c2; };
+__device__ __forceinline__ Slope slope_of(const BnbPolicyLoss& c, float share, const RowTerms& t) { return {share * t.slope, share * c.entropy_coef}; }
+__device__ __forceinline__ float gradient(float z, float lse, float c1, float c2) {
+  const float t = max_nan(z - lse, -1e4f);
+  return ex2_fast(t * LOG2E) * fmaf(c2, t, c1);
+}
+// A slice's gradients, T threads along it.  `on`: the row has weight; `at`: the action, or -1.  held: the first HELD pieces of a thread, already in hand.
+template <typename E, int T, int HELD>
+__device__ __forceinline__ void put_gradients(const E* z, E* to, int n, int t, bool on, int at, float lse, float h, Slope k, const Raw<E, 16 / sizeof(E)>* held) {
+  constexpr int N = 16 / sizeof(E);
+  const float c1 = on ? fmaf(k.c2, h, -k.dl) : 0.f;
+  auto one = [&](int j) { to[j] = on ? from_f<E>(gradient(to_f(z[j]), lse, c1, k.c2) + (j == at ? k.dl : 0.f)) : from_f<E>(0.f); };
+  const Span span = span_of(to, n);
+  const bool along = (reinterpret_cast<uintptr_t>(z) & 15) == (reinterpret_cast<uintptr_t>(to) & 15);
+  if (on && !along) {   // rows that start elsewhere in their 16 bytes than the results
+    for (int j = t; j < n; j += T) one(j);
+    return;
+  }
+  if (t < span.head) one(t);
+  if (t < span.tail) one(span.head + span.pieces * N + t);
+  const F2 by = f2(-lse), c1s = f2(c1), c2s = f2(k.c2);
+  auto piece = [&](int i, const Raw<E, N>& raw) {
+    const int j = span.head + i * N;
+    float f[N];
+    unpack<E, N>(raw, f);
+#pragma unroll
+    for (int q = 0; q < N; q += 2) {
+      const float2 d = halves(add(f2(f[q], f[q + 1]), by));
+      const F2 v = f2(max_nan(d.x, -1e4f), max_nan(d.y, -1e4f));
+      const float2 x = halves(mul(v, f2(LOG2E)));
+      const float2 r = halves(mul(f2(ex2_fast(x.x), ex2_fast(x.y)), fma(c2s, v, c1s)));
+      f[q] = r.x, f[q + 1] = r.y;
+    }
+    if ((unsigned)(at - j) < (unsigned)N) {
+#pragma unroll
+      for (int q = 0; q < N; ++q) f[q] += j + q == at ? k.dl : 0.f;
+    }
+    store<E, N>(to + j, f);
+  };
+  if (on) {
+    constexpr int UNROLL = 4;
+    int i = t;
+    if constexpr (HELD > 0) {
+#pragma unroll
+      for (int q = 0; q < HELD; ++q, i += T)
+        if (i < span.pieces) piece(i, held[q]);
+    }
+    for (; i + (UNROLL - 1) * T < span.pieces; i += UNROLL * T) {
+      Raw<E, N> raw[UNROLL];
+#pragma unroll
+      for (int q = 0; q < UNROLL; ++q) raw[q] = load_raw<E, N>(z + span.head + (int64_t)(i + q * T) * N);
+#pragma unroll
+      for (int q = 0; q < UNROLL; ++q) piece(i + q * T, raw[q]);
+    }
+    for (; i < span.pieces; i += T) piece(i, load_raw<E, N>(z + span.head + (int64_t)i * N));
+  } else {
+    for (int i = t; i < span.pieces; i += T) *reinterpret_cast<uint4*>(to + span.head + (int64_t)i * N) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// T threads a row, of CTAs of THREADS.  GRAD: the gradients for dloss = 1 are written too, from the row's logits once more: the first HELD pieces of
+// a thread from its registers, others from L2, so that memory gives and takes every number once.  A row's other numbers are read a row ahead.
+template <typename E, int T, int THREADS, bool GRAD>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_wide(const __grid_constant__ Args a) {
+  constexpr int N = 16 / sizeof(E), ROWS = THREADS / T, HELD = GRAD && T < 512 ? 4 : 0, UNROLL = 4;   // a row of 512 threads is long: few of its pieces fit
+  __shared__ double sums[ROWS][TERMS];
   __shared__ Soft joined[THREADS / 32];
   let_next_start();
   wait_for_previous();
   const BnbPolicyLoss& c = a.c;
-  const int S = c.n_slices, t = threadIdx.x % T, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Sums sum;
-  sum.start();
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / T; r < c.rows; r += (int64_t)gridDim.x * ROWS) {
-    const float w = weight_of(c, r);
-    if (w == 0.f) {
-      if (t == 0) c.logprob[r] = 0.f;
-      continue;
+  const int S = c.n_slices, t = threadIdx.x % T, group = threadIdx.x / T, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < ROWS * TERMS; i += THREADS) sums[i / TERMS][i % TERMS] = 0;
+  __syncthreads();
+  const float per_row = GRAD ? share_of_rows(a) : 0.f;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  RowIn next{};
+  int next_at = -1;
+  auto look = [&](int64_t r) {
+    if (r < c.rows) {
+      next = row_in(c, r);
+      next_at = action_of(c, r, 0);
     }
-    const E* row = static_cast<const E*>(c.logits) + r * c.logits_row;
+  };
+  look((int64_t)blockIdx.x * ROWS + group);
+  for (int64_t first = (int64_t)blockIdx.x * ROWS; first < c.rows; first += step) {
+    const int64_t r = first + group;
+    const RowIn in = next;
+    int at = next_at;
+    look(r + step);
+    const bool there = r < c.rows, on = there && in.w != 0.f;   // of all threads of a row
+    const E* row = static_cast<const E*>(c.logits) + (there ? r : 0) * c.logits_row;
+    E* const to = static_cast<E*>(a.dlogits) + (there ? r : 0) * a.width;
     float* kept = c.kept + HEAD + r * (2 * S + 1);
-    float l = 0.f, h = 0.f;
+    float l = 0.f, h = 0.f, lse = 0.f, hs = 0.f;
+    Raw<E, N> held[HELD > 0 ? HELD : 1];
     for (int s = 0; s < S; ++s) {
       const E* z = row + a.first[s];
-      const Span span = span_of(z, c.sizes[s]);
+      const Span span = span_of(z, on ? c.sizes[s] : 0);
       const E* body = z + span.head;
+      if (s && on) at = action_of(c, r, s);
+      const float taken = on && at >= 0 ? to_f(z[at]) : 0.f;
       Soft v;
       v.start();
+      int i = t;
+#pragma unroll
+      for (int k = 0; k < HELD; ++k)
+        if (i + k * T < span.pieces) held[k] = load_raw<E, N>(body + (int64_t)(i + k * T) * N);
       if (t < span.head) v.add_one(to_f(z[t]));
       if (t < span.tail) v.add_one(to_f(body[span.pieces * N + t]));
-      int i = t;
+#pragma unroll
+      for (int k = 0; k < HELD; ++k, i += T)
+        if (i < span.pieces) {
+          float f[N];
+          unpack<E, N>(held[k], f);
+          v.add(f);
+        }
       for (; i + (UNROLL - 1) * T < span.pieces; i += UNROLL * T) {
         Raw<E, N> raw[UNROLL];
 #pragma unroll
@@ -320,49 +463,54 @@ __global__ void __launch_bounds__(THREADS) k_wide(const __grid_constant__ Args a
         load<E, N>(body + (int64_t)i * N, f);
         v.add(f);
       }
-#pragma unroll
-      for (int by = 16; by; by >>= 1) v.join(shuffle(v, by));
+      if constexpr (T < 32) __syncwarp();
+      v = joined_lanes<(T < 32 ? T : 32), (T >= 32)>(v);
       if constexpr (T > 32) {
         __syncthreads();
         if (lane == 0) joined[warp] = v;
         __syncthreads();
-        v = joined[lane % (T / 32)];
-#pragma unroll
-        for (int by = T / 64; by; by >>= 1) v.join(shuffle(v, by));
+        v = joined_lanes<T / 32, true>(joined[lane % (T / 32)]);
       }
-      const int at = action_of(c, r, s);
-      const float log_s = logf(v.s), hs = v.entropy();
-      l += at < 0 || v.m == -INFINITY ? NAN : (to_f(z[at]) - v.m) - log_s;
+      const float log_s = logf(v.s);
+      hs = v.entropy();
+      lse = v.lse();
+      l += at < 0 || v.m == -INFINITY ? NAN : (taken - v.m) - log_s;
       h += hs;
-      if (t == 0) {
-        kept[2 * s] = v.lse();
+      if (t == 0 && on) {
+        kept[2 * s] = lse;
         kept[2 * s + 1] = hs;
       }
     }
-    if (t == 0) {
-      sum.add(w, row_terms(c, r, l), h);
-      kept[2 * S] = l;
-      c.logprob[r] = l;
+    RowTerms terms{};
+    if (on && (GRAD || t == 0)) terms = row_terms(c, in, l);
+    if (t == 0 && there) {
+      if (on) {
+        Sums sum = *reinterpret_cast<const Sums*>(sums[group]);   // its row's, in shared memory: no other thread needs the registers
+        sum.add(in.w, terms, h);
+        *reinterpret_cast<Sums*>(sums[group]) = sum;
+        kept[2 * S] = l;
+      }
+      c.logprob[r] = on ? l : 0.f;
     }
+    if constexpr (GRAD) {
+      const Slope k = slope_of(c, in.w * per_row, terms);
+      if (S == 1 || !on) {
+        if (there) put_gradients<E, T, HELD>(on ? row : to, to, a.width, t, on, at, lse, hs, k, held);
+      }
+      if (S > 1) {
+        if constexpr (T > 32) __syncthreads();   // what thread 0 kept of the slices
+        else __syncwarp();
+        if (on)
+          for (int s = 0; s < S; ++s)
+            put_gradients<E, T, 0>(row + a.first[s], to + a.first[s], c.sizes[s], t, true, action_of(c, r, s), kept[2 * s], kept[2 * s + 1], k, nullptr);
+      }
+    }
+    if constexpr (T < 32) __syncwarp();
   }
-  __syncthreads();
-  put_sums(a, sum, sums);
+  put_sums(a, sums, ROWS);
 }
 
 // ------------------------------------------------------------------ backward
-
-// What a row's gradients need: dl, and c2 (c1 with each slice's H).
-struct Slope { float dl, c2; };
-__device__ __forceinline__ Slope slope_of(const Args& a, int64_t r, float w) {
-  const BnbPolicyLoss& c = a.c;
-  const float share = a.dloss[0] * (w * c.kept[0]);
-  const float l = c.kept[HEAD + r * (2 * c.n_slices + 1) + 2 * c.n_slices];
-  return {share * row_terms(c, r, l).slope, share * c.entropy_coef};
-}
-__device__ __forceinline__ float gradient(float z, float lse, float c1, float c2) {
-  const float t = max_nan(z - lse, -1e4f);
-  return ex2_fast(t * LOG2E) * fmaf(c2, t, c1);
-}
 
 template <typename E>
 __global__ void __launch_bounds__(256) k_narrow_bwd(const __grid_constant__ Args a) {
@@ -382,8 +530,8 @@ __global__ void __launch_bounds__(256) k_narrow_bwd(const __grid_constant__ Args
       for (int j = 0; j < n; ++j) to[j] = from_f<E>(0.f);
       continue;
     }
-    const Slope k = slope_of(a, r, w);
     const float* kept = c.kept + HEAD + r * (2 * S + 1);
+    const Slope k = slope_of(c, a.dloss[0] * (w * c.kept[0]), row_terms(c, row_in(c, r), kept[2 * S]));
     const float lse = kept[2 * s], c1 = fmaf(k.c2, kept[2 * s + 1], -k.dl);
     const int at = action_of(c, r, s);
     const E* z = static_cast<const E*>(c.logits) + r * c.logits_row + a.first[s];
@@ -393,59 +541,40 @@ __global__ void __launch_bounds__(256) k_narrow_bwd(const __grid_constant__ Args
 
 template <typename E, int T, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_wide_bwd(const __grid_constant__ Args a) {
-  constexpr int N = 16 / sizeof(E), ROWS = THREADS / T;
+  constexpr int ROWS = THREADS / T;
   let_next_start();
   wait_for_previous();
   const BnbPolicyLoss& c = a.c;
   const int S = c.n_slices, t = threadIdx.x % T;
+  const float dloss = a.dloss[0];
+  if (a.holds_unit && dloss == 1.f) return;
   for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / T; r < c.rows; r += (int64_t)gridDim.x * ROWS) {
     const float w = weight_of(c, r);
     const bool on = w != 0.f;
-    const Slope k = on ? slope_of(a, r, w) : Slope{0.f, 0.f};
     const float* kept = c.kept + HEAD + r * (2 * S + 1);
-    for (int s = 0; s < S; ++s) {
-      const E* z = static_cast<const E*>(c.logits) + r * c.logits_row + a.first[s];
-      E* to = static_cast<E*>(a.dlogits) + r * a.width + a.first[s];
-      const int n = c.sizes[s], at = on ? action_of(c, r, s) : -1;
-      const float lse = on ? kept[2 * s] : 0.f, c1 = on ? fmaf(k.c2, kept[2 * s + 1], -k.dl) : 0.f;
-      auto one = [&](int j) { to[j] = on ? from_f<E>(gradient(to_f(z[j]), lse, c1, k.c2) + (j == at ? k.dl : 0.f)) : from_f<E>(0.f); };
-      const Span span = span_of(to, n);
-      const bool along = (reinterpret_cast<uintptr_t>(z) & 15) == (reinterpret_cast<uintptr_t>(to) & 15);
-      if (on && !along) {   // rows that start elsewhere in their 16 bytes than the results
-        for (int j = t; j < n; j += T) one(j);
-        continue;
-      }
-      if (t < span.head) one(t);
-      if (t < span.tail) one(span.head + span.pieces * N + t);
-      for (int i = t; i < span.pieces; i += T) {
-        const int j = span.head + i * N;
-        float f[N];
-        if (on) {
-          load<E, N>(z + j, f);
-#pragma unroll
-          for (int q = 0; q < N; ++q) f[q] = gradient(f[q], lse, c1, k.c2) + (j + q == at ? k.dl : 0.f);
-        } else {
-#pragma unroll
-          for (int q = 0; q < N; ++q) f[q] = 0.f;
-        }
-        store<E, N>(to + j, f);
-      }
-    }
+    const Slope k = on ? slope_of(c, dloss * (w * c.kept[0]), row_terms(c, row_in(c, r), kept[2 * S])) : Slope{0.f, 0.f};
+    for (int s = 0; s < S; ++s)
+      put_gradients<E, T, 0>(static_cast<const E*>(c.logits) + r * c.logits_row + a.first[s], static_cast<E*>(a.dlogits) + r * a.width + a.first[s], c.sizes[s], t, on,
+                             on ? action_of(c, r, s) : -1, on ? kept[2 * s] : 0.f, on ? kept[2 * s + 1] : 0.f, k, nullptr);
   }
 }
 
 // ------------------------------------------------------------------ the calls
 
-int check(const BnbPolicyLoss* c) {
-  if (!c) return BNB_ERR_NULL_POINTER;
-  if (c->rows < 0 || c->element < 0 || c->element > 2) return BNB_ERR_BAD_ARGUMENT;
+int check_slices(const BnbPolicyLoss* c) {
   if (c->n_slices < 1 || c->n_slices > BNB_MAX_SLICES) return BNB_ERR_UNSUPPORTED_DIMS;
   int64_t width = 0;
   for (int i = 0; i < c->n_slices; ++i) {
     if (c->sizes[i] < 1) return BNB_ERR_UNSUPPORTED_DIMS;
     width += c->sizes[i];
   }
-  if (width > 1 << 28 || c->rows > (int64_t)1 << 40) return BNB_ERR_UNSUPPORTED_DIMS;
+  return width > 1 << 28 ? BNB_ERR_UNSUPPORTED_DIMS : BNB_OK;
+}
+int check(const BnbPolicyLoss* c) {
+  if (!c) return BNB_ERR_NULL_POINTER;
+  if (c->rows < 0 || c->element < 0 || c->element > 2) return BNB_ERR_BAD_ARGUMENT;
+  if (const int st = check_slices(c)) return st;
+  if (c->rows > (int64_t)1 << 40) return BNB_ERR_UNSUPPORTED_DIMS;
   if (c->weights && c->mask) return BNB_ERR_BAD_ARGUMENT;
   if (!(c->clip_low >= 0.f) || !(c->clip_high >= 0.f)) return BNB_ERR_BAD_ARGUMENT;
   if (c->rows && (!c->logits || !c->actions || !c->old_logprob || !c->advantages)) return BNB_ERR_NULL_POINTER;
@@ -462,6 +591,26 @@ Args args_of(const BnbPolicyLoss& c) {
 bool narrow(const BnbPolicyLoss& c) { return *std::max_element(c.sizes, c.sizes + c.n_slices) <= NARROW; }
 int ctas_of(int64_t units, int most) { return (int)std::max<int64_t>(1, std::min<int64_t>(units, most)); }
 
+// Threads of a row: some 8 to 16 pieces of 16 bytes each, so that what a row takes besides, a chain of some 2 us, is shared by few and many rows are at
+// work.  Forward with gradients of 134 M bfloat16 logits (268 MB each way), us by width: 32768 with 256 threads 135 (512: 160), 16384
+// with 128 135 (256: 148), 8192 with 64 138 (128: 145, 256: 195), 4096 with 64 149 (32: 171), 2048 with 32 169 (256: 520).
+template <typename E, int T, int THREADS, bool GRAD>
+int launch_wide(const Args& a, int& ctas, cudaStream_t st) {
+  ctas = ctas_of((a.c.rows + THREADS / T - 1) / (THREADS / T), MAX_CTAS);   // more than there is room for: rows without weight take less
+  return launch_after(k_wide<E, T, THREADS, GRAD>, dim3(ctas), THREADS, 0, st, a);
+}
+template <typename E, bool GRAD>
+int wide(const Args& a, int& ctas, cudaStream_t st) {
+  const int64_t bytes = (int64_t)a.width * sizeof(E);
+  if (bytes <= 1024) return launch_wide<E, 8, 256, GRAD>(a, ctas, st);
+  if (bytes <= 2048) return launch_wide<E, 16, 256, GRAD>(a, ctas, st);
+  if (bytes <= 4096) return launch_wide<E, 32, 256, GRAD>(a, ctas, st);
+  if (bytes <= 16384) return launch_wide<E, 64, 64, GRAD>(a, ctas, st);
+  if (bytes <= 32768) return launch_wide<E, 128, 128, GRAD>(a, ctas, st);
+  if (bytes <= 131072) return launch_wide<E, 256, 256, GRAD>(a, ctas, st);
+  return launch_wide<E, 512, 512, GRAD>(a, ctas, st);
+}
+
 template <typename E>
 int forward(Args a, cudaStream_t st) {
   const BnbPolicyLoss& c = a.c;
@@ -472,12 +621,13 @@ int forward(Args a, cudaStream_t st) {
     if (bytes > 48 * 1024 && cudaFuncSetAttribute(k_narrow<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return BNB_ERR_LAUNCH;
     ctas = ctas_of((c.rows + t.rows - 1) / t.rows, MAX_CTAS);
     r = launch_after(k_narrow<E>, dim3(ctas), t.threads, bytes, st, a, t.rows, t.pitch, (uint32_t)((((uint64_t)1 << 32) + a.width - 1) / a.width));
-  } else if (a.width <= WARP_ROW) {
-    ctas = ctas_of((c.rows + 7) / 8, MAX_CTAS);
-    r = launch_after(k_wide<E, 32, 256>, dim3(ctas), 256, 0, st, a);
   } else {
-    ctas = ctas_of(c.rows, MAX_CTAS);
-    r = launch_after(k_wide<E, 256, 256>, dim3(ctas), 256, 0, st, a);
+    const bool grad = a.dlogits != nullptr;
+    if (grad && a.weights) {
+      a.n_weights = ctas_of((c.rows + WEIGHT_ROWS - 1) / WEIGHT_ROWS, SMS);
+      if (r = launch_after(k_weights, dim3(a.n_weights), 256, 0, st, a); r) return r;
+    }
+    r = grad ? wide<E, true>(a, ctas, st) : wide<E, false>(a, ctas, st);
   }
   return r ? r : launch_after(k_finish, dim3(1), 32 * TERMS, 0, st, a, ctas);
 }
@@ -485,8 +635,11 @@ template <typename E>
 int backward(const Args& a, cudaStream_t st) {
   const BnbPolicyLoss& c = a.c;
   if (narrow(c)) return launch_after(k_narrow_bwd<E>, dim3(ctas_of((c.rows * c.n_slices + 255) / 256, SMS * 32)), 256, 0, st, a);
-  if (a.width <= WARP_ROW) return launch_after(k_wide_bwd<E, 32, 256>, dim3(ctas_of((c.rows + 7) / 8, MAX_CTAS)), 256, 0, st, a);
-  return launch_after(k_wide_bwd<E, 256, 256>, dim3(ctas_of(c.rows, MAX_CTAS)), 256, 0, st, a);
+  const int64_t bytes = (int64_t)a.width * sizeof(E);
+  if (bytes <= 1024) return launch_after(k_wide_bwd<E, 8, 256>, dim3(ctas_of((c.rows + 31) / 32, SMS * 8)), 256, 0, st, a);
+  if (bytes <= 4096) return launch_after(k_wide_bwd<E, 32, 256>, dim3(ctas_of((c.rows + 7) / 8, SMS * 8)), 256, 0, st, a);
+  if (bytes <= 16384) return launch_after(k_wide_bwd<E, 64, 64>, dim3(ctas_of(c.rows, SMS * 32)), 64, 0, st, a);
+  return launch_after(k_wide_bwd<E, 256, 256>, dim3(ctas_of(c.rows, SMS * 4)), 256, 0, st, a);
 }
 
 }  // namespace
@@ -501,7 +654,9 @@ extern "C" size_t bnb_policy_loss_kept_bytes(const BnbPolicyLoss* c) {
   return (HEAD + (size_t)c->rows * (2 * c->n_slices + 1)) * 4;
 }
 
-extern "C" size_t bnb_policy_loss_scratch_bytes(const BnbPolicyLoss* c) { return c ? (size_t)MAX_CTAS * TERMS * sizeof(double) : 0; }
+extern "C" size_t bnb_policy_loss_scratch_bytes(const BnbPolicyLoss* c) { return c ? (size_t)(MAX_CTAS * TERMS + SMS) * sizeof(double) : 0; }
+
+extern "C" int bnb_policy_loss_takes_gradients(const BnbPolicyLoss* c) { return c && !check_slices(c) && c->element != BNB_ELEM_F16 && !narrow(*c) ? 1 : 0; }
 
 extern "C" int bnb_policy_loss_fwd(const BnbPolicyLoss* c, void* scratch, size_t scratch_bytes, void* stream) {
   if (const int st = check(c)) return st;
@@ -510,11 +665,17 @@ extern "C" int bnb_policy_loss_fwd(const BnbPolicyLoss* c, void* scratch, size_t
   if (reinterpret_cast<uintptr_t>(scratch) & 15) return BNB_ERR_MISALIGNED;
   Args a = args_of(*c);
   a.part = static_cast<double*>(scratch);
+  if (c->weights || c->mask) a.weights = a.part + MAX_CTAS * TERMS;
+  if (c->dlogits) {
+    if (!bnb_policy_loss_takes_gradients(c)) return BNB_ERR_BAD_ARGUMENT;
+    if (reinterpret_cast<uintptr_t>(c->dlogits) & 15) return BNB_ERR_MISALIGNED;
+    a.dlogits = c->dlogits;
+  }
   const auto s = static_cast<cudaStream_t>(stream);
   return c->element == BNB_ELEM_F32 ? forward<float>(a, s) : c->element == BNB_ELEM_BF16 ? forward<__nv_bfloat16>(a, s) : forward<__half>(a, s);
 }
 
-extern "C" int bnb_policy_loss_bwd(const BnbPolicyLoss* c, const float* dloss, void* dlogits, void* stream) {
+extern "C" int bnb_policy_loss_bwd(const BnbPolicyLoss* c, const float* dloss, void* dlogits, int holds_unit, void* stream) {
   if (const int st = check(c)) return st;
   if (c->rows == 0) return BNB_OK;
   if (!dloss || !dlogits) return BNB_ERR_NULL_POINTER;
@@ -522,6 +683,7 @@ extern "C" int bnb_policy_loss_bwd(const BnbPolicyLoss* c, const float* dloss, v
   Args a = args_of(*c);
   a.dloss = dloss;
   a.dlogits = dlogits;
+  a.holds_unit = holds_unit && bnb_policy_loss_takes_gradients(c);
   const auto s = static_cast<cudaStream_t>(stream);
   return c->element == BNB_ELEM_F32 ? backward<float>(a, s) : c->element == BNB_ELEM_BF16 ? backward<__nv_bfloat16>(a, s) : backward<__half>(a, s);
 }

@@ -17,7 +17,7 @@ from . import _ops, _update_ops
 def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprob: torch.Tensor, advantages: torch.Tensor, *,
                 weights: Optional[torch.Tensor] = None, ref_logprob: Optional[torch.Tensor] = None, sizes: Optional[Sequence[int]] = None,
                 clip: Union[float, Tuple[float, float]] = 0.2, kl_coef: float = 0.0,
-                entropy_coef: float = 0.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                entropy_coef: float = 0.0, grad_in_forward: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The mean over rows of  -min(ratio A, clip(ratio) A) + kl_coef k - entropy_coef H,  differentiable in the logits.
 
     ``ratio`` is exp(l - old_logprob) of the log-probability l of a row's actions, k = exp(ref_logprob - l) - (ref_logprob - l) - 1 estimates the
@@ -31,6 +31,9 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprob: torch.
             log-probability and gradient are 0.  The loss is 0 where no row has weight.
         sizes: up to 16 distributions side by side, V in total, such as (3, 7, 2); their log-probabilities and entropies add up.
         clip: how far the ratio may go from 1, in both directions or (down, up).
+        grad_in_forward: write the gradient with the forward, in one pass over the logits, where slices are wider than 64 and not float16.
+            It is what the backward returns when the loss arrives there multiplied by 1; by anything else, it is computed once more.  False leaves it to
+            the backward: for losses that are scaled.
 
     Returns:
         (loss, logprob, stats): loss () and l (..) in float32, and the means of (surrogate, k, H, whether the ratio is outside
@@ -47,5 +50,5 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logprob: torch.
     if sizes is not None and not numbers[0]:
         raise ValueError("policy_loss: sizes must name at least one slice")
     if _ops.direct(logits):
-        return _capi.host.policy_loss(logits, actions, old_logprob, advantages, ref_logprob, weights, *numbers)
+        return _capi.host.policy_loss(logits, actions, old_logprob, advantages, ref_logprob, weights, *numbers, grad_in_forward)
     return _update_ops.policy_loss(logits, actions, old_logprob, advantages, ref_logprob, weights, *numbers)[:3]

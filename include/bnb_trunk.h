@@ -651,7 +651,9 @@ int bnb_linear_bwd(const BnbLinear* call, const BnbLinearGrads* grads, void* scr
  *   old_logprob, advantages (rows); ref_logprob (rows) or NULL: k is 0
  *   weights (rows) float32, or mask (rows) bytes, or neither: 1.  Rows of weight 0 are not looked at: logprob is 0, their gradient too
  *   loss (1); stats (4): means of surrogate, k, H and of whether the ratio is beyond its clipping; logprob (rows)
- *   kept: bnb_policy_loss_kept_bytes bytes that the backward reads; scratch 16-byte aligned */
+ *   kept: bnb_policy_loss_kept_bytes bytes that the backward reads; scratch 16-byte aligned
+ *   dlogits: NULL, or, where bnb_policy_loss_takes_gradients says 1, the gradient for dloss = 1 as bnb_policy_loss_bwd writes it, in the
+ *     same pass over the logits (slices of more than 64 actions, float32 or bfloat16: in float16 a gradient that is not scaled underflows) */
 #define BNB_MAX_SLICES 16
 typedef struct {
   int64_t rows;
@@ -670,14 +672,17 @@ typedef struct {
   float* stats;
   float* logprob;
   float* kept;
+  void* dlogits;
 } BnbPolicyLoss;
+int bnb_policy_loss_takes_gradients(const BnbPolicyLoss* call);
 size_t bnb_policy_loss_kept_bytes(const BnbPolicyLoss* call);
 size_t bnb_policy_loss_scratch_bytes(const BnbPolicyLoss* call);
 int bnb_policy_loss_fwd(const BnbPolicyLoss* call, void* scratch, size_t scratch_bytes, void* stream);
 
 /* dlogits (rows, sum of sizes), contiguous, of the logits' type, for the loss's gradient dloss (1, on the device).  The call's `kept`
- * as the forward left it; its loss, stats and logprob are not read. */
-int bnb_policy_loss_bwd(const BnbPolicyLoss* call, const float* dloss, void* dlogits, void* stream);
+ * as the forward left it; its loss, stats, logprob and dlogits are not read.  holds_unit: dlogits already has the gradient for dloss = 1, from
+ * that forward, and where dloss is 1 it is left as it is. */
+int bnb_policy_loss_bwd(const BnbPolicyLoss* call, const float* dloss, void* dlogits, int holds_unit, void* stream);
 
 /* One AdamW step over many tensors at once.
  *

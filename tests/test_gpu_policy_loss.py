@@ -304,3 +304,33 @@ def test_streams_and_hooks():
     assert torch.equal(torch.autograd.grad(loss, [x])[0], want)
     loss = torch.utils.checkpoint.checkpoint(lambda v: bnb.policy_loss(v, a, old, adv)[0], x, use_reentrant=False)
     assert torch.equal(torch.autograd.grad(loss, [x])[0], want)
+
+
+def test_gradients_of_one_graph_again_and_again():
+    """The first backward may hand out what the forward wrote; later ones, other factors and changed gradients do not see each other."""
+    import boost_and_broadside_b200 as bnb
+
+    for dtype, V in ((F32, 3001), (BF16, 2048), (F16, 2048), (BF16, 300)):
+        z, acts, old, adv, ref = (t.to(DEV) for t in _inputs(20, [V], dtype))
+        a, w = acts[:, 0].contiguous(), (torch.arange(20, device=DEV) % 3 + 0.5)
+        kw = dict(ref_logprob=ref, kl_coef=0.1, entropy_coef=0.01, weights=w)
+        x = z.clone().requires_grad_(True)
+        grad = lambda loss, by: torch.autograd.grad(loss, [x], torch.tensor(by, device=DEV), retain_graph=True)[0]  # noqa: E731
+        fresh = {by: grad(bnb.policy_loss(x, a, old, adv, **kw)[0], by).clone() for by in (1.0, 2.0, 0.0)}
+        assert not fresh[0.0].any() and (dtype == F16 or torch.equal(fresh[1.0] * 2, fresh[2.0]))     # float16: numbers below its normal ones
+        for by in (1.0, 2.0):
+            assert torch.equal(grad(bnb.policy_loss(x, a, old, adv, grad_in_forward=False, **kw)[0], by), fresh[by])
+        loss = bnb.policy_loss(x, a, old, adv, **kw)[0]
+        for by in (1.0, 2.0, 1.0, 0.0, 1.0):
+            got = grad(loss, by)
+            assert torch.equal(got, fresh[by])
+            got.add_(7)                                        # what was handed out is the caller's
+        out = bnb.policy_loss(x, a, old, adv, **kw)
+        (out[0] * 0.5 + bnb.policy_loss(x, a, old, adv, **kw)[0] * 0.5).backward()
+        both = x.grad
+        assert torch.allclose(both.float(), fresh[1.0].float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-7)
+        y = bnb.policy_loss(x, a, old, adv, **kw)[0]
+        with torch.no_grad():
+            x.add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad(y, [x])

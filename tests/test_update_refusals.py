@@ -31,7 +31,7 @@ def test_policy_loss_has_no_cpu_path_and_checks_its_numbers():
 class Policy(C.Structure):
     _fields_ = [("rows", C.c_int64), ("element", C.c_int32), ("n_slices", C.c_int32), ("sizes", C.c_int32 * 16), ("logits", C.c_void_p),
                 ("logits_row", C.c_int64)] + [(n, C.c_void_p) for n in ("actions", "old", "adv", "ref", "weights", "mask")] + [
-                    (n, C.c_float) for n in ("low", "high", "kl", "entropy")] + [(n, C.c_void_p) for n in ("loss", "stats", "logprob", "kept")]
+                    (n, C.c_float) for n in ("low", "high", "kl", "entropy")] + [(n, C.c_void_p) for n in ("loss", "stats", "logprob", "kept", "dlogits")]
 
 
 def test_policy_entry_points_check_their_arguments():
@@ -54,7 +54,12 @@ def test_policy_entry_points_check_their_arguments():
     for name in ("logits", "actions", "old", "adv", "loss", "stats", "logprob", "kept"):
         assert fwd(**{name: None}) == 1, name
     assert lib.bnb_policy_loss_fwd(None, None, 0, None) == 1
-    bwd = lambda dloss, out, **over: lib.bnb_policy_loss_bwd(C.byref(call(**over)), dloss, out, None)  # noqa: E731
+    assert fwd(scratch=fake, bytes_=1 << 20, dlogits=fake) == 5                                   # narrow slices: no gradients in a forward
+    wide = (C.c_int32 * 16)(300, 2, 900)
+    takes = lambda **over: lib.bnb_policy_loss_takes_gradients(C.byref(call(**over)))  # noqa: E731
+    assert [takes(sizes=wide, element=e) for e in (0, 1, 2)] == [1, 1, 0] and takes() == 0 and takes(n_slices=0) == 0
+    assert fwd(scratch=fake, bytes_=1 << 20, dlogits=fake + 8, sizes=wide) == 2 and fwd(scratch=fake, bytes_=1 << 20, dlogits=fake, sizes=wide, element=2) == 5
+    bwd = lambda dloss, out, **over: lib.bnb_policy_loss_bwd(C.byref(call(**over)), dloss, out, 0, None)  # noqa: E731
     assert bwd(None, fake) == 1 and bwd(fake, None) == 1 and bwd(fake, fake + 2) == 2 and bwd(fake, fake, n_slices=99) == 3
     assert bwd(None, None, rows=0, logits=None) == 0
     assert lib.bnb_policy_loss_kept_bytes(C.byref(call())) == 4 * (4 + 100 * 7)
