@@ -31,6 +31,106 @@ int check(const BnbLinear* c) {
 bool recomputes(const BnbLinear& c) { return c.activation == BNB_ACT_NONE || (c.element != BNB_ELEM_F32 && c.width <= 512); }
 bool keeps(const BnbLinear& c) { return !recomputes(c); }
 
+// ------------------------------------------------------------------ few rows
+
+// A single token's layer reads its weight once and computes next to nothing: memory bounds it, and tiles of 128 rows of which one is
+// there keep too few loads on their way (1 x 4096 x 4096 bfloat16: 13.0 us with tiles and a cut depth).  Here a CTA takes NB outputs, its threads the depth in pieces of
+// 16 bytes; sums are float32, of a thread's pieces, then of a warp's lanes, then of the warps, in this order.  Float32 weights of a 16-bit
+// call are rounded to its type on the way, as the tiles' copies are.
+constexpr int FEW_THREADS = 256;
+struct FewRows {
+  const void* x;
+  const void* weight;
+  int64_t x_row;
+  int rows, width, out, x_wide;
+  Epilogue e;
+};
+template <typename T, typename E>   // eight values, of E or of float
+__device__ __forceinline__ void eight(const T* at, F2 (&f)[4]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(at);
+    f[0] = pair_up(raw.x, T{}), f[1] = pair_up(raw.y, T{}), f[2] = pair_up(raw.z, T{}), f[3] = pair_up(raw.w, T{});
+  } else {
+    const float4 a = reinterpret_cast<const float4*>(at)[0], b = reinterpret_cast<const float4*>(at)[1];
+    f[0] = f2(a.x, a.y), f[1] = f2(a.z, a.w), f[2] = f2(b.x, b.y), f[3] = f2(b.z, b.w);
+    if constexpr (!std::is_same<E, float>::value)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = pair_up(pair_of<E>(f[i]), E{});
+  }
+}
+template <typename E, typename W, int M, int NB>
+__global__ void __launch_bounds__(FEW_THREADS) k_few_rows(const __grid_constant__ FewRows p) {
+  __shared__ float sums[FEW_THREADS / 32][M * NB];
+  let_next_start();
+  wait_for_previous();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n0 = blockIdx.x * NB, pieces = p.width / 8;
+  const E* x = static_cast<const E*>(p.x);
+  const W* w = static_cast<const W*>(p.weight);
+  F2 acc[M][NB];
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[m][n] = f2(0.f);
+#pragma unroll 2
+  for (int i = threadIdx.x; i < pieces; i += FEW_THREADS) {
+    F2 ws[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) eight<W, E>(w + (int64_t)min(n0 + n, p.out - 1) * p.width + i * 8, ws[n]);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const E* row = x + (int64_t)min(m, p.rows - 1) * p.x_row + i * 8;
+      F2 xs[4];
+      if (p.x_wide) {
+        eight<E, E>(row, xs);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (sizeof(E) == 4) xs[k] = f2(row[2 * k], row[2 * k + 1]);
+          else xs[k] = f2(up(row[2 * k]), up(row[2 * k + 1]));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[m][n] = fma(xs[k], ws[n][k], acc[m][n]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const float2 s = halves(acc[m][n]);
+      float v = s.x + s.y;
+#pragma unroll
+      for (int by = 16; by; by >>= 1) v += __shfl_xor_sync(0xffffffffu, v, by);
+      if (lane == 0) sums[warp][m * NB + n] = v;
+    }
+  __syncthreads();
+  const int m = threadIdx.x / NB, c = n0 + threadIdx.x % NB;
+  if (threadIdx.x >= M * NB || m >= p.rows || c >= p.out) return;
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < FEW_THREADS / 32; ++i) v += sums[i][threadIdx.x];
+  put_linear<E>(p.e, m, c, v);
+}
+
+// Whether a call goes there: pieces of 16 bytes everywhere in the weight, depth enough for the threads, and no more rows than pay.  4096 x 4096, us:
+// bfloat16 1 row 9.1, 4 rows 11.8, 8 rows 27.9 (tiles: 13); float32 1 row 14.5, 8 rows 40 (tiles: 62).
+bool few_rows(const BnbLinear& c) {
+  return c.rows <= (c.element == BNB_ELEM_F32 ? 8 : 4) && c.width >= 1024 && c.width % 8 == 0 && reinterpret_cast<uintptr_t>(c.weight) % 16 == 0;
+}
+template <typename E, typename W>
+int few(const FewRows& p, cudaStream_t st) {
+  auto with = [&](auto kernel, int nb) { return launch_after(kernel, dim3((unsigned)((p.out + nb - 1) / nb)), FEW_THREADS, 0, st, p); };
+  if (p.rows == 1) return with(k_few_rows<E, W, 1, 4>, 4);
+  if (p.rows == 2) return with(k_few_rows<E, W, 2, 4>, 4);
+  if constexpr (sizeof(E) == 4)
+    if (p.rows > 4) return with(k_few_rows<E, W, 8, 2>, 2);
+  return with(k_few_rows<E, W, 4, 4>, 4);
+}
+
+// ------------------------------------------------------------------ slopes and sums
+
 // dz from the kept z.  A warp takes blocks of 32 x 32: z as it was kept, a row a lane, dy and dz as whole pieces of rows through shared memory (a
 // lane's own row straight from memory is 32 lines a request).
 template <typename E, int PIECES>
@@ -194,22 +294,32 @@ struct Layout {
   }
 };
 
-template <typename E, int PIECES>
-int forward(const BnbLinear& c, const Layout& l, cudaStream_t st) {
-  if (const int r = pack<E, PIECES>(l.jobs, l.n_jobs, st)) return r;
+Epilogue ends_of(const BnbLinear& c) {
+  const bool floats = c.element == BNB_ELEM_F32;
   Epilogue e{};
   e.out[0] = c.y;
-  e.ld_out = l.N;
-  e.out_kind = PIECES > 1 ? 0 : 1;
-  e.ld_h = l.ld;
+  e.ld_out = c.out;
+  e.out_kind = floats ? 0 : 1;
+  e.ld_h = round8(c.out);
   e.g = keeps(c) ? static_cast<float*>(c.kept) : nullptr;
   e.activation = c.activation;
   e.bias = c.bias;
   e.bias_kind = c.bias_element == BNB_ELEM_F32 ? 0 : 1;
   e.other = c.residual;
   e.ld_other = c.residual_row;
-  e.other_wide = reinterpret_cast<uintptr_t>(c.residual) % 16 == 0 && c.residual_row % (PIECES > 1 ? 4 : 8) == 0;
-  return multiply<E, PIECES, false, false, Out::LINEAR>({{l.x, {}}, {l.w, {}}, 1}, l.M, l.N, l.K, 1, e, l.part, st);
+  e.other_wide = reinterpret_cast<uintptr_t>(c.residual) % 16 == 0 && c.residual_row % (floats ? 4 : 8) == 0;
+  return e;
+}
+template <typename E, int PIECES>
+int forward(const BnbLinear& c, const Layout& l, cudaStream_t st) {
+  if (const int r = pack<E, PIECES>(l.jobs, l.n_jobs, st)) return r;
+  return multiply<E, PIECES, false, false, Out::LINEAR>({{l.x, {}}, {l.w, {}}, 1}, l.M, l.N, l.K, 1, ends_of(c), l.part, st);
+}
+template <typename E>
+int forward_few(const BnbLinear& c, cudaStream_t st) {
+  const int per = sizeof(E) == 4 ? 4 : 8;
+  const FewRows p{c.x, c.weight, c.x_row, (int)c.rows, c.width, c.out, reinterpret_cast<uintptr_t>(c.x) % 16 == 0 && c.x_row % per == 0, ends_of(c)};
+  return c.weight_element == BNB_ELEM_F32 ? few<E, float>(p, st) : few<E, E>(p, st);
 }
 
 template <typename E, int PIECES>
@@ -272,7 +382,7 @@ extern "C" size_t bnb_linear_kept_bytes(const BnbLinear* c) {
 }
 
 extern "C" size_t bnb_linear_scratch_bytes(const BnbLinear* c, int backward) {
-  if (check(c) || c->rows == 0) return 0;
+  if (check(c) || c->rows == 0 || (!backward && few_rows(*c))) return 0;
   // a dy that may have to be copied counts as copied: its address is not known yet
   return Layout(*c, reinterpret_cast<const void*>(1), c->out, backward != 0, nullptr).total;
 }
@@ -282,9 +392,10 @@ extern "C" int bnb_linear_fwd(const BnbLinear* c, void* scratch, size_t scratch_
   if (c->rows == 0) return BNB_OK;
   if (!c->y) return BNB_ERR_NULL_POINTER;
   if ((reinterpret_cast<uintptr_t>(c->y) | reinterpret_cast<uintptr_t>(c->kept) | reinterpret_cast<uintptr_t>(scratch)) & 15) return BNB_ERR_MISALIGNED;
+  const auto s = static_cast<cudaStream_t>(stream);
+  if (few_rows(*c)) return c->element == BNB_ELEM_F32 ? forward_few<float>(*c, s) : c->element == BNB_ELEM_BF16 ? forward_few<__nv_bfloat16>(*c, s) : forward_few<__half>(*c, s);
   const Layout l(*c, nullptr, 0, false, static_cast<uint8_t*>(scratch));
   if (!scratch || scratch_bytes < l.total) return BNB_ERR_SCRATCH_TOO_SMALL;
-  const auto s = static_cast<cudaStream_t>(stream);
   return c->element == BNB_ELEM_F32 ? forward<__nv_bfloat16, 3>(*c, l, s)
        : c->element == BNB_ELEM_BF16 ? forward<__nv_bfloat16, 1>(*c, l, s) : forward<__half, 1>(*c, l, s);
 }

@@ -79,7 +79,22 @@ __global__ void __launch_bounds__(256) k_add_parts(const float* part, int splits
   else down(static_cast<E*>(out)[at], v);
 }
 
-// The same for a linear layer: bias, activation and residual behind the sum.
+// A linear layer's result from its sum: bias, activation and residual.  E: the call's type, float among them.
+template <typename E>
+__device__ __forceinline__ void put_linear(const Epilogue& e, int64_t r, int c, float v) {
+  auto value = [](const void* from, int64_t at) {
+    if constexpr (sizeof(E) == 4) return static_cast<const float*>(from)[at];
+    else return up(static_cast<const E*>(from)[at]);
+  };
+  if (e.bias) v += e.bias_kind == 0 ? static_cast<const float*>(e.bias)[c] : value(e.bias, c);
+  if (e.g) e.g[kept_index(r, c, e.ld_h)] = v;
+  float da;
+  if (e.activation != BNB_ACT_NONE) activate_exact(e.activation, v, v, da);
+  if (e.other) v += value(e.other, r * e.ld_other + c);
+  down(static_cast<E*>(e.out[0])[r * e.ld_out + c], v);
+}
+
+// The same for a linear layer.
 template <typename E>
 __global__ void __launch_bounds__(256) k_add_linear(const __grid_constant__ Epilogue e, const float* part, int splits, int64_t m, int n) {
   __shared__ float sums[4][64];
@@ -98,13 +113,8 @@ __global__ void __launch_bounds__(256) k_add_linear(const __grid_constant__ Epil
   v = (v + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
   const int64_t r = i / n;
   const int c = (int)(i - r * n);
-  if (e.bias) v += e.bias_kind == 0 ? static_cast<const float*>(e.bias)[c] : up(static_cast<const E*>(e.bias)[c]);
-  if (e.g) e.g[kept_index(r, c, e.ld_h)] = v;
-  float da;
-  if (e.activation != BNB_ACT_NONE) activate_exact(e.activation, v, v, da);
-  const int64_t at = r * e.ld_out + c, other = r * e.ld_other + c;
-  if (e.out_kind == 0) static_cast<float*>(e.out[0])[at] = e.other ? v + static_cast<const float*>(e.other)[other] : v;
-  else down(static_cast<E*>(e.out[0])[at], e.other ? v + up(static_cast<const E*>(e.other)[other]) : v);
+  if (e.out_kind == 0) put_linear<float>(e, r, c, v);
+  else put_linear<E>(e, r, c, v);
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

@@ -70,6 +70,11 @@ CASES = [
     (1, 4100, 33, F32, False, True, "silu", False),
     (20000, 24, 48, BF16, False, False, "silu", True),       # more tiles than SMs
     (3000, 1030, 520, F16, False, False, "gelu", True),
+    (1, 1024, 7, F32, False, False, "gelu", True),           # few rows
+    (2, 1032, 5, F16, False, True, None, True),
+    (4, 2048, 33, BF16, True, True, "silu", False),
+    (7, 3080, 50, F32, False, None, "silu", False),
+    (8, 1536, 41, BF16, False, False, "gelu", True),
 ]
 
 
@@ -135,6 +140,24 @@ def test_layouts_and_empty_batches(dtype):
         assert y.shape == (0, 4, N)
         grads = torch.autograd.grad(y, [none, w, b], torch.zeros_like(y))
         assert grads[0].shape == none.shape and not any(v.any() for v in grads[1:])
+
+
+def test_few_rows_of_a_wider_tensor():
+    """Rows off every boundary, an expanded one, and weights off theirs, are the same numbers."""
+    import boost_and_broadside_b200 as bnb
+
+    g = torch.Generator().manual_seed(8)
+    for dtype in (BF16, F32):
+        big = torch.randn(3, 1024 + 11, generator=g).to(dtype).to(DEV)
+        w = torch.randn(20 * 1024 + 8, generator=g).to(dtype).to(DEV)
+        x, r = big[:, 5:1029], torch.randn(3, 31, generator=g).to(dtype).to(DEV)[:, 7:27]
+        y = bnb.linear(x, w[:20480].view(20, 1024), activation="silu", residual=r)
+        assert torch.equal(y, bnb.linear(x.contiguous(), w[:20480].view(20, 1024), activation="silu", residual=r.contiguous()))
+        off = torch.cat([w[:1], w[:20480]])[1:].view(20, 1024)                # not on 16 bytes: tiles
+        assert torch.allclose(bnb.linear(x, off, activation="silu", residual=r).float(), y.float(), rtol=torch.finfo(dtype).eps, atol=1e-3 if dtype == F32 else 1e-2)
+        one = bnb.linear(x[:1].expand(3, 1024), w[:20480].view(20, 1024))
+        assert torch.equal(one[0], one[1]) and torch.equal(one[0], one[2])
+        assert bnb.linear(x[:0], w[:20480].view(20, 1024)).shape == (0, 20)
 
 
 def test_gradient_against_differences():
