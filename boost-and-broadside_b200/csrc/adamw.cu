@@ -2,8 +2,9 @@
 //
 // Memory bounds it: 28 bytes an element of float32 with states of 32 bits, 16 with 8 bits; for the some hundred small tensors of a
 // policy, launches do, so the list of tensors is an argument of the kernel and nothing is copied to the device.  The tensors are cut into chunks of 2048
-// elements; a CTA takes chunks one behind the other, so it looks a tensor up once and then moves on.  A warp takes 256 neighbouring
-// elements, eight a lane, which are a block of 8-bit states: its scales are maxima over the warp.
+// elements, which the CTAs take in turn, so that all of them work in one place of memory at a time: with a range of chunks to each, 8-bit states, whose
+// chunks are 2 KB, took 140 us for 40 M elements instead of 108, runs of two chunks 134.  A warp takes 256 neighbouring elements, eight a lane,
+// which are a block of 8-bit states: its scales are maxima over the warp.
 //
 // Sums of the norm are 64 bits from 8 elements on and are added in a fixed order by every CTA of the step for itself.  The last CTA of a step moves the
 // tensors' counters on, when all have read them.
@@ -26,16 +27,17 @@ constexpr int SMS = 148, THREADS = 256, CHUNK = THREADS * 8, BLOCK = 256;
 constexpr int CTAS = SMS * 8;
 static_assert(CTAS == BNB_GRAD_NORM_PARTS, "a part a CTA");
 
-// Arguments of a kernel end at 32 764 bytes, and a longer list takes longer to launch.
+// Arguments of a kernel end at 32 764 bytes, and a longer list takes longer to launch.  (A copy of it in a CTA's shared memory took the norm of
+// 99 tensors from 5 to 17 us: arguments are read fast only where all lanes read the same.)
 template <int MOST> struct Tensors {
   int n;
   uint32_t chunks;
-  uint32_t first[MOST + 1];   // chunks before each tensor; all of them behind the last
+  uint32_t first[MOST + 2];   // chunks before each tensor; all of them behind the last
   BnbAdamTensor t[MOST];
 };
 constexpr int MANY = 360;
-
-// The tensor of a chunk, by all lanes of a warp: two steps where halving takes nine, each of which waits for memory.
+// The tensor of a CTA's first chunk, by all lanes of a warp: two steps where halving takes nine, each of which waits for memory.  A later chunk's is a few
+// tensors on.
 template <int MOST>
 __device__ __forceinline__ int tensor_of(const Tensors<MOST>& l, uint32_t chunk) {
   constexpr int STRIDE = (MOST + 31) / 32;
@@ -44,6 +46,10 @@ __device__ __forceinline__ int tensor_of(const Tensors<MOST>& l, uint32_t chunk)
   const int i = part * STRIDE + lane;
   const unsigned in = __ballot_sync(0xffffffffu, lane < STRIDE && i < l.n && l.first[min(i, MOST)] <= chunk);
   return part * STRIDE + __popc(in) - 1;
+}
+template <int MOST>
+__device__ __forceinline__ void move_on(const Tensors<MOST>& l, int& i, uint32_t chunk) {
+  while (l.first[i + 1] <= chunk) ++i;
 }
 
 // Eight neighbouring elements from `at` on of `n`; `wide`: all there, on their natural boundary of eight.
@@ -179,11 +185,10 @@ __global__ void __launch_bounds__(THREADS) k_norm(const __grid_constant__ Tensor
   let_next_start();
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t c0 = (uint64_t)l.chunks * blockIdx.x / gridDim.x, c1 = (uint64_t)l.chunks * (blockIdx.x + 1) / gridDim.x;
   double sum = 0;
-  int i = c0 < c1 ? tensor_of(l, c0) : 0;
-  for (uint32_t c = c0; c < c1; ++c) {
-    while (l.first[i + 1] <= c) ++i;
+  int i = blockIdx.x < l.chunks ? tensor_of(l, blockIdx.x) : 0;
+  for (uint32_t c = blockIdx.x; c < l.chunks; c += gridDim.x) {
+    move_on(l, i, c);
     const BnbAdamTensor& t = l.t[i];
     const int64_t at = (int64_t)(c - l.first[i]) * CHUNK + threadIdx.x * 8;
     if (at >= t.n) continue;
@@ -236,8 +241,7 @@ __device__ __forceinline__ bool clipping(const Hyper& h, double (&sums)[THREADS 
 }
 // A tensor's step: the learning rate and the root's factor with their corrections, the key of its random numbers.
 struct Rates { float rate, root; uint32_t key; };
-__device__ __forceinline__ Rates rates_of(const Hyper& h, float lr, const float* step) {
-  const float steps = *step + 1.f;
+__device__ __forceinline__ Rates rates_of(const Hyper& h, float lr, float steps) {
   return {lr / -expm1f(steps * h.log1), 1.f / sqrtf(-expm1f(steps * h.log2_)), h.c.seed * 0x5D2F63B9u + (uint32_t)steps * 0x3C6EF36Bu};
 }
 // Eight elements: m and v come multiplied by their betas; with EIGHT, v goes back as its root.
@@ -286,6 +290,7 @@ struct Piece {
   float m[EIGHT ? 1 : 8], v[EIGHT ? 1 : 8];
   uint2 codes_m, codes_v;
   float scale_m, scale_v;
+  float step;       // the tensor's
   int64_t at;       // of the lane's first element
   int tensor;
 };
@@ -295,24 +300,30 @@ struct Piece {
 // 64 registers 159, two 168).  States of 32 bits are bound by memory, 98 % of the measured copy rate with float32 parameters; 16-bit ones leave fewer bytes
 // on their way, 79 % (two CTAs an SM 69 %; four 89 %, but float32 92 %).
 constexpr int RESIDENT = 3;
-template <int MOST, bool EIGHT>
+// TYPE: all parameters' element, or MIXED.
+constexpr int MIXED = -1;
+template <int MOST, bool EIGHT, int TYPE>
 __global__ void __launch_bounds__(THREADS, RESIDENT) k_step(const __grid_constant__ Tensors<MOST> l, const __grid_constant__ Hyper h) {
   __shared__ double sums[THREADS / 32];
   let_next_start();
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t c0 = (uint64_t)l.chunks * blockIdx.x / gridDim.x, c1 = (uint64_t)l.chunks * (blockIdx.x + 1) / gridDim.x;
-  int i = c0 < c1 ? tensor_of(l, c0) : 0, known = -1;
+  const uint32_t chunks = l.chunks;
+  const float lr = h.c.lr_device ? *h.c.lr_device : h.c.lr, decay = lr * h.c.weight_decay;
+  int known = -1, i = blockIdx.x < chunks ? tensor_of(l, blockIdx.x) : 0;
+  auto element = [](const BnbAdamTensor& t) { return TYPE == MIXED ? t.element : TYPE; };
   auto fetch = [&](uint32_t c, Piece<EIGHT>& x) {
-    while (l.first[i + 1] <= c) ++i;
+    if (c >= chunks) return;
+    move_on(l, i, c);
     const BnbAdamTensor& t = l.t[i];
     const int64_t start = (int64_t)(c - l.first[i]) * CHUNK + warp * BLOCK, at = start + lane * 8;
     x.at = at;
     x.tensor = i;
     if (start >= t.n) return;   // the warp's
+    x.step = *t.step;
     const bool whole = at + 8 <= t.n;
-    take_any(t.element, t.p, at, t.n, whole && values_lie_well(t.element, t.p), x.p);
-    take_any(t.element, t.g, at, t.n, whole && values_lie_well(t.element, t.g), x.g);
+    take_any(element(t), t.p, at, t.n, whole && values_lie_well(element(t), t.p), x.p);
+    take_any(element(t), t.g, at, t.n, whole && values_lie_well(element(t), t.g), x.g);
     if constexpr (EIGHT) {
       x.codes_m = take_codes(static_cast<const uint8_t*>(t.m), at, t.n, whole && on(t.m, 8));
       x.codes_v = take_codes(static_cast<const uint8_t*>(t.v), at, t.n, whole && on(t.v, 8));
@@ -324,21 +335,20 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_step(const __grid_constan
     }
   };
   Piece<EIGHT> x;
-  if (c0 < c1) fetch(c0, x);
-  const float lr = h.c.lr_device ? *h.c.lr_device : h.c.lr, decay = lr * h.c.weight_decay;
+  fetch(blockIdx.x, x);
   float clip;
   if (!clipping(h, sums, clip)) return;   // while the first loads are on their way; all CTAs do: nobody counts
   Rates k{};
-  for (uint32_t c = c0; c < c1; ++c) {
+  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
     const BnbAdamTensor& t = l.t[x.tensor];
     const int64_t at = x.at, start = at - lane * 8;
     if (start >= t.n) {   // the warp's
-      if (c + 1 < c1) fetch(c + 1, x);
+      fetch(c + gridDim.x, x);
       continue;
     }
     if (known != x.tensor) {
       known = x.tensor;
-      k = rates_of(h, lr, t.step);
+      k = rates_of(h, lr, x.step + 1.f);
     }
     const bool whole = at + 8 <= t.n;
     F2 m[4], v[4];
@@ -354,12 +364,12 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_step(const __grid_constan
       for (int j = 0; j < 4; ++j) m[j] = mul(f2(x.m[2 * j], x.m[2 * j + 1]), f2(h.beta1)), v[j] = mul(f2(x.v[2 * j], x.v[2 * j + 1]), f2(h.beta2));
     }
     update<EIGHT>(h, k, clip, decay, x.g, x.p, m, v);
-    put_any(t.element, t.p, at, t.n, whole && values_lie_well(t.element, t.p), x.p);
+    put_any(element(t), t.p, at, t.n, whole && values_lie_well(element(t), t.p), x.p);
     float ms[8], vs[8];
     flat(m, ms);
     flat(v, vs);
     if constexpr (EIGHT) {
-      if (c + 1 < c1) fetch(c + 1, x);
+      fetch(c + gridDim.x, x);
       float most_m = 0.f, most_r = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) k_step(const __grid_constan
     } else {
       put(static_cast<float*>(t.m), at, t.n, whole && on(t.m, 32), ms);
       put(static_cast<float*>(t.v), at, t.n, whole && on(t.v, 32), vs);
-      if (c + 1 < c1) fetch(c + 1, x);
+      fetch(c + gridDim.x, x);
     }
   }
   count(l, h.c.control);
@@ -429,7 +439,7 @@ Tensors<MOST> list_of(const BnbAdamTensor* t, int n) {
     l.first[i] = l.chunks;
     l.chunks += (uint32_t)((t[i].n + CHUNK - 1) / CHUNK);
   }
-  for (int i = n; i <= MOST; ++i) l.first[i] = l.chunks;
+  for (int i = n; i < MOST + 2; ++i) l.first[i] = l.chunks;
   return l;
 }
 unsigned ctas_of(uint32_t chunks) { return std::max(1u, std::min(chunks, (uint32_t)CTAS)); }
@@ -450,8 +460,15 @@ int norm(const BnbAdamTensor* t, int n, double* parts, bool add, cudaStream_t st
 template <int MOST>
 int step(const BnbAdamTensor* t, int n, const Hyper& h, cudaStream_t st) {
   const Tensors<MOST> l = list_of<MOST>(t, n);
-  return h.c.state_bits == 8 ? launch_after(k_step<MOST, true>, dim3(std::min(ctas_of(l.chunks), (unsigned)(SMS * RESIDENT))), THREADS, 0, st, l, h)
-                             : launch_after(k_step<MOST, false>, dim3(ctas_of(l.chunks)), THREADS, 0, st, l, h);
+  int type = n ? t[0].element : (int)MIXED;
+  for (int i = 1; i < n; ++i) type = t[i].element == type ? type : MIXED;
+  const unsigned all = ctas_of(l.chunks), wave = std::min(all, (unsigned)(SMS * RESIDENT));
+  auto with = [&](auto kernel, unsigned ctas) { return launch_after(kernel, dim3(ctas), THREADS, 0, st, l, h); };
+  if (h.c.state_bits == 8)
+    return type == BNB_ELEM_F32 ? with(k_step<MOST, true, BNB_ELEM_F32>, wave) : type == BNB_ELEM_BF16 ? with(k_step<MOST, true, BNB_ELEM_BF16>, wave)
+         : type == BNB_ELEM_F16 ? with(k_step<MOST, true, BNB_ELEM_F16>, wave) : with(k_step<MOST, true, MIXED>, wave);
+  return type == BNB_ELEM_F32 ? with(k_step<MOST, false, BNB_ELEM_F32>, all) : type == BNB_ELEM_BF16 ? with(k_step<MOST, false, BNB_ELEM_BF16>, all)
+       : type == BNB_ELEM_F16 ? with(k_step<MOST, false, BNB_ELEM_F16>, all) : with(k_step<MOST, false, MIXED>, all);
 }
 
 }  // namespace
