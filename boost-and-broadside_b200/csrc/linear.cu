@@ -284,7 +284,7 @@ struct Layout {
     const int t = pieces > 1 ? 6 : 1, most = pieces > 1 ? MOST<3> : MOST<1>;
     size_t parts = 0;
     if (!backward) {
-      parts = part_bytes(M, N, K, 1, t, most);
+      parts = part_bytes(M, N, K, 1, t, most_of_linear(pieces, (int)((K + BK - 1) / BK)));
     } else {
       dz = c.activation == BNB_ACT_NONE ? operand(dy, M, N, dy_row, c.element) : Operand{take((size_t)pieces * M * ld * 2), M, N, ld, M * ld};
       parts = std::max(part_bytes(M, K, N, 1, t, most), part_bytes(N, K, M, 1, t, most));

@@ -174,10 +174,10 @@ inline Shaped shape_of(int64_t m, int64_t n, int jobs, int steps, int most, int 
 
 template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT>
 int launch(const Product& p, int tiles, cudaStream_t st) {
-  constexpr uint32_t bytes = Shape<BN, OUT>::BYTES;
+  constexpr uint32_t bytes = Shape<BN, OUT, PIECES>::BYTES;
   auto kernel = k_product<E, PIECES, A_MN, B_MN, BN, OUT>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return BNB_ERR_LAUNCH;
-  return launch_after(kernel, dim3(std::min(tiles, SMS)), CTA, bytes, st, p);
+  return launch_after(kernel, dim3(std::min(tiles, SMS)), Crew<PIECES, BN, OUT>::THREADS, bytes, st, p);
 }
 
 // Pieces of a float32 product that are not below 2^-24 of it, smallest first.
@@ -187,6 +187,10 @@ struct Sides { Operand a[2], b[3]; int segments; };   // segments: a[s] b[s]^T a
 
 // Widths of tiles that are built: two sets of accumulators are 512 columns, and float32 adds runs in a third.
 template <int PIECES> constexpr int MOST = PIECES > 1 ? 128 : 256;
+
+// A linear layer's widest tile: narrow ones are bound by their epilogues, which have more warps at 128 columns.  65536 rows x 512 outputs with GELU, us with tiles
+// of 256 and 128 columns: width 128 42.1 and 39.0, 512 50.6 and 49.4; 8192 x 1024 x 4096 75.0 and 79.6.
+inline int most_of_linear(int pieces, int k_steps) { return pieces > 1 || k_steps <= 8 ? 128 : 256; }
 
 template <typename E, int PIECES, bool A_MN, bool B_MN, Out OUT>
 int at_width(const Product& p, int bn, int tiles, cudaStream_t st) {
@@ -214,8 +218,9 @@ int multiply(const Sides& s, int64_t m, int64_t n, int64_t depth, int jobs, cons
   }
   constexpr bool again = OUT == Out::AGAIN;
   constexpr int LEAST = OUT == Out::GATE ? 128 : 64, OF = OUT == Out::GATE ? 2 : 1;
+  const int most = is_linear<OUT> ? most_of_linear(PIECES, p.k_steps) : MOST<PIECES>;
   Shaped z = again ? Shaped{64, (int)((m + BM - 1) / BM * ((n + 63) / 64)), 1, p.k_steps}
-                   : shape_of(m, n, jobs, p.k_steps * p.terms, MOST<PIECES>, LEAST, OF, OUT == Out::VALUES || OUT == Out::LINEAR);
+                   : shape_of(m, n, jobs, p.k_steps * p.terms, most, LEAST, OF, OUT == Out::VALUES || OUT == Out::LINEAR);
   p.splits = z.splits;
   p.split_steps = z.split_steps;
   p.m_tiles = (int)((m + BM - 1) / BM);

@@ -30,7 +30,6 @@ constexpr int BM = 128, BK = 64;              // tile rows; depth of a stage
 constexpr int MAX_TERMS = 12;                 // two segments of six
 constexpr int FLUSH = 4;                      // stages of a run
 constexpr int OUT_WARPS = 16, CTA = 32 * (2 + OUT_WARPS);
-constexpr uint32_t OUT_BYTES = OUT_WARPS * 2048;   // shared memory of the results on their way out
 constexpr uint32_t A_BYTES = BM * BK * 2, SLAB = 64 * BK * 2;   // SLAB: 64 rows or columns by 64
 enum : int { W_FULL = 101, W_EMPTY = 102, W_ACC = 103, W_DRAINED = 104 };
 
@@ -88,8 +87,9 @@ __device__ __forceinline__ Tile tile_of(const Product& p, int i) {
 }
 
 constexpr int MAX_STAGES = 8;
+constexpr int MAX_SETS = 3;
 struct Frame2 {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc[2], drained[2];
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc[MAX_SETS], drained[MAX_SETS];
   alignas(8) int aborted[4];   // see mbar_wait: the last two hold an address
   int status;
   uint32_t tmem;
@@ -187,11 +187,21 @@ __device__ __forceinline__ void put_operand(void* base, int64_t piece_stride, in
 template <typename E> struct Format { static constexpr uint32_t BITS = 0; };
 template <> struct Format<__nv_bfloat16> { static constexpr uint32_t BITS = (1u << 7) | (1u << 10); };
 
-template <int BN, Out OUT>
+// Who takes out: WARPS in GROUPS that take tiles in turn, and as many sets of accumulators at least.  A linear layer's tiles of 128 columns have three of each: its
+// epilogue is most of a narrow layer's time and waits in chains, which more warps fill (see at_width's callers).
+template <int PIECES, int BN, Out OUT>
+struct Crew {
+  static constexpr bool MORE = is_linear<OUT> && PIECES == 1 && BN == 128;
+  static constexpr int WARPS = MORE ? 24 : OUT_WARPS, GROUPS = PIECES > 1 || OUT == Out::BACK ? 1 : MORE ? 3 : 2, SETS = MORE ? 3 : 2, THREADS = 32 * (2 + WARPS);
+};
+
+template <int BN, Out OUT, int PIECES = 1>
 struct Shape {
+  static constexpr int WARPS = Crew<PIECES, BN, OUT>::WARPS;
+  static constexpr uint32_t OUT_BYTES = WARPS * 2048;   // shared memory of the results on their way out
   static constexpr uint32_t B_BYTES = BN * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
   static constexpr int COLS = OUT == Out::GATE ? BN / 2 : OUT == Out::AGAIN ? BN / 3 : BN;   // of the output
-  static constexpr uint32_t BIAS = is_linear<OUT> ? OUT_WARPS * 128 : 0;   // a warp's bias of a segment
+  static constexpr uint32_t BIAS = is_linear<OUT> ? WARPS * 128 : 0;   // a warp's bias of a segment
   static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_BYTES - BIAS) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
   static constexpr uint32_t OUT_AT = STAGES * STAGE, BIAS_AT = OUT_AT + OUT_BYTES, FRAME = BIAS_AT + BIAS, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
 };
@@ -264,10 +274,12 @@ __device__ __forceinline__ F2 pair_up(uint32_t v, __half) {
 // sets of accumulators for one tile, has one group, and so has BACK: it waits for g and u from memory most, and 16 columns a warp leave
 // the registers to have all of a segment's on their way at once (128 us against 113 at 8192 x 1024 x 4096).
 template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT>
-static __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant__ Product p) {
-  using S = Shape<BN, OUT>;
+static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_product(const __grid_constant__ Product p) {
+  using S = Shape<BN, OUT, PIECES>;
+  using C = Crew<PIECES, BN, OUT>;
   constexpr bool EXACT = PIECES > 1;
-  constexpr int GROUPS = EXACT || OUT == Out::BACK ? 1 : 2, PARTS = OUT_WARPS / 4 / GROUPS;
+  constexpr int GROUPS = C::GROUPS, SETS = C::SETS, PARTS = C::WARPS / 4 / GROUPS;
+  static_assert(SETS <= MAX_SETS && SETS * BN <= 512 && (GROUPS == 1 || GROUPS == SETS), "a group's tiles have a set of their own");
   static_assert(!EXACT || 3 * BN <= 512, "two sets of accumulators and their sum");
   constexpr uint32_t SUM = 2 * BN;   // float32: where runs are added
   extern __shared__ uint8_t raw_smem[];
@@ -283,9 +295,9 @@ static __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant
       mbar_init(smem_u32(&f.full[i]), 1);
       mbar_init(smem_u32(&f.empty[i]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < SETS; ++i) {
       mbar_init(smem_u32(&f.acc[i]), 1);
-      mbar_init(smem_u32(&f.drained[i]), OUT_WARPS / GROUPS);
+      mbar_init(smem_u32(&f.drained[i]), C::WARPS / GROUPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -366,8 +378,8 @@ static __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant
       const Tile t = tile_of(p, i);
       const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps);
       for (int s = s0; s < s1; ++done) {
-        const int set = done & 1, end = run_end(s, s1);
-        if (done >= 2) wait(f.drained[set], done / 2 - 1, W_DRAINED);
+        const int set = done % SETS, end = run_end(s, s1);
+        if (done >= SETS) wait(f.drained[set], done / SETS - 1, W_DRAINED);
         tc_fence_after();
         for (uint32_t acc = 0; s < end; ++s, ++step, acc = 1) {
           const int slot = step % S::STAGES;
@@ -400,7 +412,7 @@ static __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant
     // taking out: this warp's 32 rows (a quarter of tensor memory is a warp's by its number) and a part of every 64 columns
     constexpr int SEG = 64 / PARTS;   // columns of a warp among 64
     const int quarter = warp & 3, group = ((warp - 2) >> 2) % GROUPS, part = ((warp - 2) >> 2) / GROUPS;
-    uint8_t* rows = smem + S::OUT_AT + quarter * 8192 + group * 4096;      // of the warps that share rows
+    uint8_t* rows = smem + S::OUT_AT + quarter * (C::WARPS * 512) + group * 4096;      // of the warps that share rows
     uint8_t* stage = smem + S::OUT_AT + (warp - 2) * 2048;                  // of this one
     auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter * GROUPS + group), "n"(32 * PARTS) : "memory"); };
     const Epilogue& e = p.e;
@@ -414,12 +426,12 @@ static __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant
     int done = group, turn = 0;
     for (int i = blockIdx.x + group * gridDim.x; i < tiles; i += GROUPS * gridDim.x) {
       const Tile t = tile_of(p, i);
-      uint32_t acc = lanes + (done & 1) * BN;
+      uint32_t acc = lanes + (done % SETS) * BN;
       if constexpr (EXACT) {
         const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps);
         for (int s = s0; s < s1; ++done) {
-          const int set = done & 1;
-          wait(f.acc[set], done / 2, W_ACC);
+          const int set = done % SETS;
+          wait(f.acc[set], done / SETS, W_ACC);
           tc_fence_after();
           // the columns that this warp takes out below
 #pragma unroll 1
@@ -440,7 +452,7 @@ static __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant
         }
         acc = lanes + SUM;
       }
-      const int set = done & 1;
+      const int set = done % SETS;
       const int64_t row0 = (int64_t)t.m * BM + 32 * quarter;
       // kept g and u: a block of 32 x 32 is eight requests of a float4 a lane, its row's
       auto kept_at = [&](float* base_, int col, int q) {
@@ -450,7 +462,7 @@ static __global__ void __launch_bounds__(CTA, 1) k_product(const __grid_constant
       // A tile's accumulators are waited for once, and given back as soon as the last of them are in registers.
       bool waited = EXACT, released = EXACT;
       auto ready = [&] {
-        if (!waited) wait(f.acc[set], done / 2, W_ACC), waited = true;
+        if (!waited) wait(f.acc[set], done / SETS, W_ACC), waited = true;
         tc_fence_after();
       };
 #pragma unroll 1
