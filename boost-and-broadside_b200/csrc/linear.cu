@@ -6,8 +6,8 @@
 // operations for each of rows x width x out forward and twice that backward: the tensor cores bound it, or, for few rows or a small width, memory.
 //
 // The backward of an activation needs z as it was before any rounding.  Either it is computed once more, with dy taken to dz behind it
-// (Out::SLOPE), or the forward keeps it in float32 (see recomputes).  dz is rounded to the operands' type: it is an operand of the two
-// products behind it, and the bias's gradient is the sum of the same numbers.  Without an activation dz is dy as it lies.
+// (Out::SLOPE), or the forward keeps it in float32 (see recomputes).  dz is rounded to the operands' type, as an operand of the two
+// products behind it; the bias's gradient sums it before that.  Without an activation dz is dy as it lies.
 #include "product_calls.cuh"
 
 namespace bnb {
@@ -131,10 +131,12 @@ int few(const FewRows& p, cudaStream_t st) {
 
 // ------------------------------------------------------------------ slopes and sums
 
-// dz from the kept z.  A warp takes blocks of 32 x 32: z as it was kept, a row a lane, dy and dz as whole pieces of rows through shared memory (a
-// lane's own row straight from memory is 32 lines a request).
+// dz from the kept z.  A warp takes blocks of 32 x 32 of the same columns, eight warps side by side: z as it was kept, a row a lane, dy and dz as whole pieces of rows
+// through shared memory (a lane's own row straight from memory is 32 lines a request).  sums: null, or (gridDim.y, n) sums over the rows before dz
+// is rounded, a lane's rows one behind the other, then the lanes.
 template <typename E, int PIECES>
-__global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, int64_t ld_dy, int wide, int activation, int64_t m, int n, void* dz, int64_t ld, int64_t piece_stride) {
+__global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, int64_t ld_dy, int wide, int activation, int64_t m, int n, void* dz, int64_t ld, int64_t piece_stride,
+                                               float* sums) {
   constexpr bool EXACT = PIECES > 1;
   using T = std::conditional_t<EXACT, float, E>;
   constexpr int N = 16 / sizeof(T), ROW = 32 / N;   // pieces of a block's row: 4, float32 8
@@ -144,11 +146,16 @@ __global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, i
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4* const mine = staged[warp];
   auto spot = [](int r, int q) { return r * ROW + (q ^ ((r / (8 / ROW)) % ROW)); };
-  const int64_t columns = (ld + 31) / 32, blocks = (m + 31) / 32 * columns;
-  for (int64_t b = (int64_t)blockIdx.x * 8 + warp; b < blocks; b += (int64_t)gridDim.x * 8) {
-    const int64_t r0 = b / columns * 32;
-    const int c0 = (int)(b % columns) * 32;
-    const float4* kept = reinterpret_cast<const float4*>(z) + b * 256 + lane;
+  const int64_t columns = (ld + 31) / 32, blocks = (m + 31) / 32;
+  const int64_t column = (int64_t)blockIdx.x * 8 + warp;
+  if (column >= columns) return;
+  const int c0 = (int)column * 32;
+  F2 total[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) total[k] = f2(0.f);
+  for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
+    const int64_t r0 = b * 32;
+    const float4* kept = reinterpret_cast<const float4*>(z) + (b * columns + column) * 256 + lane;
     float4 zs[8];
     uint4 in[ROW];
 #pragma unroll
@@ -162,10 +169,11 @@ __global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, i
 #pragma unroll
     for (int q = 0; q < ROW; ++q) mine[spot(q * (32 / ROW) + lane / ROW, lane % ROW)] = in[q];
     __syncwarp();
+    const bool row = r0 + lane < m;   // nothing was kept behind the last row and column
     F2 v[16];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const bool there[4] = {c0 + 4 * q < n, c0 + 4 * q + 1 < n, c0 + 4 * q + 2 < n, c0 + 4 * q + 3 < n};   // nothing was kept behind the last column
+      const bool there[4] = {row && c0 + 4 * q < n, row && c0 + 4 * q + 1 < n, row && c0 + 4 * q + 2 < n, row && c0 + 4 * q + 3 < n};
       F2 a, d0, d1;
       activate<EXACT, true>(activation, f2(there[0] ? zs[q].x : 0.f, there[1] ? zs[q].y : 0.f), a, d0);
       activate<EXACT, true>(activation, f2(there[2] ? zs[q].z : 0.f, there[3] ? zs[q].w : 0.f), a, d1);
@@ -179,6 +187,8 @@ __global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, i
         v[2 * q + 1] = mul(d1, pair_up(raw.y, E{}));
       }
     }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) total[k] = add(total[k], v[k]);
     // the results: four pieces of a row, whatever dy was
     auto out = [](int r, int q) { return r * 4 + (q ^ ((r / 2) % 4)); };
 #pragma unroll
@@ -202,9 +212,17 @@ __global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, i
       }
     }
   }
+  if (!sums) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const F2 eight[4] = {total[4 * q], total[4 * q + 1], total[4 * q + 2], total[4 * q + 3]};
+    const float s = column_sum(eight, lane);
+    const int c = c0 + 8 * q + lane / 4;
+    if (lane % 4 == 0 && c < n) sums[(int64_t)blockIdx.y * n + c] = s;
+  }
 }
 
-// Sums over rows of operand pieces: 64 columns and a share of the rows a CTA, 32 threads' rows added in a fixed order.
+// Sums over rows of operand pieces (PIECES 0: of float32 rows without padding): 64 columns and a share of the rows a CTA, 32 threads' rows added in a fixed order.
 template <typename E, int PIECES>
 __global__ void __launch_bounds__(256) k_column_sums(const Operand o, float* part, int n) {
   __shared__ float sums[32][65];
@@ -213,7 +231,13 @@ __global__ void __launch_bounds__(256) k_column_sums(const Operand o, float* par
   const int q = threadIdx.x % 8, t = threadIdx.x / 8, col = blockIdx.x * 64 + q * 8;
   const int64_t r0 = o.rows * blockIdx.y / gridDim.y, r1 = o.rows * (blockIdx.y + 1) / gridDim.y;
   float v[8] = {};
-  if (col < o.ld) {
+  if constexpr (PIECES == 0) {
+    const float* from = static_cast<const float*>(o.data) + col;
+    for (int64_t r = r0 + t; r < r1; r += 32)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col + k < n) v[k] += from[r * o.ld + k];
+  } else if (col < o.ld) {
     constexpr int UNROLL = 4;   // rows whose loads are on their way together
     const E* from = static_cast<const E*>(o.data) + col;
     auto add_row = [&](const uint4 (&raw)[PIECES]) {
@@ -254,19 +278,23 @@ __global__ void __launch_bounds__(256) k_column_sums(const Operand o, float* par
 // How many CTAs share the rows: six an SM, no fewer than 128 rows each.
 int row_shares(int64_t rows, int n) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 127) / 128, SMS * 6 / ((n + 63) / 64))); }
 
+// How many CTAs share the row blocks of k_slope: four an SM.
+int slope_shares(int64_t rows, int64_t ld) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 31) / 32, SMS * 4 / ((ld + 255) / 256))); }
+
 // Where everything of a call stands in its scratch; sizes alone with base = null.
 struct Layout {
   int pieces;
   int64_t M, K, N, ld;
   Operand x, w, dz;
   float* part;
-  float* sums;
+  float* sums;     // of a bias's gradient: shares of rows
+  float* blocks;   // of the rows' 32s, where z is computed once more
   PackJobs jobs;
   int n_jobs;
   size_t total;
 
   Layout(const BnbLinear& c, const void* dy, int64_t dy_row, bool backward, uint8_t* base)
-      : pieces(c.element == BNB_ELEM_F32 ? 3 : 1), M(c.rows), K(c.width), N(c.out), ld(round8(c.out)), dz{}, part(nullptr), sums(nullptr), jobs{}, n_jobs(0), total(0) {
+      : pieces(c.element == BNB_ELEM_F32 ? 3 : 1), M(c.rows), K(c.width), N(c.out), ld(round8(c.out)), dz{}, part(nullptr), sums(nullptr), blocks(nullptr), jobs{}, n_jobs(0), total(0) {
     auto take = [&](size_t bytes) {
       uint8_t* at = base ? base + total : nullptr;
       total += round256(bytes);
@@ -288,7 +316,8 @@ struct Layout {
     } else {
       dz = c.activation == BNB_ACT_NONE ? operand(dy, M, N, dy_row, c.element) : Operand{take((size_t)pieces * M * ld * 2), M, N, ld, M * ld};
       parts = std::max(part_bytes(M, K, N, 1, t, most), part_bytes(N, K, M, 1, t, most));
-      sums = reinterpret_cast<float*>(take((size_t)row_shares(M, (int)N) * N * 4));
+      sums = reinterpret_cast<float*>(take((size_t)std::max(row_shares(M, (int)N), slope_shares(M, ld)) * N * 4));
+      if (c.activation != BNB_ACT_NONE && recomputes(c)) blocks = reinterpret_cast<float*>(take((size_t)((M + 31) / 32) * N * 4));
     }
     part = reinterpret_cast<float*>(take(parts));
   }
@@ -325,13 +354,13 @@ int forward_few(const BnbLinear& c, cudaStream_t st) {
 template <typename E, int PIECES>
 int backward(const BnbLinear& c, const BnbLinearGrads& g, const Layout& l, cudaStream_t st) {
   if (const int r = pack<E, PIECES>(l.jobs, l.n_jobs, st)) return r;
-  int r = BNB_OK;
+  int r = BNB_OK, shares = 0;   // of sums that are there already
   if (c.activation != BNB_ACT_NONE) {
     const int wide = reinterpret_cast<uintptr_t>(g.dy) % 16 == 0 && g.dy_row % (PIECES > 1 ? 4 : 8) == 0;
     if (keeps(c)) {
-      const int64_t blocks = (l.M + 31) / 32 * ((l.ld + 31) / 32);
-      r = launch_after(k_slope<E, PIECES>, dim3((unsigned)std::min<int64_t>((blocks + 7) / 8, SMS * 8)), 256, 0, st, static_cast<const float*>(c.kept), g.dy, g.dy_row, wide,
-                       (int)c.activation, l.M, (int)l.N, const_cast<void*>(l.dz.data), l.ld, l.dz.piece_stride);
+      shares = slope_shares(l.M, l.ld);
+      r = launch_after(k_slope<E, PIECES>, dim3((unsigned)((l.ld + 255) / 256), (unsigned)shares), 256, 0, st, static_cast<const float*>(c.kept), g.dy, g.dy_row, wide,
+                       (int)c.activation, l.M, (int)l.N, const_cast<void*>(l.dz.data), l.ld, l.dz.piece_stride, g.dbias ? l.sums : nullptr);
     } else if constexpr (PIECES == 1) {
       Epilogue e{};
       e.h = const_cast<void*>(l.dz.data);
@@ -342,6 +371,7 @@ int backward(const BnbLinear& c, const BnbLinearGrads& g, const Layout& l, cudaS
       e.other = g.dy;
       e.ld_other = g.dy_row;
       e.other_wide = wide;
+      e.part = g.dbias ? l.blocks : nullptr;
       r = multiply<E, PIECES, false, false, Out::SLOPE>({{l.x, {}}, {l.w, {}}, 1}, l.M, l.N, l.K, 1, e, nullptr, st);
     }
   }
@@ -360,8 +390,14 @@ int backward(const BnbLinear& c, const BnbLinearGrads& g, const Layout& l, cudaS
     if (r = multiply<E, PIECES, true, true, Out::VALUES>({{l.dz, {}}, {l.x, {}}, 1}, l.N, l.K, l.M, 1, e, l.part, st); r) return r;
   }
   if (g.dbias) {
-    const int shares = row_shares(l.M, (int)l.N);
-    if (r = launch_after(k_column_sums<E, PIECES>, dim3((unsigned)((l.N + 63) / 64), shares), 256, 0, st, l.dz, l.sums, (int)l.N); r) return r;
+    if (!shares) {
+      const Operand blocks{l.blocks, (l.M + 31) / 32, l.N, l.N, 0};
+      const Operand& from = l.blocks ? blocks : l.dz;
+      shares = row_shares(from.rows, (int)l.N);
+      const dim3 grid((unsigned)((l.N + 63) / 64), (unsigned)shares);
+      r = l.blocks ? launch_after(k_column_sums<E, 0>, grid, 256, 0, st, from, l.sums, (int)l.N) : launch_after(k_column_sums<E, PIECES>, grid, 256, 0, st, from, l.sums, (int)l.N);
+      if (r) return r;
+    }
     count_launch();
     k_add_parts<E><<<(unsigned)((l.N + 63) / 64), 256, 0, st>>>(l.sums, shares, l.N, 1, g.dbias, nullptr, c.bias_element == BNB_ELEM_F32 ? 0 : 1);
     return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;

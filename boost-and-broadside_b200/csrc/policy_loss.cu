@@ -129,11 +129,14 @@ struct RowIn { float w, old, advantage, ref; };
 __device__ __forceinline__ RowIn row_in(const BnbPolicyLoss& c, int64_t r) {
   return {weight_of(c, r), c.old_logprob[r], c.advantages[r], c.ref_logprob ? c.ref_logprob[r] : 0.f};
 }
+// How far a row's log-probability is from the old and the reference policy's: from 64 bits, since a rounding of l is many of a difference's.
+struct Moved { float old, ref; };   // l - old, ref - l
+__device__ __forceinline__ Moved moved(const RowIn& x, double l) { return {(float)(l - x.old), (float)(x.ref - l)}; }
 // A row's terms and the loss's slope in l.
 struct RowTerms { float surrogate, kl, clipped, slope; };
-__device__ __forceinline__ RowTerms row_terms(const BnbPolicyLoss& c, const RowIn& x, float l) {
+__device__ __forceinline__ RowTerms row_terms(const BnbPolicyLoss& c, const RowIn& x, Moved by) {
   RowTerms v;
-  const float a = x.advantage, ratio = expf(l - x.old);
+  const float a = x.advantage, ratio = expf(by.old);
   const float lo = 1.f - c.clip_low, hi = 1.f + c.clip_high, held = ratio < lo ? lo : ratio > hi ? hi : ratio;
   const float free_ = ratio * a, bound = held * a;
   v.surrogate = free_ <= bound ? free_ : bound != bound || free_ == free_ ? bound : free_;   // NaN stays NaN
@@ -141,7 +144,7 @@ __device__ __forceinline__ RowTerms row_terms(const BnbPolicyLoss& c, const RowI
   v.clipped = ratio < lo || ratio > hi ? 1.f : 0.f;
   v.kl = 0.f;
   if (c.ref_logprob) {
-    const float d = x.ref - l, grown = expm1f(d);
+    const float d = by.ref, grown = expm1f(d);
     v.kl = grown - d;
     if (c.kl_coef != 0.f) v.slope = fmaf(-c.kl_coef, grown, v.slope);
   }
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(512) k_narrow(const __grid_constant__ Args a, 
     __syncthreads();
     const int64_t r = r0 + row;
     const float w = row < rows ? weight_of(c, r) : 0.f;
-    float* kept = c.kept + HEAD + r * (2 * S + 1);
+    float* kept = c.kept + HEAD + r * (2 * S + 2);
     if (row < rows && w != 0.f) {
       const float* z = tile + row * pitch + a.first[slice];
       const int n = c.sizes[slice];
@@ -293,17 +296,21 @@ __global__ void __launch_bounds__(512) k_narrow(const __grid_constant__ Args a, 
     }
     __syncthreads();
     if (tid < rows) {
-      float l = 0.f, h = 0.f;
+      double l = 0;
+      float h = 0.f;
       if (w != 0.f) {
         for (int i = 0; i < S; ++i) {
           const float2 v = slice_results[i * tile_rows + tid];
           l += v.x;
           h += v.y;
         }
-        s.add(w, row_terms(c, row_in(c, r), l), h);
-        kept[2 * S] = l;
+        const RowIn in = row_in(c, r);
+        const Moved by = moved(in, l);
+        s.add(w, row_terms(c, in, by), h);
+        kept[2 * S] = by.old;
+        kept[2 * S + 1] = by.ref;
       }
-      c.logprob[r] = l;
+      c.logprob[r] = (float)l;
     }
   }
 #pragma unroll
@@ -423,8 +430,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_wide(const __grid_c
     const bool there = r < c.rows, on = there && in.w != 0.f;   // of all threads of a row
     const E* row = static_cast<const E*>(c.logits) + (there ? r : 0) * c.logits_row;
     E* const to = static_cast<E*>(a.dlogits) + (there ? r : 0) * a.width;
-    float* kept = c.kept + HEAD + r * (2 * S + 1);
-    float l = 0.f, h = 0.f, lse = 0.f, hs = 0.f;
+    float* kept = c.kept + HEAD + r * (2 * S + 2);
+    double l = 0;
+    float h = 0.f, lse = 0.f, hs = 0.f;
     Raw<E, N> held[HELD > 0 ? HELD : 1];
     for (int s = 0; s < S; ++s) {
       const E* z = row + a.first[s];
@@ -482,15 +490,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_wide(const __grid_c
       }
     }
     RowTerms terms{};
-    if (on && (GRAD || t == 0)) terms = row_terms(c, in, l);
+    const Moved by = moved(in, l);
+    if (on && (GRAD || t == 0)) terms = row_terms(c, in, by);
     if (t == 0 && there) {
       if (on) {
         Sums sum = *reinterpret_cast<const Sums*>(sums[group]);   // its row's, in shared memory: no other thread needs the registers
         sum.add(in.w, terms, h);
         *reinterpret_cast<Sums*>(sums[group]) = sum;
-        kept[2 * S] = l;
+        kept[2 * S] = by.old;
+        kept[2 * S + 1] = by.ref;
       }
-      c.logprob[r] = on ? l : 0.f;
+      c.logprob[r] = on ? (float)l : 0.f;
     }
     if constexpr (GRAD) {
       const Slope k = slope_of(c, in.w * per_row, terms);
@@ -530,8 +540,8 @@ __global__ void __launch_bounds__(256) k_narrow_bwd(const __grid_constant__ Args
       for (int j = 0; j < n; ++j) to[j] = from_f<E>(0.f);
       continue;
     }
-    const float* kept = c.kept + HEAD + r * (2 * S + 1);
-    const Slope k = slope_of(c, a.dloss[0] * (w * c.kept[0]), row_terms(c, row_in(c, r), kept[2 * S]));
+    const float* kept = c.kept + HEAD + r * (2 * S + 2);
+    const Slope k = slope_of(c, a.dloss[0] * (w * c.kept[0]), row_terms(c, row_in(c, r), {kept[2 * S], kept[2 * S + 1]}));
     const float lse = kept[2 * s], c1 = fmaf(k.c2, kept[2 * s + 1], -k.dl);
     const int at = action_of(c, r, s);
     const E* z = static_cast<const E*>(c.logits) + r * c.logits_row + a.first[s];
@@ -551,8 +561,8 @@ __global__ void __launch_bounds__(THREADS) k_wide_bwd(const __grid_constant__ Ar
   for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / T; r < c.rows; r += (int64_t)gridDim.x * ROWS) {
     const float w = weight_of(c, r);
     const bool on = w != 0.f;
-    const float* kept = c.kept + HEAD + r * (2 * S + 1);
-    const Slope k = on ? slope_of(c, dloss * (w * c.kept[0]), row_terms(c, row_in(c, r), kept[2 * S])) : Slope{0.f, 0.f};
+    const float* kept = c.kept + HEAD + r * (2 * S + 2);
+    const Slope k = on ? slope_of(c, dloss * (w * c.kept[0]), row_terms(c, row_in(c, r), {kept[2 * S], kept[2 * S + 1]})) : Slope{0.f, 0.f};
     for (int s = 0; s < S; ++s)
       put_gradients<E, T, 0>(static_cast<const E*>(c.logits) + r * c.logits_row + a.first[s], static_cast<E*>(a.dlogits) + r * a.width + a.first[s], c.sizes[s], t, on,
                              on ? action_of(c, r, s) : -1, on ? kept[2 * s] : 0.f, on ? kept[2 * s + 1] : 0.f, k, nullptr);
@@ -651,7 +661,7 @@ using namespace bnb::policy;
 
 extern "C" size_t bnb_policy_loss_kept_bytes(const BnbPolicyLoss* c) {
   if (!c || c->n_slices < 1 || c->n_slices > BNB_MAX_SLICES || c->rows < 0) return 0;
-  return (HEAD + (size_t)c->rows * (2 * c->n_slices + 1)) * 4;
+  return (HEAD + (size_t)c->rows * (2 * c->n_slices + 2)) * 4;
 }
 
 extern "C" size_t bnb_policy_loss_scratch_bytes(const BnbPolicyLoss* c) { return c ? (size_t)(MAX_CTAS * TERMS + SMS) * sizeof(double) : 0; }

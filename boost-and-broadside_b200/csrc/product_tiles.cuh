@@ -40,13 +40,13 @@ enum : int { W_FULL = 101, W_EMPTY = 102, W_ACC = 103, W_DRAINED = 104 };
 //   BACK     columns are dh: dg = dh u act'(g), du = dh act(g), h = act(g) u as operand pieces, from the kept g and u
 //   AGAIN    the same with g and u computed once more: a stage holds x and dy, and 64 columns of all three weights
 //   LINEAR   z = sum + bias, out[0] = act(z) + other (m, n); z itself where it is kept
-//   SLOPE    the same z: other act'(z) as operand pieces (16 bits)
+//   SLOPE    the same z: other act'(z) as operand pieces (16 bits), and its sums over 32 rows before it is rounded
 enum class Out : int { VALUES, PARTIAL, GATE, BACK, AGAIN, LINEAR, SLOPE };
 template <Out OUT> constexpr bool is_linear = OUT == Out::LINEAR || OUT == Out::SLOPE;
 
 struct Epilogue {
   void* out[2];
-  float* part;
+  float* part;          // SLOPE: sums (m / 32, n), or null
   void* h;              // operand pieces (pieces, m, ld_h)
   void* dg;
   void* du;
@@ -267,6 +267,21 @@ __device__ __forceinline__ F2 pair_up(uint32_t v, __nv_bfloat16) { return unpack
 __device__ __forceinline__ F2 pair_up(uint32_t v, __half) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
   return f2(f.x, f.y);
+}
+
+// Sums over a warp of eight columns, of which every lane has a row: lane 4 c has column c's.  Lanes give away half of their columns a step while there are
+// several: nine shuffles where one column after the other takes forty.
+__device__ __forceinline__ float column_sum(const F2 (&v)[4], int lane) {
+  auto swap = [](F2 x, int by) {
+    const float2 f = halves(x);
+    return f2(__shfl_xor_sync(0xffffffffu, f.x, by), __shfl_xor_sync(0xffffffffu, f.y, by));
+  };
+  const bool b16 = lane & 16, b8 = lane & 8, b4 = lane & 4;
+  const F2 p = add(b16 ? v[2] : v[0], swap(b16 ? v[0] : v[2], 16)), q = add(b16 ? v[3] : v[1], swap(b16 ? v[1] : v[3], 16));   // columns 4-7 or 0-3
+  const float2 r = halves(add(b8 ? q : p, swap(b8 ? p : q, 8)));
+  float s = (b4 ? r.y : r.x) + __shfl_xor_sync(0xffffffffu, b4 ? r.x : r.y, 4);
+  s += __shfl_xor_sync(0xffffffffu, s, 2);
+  return s + __shfl_xor_sync(0xffffffffu, s, 1);
 }
 
 // Sixteen warps take out in two groups, tiles in turn: while one group waits for accumulators, for its rows or for memory, the other
@@ -615,8 +630,18 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
               for (int k = 0; k < 4; ++k) activate<false, OUT == Out::SLOPE>(e.activation, v[k], a[k], da[k]);
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) bits[k] = pair_of<E>(OUT == Out::SLOPE ? mul(pair_up(o[k], E{}), da[k]) : e.other ? add(a[k], pair_up(o[k], E{})) : a[k]);
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (OUT == Out::SLOPE) a[k] = mul(pair_up(o[k], E{}), da[k]);
+              else if (e.other) a[k] = add(a[k], pair_up(o[k], E{}));
+              bits[k] = pair_of<E>(a[k]);
+            }
             *at = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+            if constexpr (OUT == Out::SLOPE) {
+              if (e.part && row0 < p.m) {
+                const float s = column_sum(a, lane);
+                if (lane % 4 == 0 && col0 + k0 + lane / 4 < p.n) e.part[(row0 >> 5) * p.n + col0 + k0 + lane / 4] = s;
+              }
+            }
           }
           meet();
           E* to = static_cast<E*>(OUT == Out::SLOPE ? e.h : e.out[0]);

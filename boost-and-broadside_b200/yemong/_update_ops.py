@@ -84,7 +84,7 @@ def _(logits, actions, old_logprob, advantages, ref_logprob, weights, sizes, cli
     rows = logits.numel() // logits.shape[-1]
     f = {"dtype": torch.float32}
     return (logits.new_empty((), **f), logits.new_empty(logits.shape[:-1], **f), logits.new_empty(4, **f),
-            logits.new_empty(4 + rows * (2 * max(1, len(sizes)) + 1), **f))
+            logits.new_empty(4 + rows * (2 * max(1, len(sizes)) + 2), **f))
 
 
 @torch.library.custom_op("bnb_b200::policy_loss_backward", mutates_args=(), device_types="cuda")

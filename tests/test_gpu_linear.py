@@ -43,9 +43,10 @@ def _bounds(x, w, b, r, dy, act):
     ey = ez if act is None else 1.13 * ez + 4e-7 * (1 + z.abs())
     ey = ey + 2.0 ** -23 * (a.detach().abs() + y.abs())
     dz = DY * da
-    edz = torch.zeros_like(dz) if act is None else DY.abs() * (0.8 * ez + 1e-6) + (2.0 ** -23 + e) * dz.abs() + small
+    wide = torch.zeros_like(dz) if act is None else DY.abs() * (0.8 * ez + 1e-6) + 2.0 ** -23 * dz.abs()     # before it is rounded as an operand
+    edz = wide if act is None else wide + e * dz.abs() + small
     return [(y, ey), (dz @ W, edz @ W.abs() + s(N) * (dz.abs() @ W.abs())), (dz.T @ X, edz.T @ X.abs() + s(M) * (dz.abs().T @ X.abs())),
-            (dz.sum(0), edz.sum(0) + (M / 32 + 100) * 2.0 ** -24 * dz.abs().sum(0))]
+            (dz.sum(0), wide.sum(0) + (M / 32 + 100) * 2.0 ** -24 * dz.abs().sum(0))]
 
 
 CASES = [

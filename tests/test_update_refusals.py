@@ -62,7 +62,7 @@ def test_policy_entry_points_check_their_arguments():
     bwd = lambda dloss, out, **over: lib.bnb_policy_loss_bwd(C.byref(call(**over)), dloss, out, 0, None)  # noqa: E731
     assert bwd(None, fake) == 1 and bwd(fake, None) == 1 and bwd(fake, fake + 2) == 2 and bwd(fake, fake, n_slices=99) == 3
     assert bwd(None, None, rows=0, logits=None) == 0
-    assert lib.bnb_policy_loss_kept_bytes(C.byref(call())) == 4 * (4 + 100 * 7)
+    assert lib.bnb_policy_loss_kept_bytes(C.byref(call())) == 4 * (4 + 100 * 8)
     assert lib.bnb_policy_loss_scratch_bytes(C.byref(call())) > 0
 
 
@@ -75,7 +75,7 @@ def test_operators_have_shape_only_fakes():
         z = torch.empty(5, 3, 12, device="cuda", dtype=torch.bfloat16)
         a, v = torch.empty(5, 3, 3, device="cuda", dtype=torch.int64), torch.empty(5, 3, device="cuda")
         loss, l, stats, kept = ops.policy_loss(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0)
-        assert loss.shape == () and loss.dtype == torch.float32 and l.shape == (5, 3) and stats.shape == (4,) and kept.numel() == 4 + 15 * 7
+        assert loss.shape == () and loss.dtype == torch.float32 and l.shape == (5, 3) and stats.shape == (4,) and kept.numel() == 4 + 15 * 8
         y, kept_z = ops.linear(z, torch.empty(20, 12, device="cuda"), None, None, 2, True)
         assert y.shape == (5, 3, 20) and y.dtype == z.dtype and kept_z.numel() == 0
         assert ops.linear(z.float(), torch.empty(20, 12, device="cuda"), None, None, 2, True)[1].numel() == 4 * 32 * 32
