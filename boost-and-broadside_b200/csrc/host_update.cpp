@@ -4,6 +4,7 @@
 
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <tuple>
 
 namespace bnb {
@@ -330,6 +331,17 @@ class AdamWPlan {
       }
       groups_.push_back(std::move(entries));
     }
+    // elements of two parameters at one place would be updated at the same time
+    std::vector<std::pair<uintptr_t, uintptr_t>> places;
+    for (const auto& entries : groups_)
+      for (const Entry& e : entries)
+        if (e.p.numel() && e.p.is_non_overlapping_and_dense()) {
+          const auto at = reinterpret_cast<uintptr_t>(e.p.data_ptr());
+          places.emplace_back(at, at + e.p.numel() * e.p.element_size());
+        }
+    std::sort(places.begin(), places.end());
+    for (size_t i = 1; i < places.size(); ++i)
+      if (places[i].first < places[i - 1].second) throw py::value_error("AdamW: two parameters share memory");
     PyObject *key, *value;
     for (Py_ssize_t i = 0; PyDict_Next(state.ptr(), &i, &key, &value);) states_.emplace_back(py::reinterpret_borrow<py::object>(key), py::reinterpret_borrow<py::object>(value));
   }

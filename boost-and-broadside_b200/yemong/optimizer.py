@@ -133,6 +133,8 @@ class AdamW(torch.optim.Optimizer):
                 self.grad_norm = None
                 return loss
             norm = self._launch()
+            if norm is False:
+                raise RuntimeError("AdamW: parameter groups must be lists of parameters that stay as they are during a step")
         self.grad_norm = norm
         return loss
 

@@ -275,6 +275,12 @@ def test_saved_and_loaded():
         assert all(torch.equal(a, b) for a, b in zip(ps, twin))
         with pytest.raises(ValueError, match="does not fit"):
             bnb.AdamW(twin, state_bits=40 - bits).load_state_dict(opt.state_dict())
+    both = copy.deepcopy((ps, opt))                          # a copy of parameters and optimizer goes on by itself
+    for a, b in zip(both[0], ps):
+        a.grad = b.grad.clone()
+    both[1].step()
+    opt.step()
+    assert all(torch.equal(a, b) for a, b in zip(both[0], ps)) and float(both[1].grad_norm) == float(opt.grad_norm)
     ps, g = _params([(300,), (65, 7)], [F32, F32])
     twin = [torch.nn.Parameter(p.detach().clone()) for p in ps]
     _gradients(ps, g)
@@ -321,6 +327,11 @@ def test_another_stream_and_refusals():
     strided.grad = torch.zeros(10, device=DEV)
     with pytest.raises(ValueError, match="densely"):
         bnb.AdamW([strided]).step()
+    whole = torch.zeros(300, device=DEV)
+    shared = [torch.nn.Parameter(whole[:200]), torch.nn.Parameter(whole[199:])]
+    shared[0].grad = torch.zeros(200, device=DEV)
+    with pytest.raises(ValueError, match="share memory"):
+        bnb.AdamW(shared).step()
     version = ps[0]._version
     assert torch.equal(was, ps[0]) and float(one.state[ps[0]]["step"]) == 1
     one.step()

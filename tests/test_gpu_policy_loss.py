@@ -83,6 +83,9 @@ CASES = [
     (4, [5001], F32, None, True, True, 1.0),
     (3, [40003], BF16, "mask", True, False, 1.0),
     (2, [33001], F16, None, False, True, 8.0),
+    (3, [33003], F32, "mask", True, False, 1.0),             # rows of more than 128 KB
+    (70, [100], BF16, "float", False, True, 2.0),            # several rows a warp, some of them without weight
+    (45, [999], F32, "mask", True, False, 1.0),
 ]
 
 
