@@ -38,6 +38,32 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// The largest of several pieces; NaN is passed over.
+__device__ __forceinline__ uint32_t larger_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t larger_pair(uint32_t a, uint32_t b, __half) {
+  const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename E, int N, int B>
+__device__ __forceinline__ float top_of(const Raw<E, N> (&raw)[B]) {
+  if constexpr (sizeof(E) == 2) {
+    uint32_t top = raw[0].w[0];
+#pragma unroll
+    for (int i = 1; i < 4 * B; ++i) top = larger_pair(top, raw[i / 4].w[i % 4], E{});
+    float f[2];
+    unpack<E, 2>(Raw<E, 2>{{top}}, f);
+    return fmaxf(f[0], f[1]);
+  } else {
+    float top = __uint_as_float(raw[0].w[0]);
+#pragma unroll
+    for (int i = 1; i < 4 * B; ++i) top = fmaxf(top, __uint_as_float(raw[i / 4].w[i % 4]));
+    return top;
+  }
+}
+
 // e^t summed, and e^t t, with t = z - m.
 struct Soft {
   float m, s, u;
@@ -59,13 +85,9 @@ struct Soft {
     if (z > m) raise(z);
     term(z, base());
   }
-  // N values, two an instruction where there is one; their sums apart until all are there.
+  // N values, none above m, two an instruction where there is one; their sums apart until all are there.
   template <int N>
-  __device__ __forceinline__ void add(const float (&z)[N]) {
-    float top = z[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
-    if (top > m) raise(top);
+  __device__ __forceinline__ void terms(const float (&z)[N]) {
     const F2 b = f2(-base());
     F2 ss = f2(0.f), us = f2(0.f);
 #pragma unroll
@@ -80,6 +102,26 @@ struct Soft {
     const float2 a = halves(ss), c = halves(us);
     s += a.x + a.y;
     u += c.x + c.y;
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const float (&z)[N]) {
+    float top = z[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
+    if (top > m) raise(top);
+    terms(z);
+  }
+  // Several pieces together, 16-bit ones compared two an instruction as they lie: one look at the maximum for all of them.
+  template <typename E, int N, int B>
+  __device__ __forceinline__ void add_pieces(const Raw<E, N> (&raw)[B]) {
+    const float top = top_of<E, N, B>(raw);
+    if (top > m) raise(top);
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      float f[N];
+      unpack<E, N>(raw[k], f);
+      terms(f);
+    }
   }
   __device__ __forceinline__ float lse() const { return m == -INFINITY ? NAN : m + logf(s); }
   __device__ __forceinline__ float entropy() const { return m == -INFINITY ? NAN : logf(s) - u / s; }
@@ -448,23 +490,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_wide(const __grid_c
         if (i + k * T < span.pieces) held[k] = load_raw<E, N>(body + (int64_t)(i + k * T) * N);
       if (t < span.head) v.add_one(to_f(z[t]));
       if (t < span.tail) v.add_one(to_f(body[span.pieces * N + t]));
+      if (HELD > 0 && span.pieces >= HELD * T) {
+        if constexpr (HELD > 0) v.template add_pieces<E, N, HELD>(held);
+        i += HELD * T;
+      } else {
 #pragma unroll
-      for (int k = 0; k < HELD; ++k, i += T)
-        if (i < span.pieces) {
-          float f[N];
-          unpack<E, N>(held[k], f);
-          v.add(f);
-        }
+        for (int k = 0; k < HELD; ++k, i += T)
+          if (i < span.pieces) {
+            float f[N];
+            unpack<E, N>(held[k], f);
+            v.add(f);
+          }
+      }
       for (; i + (UNROLL - 1) * T < span.pieces; i += UNROLL * T) {
         Raw<E, N> raw[UNROLL];
 #pragma unroll
         for (int k = 0; k < UNROLL; ++k) raw[k] = load_raw<E, N>(body + (int64_t)(i + k * T) * N);
-#pragma unroll
-        for (int k = 0; k < UNROLL; ++k) {
-          float f[N];
-          unpack<E, N>(raw[k], f);
-          v.add(f);
-        }
+        v.template add_pieces<E, N, UNROLL>(raw);
       }
       for (; i < span.pieces; i += T) {
         float f[N];
