@@ -5,9 +5,10 @@
 // Forward is one launch: bias, activation and residual enter where the sums leave tensor memory (Out::LINEAR of product_tiles.cuh).  A product of two
 // operations for each of rows x width x out forward and twice that backward: the tensor cores bound it, or, for few rows or a small width, memory.
 //
-// The backward of an activation needs z as it was before any rounding.  Either it is computed once more, with dy taken to dz behind it
-// (Out::SLOPE), or the forward keeps it in float32 (see recomputes).  dz is rounded to the operands' type, as an operand of the two
-// products behind it; the bias's gradient sums it before that.  Without an activation dz is dy as it lies.
+// The backward of an activation reads what the forward kept of it: act'(z) in 16 bits, or z in float32 (see keeps_slopes).  Up to a width of some 400 computing z once more
+// moves fewer bytes, but its second epilogue takes longer than they do: 65536 x 128 x 512 bfloat16 forward and backward 152 us, 145 with slopes kept
+// (float16, with z kept: 151 and 158); 16384 x 512 x 2048 214 and 188; 8192 x 1024 x 4096 with z kept 250, with slopes 231.  dz is rounded to the operands' type, as an
+// operand of the two products behind it; the bias's gradient sums it before that.  Without an activation dz is dy as it lies.
 #include "product_calls.cuh"
 
 namespace bnb {
@@ -25,11 +26,10 @@ int check(const BnbLinear* c) {
   return BNB_OK;
 }
 
-// Whether the backward computes z once more: keeping it costs 8 bytes a result, written and read, computing it 2 width operations.
-// At the measured rates (6.5 TB/s, 1.4 PFLOP/s) they are even at a width of 860, and keeping holds the memory; float32 takes six times
-// the products, and keeps.
-bool recomputes(const BnbLinear& c) { return c.activation == BNB_ACT_NONE || (c.element != BNB_ELEM_F32 && c.width <= 512); }
-bool keeps(const BnbLinear& c) { return !recomputes(c); }
+bool keeps(const BnbLinear& c) { return c.activation != BNB_ACT_NONE; }
+// Whether the forward keeps act'(z) in 16 bits (see KEPT_SCALE) or z in float32.  Where dz becomes an operand of bfloat16 and its sums a bias's gradient of bfloat16, both are
+// rounded to a relative 2^-9, which a slope's 2^-12 leaves as it is.  Beside float16's rounding, and in a bias's gradient in float32, it would show.
+bool keeps_slopes(const BnbLinear& c) { return keeps(c) && c.element == BNB_ELEM_BF16 && (!c.bias || c.bias_element == BNB_ELEM_BF16); }
 
 // ------------------------------------------------------------------ few rows
 
@@ -131,21 +131,38 @@ int few(const FewRows& p, cudaStream_t st) {
 
 // ------------------------------------------------------------------ slopes and sums
 
-// dz from the kept z.  A warp takes blocks of 32 x 32 of the same columns, eight warps side by side: z as it was kept, a row a lane, dy and dz as whole pieces of rows
-// through shared memory (a lane's own row straight from memory is 32 lines a request).  sums: null, or (gridDim.y, n) sums over the rows before dz
-// is rounded, a lane's rows one behind the other, then the lanes.
-template <typename E, int PIECES>
-__global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, int64_t ld_dy, int wide, int activation, int64_t m, int n, void* dz, int64_t ld, int64_t piece_stride,
-                                               float* sums) {
+// Sums over a warp of eight columns, of which every lane has a row: lane 4 c has column c's.  Lanes give away half of their columns a step while there are
+// several: nine shuffles where one column after the other takes forty.
+__device__ __forceinline__ float column_sum(const F2 (&v)[4], int lane) {
+  auto swap = [](F2 x, int by) {
+    const float2 f = halves(x);
+    return f2(__shfl_xor_sync(0xffffffffu, f.x, by), __shfl_xor_sync(0xffffffffu, f.y, by));
+  };
+  const bool b16 = lane & 16, b8 = lane & 8, b4 = lane & 4;
+  const F2 p = add(b16 ? v[2] : v[0], swap(b16 ? v[0] : v[2], 16)), q = add(b16 ? v[3] : v[1], swap(b16 ? v[1] : v[3], 16));   // columns 4-7 or 0-3
+  const float2 r = halves(add(b8 ? q : p, swap(b8 ? p : q, 8)));
+  float s = (b4 ? r.y : r.x) + __shfl_xor_sync(0xffffffffu, b4 ? r.x : r.y, 4);
+  s += __shfl_xor_sync(0xffffffffu, s, 2);
+  return s + __shfl_xor_sync(0xffffffffu, s, 1);
+}
+
+// dz from the kept slopes, or from the kept z.  A warp takes blocks of 32 x 32 of the same columns, eight warps side by side: what was kept, a row a lane, dy and dz as
+// whole pieces of rows through shared memory (a lane's own row straight from memory is 32 lines a request).  sums: null, or (gridDim.y, n) sums over the
+// rows before dz is rounded, a lane's rows one behind the other, then the lanes.
+template <int PIECES> constexpr int SLOPE_CTAS = PIECES > 1 ? 1 : 2;   // of an SM
+template <typename E, int PIECES, bool SLOPES>
+__global__ void __launch_bounds__(256, SLOPE_CTAS<PIECES>) k_slope(const uint4* kept, const void* dy, int64_t ld_dy, int wide, int activation, int64_t m, int n, void* dz, int64_t ld,
+                                                                       int64_t piece_stride, float* sums) {
   constexpr bool EXACT = PIECES > 1;
   using T = std::conditional_t<EXACT, float, E>;
-  constexpr int N = 16 / sizeof(T), ROW = 32 / N;   // pieces of a block's row: 4, float32 8
+  constexpr int N = 16 / sizeof(T), ROW = 32 / N, KEPT = SLOPES ? 4 : 8;   // pieces of a block's row: 4, float32 8
   __shared__ uint4 staged[8][32 * ROW];
   let_next_start();
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint4* const mine = staged[warp];
   auto spot = [](int r, int q) { return r * ROW + (q ^ ((r / (8 / ROW)) % ROW)); };
+  auto out = [](int r, int q) { return r * 4 + (q ^ ((r / 2) % 4)); };   // dz: four pieces of a row, whatever dy was
   const int64_t columns = (ld + 31) / 32, blocks = (m + 31) / 32;
   const int64_t column = (int64_t)blockIdx.x * 8 + warp;
   if (column >= columns) return;
@@ -153,58 +170,77 @@ __global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, i
   F2 total[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) total[k] = f2(0.f);
-  for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
-    const int64_t r0 = b * 32;
-    const float4* kept = reinterpret_cast<const float4*>(z) + (b * columns + column) * 256 + lane;
-    float4 zs[8];
-    uint4 in[ROW];
+  uint4 held[KEPT], in[ROW];
+  auto fetch = [&](int64_t b) {
+    const uint4* from = kept + (b * columns + column) * KEPT * 32 + lane;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) zs[q] = kept[q * 32];
+    for (int q = 0; q < KEPT; ++q) held[q] = from[q * 32];
 #pragma unroll
     for (int q = 0; q < ROW; ++q) {
-      const int r = q * (32 / ROW) + lane / ROW, c = c0 + lane % ROW * N;
-      in[q] = r0 + r < m && c < n ? get16(static_cast<const T*>(dy) + (r0 + r) * ld_dy, c, n, wide) : make_uint4(0u, 0u, 0u, 0u);
+      const int64_t r = b * 32 + q * (32 / ROW) + lane / ROW;
+      const int c = c0 + lane % ROW * N;
+      in[q] = r < m && c < n ? get16(static_cast<const T*>(dy) + r * ld_dy, c, n, wide) : make_uint4(0u, 0u, 0u, 0u);
     }
+  };
+  for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
+    const int64_t r0 = b * 32;
+    fetch(b);
     __syncwarp();
 #pragma unroll
     for (int q = 0; q < ROW; ++q) mine[spot(q * (32 / ROW) + lane / ROW, lane % ROW)] = in[q];
     __syncwarp();
-    const bool row = r0 + lane < m;   // nothing was kept behind the last row and column
+    const int there = r0 + lane < m ? n - c0 : 0;   // columns of this row; nothing was kept behind the last row and column
     F2 v[16];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const bool there[4] = {row && c0 + 4 * q < n, row && c0 + 4 * q + 1 < n, row && c0 + 4 * q + 2 < n, row && c0 + 4 * q + 3 < n};
-      F2 a, d0, d1;
-      activate<EXACT, true>(activation, f2(there[0] ? zs[q].x : 0.f, there[1] ? zs[q].y : 0.f), a, d0);
-      activate<EXACT, true>(activation, f2(there[2] ? zs[q].z : 0.f, there[3] ? zs[q].w : 0.f), a, d1);
-      if constexpr (EXACT) {
-        const uint4 raw = mine[spot(lane, q)];
-        v[2 * q] = mul(d0, f2(__uint_as_float(raw.x), __uint_as_float(raw.y)));
-        v[2 * q + 1] = mul(d1, f2(__uint_as_float(raw.z), __uint_as_float(raw.w)));
-      } else {
-        const uint2 raw = reinterpret_cast<const uint2*>(&mine[spot(lane, q / 2)])[q % 2];
-        v[2 * q] = mul(d0, pair_up(raw.x, E{}));
-        v[2 * q + 1] = mul(d1, pair_up(raw.y, E{}));
-      }
-    }
+    for (int q = 0; q < 4; ++q) {   // eight columns
+      F2 d[4], a;
+      if constexpr (SLOPES) {
+        const uint32_t raw[4] = {held[q].x, held[q].y, held[q].z, held[q].w};
 #pragma unroll
-    for (int k = 0; k < 16; ++k) total[k] = add(total[k], v[k]);
-    // the results: four pieces of a row, whatever dy was
-    auto out = [](int r, int q) { return r * 4 + (q ^ ((r / 2) % 4)); };
+        for (int k = 0; k < 4; ++k) {
+          const float2 s = halves(pair_up(raw[k], __half{}));
+          d[k] = mul(f2(8 * q + 2 * k < there ? s.x : 0.f, 8 * q + 2 * k + 1 < there ? s.y : 0.f), f2(1.f / KEPT_SCALE));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint4 z = held[2 * q + k / 2];
+          const float x = __uint_as_float(k % 2 ? z.z : z.x), y = __uint_as_float(k % 2 ? z.w : z.y);
+          activate<EXACT, true>(activation, f2(8 * q + 2 * k < there ? x : 0.f, 8 * q + 2 * k + 1 < there ? y : 0.f), a, d[k]);
+        }
+      }
+      if constexpr (EXACT) {
+        const uint4 raw[2] = {mine[spot(lane, 2 * q)], mine[spot(lane, 2 * q + 1)]};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          v[4 * q + k] = mul(d[k], k % 2 ? f2(__uint_as_float(raw[k / 2].z), __uint_as_float(raw[k / 2].w)) : f2(__uint_as_float(raw[k / 2].x), __uint_as_float(raw[k / 2].y)));
+      } else {
+        uint4* const at = &mine[spot(lane, q)];   // dz's place too
+        const uint4 raw = *at;
+        const uint32_t g[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[4 * q + k] = mul(d[k], pair_up(g[k], E{}));
+        *at = make_uint4(pair_of<E>(v[4 * q]), pair_of<E>(v[4 * q + 1]), pair_of<E>(v[4 * q + 2]), pair_of<E>(v[4 * q + 3]));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) total[4 * q + k] = add(total[4 * q + k], v[4 * q + k]);
+    }
 #pragma unroll
     for (int piece = 0; piece < PIECES; ++piece) {
       __syncwarp();
+      if constexpr (EXACT) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t bits[4];
+        for (int q = 0; q < 4; ++q) {
+          uint32_t bits[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          bits[k] = pair_of<E>(v[4 * q + k]);
-          if constexpr (EXACT) v[4 * q + k] = add(v[4 * q + k], mul(pair_up(bits[k], E{}), f2(-1.f)));
+          for (int k = 0; k < 4; ++k) {
+            bits[k] = pair_of<E>(v[4 * q + k]);
+            v[4 * q + k] = add(v[4 * q + k], mul(pair_up(bits[k], E{}), f2(-1.f)));
+          }
+          mine[out(lane, q)] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
         }
-        mine[out(lane, q)] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+        __syncwarp();
       }
-      __syncwarp();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int r = q * 8 + lane / 4, c = c0 + lane % 4 * 8;
@@ -222,7 +258,7 @@ __global__ void __launch_bounds__(256) k_slope(const float* z, const void* dy, i
   }
 }
 
-// Sums over rows of operand pieces (PIECES 0: of float32 rows without padding): 64 columns and a share of the rows a CTA, 32 threads' rows added in a fixed order.
+// Sums over rows of operand pieces: 64 columns and a share of the rows a CTA, 32 threads' rows added in a fixed order.
 template <typename E, int PIECES>
 __global__ void __launch_bounds__(256) k_column_sums(const Operand o, float* part, int n) {
   __shared__ float sums[32][65];
@@ -231,13 +267,7 @@ __global__ void __launch_bounds__(256) k_column_sums(const Operand o, float* par
   const int q = threadIdx.x % 8, t = threadIdx.x / 8, col = blockIdx.x * 64 + q * 8;
   const int64_t r0 = o.rows * blockIdx.y / gridDim.y, r1 = o.rows * (blockIdx.y + 1) / gridDim.y;
   float v[8] = {};
-  if constexpr (PIECES == 0) {
-    const float* from = static_cast<const float*>(o.data) + col;
-    for (int64_t r = r0 + t; r < r1; r += 32)
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (col + k < n) v[k] += from[r * o.ld + k];
-  } else if (col < o.ld) {
+  if (col < o.ld) {
     constexpr int UNROLL = 4;   // rows whose loads are on their way together
     const E* from = static_cast<const E*>(o.data) + col;
     auto add_row = [&](const uint4 (&raw)[PIECES]) {
@@ -288,13 +318,12 @@ struct Layout {
   Operand x, w, dz;
   float* part;
   float* sums;     // of a bias's gradient: shares of rows
-  float* blocks;   // of the rows' 32s, where z is computed once more
   PackJobs jobs;
   int n_jobs;
   size_t total;
 
   Layout(const BnbLinear& c, const void* dy, int64_t dy_row, bool backward, uint8_t* base)
-      : pieces(c.element == BNB_ELEM_F32 ? 3 : 1), M(c.rows), K(c.width), N(c.out), ld(round8(c.out)), dz{}, part(nullptr), sums(nullptr), blocks(nullptr), jobs{}, n_jobs(0), total(0) {
+      : pieces(c.element == BNB_ELEM_F32 ? 3 : 1), M(c.rows), K(c.width), N(c.out), ld(round8(c.out)), dz{}, part(nullptr), sums(nullptr), jobs{}, n_jobs(0), total(0) {
     auto take = [&](size_t bytes) {
       uint8_t* at = base ? base + total : nullptr;
       total += round256(bytes);
@@ -317,7 +346,6 @@ struct Layout {
       dz = c.activation == BNB_ACT_NONE ? operand(dy, M, N, dy_row, c.element) : Operand{take((size_t)pieces * M * ld * 2), M, N, ld, M * ld};
       parts = std::max(part_bytes(M, K, N, 1, t, most), part_bytes(N, K, M, 1, t, most));
       sums = reinterpret_cast<float*>(take((size_t)std::max(row_shares(M, (int)N), slope_shares(M, ld)) * N * 4));
-      if (c.activation != BNB_ACT_NONE && recomputes(c)) blocks = reinterpret_cast<float*>(take((size_t)((M + 31) / 32) * N * 4));
     }
     part = reinterpret_cast<float*>(take(parts));
   }
@@ -330,7 +358,8 @@ Epilogue ends_of(const BnbLinear& c) {
   e.ld_out = c.out;
   e.out_kind = floats ? 0 : 1;
   e.ld_h = round8(c.out);
-  e.g = keeps(c) ? static_cast<float*>(c.kept) : nullptr;
+  if (keeps_slopes(c)) e.slopes = static_cast<__half*>(c.kept);
+  else if (keeps(c)) e.g = static_cast<float*>(c.kept);
   e.activation = c.activation;
   e.bias = c.bias;
   e.bias_kind = c.bias_element == BNB_ELEM_F32 ? 0 : 1;
@@ -355,25 +384,15 @@ template <typename E, int PIECES>
 int backward(const BnbLinear& c, const BnbLinearGrads& g, const Layout& l, cudaStream_t st) {
   if (const int r = pack<E, PIECES>(l.jobs, l.n_jobs, st)) return r;
   int r = BNB_OK, shares = 0;   // of sums that are there already
-  if (c.activation != BNB_ACT_NONE) {
+  if (keeps(c)) {
     const int wide = reinterpret_cast<uintptr_t>(g.dy) % 16 == 0 && g.dy_row % (PIECES > 1 ? 4 : 8) == 0;
-    if (keeps(c)) {
-      shares = slope_shares(l.M, l.ld);
-      r = launch_after(k_slope<E, PIECES>, dim3((unsigned)((l.ld + 255) / 256), (unsigned)shares), 256, 0, st, static_cast<const float*>(c.kept), g.dy, g.dy_row, wide,
-                       (int)c.activation, l.M, (int)l.N, const_cast<void*>(l.dz.data), l.ld, l.dz.piece_stride, g.dbias ? l.sums : nullptr);
-    } else if constexpr (PIECES == 1) {
-      Epilogue e{};
-      e.h = const_cast<void*>(l.dz.data);
-      e.ld_h = l.ld;
-      e.activation = c.activation;
-      e.bias = c.bias;
-      e.bias_kind = c.bias_element == BNB_ELEM_F32 ? 0 : 1;
-      e.other = g.dy;
-      e.ld_other = g.dy_row;
-      e.other_wide = wide;
-      e.part = g.dbias ? l.blocks : nullptr;
-      r = multiply<E, PIECES, false, false, Out::SLOPE>({{l.x, {}}, {l.w, {}}, 1}, l.M, l.N, l.K, 1, e, nullptr, st);
-    }
+    shares = slope_shares(l.M, l.ld);
+    auto slope = [&](auto kernel) {
+      return launch_after(kernel, dim3((unsigned)((l.ld + 255) / 256), (unsigned)shares), 256, 0, st, static_cast<const uint4*>(c.kept), g.dy, g.dy_row, wide,
+                          (int)c.activation, l.M, (int)l.N, const_cast<void*>(l.dz.data), l.ld, l.dz.piece_stride, g.dbias ? l.sums : nullptr);
+    };
+    if constexpr (std::is_same<E, __nv_bfloat16>::value && PIECES == 1) r = keeps_slopes(c) ? slope(k_slope<E, 1, true>) : slope(k_slope<E, 1, false>);
+    else r = slope(k_slope<E, PIECES, false>);
   }
   if (r) return r;
   Epilogue e{};
@@ -391,12 +410,8 @@ int backward(const BnbLinear& c, const BnbLinearGrads& g, const Layout& l, cudaS
   }
   if (g.dbias) {
     if (!shares) {
-      const Operand blocks{l.blocks, (l.M + 31) / 32, l.N, l.N, 0};
-      const Operand& from = l.blocks ? blocks : l.dz;
-      shares = row_shares(from.rows, (int)l.N);
-      const dim3 grid((unsigned)((l.N + 63) / 64), (unsigned)shares);
-      r = l.blocks ? launch_after(k_column_sums<E, 0>, grid, 256, 0, st, from, l.sums, (int)l.N) : launch_after(k_column_sums<E, PIECES>, grid, 256, 0, st, from, l.sums, (int)l.N);
-      if (r) return r;
+      shares = row_shares(l.M, (int)l.N);
+      if (r = launch_after(k_column_sums<E, PIECES>, dim3((unsigned)((l.N + 63) / 64), (unsigned)shares), 256, 0, st, l.dz, l.sums, (int)l.N); r) return r;
     }
     count_launch();
     k_add_parts<E><<<(unsigned)((l.N + 63) / 64), 256, 0, st>>>(l.sums, shares, l.N, 1, g.dbias, nullptr, c.bias_element == BNB_ELEM_F32 ? 0 : 1);
@@ -414,7 +429,7 @@ using namespace bnb::product;
 
 extern "C" size_t bnb_linear_kept_bytes(const BnbLinear* c) {
   if (check(c)) return 0;
-  return keeps(*c) ? (size_t)round32(c->rows) * round32(c->out) * 4 : 0;
+  return keeps(*c) ? (size_t)round32(c->rows) * round32(c->out) * (keeps_slopes(*c) ? 2 : 4) : 0;
 }
 
 extern "C" size_t bnb_linear_scratch_bytes(const BnbLinear* c, int backward) {

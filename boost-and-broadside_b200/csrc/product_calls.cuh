@@ -88,8 +88,9 @@ __device__ __forceinline__ void put_linear(const Epilogue& e, int64_t r, int c, 
   };
   if (e.bias) v += e.bias_kind == 0 ? static_cast<const float*>(e.bias)[c] : value(e.bias, c);
   if (e.g) e.g[kept_index(r, c, e.ld_h)] = v;
-  float da;
+  float da = 1.f;
   if (e.activation != BNB_ACT_NONE) activate_exact(e.activation, v, v, da);
+  if (e.slopes) e.slopes[kept_slope_index(r, c, e.ld_h)] = __float2half_rn(da * KEPT_SCALE);
   if (e.other) v += value(e.other, r * e.ld_other + c);
   down(static_cast<E*>(e.out[0])[r * e.ld_out + c], v);
 }
@@ -218,7 +219,7 @@ int multiply(const Sides& s, int64_t m, int64_t n, int64_t depth, int jobs, cons
   }
   constexpr bool again = OUT == Out::AGAIN;
   constexpr int LEAST = OUT == Out::GATE ? 128 : 64, OF = OUT == Out::GATE ? 2 : 1;
-  const int most = is_linear<OUT> ? most_of_linear(PIECES, p.k_steps) : MOST<PIECES>;
+  const int most = OUT == Out::LINEAR ? most_of_linear(PIECES, p.k_steps) : MOST<PIECES>;
   Shaped z = again ? Shaped{64, (int)((m + BM - 1) / BM * ((n + 63) / 64)), 1, p.k_steps}
                    : shape_of(m, n, jobs, p.k_steps * p.terms, most, LEAST, OF, OUT == Out::VALUES || OUT == Out::LINEAR);
   p.splits = z.splits;

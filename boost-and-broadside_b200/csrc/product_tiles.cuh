@@ -39,24 +39,23 @@ enum : int { W_FULL = 101, W_EMPTY = 102, W_ACC = 103, W_DRAINED = 104 };
 //   GATE     columns come in pairs of tiles, g and u: h = act(g) u as operand pieces; g and u themselves where they are kept
 //   BACK     columns are dh: dg = dh u act'(g), du = dh act(g), h = act(g) u as operand pieces, from the kept g and u
 //   AGAIN    the same with g and u computed once more: a stage holds x and dy, and 64 columns of all three weights
-//   LINEAR   z = sum + bias, out[0] = act(z) + other (m, n); z itself where it is kept
-//   SLOPE    the same z: other act'(z) as operand pieces (16 bits), and its sums over 32 rows before it is rounded
-enum class Out : int { VALUES, PARTIAL, GATE, BACK, AGAIN, LINEAR, SLOPE };
-template <Out OUT> constexpr bool is_linear = OUT == Out::LINEAR || OUT == Out::SLOPE;
+//   LINEAR   z = sum + bias, out[0] = act(z) + other (m, n); z itself or act'(z) where it is kept
+enum class Out : int { VALUES, PARTIAL, GATE, BACK, AGAIN, LINEAR };
 
 struct Epilogue {
   void* out[2];
-  float* part;          // SLOPE: sums (m / 32, n), or null
+  float* part;
   void* h;              // operand pieces (pieces, m, ld_h)
   void* dg;
   void* du;
   float* g;             // kept: blocks of 32 rows by 32 columns, see kept_at
   float* u;
+  __half* slopes;       // LINEAR of bfloat16: act'(z), kept instead of z; see kept_slope_index
   int64_t ld_out, ld_h, piece_stride;
   int out_kind;         // 0: float32, 1: the operands' type
   int activation;       // BNB_ACT_SILU or BNB_ACT_GELU; a linear layer's also BNB_ACT_NONE
   const void* bias;     // (n), or null
-  const void* other;    // LINEAR: (m, n) of the results' type to be added, or null; SLOPE: dy
+  const void* other;    // LINEAR: (m, n) of the results' type to be added, or null
   int64_t ld_other;
   int bias_kind, other_wide;   // bias_kind: 0 float32, 1 the operands' type; other_wide: rows of `other` start on 16 bytes
 };
@@ -151,6 +150,12 @@ __device__ __forceinline__ int64_t kept_index(int64_t r, int c, int64_t ld) {
   return ((((r >> 5) * ((ld + 31) >> 5) + (c >> 5)) * 8 + ((c & 31) >> 2)) * 32 + (r & 31)) * 4 + (c & 3);
 }
 
+// Slopes are kept times 2^15 in float16, to a relative 2^-12 from 2e-9 to 1.99.  Blocks as before, each four requests of eight columns a lane.
+constexpr float KEPT_SCALE = 32768.f;
+__device__ __forceinline__ int64_t kept_slope_index(int64_t r, int c, int64_t ld) {
+  return ((((r >> 5) * ((ld + 31) >> 5) + (c >> 5)) * 4 + ((c & 31) >> 3)) * 32 + (r & 31)) * 8 + (c & 7);
+}
+
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __half) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -191,7 +196,7 @@ template <> struct Format<__nv_bfloat16> { static constexpr uint32_t BITS = (1u 
 // epilogue is most of a narrow layer's time and waits in chains, which more warps fill (see at_width's callers).
 template <int PIECES, int BN, Out OUT>
 struct Crew {
-  static constexpr bool MORE = is_linear<OUT> && PIECES == 1 && BN == 128;
+  static constexpr bool MORE = OUT == Out::LINEAR && PIECES == 1 && BN == 128;
   static constexpr int WARPS = MORE ? 24 : OUT_WARPS, GROUPS = PIECES > 1 || OUT == Out::BACK ? 1 : MORE ? 3 : 2, SETS = MORE ? 3 : 2, THREADS = 32 * (2 + WARPS);
 };
 
@@ -201,7 +206,7 @@ struct Shape {
   static constexpr uint32_t OUT_BYTES = WARPS * 2048;   // shared memory of the results on their way out
   static constexpr uint32_t B_BYTES = BN * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
   static constexpr int COLS = OUT == Out::GATE ? BN / 2 : OUT == Out::AGAIN ? BN / 3 : BN;   // of the output
-  static constexpr uint32_t BIAS = is_linear<OUT> ? WARPS * 128 : 0;   // a warp's bias of a segment
+  static constexpr uint32_t BIAS = OUT == Out::LINEAR ? WARPS * 128 : 0;   // a warp's bias of a segment
   static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_BYTES - BIAS) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
   static constexpr uint32_t OUT_AT = STAGES * STAGE, BIAS_AT = OUT_AT + OUT_BYTES, FRAME = BIAS_AT + BIAS, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
 };
@@ -267,21 +272,6 @@ __device__ __forceinline__ F2 pair_up(uint32_t v, __nv_bfloat16) { return unpack
 __device__ __forceinline__ F2 pair_up(uint32_t v, __half) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
   return f2(f.x, f.y);
-}
-
-// Sums over a warp of eight columns, of which every lane has a row: lane 4 c has column c's.  Lanes give away half of their columns a step while there are
-// several: nine shuffles where one column after the other takes forty.
-__device__ __forceinline__ float column_sum(const F2 (&v)[4], int lane) {
-  auto swap = [](F2 x, int by) {
-    const float2 f = halves(x);
-    return f2(__shfl_xor_sync(0xffffffffu, f.x, by), __shfl_xor_sync(0xffffffffu, f.y, by));
-  };
-  const bool b16 = lane & 16, b8 = lane & 8, b4 = lane & 4;
-  const F2 p = add(b16 ? v[2] : v[0], swap(b16 ? v[0] : v[2], 16)), q = add(b16 ? v[3] : v[1], swap(b16 ? v[1] : v[3], 16));   // columns 4-7 or 0-3
-  const float2 r = halves(add(b8 ? q : p, swap(b8 ? p : q, 8)));
-  float s = (b4 ? r.y : r.x) + __shfl_xor_sync(0xffffffffu, b4 ? r.x : r.y, 4);
-  s += __shfl_xor_sync(0xffffffffu, s, 2);
-  return s + __shfl_xor_sync(0xffffffffu, s, 1);
 }
 
 // Sixteen warps take out in two groups, tiles in turn: while one group waits for accumulators, for its rows or for memory, the other
@@ -490,9 +480,9 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
           if (!EXACT && last && k + 8 == SEG) release(set), released = true;
         };
         // a linear layer: the rows of `other` as whole rows and the bias, on their way before the accumulators are waited for
-        uint4 others[is_linear<OUT> && !EXACT ? 8 / PARTS : 1];
+        uint4 others[OUT == Out::LINEAR && !EXACT ? 8 / PARTS : 1];
         float* bias = reinterpret_cast<float*>(smem + S::BIAS_AT + (warp - 2) * 128);
-        if constexpr (is_linear<OUT>) {
+        if constexpr (OUT == Out::LINEAR) {
           float b = 0.f;
           if (e.bias && lane < SEG && col0 + lane < p.n)
             b = e.bias_kind == 0 ? static_cast<const float*>(e.bias)[col0 + lane] : up(static_cast<const E*>(e.bias)[col0 + lane]);
@@ -591,7 +581,7 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
               });
             }
           }
-        } else if constexpr (is_linear<OUT> && !EXACT) {
+        } else if constexpr (OUT == Out::LINEAR && !EXACT) {
           meet();   // what stood there is written
           if (e.other) {
 #pragma unroll
@@ -613,44 +603,39 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
             F2 v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = add(pair(z, k), b[k]);
-            if constexpr (OUT == Out::LINEAR) {
-              if (e.g && in)
+            if (e.g && in)
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                  const float2 x = halves(v[2 * q]), y = halves(v[2 * q + 1]);
-                  *kept_at(e.g, col0 + k0, q) = make_float4(x.x, x.y, y.x, y.y);
-                }
-            }
+              for (int q = 0; q < 2; ++q) {
+                const float2 x = halves(v[2 * q]), y = halves(v[2 * q + 1]);
+                *kept_at(e.g, col0 + k0, q) = make_float4(x.x, x.y, y.x, y.y);
+              }
             F2 a[4], da[4];
             if (e.activation == BNB_ACT_NONE) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) a[k] = v[k], da[k] = f2(1.f);
+              for (int k = 0; k < 4; ++k) a[k] = v[k];
+            } else if (std::is_same<E, __nv_bfloat16>::value && e.slopes) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) activate<false, true>(e.activation, v[k], a[k], da[k]);
+              uint32_t d[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) d[k] = pair_of<__half>(mul(da[k], f2(KEPT_SCALE)));
+              if (in) *reinterpret_cast<uint4*>(e.slopes + kept_slope_index(row0 + lane, col0 + k0, e.ld_h)) = make_uint4(d[0], d[1], d[2], d[3]);
             } else {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) activate<false, OUT == Out::SLOPE>(e.activation, v[k], a[k], da[k]);
+              for (int k = 0; k < 4; ++k) activate<false, false>(e.activation, v[k], a[k], da[k]);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              if constexpr (OUT == Out::SLOPE) a[k] = mul(pair_up(o[k], E{}), da[k]);
-              else if (e.other) a[k] = add(a[k], pair_up(o[k], E{}));
+              if (e.other) a[k] = add(a[k], pair_up(o[k], E{}));
               bits[k] = pair_of<E>(a[k]);
             }
             *at = make_uint4(bits[0], bits[1], bits[2], bits[3]);
-            if constexpr (OUT == Out::SLOPE) {
-              if (e.part && row0 < p.m) {
-                const float s = column_sum(a, lane);
-                if (lane % 4 == 0 && col0 + k0 + lane / 4 < p.n) e.part[(row0 >> 5) * p.n + col0 + k0 + lane / 4] = s;
-              }
-            }
           }
           meet();
-          E* to = static_cast<E*>(OUT == Out::SLOPE ? e.h : e.out[0]);
-          const int64_t ld = OUT == Out::SLOPE ? e.ld_h : e.ld_out;
-          const int cols = OUT == Out::SLOPE ? (int)e.ld_h : p.n;   // an operand's rows are padded with zeros
           take_rows<PARTS>(rows, part, lane, [&](int r, int c, uint4 raw) {
-            if (row0 + r < p.m) put16(to + (row0 + r) * ld, first + c, cols, ld % 8 == 0, raw);
+            if (row0 + r < p.m) put16(static_cast<E*>(e.out[0]) + (row0 + r) * e.ld_out, first + c, p.n, e.ld_out % 8 == 0, raw);
           });
-        } else if constexpr (is_linear<OUT>) {
+        } else if constexpr (OUT == Out::LINEAR) {
           // float32: 16 columns at a time
 #pragma unroll
           for (int k0 = 0; k0 < SEG; k0 += 16) {

@@ -24,11 +24,10 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], residual: Optional
 
 @linear.register_fake
 def _(x, weight, bias, residual, activation, keep):
-    # as bnb_linear_kept_bytes: without an activation nothing is kept, and narrow 16-bit calls compute z once more
-    recomputes = activation == 0 or (x.dtype != torch.float32 and x.shape[-1] <= 512)
+    # as bnb_linear_kept_bytes: slopes in 16 bits, or z in 32; without an activation nothing
     rows = x.numel() // x.shape[-1]
-    kept = 4 * ((rows + 31) // 32 * 32) * ((weight.shape[0] + 31) // 32 * 32)
-    return x.new_empty((*x.shape[:-1], weight.shape[0])), x.new_empty(kept if keep and not recomputes else 0, dtype=torch.uint8)
+    kept = (2 if x.dtype == torch.bfloat16 and (bias is None or bias.dtype == x.dtype) else 4) * ((rows + 31) // 32 * 32) * ((weight.shape[0] + 31) // 32 * 32)
+    return x.new_empty((*x.shape[:-1], weight.shape[0])), x.new_empty(kept if keep and activation else 0, dtype=torch.uint8)
 
 
 @torch.library.custom_op("bnb_b200::linear_backward", mutates_args=(), device_types="cuda")

@@ -28,7 +28,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
     Returns:
         (.., N) in x's type, rounded once.  16-bit calls: products of 16-bit operands summed in float32; the gradient before the activation is
-        rounded to x's type as an operand of the next products, but not for the bias's gradient, its sum.  float32 calls: float32
+        rounded to x's type as an operand of the next products, but not for the bias's gradient, its sum.  Between forward and backward, bfloat16
+        calls keep the activation's slopes in 16 bits (relative 2^-12), calls with a float32 bias, float16 and float32 ones the sums in 32.  float32 calls: float32
         products, of numbers in pieces, so that an infinity, or a number above 3.39e38, comes out as NaN.
     """
     act = activation_code("linear", activation, (None, "silu", "gelu"))

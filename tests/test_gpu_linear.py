@@ -61,11 +61,11 @@ CASES = [
     (129, 72, 129, BF16, False, True, "silu", False),
     (300, 130, 257, F32, False, False, None, False),
     (301, 522, 130, F32, False, False, "silu", True),
-    (300, 513, 200, BF16, False, False, "gelu", True),       # z is kept
+    (300, 513, 200, BF16, False, False, "gelu", True),       # wide, slopes kept
     (200, 640, 321, F16, True, None, "silu", False),
-    (200, 512, 64, BF16, False, False, "silu", True),        # z is computed again
+    (200, 512, 64, BF16, False, False, "silu", True),        # narrow
     (2500, 96, 40, BF16, False, False, "gelu", True),        # the weight's gradient over a cut depth
-    (5, 4096, 100, BF16, False, False, "gelu", True),        # a cut depth, z kept by its sums
+    (5, 4096, 100, BF16, False, False, "gelu", True),        # a cut depth, slopes kept by its sums
     (3, 4096, 4096, F16, False, False, None, True),
     (40, 2600, 70, F32, False, False, "gelu", True),
     (1, 4100, 33, F32, False, True, "silu", False),
@@ -76,6 +76,8 @@ CASES = [
     (4, 2048, 33, BF16, True, True, "silu", False),
     (7, 3080, 50, F32, False, None, "silu", False),
     (8, 1536, 41, BF16, False, False, "gelu", True),
+    (3, 1024, 9, BF16, False, None, "gelu", False),          # few rows, slopes kept
+    (130, 64, 40, BF16, True, True, "gelu", True),           # z kept, for the bias's gradient in float32
 ]
 
 
@@ -159,6 +161,21 @@ def test_few_rows_of_a_wider_tensor():
         one = bnb.linear(x[:1].expand(3, 1024), w[:20480].view(20, 1024))
         assert torch.equal(one[0], one[1]) and torch.equal(one[0], one[2])
         assert bnb.linear(x[:0], w[:20480].view(20, 1024)).shape == (0, 20)
+
+
+def test_small_slopes():
+    """Slopes from 1 to 4e-11 through what is kept of a bfloat16 call: relative 2^-12, a rounding as the operand dz and one as dx (2^-9 each, and their product), the
+    logistic's and its factor's in float32 (s (1 + |z|) 2^-20), and half a step of the smallest numbers kept, 2^-25 2^-15."""
+    import boost_and_broadside_b200 as bnb
+
+    x = -torch.linspace(-3, 27, 301).to(BF16)[:, None]
+    one = torch.ones(1, 1, dtype=BF16, device=DEV)
+    leaf = x.to(DEV).requires_grad_(True)
+    got = torch.autograd.grad(bnb.linear(leaf, one, activation="silu"), [leaf], torch.ones(301, 1, dtype=BF16, device=DEV))[0]
+    z = x.double()
+    s = torch.sigmoid(z)
+    d = s * (1 + z * (1 - s))
+    _within(got, d, (2 ** -8 + 2 ** -11) * d.abs() + s * (1 + z.abs()) * 2 ** -20 + 2 ** -40, "dx")
 
 
 def test_gradient_against_differences():

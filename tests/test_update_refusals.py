@@ -77,7 +77,7 @@ def test_operators_have_shape_only_fakes():
         loss, l, stats, kept = ops.policy_loss(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0)
         assert loss.shape == () and loss.dtype == torch.float32 and l.shape == (5, 3) and stats.shape == (4,) and kept.numel() == 4 + 15 * 8
         y, kept_z = ops.linear(z, torch.empty(20, 12, device="cuda"), None, None, 2, True)
-        assert y.shape == (5, 3, 20) and y.dtype == z.dtype and kept_z.numel() == 0
+        assert y.shape == (5, 3, 20) and y.dtype == z.dtype and kept_z.numel() == 32 * 32 * 2
         assert ops.linear(z.float(), torch.empty(20, 12, device="cuda"), None, None, 2, True)[1].numel() == 4 * 32 * 32
         assert ops.policy_loss_backward(z, a, v, v, None, None, [3, 7, 2], 0.2, 0.2, 0.0, 0.0, kept, loss).shape == z.shape
 
@@ -183,10 +183,11 @@ def test_linear_checks_its_arguments():
     assert fwd(weight=None) == 1 and fwd(x=None) == 1 and fwd(y=None) == 1
     assert fwd(y=fake + 4) == 2 and fwd() == 6 and fwd(rows=0) == 0
     kept = lambda **over: lib.bnb_linear_kept_bytes(C.byref(call(**over)))  # noqa: E731
-    assert kept() == 0 and kept(width=600, activation=0) == 0                # computed once more; no activation
-    assert kept(width=600) == 128 * 128 * 4 and kept(element=0, weight_element=0, bias_element=0) == 128 * 128 * 4
+    assert kept(activation=0) == 0 and kept() == 128 * 128 * 2 and kept(bias=None, bias_element=0) == 128 * 128 * 2   # slopes in 16 bits
+    for over in (dict(bias_element=0), dict(element=2, weight_element=2, bias_element=2), dict(element=0, weight_element=0, bias_element=0)):
+        assert kept(**over) == 128 * 128 * 4                                  # z in float32
     assert lib.bnb_linear_scratch_bytes(C.byref(call()), 1) > lib.bnb_linear_scratch_bytes(C.byref(call()), 0)
     bwd = lambda g, **over: lib.bnb_linear_bwd(C.byref(call(**over)), C.byref(g) if g else None, None, 0, None)  # noqa: E731
     assert bwd(None) == 1 and bwd(LinearGrads(None, 128, fake, fake, fake)) == 1
     assert bwd(LinearGrads(fake, 128, fake, fake, fake), width=600) == 1     # nothing kept
-    assert bwd(LinearGrads(fake, 128, fake + 8, fake, fake)) == 2 and bwd(LinearGrads(fake, 128, fake, fake, fake)) == 6
+    assert bwd(LinearGrads(fake, 128, fake + 8, fake, fake), kept=fake) == 2 and bwd(LinearGrads(fake, 128, fake, fake, fake), kept=fake) == 6
