@@ -12,9 +12,10 @@
 #include "launch_count.h"
 
 namespace bnb {
+// CTAs of a cluster lie side by side in x.
 template <class... P, class... A>
-inline int launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
-  cudaLaunchAttribute at[1];
+inline int launch_clusters_after(unsigned cluster, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
@@ -24,9 +25,19 @@ inline int launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_
   cfg.stream = st;
   cfg.attrs = at;
   cfg.numAttrs = 1;
+  if (cluster > 1) {
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
   count_launch();
   if (cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...) == cudaSuccess) return BNB_OK;
   (void)cudaGetLastError();
   return BNB_ERR_LAUNCH;
+}
+template <class... P, class... A>
+inline int launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
+  return launch_clusters_after(1, kernel, grid, threads, smem, st, std::forward<A>(args)...);
 }
 }  // namespace bnb

@@ -148,11 +148,16 @@ inline bool map_of(CUtensorMap& m, const Operand& o, int pieces, int box_rows, b
 
 // ------------------------------------------------------------------ products
 
-struct Shaped { int bn, tiles, splits, split_steps; };
+// Clocks of a stage of two CTAs on 256 x 256, see shape_of.
+constexpr double PAIR_STAGE = 640.0;
+struct Shaped { int bn, tiles, splits, split_steps; bool pair; };
 // The width of a tile: the one with the least time.  A stage moves (128 + BN) rows of 128 bytes into shared memory and the products read
 // them once from there, at 128 bytes a clock: 2 (128 + BN) clocks, more than the products themselves take at any BN up to 256 (measured:
 // 790 clocks a stage at 256).  A tile's fixed cost (fill, the last results) is about 1200.  Then, where tiles leave SMs idle and results can be
-// added, the depth is cut so that all have work, no part below 8 stages; the sums' launch costs some 6000 clocks.
+// added, the depth is cut so that all have work, no part below 8 stages; the sums' launch costs some 6000 clocks.  Two CTAs on 256 x 256 (16-bit operands) each hold their rows
+// and half of the columns' operand: 2 (128 + 128) clocks of shared memory, as much as the products take.  8192 x 4096 outputs, us of one and of two CTAs to a tile: width
+// 4096 231 and 187, 2048 121 and 101, 1024 70 and 68 (its results bound it); a stage is 0.79 of a single one's there, and counts for a little more, since 74 pairs divide work less
+// evenly than 148 CTAs (4736 rows, five rounds for four: 136 and 153).
 inline Shaped shape_of(int64_t m, int64_t n, int jobs, int steps, int most, int least, int out_of_bn, bool may_split) {
   const int64_t mt = (m + BM - 1) / BM;
   Shaped best{};
@@ -165,19 +170,25 @@ inline Shaped shape_of(int64_t m, int64_t n, int jobs, int steps, int most, int 
       splits = (steps + split_steps - 1) / split_steps;
       const double rounds = (double)((tiles * splits + SMS - 1) / SMS), c = rounds * (split_steps * 2.0 * (BM + bn) + 1200.0) + (splits > 1 ? 6000.0 : 0.0);
       if (best.bn == 0 || c < cost) {
-        best = {bn, (int)tiles, splits, split_steps};
+        best = {bn, (int)tiles, splits, split_steps, false};
         cost = c;
       }
     }
   }
+  if (may_split && most == 256) {
+    const int64_t tiles = (mt + 1) / 2 * ((n + 255) / 256) * jobs;
+    const double rounds = (double)((tiles + SMS / 2 - 1) / (SMS / 2)), c = rounds * (steps * PAIR_STAGE + 1200.0);
+    if (c < cost) best = {256, (int)tiles, 1, steps, true};
+  }
   return best;
 }
 
-template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT>
+template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT, bool PAIR = false>
 int launch(const Product& p, int tiles, cudaStream_t st) {
-  constexpr uint32_t bytes = Shape<BN, OUT, PIECES>::BYTES;
-  auto kernel = k_product<E, PIECES, A_MN, B_MN, BN, OUT>;
+  constexpr uint32_t bytes = Shape<BN, OUT, PIECES, PAIR>::BYTES;
+  auto kernel = k_product<E, PIECES, A_MN, B_MN, BN, OUT, PAIR>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return BNB_ERR_LAUNCH;
+  if constexpr (PAIR) return launch_clusters_after(2, kernel, dim3(2 * std::min(tiles, SMS / 2)), Crew<PIECES, BN, OUT>::THREADS, bytes, st, p);
   return launch_after(kernel, dim3(std::min(tiles, SMS)), Crew<PIECES, BN, OUT>::THREADS, bytes, st, p);
 }
 
@@ -194,7 +205,9 @@ template <int PIECES> constexpr int MOST = PIECES > 1 ? 128 : 256;
 inline int most_of_linear(int pieces, int k_steps) { return pieces > 1 || k_steps <= 8 ? 128 : 256; }
 
 template <typename E, int PIECES, bool A_MN, bool B_MN, Out OUT>
-int at_width(const Product& p, int bn, int tiles, cudaStream_t st) {
+int at_width(const Product& p, int bn, int tiles, bool pair, cudaStream_t st) {
+  if constexpr (PIECES == 1 && (OUT == Out::VALUES || OUT == Out::LINEAR))
+    if (pair) return launch<E, PIECES, A_MN, B_MN, 256, OUT, true>(p, tiles, st);
   if constexpr (PIECES == 1)
     if (bn == 256) return launch<E, PIECES, A_MN, B_MN, 256, OUT>(p, tiles, st);
   if (bn == 128) return launch<E, PIECES, A_MN, B_MN, 128, OUT>(p, tiles, st);
@@ -220,18 +233,18 @@ int multiply(const Sides& s, int64_t m, int64_t n, int64_t depth, int jobs, cons
   constexpr bool again = OUT == Out::AGAIN;
   constexpr int LEAST = OUT == Out::GATE ? 128 : 64, OF = OUT == Out::GATE ? 2 : 1;
   const int most = OUT == Out::LINEAR ? most_of_linear(PIECES, p.k_steps) : MOST<PIECES>;
-  Shaped z = again ? Shaped{64, (int)((m + BM - 1) / BM * ((n + 63) / 64)), 1, p.k_steps}
+  Shaped z = again ? Shaped{64, (int)((m + BM - 1) / BM * ((n + 63) / 64)), 1, p.k_steps, false}
                    : shape_of(m, n, jobs, p.k_steps * p.terms, most, LEAST, OF, OUT == Out::VALUES || OUT == Out::LINEAR);
   p.splits = z.splits;
   p.split_steps = z.split_steps;
-  p.m_tiles = (int)((m + BM - 1) / BM);
+  p.m_tiles = (int)((m + (z.pair ? 2 * BM : BM) - 1) / (z.pair ? 2 * BM : BM));
   p.n_tiles = (int)((n + z.bn / OF - 1) / (z.bn / OF));
   p.host_status = host_status_word(st);
   constexpr bool half = std::is_same<E, __half>::value;
   const int a_maps = again ? 2 : jobs > 1 ? jobs : s.segments, b_maps = again ? 3 : OUT == Out::GATE ? 2 : s.segments;
   bool ok = has_context();
   for (int i = 0; i < a_maps; ++i) ok = ok && map_of(p.a[i], s.a[i], PIECES, A_MN ? BK : BM, half);
-  for (int i = 0; i < b_maps; ++i) ok = ok && map_of(p.b[i], s.b[i], PIECES, again || B_MN ? BK : z.bn / OF, half);
+  for (int i = 0; i < b_maps; ++i) ok = ok && map_of(p.b[i], s.b[i], PIECES, again || B_MN ? BK : z.pair ? z.bn / 2 : z.bn / OF, half);
   if (!ok) return BNB_ERR_LAUNCH;
   const int total = z.tiles * z.splits;
   if constexpr (again) {
@@ -239,22 +252,22 @@ int multiply(const Sides& s, int64_t m, int64_t n, int64_t depth, int jobs, cons
   } else if constexpr (OUT == Out::LINEAR) {
     if (z.splits > 1) {
       p.e.part = part;
-      if (const int r = at_width<E, PIECES, A_MN, B_MN, Out::PARTIAL>(p, z.bn, total, st)) return r;
+      if (const int r = at_width<E, PIECES, A_MN, B_MN, Out::PARTIAL>(p, z.bn, total, z.pair, st)) return r;
       return launch_after(k_add_linear<E>, dim3((unsigned)((m * n + 63) / 64)), 256, 0, st, p.e, (const float*)part, z.splits, m, (int)n);
     }
-    return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, st);
+    return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, z.pair, st);
   } else if constexpr (OUT == Out::VALUES) {
     if (z.splits > 1) {
       p.e.part = part;
-      if (const int r = at_width<E, PIECES, A_MN, B_MN, Out::PARTIAL>(p, z.bn, total, st)) return r;
+      if (const int r = at_width<E, PIECES, A_MN, B_MN, Out::PARTIAL>(p, z.bn, total, z.pair, st)) return r;
       const int64_t cells = m * n;
       count_launch();
       k_add_parts<E><<<(unsigned)((cells * jobs + 63) / 64), 256, 0, st>>>(part, z.splits, cells, jobs, e.out[0], e.out[1], e.out_kind);
       return cudaGetLastError() == cudaSuccess ? BNB_OK : BNB_ERR_LAUNCH;
     }
-    return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, st);
+    return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, z.pair, st);
   } else {
-    return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, st);
+    return at_width<E, PIECES, A_MN, B_MN, OUT>(p, z.bn, total, z.pair, st);
   }
 }
 inline size_t part_bytes(int64_t m, int64_t n, int64_t depth, int jobs, int terms, int most) {

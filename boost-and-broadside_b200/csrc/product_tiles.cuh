@@ -4,7 +4,8 @@
 // out (m, n) = sum over terms of A_t (m, k) B_t (n, k)^T.  One persistent CTA per SM walks over tiles of 128 x BN; a warp fetches (TMA
 // boxes of 64 elements by 64 to 256, 128-byte swizzle, zeros outside the tensors, so that no size has to be a multiple of a
 // tile), a warp issues the products, sixteen warps take finished accumulators out of tensor memory.  There are two accumulators: a tile's
-// products run while the tile before is written out.
+// products run while the tile before is written out.  Wide tiles of large products are 256 x 256 and have two CTAs (cta_group::2), which read each other's half of the columns'
+// operand: one alone is bound by shared memory, which writes and reads (128 + 256) 128 bytes for 512 clocks of products.
 //
 // An operand may lie in memory with its depth innermost (K-major) or with its rows innermost (MN-major): the same boxes, other descriptor
 // bits.  So no operand of the backward is transposed in memory.
@@ -76,10 +77,53 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
                ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 
+// Two CTAs of a cluster on one tile (cta_group::2): the first one's products read both's shared memory and write both's tensor memory.
+__device__ __forceinline__ uint32_t rank_of_pair() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {   // the first CTA's address of the same place
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar_in_first) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar_in_first) : "memory");
+}
+__device__ __forceinline__ void arrive_in_first(uint32_t bar_in_first) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_in_first) : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t elected, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(0x40004040u), "r"(elected) : "memory");
+}
+__device__ __forceinline__ void commit_pair_if(uint32_t elected, uint32_t bar) {   // this barrier of both CTAs
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}"
+      ::"r"(bar), "r"(elected), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t smem_dst, uint32_t cols) {   // a warp of each
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+
 struct Tile { int job, split, m, n; };
-// Neighbouring CTAs take tiles of up to 16 row tiles by as many column tiles as it takes: their operands come from L2.
+// Neighbouring CTAs take tiles of up to 16 row tiles (GM, of pairs 8) by as many column tiles as it takes: their operands come from L2.
+template <int GM>
 __device__ __forceinline__ Tile tile_of(const Product& p, int i) {
-  constexpr int GM = 16;
   const int per = p.m_tiles * p.n_tiles, js = i / per, rest = i - js * per;
   const int g = rest / (GM * p.n_tiles), in = rest - g * GM * p.n_tiles, first = g * GM, gm = min(GM, p.m_tiles - first);
   return {js % p.jobs, js / p.jobs, first + in % gm, in / gm};
@@ -200,11 +244,11 @@ struct Crew {
   static constexpr int WARPS = MORE ? 24 : OUT_WARPS, GROUPS = PIECES > 1 || OUT == Out::BACK ? 1 : MORE ? 3 : 2, SETS = MORE ? 3 : 2, THREADS = 32 * (2 + WARPS);
 };
 
-template <int BN, Out OUT, int PIECES = 1>
+template <int BN, Out OUT, int PIECES = 1, bool PAIR = false>
 struct Shape {
   static constexpr int WARPS = Crew<PIECES, BN, OUT>::WARPS;
   static constexpr uint32_t OUT_BYTES = WARPS * 2048;   // shared memory of the results on their way out
-  static constexpr uint32_t B_BYTES = BN * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
+  static constexpr uint32_t B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
   static constexpr int COLS = OUT == Out::GATE ? BN / 2 : OUT == Out::AGAIN ? BN / 3 : BN;   // of the output
   static constexpr uint32_t BIAS = OUT == Out::LINEAR ? WARPS * 128 : 0;   // a warp's bias of a segment
   static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_BYTES - BIAS) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
@@ -278,13 +322,14 @@ __device__ __forceinline__ F2 pair_up(uint32_t v, __half) {
 // computes.  (All sixteen on a tile at once wait together: 71 us for dh and its gradients at 65 536 x 128 x 512.)  Float32, whose runs need both
 // sets of accumulators for one tile, has one group, and so has BACK: it waits for g and u from memory most, and 16 columns a warp leave
 // the registers to have all of a segment's on their way at once (128 us against 113 at 8192 x 1024 x 4096).
-template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT>
+template <typename E, int PIECES, bool A_MN, bool B_MN, int BN, Out OUT, bool PAIR>
 static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_product(const __grid_constant__ Product p) {
-  using S = Shape<BN, OUT, PIECES>;
+  using S = Shape<BN, OUT, PIECES, PAIR>;
   using C = Crew<PIECES, BN, OUT>;
   constexpr bool EXACT = PIECES > 1;
   constexpr int GROUPS = C::GROUPS, SETS = C::SETS, PARTS = C::WARPS / 4 / GROUPS;
   static_assert(SETS <= MAX_SETS && SETS * BN <= 512 && (GROUPS == 1 || GROUPS == SETS), "a group's tiles have a set of their own");
+  static_assert(!PAIR || (BN == 256 && PIECES == 1 && (OUT == Out::VALUES || OUT == Out::LINEAR)), "256 x 256, half of the columns' operand in each");
   static_assert(!EXACT || 3 * BN <= 512, "two sets of accumulators and their sum");
   constexpr uint32_t SUM = 2 * BN;   // float32: where runs are added
   extern __shared__ uint8_t raw_smem[];
@@ -302,16 +347,18 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
     }
     for (int i = 0; i < SETS; ++i) {
       mbar_init(smem_u32(&f.acc[i]), 1);
-      mbar_init(smem_u32(&f.drained[i]), C::WARPS / GROUPS);
+      mbar_init(smem_u32(&f.drained[i]), (PAIR ? 2 : 1) * C::WARPS / GROUPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
     __syncwarp();
-    tmem_alloc(smem_u32(&f.tmem), 512);
+    if constexpr (PAIR) tmem_alloc_pair(smem_u32(&f.tmem), 512);
+    else tmem_alloc(smem_u32(&f.tmem), 512);
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) pair_sync();   // both's barriers are there
   tc_fence_after();
   let_next_start();
   wait_for_previous();
@@ -320,26 +367,32 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
   const int tiles = p.m_tiles * p.n_tiles * p.jobs * p.splits, all_steps = p.k_steps * p.terms;
   // The end of the run of stages that begins at s: all of a tile's, or, in float32, all of the small terms, then FLUSH at a time.
   const int small = EXACT ? all_steps - all_steps / 6 : all_steps;
+  const int rank = PAIR ? (int)rank_of_pair() : 0, walker = PAIR ? blockIdx.x / 2 : blockIdx.x, walkers = PAIR ? gridDim.x / 2 : gridDim.x;
+  constexpr int GM = PAIR ? 8 : 16;
   auto run_end = [&](int s, int s1) { return !EXACT ? s1 : s < small ? min(s1, small) : min(s1, s + FLUSH); };
 
   if (warp == 0) {
     // fetching
     int step = 0;
     const uint32_t el = elect_one();
-    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
-      const Tile t = tile_of(p, i);
+    for (int i = walker; i < tiles; i += walkers) {
+      const Tile t = tile_of<GM>(p, i);
       const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps);
       int term = s0 / p.k_steps, k = s0 - term * p.k_steps;
-      const int m0 = t.m * BM, n0 = t.n * S::COLS;
+      const int m0 = (PAIR ? 2 * t.m + rank : t.m) * BM, n0 = t.n * S::COLS + (PAIR ? rank * (BN / 2) : 0);
       for (int s = s0; s < s1; ++s, ++step) {
         const int slot = step % S::STAGES;
         if (step >= S::STAGES) wait(f.empty[slot], step / S::STAGES - 1, W_EMPTY);
         if (el) {
-          const uint32_t bar = smem_u32(&f.full[slot]), at = base + slot * S::STAGE;
+          const uint32_t own = smem_u32(&f.full[slot]), bar = PAIR ? in_first(own) : own, at = base + slot * S::STAGE;
+          auto load = [](uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+            if constexpr (PAIR) tma_load_pair(dst, map, x, y, z, bar);
+            else tma_load(dst, map, x, y, z, bar);
+          };
           const CUtensorMap* am = &p.a[p.jobs > 1 ? t.job : p.a_map[term]];
           const CUtensorMap* bm = &p.b[p.b_map[term]];
           const int ap = p.a_piece[term], bp = p.b_piece[term], kc = k * BK;
-          mbar_expect_tx(bar, S::STAGE);
+          if (rank == 0) mbar_expect_tx(own, (PAIR ? 2 : 1) * S::STAGE);
           if constexpr (OUT == Out::AGAIN) {
             tma_load(at, &p.a[0], kc, m0, 0, bar);
             tma_load(at + A_BYTES, &p.a[1], kc, m0, 0, bar);
@@ -350,18 +403,18 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
             const uint32_t bt = at + A_BYTES;
             if constexpr (A_MN) {
 #pragma unroll
-              for (int j = 0; j < BM / 64; ++j) tma_load(at + j * SLAB, am, m0 + 64 * j, kc, ap, bar);
+              for (int j = 0; j < BM / 64; ++j) load(at + j * SLAB, am, m0 + 64 * j, kc, ap, bar);
             } else {
-              tma_load(at, am, kc, m0, ap, bar);
+              load(at, am, kc, m0, ap, bar);
             }
             if constexpr (OUT == Out::GATE) {
               tma_load(bt, &p.b[0], kc, n0, bp, bar);
               tma_load(bt + S::B_BYTES / 2, &p.b[1], kc, n0, bp, bar);
             } else if constexpr (B_MN) {
 #pragma unroll
-              for (int j = 0; j < BN / 64; ++j) tma_load(bt + j * SLAB, bm, n0 + 64 * j, kc, bp, bar);
+              for (int j = 0; j < (PAIR ? BN / 2 : BN) / 64; ++j) load(bt + j * SLAB, bm, n0 + 64 * j, kc, bp, bar);
             } else {
-              tma_load(bt, bm, kc, n0, bp, bar);
+              load(bt, bm, kc, n0, bp, bar);
             }
           }
         }
@@ -370,17 +423,24 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
       }
     }
     // every copy has landed before the CTA may leave
-    for (int s = max(0, step - S::STAGES); s < step; ++s) wait(f.full[s % S::STAGES], s / S::STAGES, W_FULL);
+    for (int s = max(0, step - S::STAGES); s < step; ++s) {
+      if (rank == 0) wait(f.full[s % S::STAGES], s / S::STAGES, W_FULL);   // a pair's: the first CTA's barriers count both's copies, and both leave together
+      if constexpr (PAIR) wait(f.empty[s % S::STAGES], s / S::STAGES, W_EMPTY);   // arrivals from the other CTA
+    }
   } else if (warp == 1) {
     // issuing
-    constexpr uint32_t COMMON = (1u << 4) | Format<E>::BITS | ((uint32_t)(BM >> 4) << 24);
+    constexpr uint32_t COMMON = (1u << 4) | Format<E>::BITS | ((uint32_t)((PAIR ? 2 * BM : BM) >> 4) << 24);
     constexpr uint32_t MN_A = 1u << 15, MN_B = 1u << 16;
     constexpr uint32_t A_K = A_MN ? 128 : 2, B_K = B_MN ? 128 : 2;   // 16 of depth in descriptor units (16 bytes)
     const uint32_t el = elect_one(), tm = uniform(tmem);
     auto low = [](uint32_t addr, bool mn) { return ((addr & 0x3FFFFu) >> 4) | (mn ? (SLAB >> 4) << 16 : 1u << 16); };
     int step = 0, done = 0;
-    for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
-      const Tile t = tile_of(p, i);
+    auto commit = [&](uint64_t& bar) {
+      if constexpr (PAIR) commit_pair_if(el, smem_u32(&bar));
+      else tc_commit_if(el, smem_u32(&bar));
+    };
+    for (int i = rank == 0 ? walker : tiles; i < tiles; i += walkers) {   // a pair's products: the first CTA
+      const Tile t = tile_of<GM>(p, i);
       const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps);
       for (int s = s0; s < s1; ++done) {
         const int set = done % SETS, end = run_end(s, s1);
@@ -405,11 +465,12 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
             const uint32_t a_lo = uniform(low(at, A_MN)), b_lo = uniform(low(at + A_BYTES, B_MN));
 #pragma unroll
             for (uint32_t k = 0; k < BK / 16; ++k)
-              mma_one<false>(el, tm + set * BN, a_lo + A_K * k, b_lo + B_K * k, IDESC, acc || k ? 1u : 0u);
+              if constexpr (PAIR) mma_pair(el, tm + set * BN, a_lo + A_K * k, b_lo + B_K * k, IDESC, acc || k ? 1u : 0u);
+              else mma_one<false>(el, tm + set * BN, a_lo + A_K * k, b_lo + B_K * k, IDESC, acc || k ? 1u : 0u);
           }
-          tc_commit_if(el, smem_u32(&f.empty[slot]));
+          commit(f.empty[slot]);
         }
-        tc_commit_if(el, smem_u32(&f.acc[set]));
+        commit(f.acc[set]);
         __syncwarp();
       }
     }
@@ -425,12 +486,15 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
     auto release = [&](int set) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&f.drained[set]));
+      if (lane == 0) {
+        if constexpr (PAIR) arrive_in_first(in_first(smem_u32(&f.drained[set])));
+        else mbar_arrive(smem_u32(&f.drained[set]));
+      }
     };
     auto pair = [](const uint32_t (&v)[8], int k) { return f2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])); };
     int done = group, turn = 0;
-    for (int i = blockIdx.x + group * gridDim.x; i < tiles; i += GROUPS * gridDim.x) {
-      const Tile t = tile_of(p, i);
+    for (int i = walker + group * walkers; i < tiles; i += GROUPS * walkers) {
+      const Tile t = tile_of<GM>(p, i);
       uint32_t acc = lanes + (done % SETS) * BN;
       if constexpr (EXACT) {
         const int s0 = t.split * p.split_steps, s1 = min(all_steps, s0 + p.split_steps);
@@ -458,7 +522,7 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
         acc = lanes + SUM;
       }
       const int set = done % SETS;
-      const int64_t row0 = (int64_t)t.m * BM + 32 * quarter;
+      const int64_t row0 = (PAIR ? 2 * (int64_t)t.m + rank : (int64_t)t.m) * BM + 32 * quarter;
       // kept g and u: a block of 32 x 32 is eight requests of a float4 a lane, its row's
       auto kept_at = [&](float* base_, int col, int q) {
         const int64_t block = (row0 >> 5) * ((e.ld_h + 31) >> 5) + (col >> 5);
@@ -710,9 +774,11 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
   if (f.aborted[0] && warp == 0)   // copies may still be on their way here
     for (int i = 0; i < 64; ++i) __nanosleep(1000);
   __syncthreads();
+  if constexpr (PAIR) pair_sync();   // neither leaves while the other's products, copies or arrivals may reach it
   if (warp == 0) {
     __syncwarp();
-    tmem_dealloc(tmem, 512);
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 

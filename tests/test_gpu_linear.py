@@ -77,6 +77,9 @@ CASES = [
     (7, 3080, 50, F32, False, None, "silu", False),
     (8, 1536, 41, BF16, False, False, "gelu", True),
     (3, 1024, 9, BF16, False, None, "gelu", False),          # few rows, slopes kept
+    (4400, 520, 2100, BF16, False, False, "gelu", True),     # tiles of two CTAs, the last one's second without rows
+    (2050, 4100, 1000, F16, False, None, None, False),
+    (4500, 600, 2056, BF16, True, True, "silu", False),
     (130, 64, 40, BF16, True, True, "gelu", True),           # z kept, for the bias's gradient in float32
 ]
 
