@@ -250,7 +250,7 @@ struct Shape {
   static constexpr uint32_t OUT_BYTES = WARPS * 2048;   // shared memory of the results on their way out
   static constexpr uint32_t B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2, STAGE = (OUT == Out::AGAIN ? 2 : 1) * A_BYTES + B_BYTES;
   static constexpr int COLS = OUT == Out::GATE ? BN / 2 : OUT == Out::AGAIN ? BN / 3 : BN;   // of the output
-  static constexpr uint32_t BIAS = OUT == Out::LINEAR ? WARPS * 128 : 0;   // a warp's bias of a segment
+  static constexpr uint32_t BIAS = OUT == Out::LINEAR ? WARPS * COLS * 2 : 0;   // a warp's bias of its part of a tile, 32 columns of 64 at most
   static constexpr int FIT = (int)((227 * 1024 - 1024 - sizeof(Frame2) - OUT_BYTES - BIAS) / STAGE), STAGES = FIT < MAX_STAGES ? FIT : MAX_STAGES;
   static constexpr uint32_t OUT_AT = STAGES * STAGE, BIAS_AT = OUT_AT + OUT_BYTES, FRAME = BIAS_AT + BIAS, BYTES = FRAME + sizeof(Frame2) + 1024;   // 1024: to the swizzle's boundary
 };
@@ -534,6 +534,21 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
         if (!waited) wait(f.acc[set], done / SETS, W_ACC), waited = true;
         tc_fence_after();
       };
+      float* tile_bias = reinterpret_cast<float*>(smem + S::BIAS_AT + (warp - 2) * (S::COLS * 2));
+      if constexpr (OUT == Out::LINEAR) {
+        float b[S::COLS / 64];
+#pragma unroll
+        for (int i = 0; i < S::COLS / 64; ++i) {
+          const int col = t.n * S::COLS + 64 * i + part * SEG + lane;
+          b[i] = 0.f;
+          if (e.bias && lane < SEG && col < p.n) b[i] = e.bias_kind == 0 ? static_cast<const float*>(e.bias)[col] : up(static_cast<const E*>(e.bias)[col]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < S::COLS / 64; ++i)
+          if (lane < SEG) tile_bias[i * SEG + lane] = b[i];
+        __syncwarp();
+      }
 #pragma unroll 1
       for (int c64 = 0; c64 < S::COLS; c64 += 64) {
         const int first = t.n * S::COLS + c64, c0 = c64 + part * SEG, col0 = first + part * SEG;
@@ -543,25 +558,17 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
           tmem_wait_ld();
           if (!EXACT && last && k + 8 == SEG) release(set), released = true;
         };
-        // a linear layer: the rows of `other` as whole rows and the bias, on their way before the accumulators are waited for
+        // a linear layer: the rows of `other` as whole rows, on their way before the accumulators are waited for
         uint4 others[OUT == Out::LINEAR && !EXACT ? 8 / PARTS : 1];
-        float* bias = reinterpret_cast<float*>(smem + S::BIAS_AT + (warp - 2) * 128);
-        if constexpr (OUT == Out::LINEAR) {
-          float b = 0.f;
-          if (e.bias && lane < SEG && col0 + lane < p.n)
-            b = e.bias_kind == 0 ? static_cast<const float*>(e.bias)[col0 + lane] : up(static_cast<const E*>(e.bias)[col0 + lane]);
-          if constexpr (!EXACT) {
-            if (e.other)
+        const float* bias = tile_bias + c64 / 64 * SEG;
+        if constexpr (OUT == Out::LINEAR && !EXACT) {
+          if (e.other)
 #pragma unroll
-              for (int i = 0; i < 8 / PARTS; ++i) {
-                const int r = (32 / PARTS) * part + i * 4 + lane / 8;
-                others[i] = row0 + r < p.m ? get16(static_cast<const E*>(e.other) + (row0 + r) * e.ld_other, first + 8 * (lane % 8), p.n, e.other_wide)
-                                           : make_uint4(0u, 0u, 0u, 0u);
-              }
-          }
-          __syncwarp();
-          bias[lane] = b;
-          __syncwarp();
+            for (int i = 0; i < 8 / PARTS; ++i) {
+              const int r = (32 / PARTS) * part + i * 4 + lane / 8;
+              others[i] = row0 + r < p.m ? get16(static_cast<const E*>(e.other) + (row0 + r) * e.ld_other, first + 8 * (lane % 8), p.n, e.other_wide)
+                                         : make_uint4(0u, 0u, 0u, 0u);
+            }
         }
         uint4 kept[OUT == Out::BACK ? 2 : 1][SEG / 4];
         if constexpr (OUT == Out::BACK) {
@@ -652,10 +659,11 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
             for (int i = 0; i < 8 / PARTS; ++i) *reinterpret_cast<uint4*>(rows + row_piece((32 / PARTS) * part + i * 4 + lane / 8, lane % 8)) = others[i];
             meet();
           }
+          uint32_t next[8];   // on their way while the eight columns before are worked on
+          tmem_ld8_nowait(acc + c0, next);
 #pragma unroll
           for (int k0 = 0; k0 < SEG; k0 += 8) {
             uint32_t z[8], bits[4], o[4] = {0u, 0u, 0u, 0u};
-            tmem_ld8_nowait(acc + c0 + k0, z);
             uint4* at = reinterpret_cast<uint4*>(rows + row_piece(lane, (part * SEG + k0) / 8));   // this lane's own
             const float4 b0 = *reinterpret_cast<const float4*>(bias + k0), b1 = *reinterpret_cast<const float4*>(bias + k0 + 4);
             if (e.other) {
@@ -663,6 +671,9 @@ static __global__ void __launch_bounds__(Crew<PIECES, BN, OUT>::THREADS, 1) k_pr
               o[0] = raw.x, o[1] = raw.y, o[2] = raw.z, o[3] = raw.w;
             }
             taken(k0);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] = next[k];
+            if (k0 + 8 < SEG) tmem_ld8_nowait(acc + c0 + k0 + 8, next);
             const F2 b[4] = {f2(b0.x, b0.y), f2(b0.z, b0.w), f2(b1.x, b1.y), f2(b1.z, b1.w)};
             F2 v[4];
 #pragma unroll
