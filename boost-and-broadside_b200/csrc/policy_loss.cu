@@ -271,6 +271,7 @@ __device__ __forceinline__ float share_of_rows(const Args& a) {
 
 // ------------------------------------------------------------------ narrow slices
 
+constexpr int NARROW_WARPS = 16;   // of a CTA, at most
 struct Tile { int rows, threads, pitch; size_t bytes; };
 // Rows of a tile by how many slices they have; floats in shared memory, rows an odd number of them apart.
 Tile tile_of(int slices, int width) {
@@ -282,9 +283,9 @@ Tile tile_of(int slices, int width) {
   return t;
 }
 template <typename E>
-__global__ void __launch_bounds__(512) k_narrow(const __grid_constant__ Args a, int tile_rows, int pitch, uint32_t per_width) {
+__global__ void __launch_bounds__(32 * NARROW_WARPS) k_narrow(const __grid_constant__ Args a, int tile_rows, int pitch, uint32_t per_width) {
   extern __shared__ float tile[];
-  __shared__ double sums[16][TERMS];
+  __shared__ double sums[NARROW_WARPS][TERMS];
   let_next_start();
   wait_for_previous();
   const BnbPolicyLoss& c = a.c;
@@ -670,7 +671,7 @@ int forward(Args a, cudaStream_t st) {
   if (narrow(c)) {
     const Tile t = tile_of(c.n_slices, a.width);
     const size_t bytes = t.bytes + 8;
-    if (bytes > 48 * 1024 && cudaFuncSetAttribute(k_narrow<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return BNB_ERR_LAUNCH;
+    if (bytes + NARROW_WARPS * TERMS * sizeof(double) > 48 * 1024 && cudaFuncSetAttribute(k_narrow<E>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return BNB_ERR_LAUNCH;
     ctas = ctas_of((c.rows + t.rows - 1) / t.rows, MAX_CTAS);
     r = launch_after(k_narrow<E>, dim3(ctas), t.threads, bytes, st, a, t.rows, t.pitch, (uint32_t)((((uint64_t)1 << 32) + a.width - 1) / a.width));
   } else {

@@ -71,6 +71,9 @@ CASES = [
     (16, [3, 7, 2], F32, "mask", False, False, 1.0),
     (1000, [3, 7, 2], BF16, "mask", True, True, 0.25),
     (129, [3, 7, 2], F16, "float", True, True, 300.0),
+    (130, [40, 30, 10, 7], F32, None, False, False, 1.0),            # tiles that take nearly 48 KB of shared memory: with four slices,
+    (70, [30, 25, 20, 25, 20, 25, 20, 10], BF16, "mask", True, False, 1.0),   # eight
+    (40, [22] * 15 + [19], F16, None, False, True, 80.0),            # and sixteen
     (200, [64], BF16, "float", True, False, 1.0),
     (77, [64, 1, 64, 63, 2, 5, 11, 64, 3], F32, None, True, True, 1.0),
     (50, [5] * 16, F16, "mask", False, False, 100.0),
