@@ -646,7 +646,8 @@ int ctas_of(int64_t units, int most) { return (int)std::max<int64_t>(1, std::min
 
 // Threads of a row: some 8 to 16 pieces of 16 bytes each, so that what a row takes besides, a chain of some 2 us, is shared by few and many rows are at
 // work.  Forward with gradients of 134 M bfloat16 logits (268 MB each way), us by width: 32768 with 256 threads 135 (512: 160), 16384
-// with 128 135 (256: 148), 8192 with 64 138 (128: 145, 256: 195), 4096 with 64 149 (32: 171), 2048 with 32 169 (256: 520).
+// with 128 135 (256: 148), 8192 with 64 138 (128: 145, 256: 195), 4096 with 64 149 (32: 171), 2048 with 32 169 (256: 520);
+// since then, with one maximum for four pieces, 118, 120, 123 and, 2048 wide, 137.
 template <typename E, int T, int THREADS, bool GRAD>
 int launch_wide(const Args& a, int& ctas, cudaStream_t st) {
   ctas = ctas_of((a.c.rows + THREADS / T - 1) / (THREADS / T), MAX_CTAS);   // more than there is room for: rows without weight take less
