@@ -258,3 +258,35 @@ def test_what_is_not_finite_stays_in_its_rows():
             spoiled[9, 0] = float("inf")
             grad, = torch.autograd.grad(y, [bad], spoiled)
             assert not grad[9].isfinite().any() and grad[10:].isfinite().all() and grad[:7].isfinite().all()
+
+
+def test_large_products_in_a_graph():
+    """Tiles of two CTAs, several launches behind one another, captured and replayed with other numbers, beside the same call on another stream."""
+    import boost_and_broadside_b200 as bnb
+
+    g = torch.Generator().manual_seed(21)
+    M, K, N = 4400, 640, 2100
+    x, w, b, dy = [torch.randn(*s, generator=g).to(BF16).to(DEV) for s in ((M, K), (N, K), (N,), (M, N))]
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def call():
+        y = bnb.linear(*leaves, activation="gelu")
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for scale in (1.0, -0.5):
+        with torch.no_grad():
+            x.mul_(scale)
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            other = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(got, other)) and all(torch.equal(a, e) for a, e in zip(got, call()))
